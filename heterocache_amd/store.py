@@ -254,6 +254,45 @@ class KVStore:
         self.host_len += 1
         self._headroom -= 1
 
+    def append_rotated(self, q, k, v, cos, sin, counts=None, out=None, stream=None):
+        """Turn new queries [B, Hq, T, 128] and keys [B, Hkv, T, 128] by their
+        rotation tables and append keys and values to rows b * Hkv + h, the
+        lengths advancing with them (ops.append_rotated).  Returns the turned
+        queries.
+
+        counts: tokens of each sequence to append (host integers, at most T;
+        None: all T): the rest is padding.  Raises the reference's "Layer i
+        OOM." when a row has no room.
+        """
+        rows, T = k.shape[0] * k.shape[1], k.shape[2]
+        if rows != self.rows:
+            raise ValueError(f"keys of {rows} rows for a store of {self.rows}")
+        dev_counts = add = None
+        if counts is None:
+            if self._headroom < T:
+                raise self._oom()
+        else:
+            counts = np.asarray(counts, dtype=np.int64).reshape(-1)
+            if len(counts) != k.shape[0] or (counts < 0).any() or (counts > T).any():
+                raise ValueError(f"counts must be one integer in 0..{T} per sequence")
+            add = np.repeat(counts, k.shape[1]).astype(np.int32)
+            if (self.host_len + add > self.host_cap).any():
+                raise self._oom()
+            if stream is not None:
+                with torch.cuda.stream(stream):
+                    dev_counts = ops.to_device(counts, self.device, torch.int32)
+            else:
+                dev_counts = ops.to_device(counts, self.device, torch.int32)
+        out = ops.append_rotated(q, k, v, cos, sin, self.k, self.v, self.row_tile_off, self.row_len, self.row_cap,
+                                 counts=dev_counts, out=out, len_out=self.row_len, status=self.status, stream=stream)
+        if add is None:
+            self.host_len += np.int32(T)
+            self._headroom -= T
+        else:
+            self.host_len += add
+            self._headroom = int((self.host_cap - self.host_len).min()) if self.rows else 0
+        return out
+
     # -- readers -----------------------------------------------------------
     def read_rows(self, rows, count):
         if count > int(self.host_cap[np.asarray(rows, dtype=np.int64)].min()):
@@ -284,6 +323,45 @@ class KVStore:
             self._headroom -= 1
         return out
 
+    def attend_shared(self, q, prefix, scale, out=None, stream=None):
+        """Attention of queries [B, Hq, Q, 128] (the last Q tokens of these
+        rows) over the shared `prefix`, a KVStore of Hkv rows or None, and
+        over this store's rows b * Hkv + h: [B, Q, Hq, 128]
+        (ops.shared_attn).  Lengths are read on the device: a captured call
+        replays while the rows grow."""
+        B = q.shape[0]
+        if B == 0 or self.rows % B:
+            raise ValueError(f"{self.rows} rows for {B} sequences")
+        kv = self.rows // B
+        pre = None
+        ptiles = 0
+        if prefix is not None:
+            if prefix.rows != kv:
+                raise ValueError(f"a prefix of {prefix.rows} rows for {kv} KV heads")
+            pre = (prefix.k, prefix.v, prefix.row_tile_off, prefix.row_len)
+            ptiles = int(prefix.host_len.sum()) // TILE + kv
+        return ops.shared_attn(q, pre, (self.k, self.v, self.row_tile_off, self.row_len), kv, scale, prefix_tiles=ptiles,
+                               row_tiles=int(self.host_len.max(initial=0)) // TILE + 1, out=out, stream=stream)
+
+    def block_index(self, block=64):
+        """An index of this store's key blocks of `block` tokens for
+        attend_blocks (empty until its update)."""
+        return BlockIndex(self, block)
+
+    def attend_blocks(self, q, index, keep, scale, sink=1, local=2, out=None, stream=None):
+        """Attention of queries [B, Hq, Q, 128] (the last Q tokens of their
+        rows) over `keep` blocks of each row: its first `sink`, last `local`
+        and those that score highest for the query (ops.block_select,
+        ops.block_attn).  Returns (out [B, Q, Hq, 128], idx [rows, Q, keep],
+        counts [rows, Q]).  The index must hold every complete block."""
+        if index.store is not self:
+            raise ValueError("the index is another store's")
+        idx, counts = ops.block_select(q, index.bounds, index.exps, index.row_block_off, self.row_len, index.block,
+                                       index.max_blocks, keep, sink=sink, local=local, stream=stream)
+        out = ops.block_attn(q, self.k, self.v, self.row_tile_off, self.row_len, idx, counts, index.block, scale,
+                             out=out, stream=stream)
+        return out, idx, counts
+
     def _oom(self):
         name = "?" if self.layer_idx is None else self.layer_idx
         return RuntimeError(f"Layer {name} OOM.")
@@ -305,3 +383,45 @@ class KVStore:
             if e.code == _lib.HC_ERR_CAPACITY:
                 raise self._oom() from e
             raise
+
+
+class BlockIndex:
+    """8-bit channel bounds of a store's complete key blocks, from which
+    KVStore.attend_blocks picks the blocks a query reads.
+
+    bounds int8 [blocks, 2, 128] (maxima, minima), exps int8 [blocks]: see
+    hc_block_bounds in include/hc.h.  A block's entry stays valid while its
+    keys stay: after tokens were appended, update(new_tokens) adds the blocks
+    they completed; after rows were rewritten, update() takes all again.
+    """
+
+    def __init__(self, store, block):
+        block = int(block)
+        if block < TILE or block % TILE:
+            raise ValueError(f"block must be a positive multiple of {TILE}, got {block}")
+        self.store = store
+        self.block = block
+        whole = store.host_cap // block
+        off = np.zeros(store.rows, dtype=np.int64)
+        if store.rows > 1:
+            off[1:] = np.cumsum(whole)[:-1]
+        n = max(int(whole.sum()), 1)
+        self.max_blocks = int((-(-store.host_cap // block)).max(initial=0))
+        self.row_block_off = torch.as_tensor(off, dtype=torch.int64).to(store.device)
+        self.bounds = torch.zeros((n, 2, HEAD_DIM), dtype=torch.int8, device=store.device)
+        self.exps = torch.zeros(n, dtype=torch.int8, device=store.device)
+
+    def update(self, new_tokens=None, stream=None):
+        """Take the bounds of every complete block, or with new_tokens of
+        those that each row's last new_tokens tokens completed."""
+        s = self.store
+        if new_tokens is None:
+            span, fresh = int(s.host_len.max(initial=0)) // self.block, 0
+        else:
+            fresh = int(new_tokens)
+            if fresh < 0:
+                raise ValueError(f"new_tokens={fresh}")
+            span = -(-fresh // self.block)
+        if span:
+            ops.block_bounds(s.k, s.row_tile_off, s.row_len, self.row_block_off, self.block, self.bounds, self.exps,
+                             span, fresh=fresh, stream=stream)

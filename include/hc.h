@@ -544,6 +544,116 @@ size_t hc_drift_scratch_size(int njobs, int span);
 int hc_drift_decide(const int32_t* counts, int npiv, int batch, int steps, int K, double threshold, float* overlap,
                     double* median, int32_t* trigger, void* stream);
 
+/*
+ * Rotated append: the new queries and keys of `tokens` positions turned by
+ * their rotation tables, keys and values stored into the ragged store, in one
+ * pass over them.  For every query and key head, with 128-channel tables
+ * cos, sin of each (sequence, token):
+ *   x'[d]      = x[d] * cos[d] - x[d + 64] * sin[d]              d < 64
+ *   x'[d + 64] = x[d + 64] * cos[d + 64] + x[d] * sin[d + 64]
+ * formed in float32 and rounded once.  q_out receives every query, padding
+ * included (q_out may be q itself).  Of sequence b the first counts[b] tokens
+ * (counts NULL: all; clamped to [0, tokens]) are stored: token t of head h
+ * goes to slot row_len[r] + t of row r = b * kv_heads + h.
+ * len_out (optional, int32 [rows]): receives row_len[r] + counts[b]; it may be
+ * row_len itself (the lengths advance) or a tensor that does not overlap it.
+ * A row whose tokens exceed row_cap[r] is left unchanged, its length too, and
+ * sets bit 0 of *status (optional; hc_read_status).
+ * q, q_out, k, v: base + b*strides[0] + h*strides[1] + t*strides[2] + c
+ * (element strides, 16-byte multiples, 16-byte aligned bases); tables: base +
+ * b*table_batch_stride + t*table_tok_stride + c, of dtype table_dtype (the
+ * tensors' or float32); a zero batch stride shares one table.
+ * Stands beside hc_append, which takes one turned token a row; replaces the
+ * model's rotary embedding of the new tokens and the append that follows it
+ * (heterocache/cache_utils.py:970-1005).
+ */
+int hc_append_rotated(int dtype, int table_dtype, const void* q, const int64_t* q_strides, void* q_out,
+                      const int64_t* q_out_strides, const void* k, const int64_t* k_strides, const void* v,
+                      const int64_t* v_strides, const void* cos, const void* sin, int64_t table_batch_stride,
+                      int64_t table_tok_stride, void* kstore, void* vstore, const int64_t* row_tile_off,
+                      const int32_t* row_len, const int32_t* row_cap, int32_t* len_out, const int32_t* counts,
+                      int batch, int q_heads, int kv_heads, int tokens, int32_t* status, void* stream);
+
+/*
+ * Attention of a batch over one shared prefix and each sequence's own rows:
+ *   out[b, h, i] = softmax over {prefix row kv, tokens t < prefix_len[kv]} and
+ *                  {row b * kv_heads + kv, tokens t < row_len - queries + 1 + i}
+ * of scale * q[b, h, i] . k_t, times their values; kv = h / (q_heads /
+ * kv_heads).  The queries are the last `queries` tokens of the rows (1: a
+ * decode step); zeros where nothing is visible.  The prefix is a store of
+ * kv_heads rows, each of its own length (a prompt kept whole or compressed
+ * per head), and is read once for all sequences.  prefix_len NULL: no prefix;
+ * row_len NULL: no rows of their own.  prefix_tiles, row_tiles: tiles of all
+ * prefix rows and of the longest own row that the call should be cut for
+ * (bounds such as the capacities; they set the grid and the workspace, and
+ * any device lengths are attended whole whatever they are, so a captured
+ * call replays while the rows grow).
+ * q, out: base + b*strides[0] + h*strides[1] + i*strides[2] + c, q's strides
+ * 16-byte multiples; at most 16 query heads a KV head and 2^24 query rows;
+ * scale finite and positive.  workspace: hc_shared_workspace_size bytes,
+ * 16-byte aligned, no initialisation; calls that overlap in time need their
+ * own.  Matrix products on the input type, softmax and sums in float32.
+ * Stands beside hc_decode_attn, which would read the prefix once a sequence;
+ * no counterpart in the reference, whose cache serves one sequence.
+ */
+int hc_shared_attn(int dtype, const void* q, const int64_t* q_strides, const void* kprefix, const void* vprefix,
+                   const int64_t* prefix_tile_off, const int32_t* prefix_len, int64_t prefix_tiles, const void* kstore,
+                   const void* vstore, const int64_t* row_tile_off, const int32_t* row_len, int64_t row_tiles,
+                   void* out, const int64_t* out_strides, int batch, int q_heads, int kv_heads, int queries,
+                   float scale, void* workspace, size_t workspace_bytes, void* stream);
+size_t hc_shared_workspace_size(int dtype, int batch, int q_heads, int kv_heads, int queries, int64_t prefix_tiles,
+                                int64_t row_tiles);
+
+/*
+ * Attention over the key blocks that a score selects for each query, in three
+ * calls.  A block is `block` tokens (a multiple of 32) of a row.  No
+ * counterpart in the reference, which reads a kept head whole; for rows that
+ * keep their whole prompt (its volatile and pivot heads).
+ *
+ * hc_block_bounds: of complete blocks, bounds int8 [block][2][128] (channel
+ * maxima, then minima, of the keys) and exps int8 [block]:
+ *   e = the least exponent in [-48, 48] with max |k| <= 127 * 2^e,
+ *   hi = ceil(max_t k_t / 2^e), lo = floor(min_t k_t / 2^e)   (-127 .. 127);
+ * NaN keys are passed over.  Block j of row r lies at row_block_off[r] + j.
+ * Of each row the last `span` complete blocks are taken, with fresh > 0 only
+ * those that its last `fresh` tokens completed.  A row whose stored keys
+ * change must have its blocks taken again.
+ */
+int hc_block_bounds(int dtype, const void* kstore, const int64_t* row_tile_off, const int32_t* row_len,
+                    const int64_t* row_block_off, int rows, int block, int span, int fresh, int8_t* bounds,
+                    int8_t* exps, void* stream);
+/*
+ * hc_block_select: the blocks that each query of each row keeps.  With q8 =
+ * rint(q / 2^eq) (eq found as e above) a block scores
+ *   max over the row's query heads of 2^(eq + e) * sum_d max(q8_d hi_d, q8_d lo_d),
+ * a sum of whole numbers, so the score is exact and the selection does not
+ * depend on batch, grid or order.  Query i sees row_len - queries + 1 + i
+ * tokens; of its visible blocks it keeps the first `sink`, the last `local`
+ * (at least 1: the unfinished block is never scored) and the best of the
+ * others, equal scores to the lower block: `keep` in all, or every block if
+ * there are no more.  idx int32 [rows][queries][keep]: ascending, -1 past
+ * counts int32 [rows][queries].  max_blocks: visible blocks that scratch
+ * (hc_block_select_scratch_size bytes, no initialisation) has room for; a
+ * query that sees more gets counts -1 and no block.
+ */
+int hc_block_select(int dtype, const void* q, const int64_t* q_strides, const int8_t* bounds, const int8_t* exps,
+                    const int64_t* row_block_off, const int32_t* row_len, int batch, int q_heads, int kv_heads,
+                    int queries, int block, int max_blocks, int keep, int sink, int local, int32_t* idx,
+                    int32_t* counts, void* scratch, size_t scratch_bytes, void* stream);
+size_t hc_block_select_scratch_size(int batch, int kv_heads, int queries, int max_blocks);
+/*
+ * hc_block_attn: out[b, h, i] = softmax(scale * q . k_t) v_t over the visible
+ * tokens of the blocks idx[r][i][0 .. counts[r][i]) (distinct, in any order;
+ * an entry that is no visible block of the row is passed over; counts -1:
+ * NaN).  Layouts as hc_shared_attn's; workspace:
+ * hc_block_attn_workspace_size bytes (may be 0).
+ */
+int hc_block_attn(int dtype, const void* q, const int64_t* q_strides, const void* kstore, const void* vstore,
+                  const int64_t* row_tile_off, const int32_t* row_len, const int32_t* idx, const int32_t* counts,
+                  int keep, int block, void* out, const int64_t* out_strides, int batch, int q_heads, int kv_heads,
+                  int queries, float scale, void* workspace, size_t workspace_bytes, void* stream);
+size_t hc_block_attn_workspace_size(int batch, int q_heads, int kv_heads, int queries, int block, int keep);
+
 #ifdef __cplusplus
 }
 #endif
