@@ -500,7 +500,7 @@ extern "C" int hc_block_attn(int dtype, const void* q, const int64_t* q_strides,
     r.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + p.part_o);
   }
   hipStream_t s = (hipStream_t)stream;
-  if ((rc = launch_rows_attn(dtype, r, s)) || p.nsplit == 1) return rc;
+  if ((rc = launch_block_rows(dtype, r, s)) || p.nsplit == 1) return rc;
   MergeArgs mg = {};
   mg.row_o = r.part_o, mg.row_ml = r.part_ml, mg.nsplit = p.nsplit;
   mg.Hkv = kv_heads, mg.G = G, mg.Q = queries, mg.out = out;

@@ -287,6 +287,10 @@ __device__ __forceinline__ void rows4_transpose(float (&e)[4]) {
 __device__ __forceinline__ void lds_dma16(const void* src, void* lds) {
   __builtin_amdgcn_global_load_lds(src, lds, 16, 0, 0);
 }
+// lds_dma16 with the nontemporal hint, for data that one workgroup reads.
+__device__ __forceinline__ void lds_dma16_stream(const void* src, void* lds) {
+  __builtin_amdgcn_global_load_lds(src, lds, 16, 0, 2);
+}
 // s_waitcnt vmcnt(0): every LDS-DMA load of this wave has landed.
 __device__ __forceinline__ void wait_lds_dma() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 // s_waitcnt vmcnt(N): all but this wave's N most recent vector loads have

@@ -1,6 +1,6 @@
-// Attention of a wave over 32-token tiles of the ragged store, shared by the
-// kernels that read rows straight from memory into MFMA operands (a batch's
-// own rows beside a shared prefix; the kept blocks of a row).
+// Attention over 32-token tiles of the ragged store, shared by the kernels
+// that read rows straight from memory into MFMA operands (a batch's own rows
+// beside a shared prefix; the kept blocks of a row).
 //
 // A wave holds up to 16 query columns: lane l serves column l % 16 and the
 // k-group l / 16.  Each column has a limit, the first token it does not see.
@@ -38,31 +38,24 @@ __device__ __forceinline__ void zero_tail(typename Elem<T>::vec8& v, int tok0, i
     if (tok0 + 16 * (e >> 2) + 4 * g + (e & 3) >= end) set8<T>(v, e, 0.f);
 }
 
-// Tokens tok0 + [0, 32) of a row, their K and V operands in kr and vr.  lim:
-// this lane's column limit; lim_lo <= lim <= lim_hi over the wave's columns
-// (both uniform), and equal unless MIXED.  scale_log2 > 0.
-template <typename T, bool MIXED>
-__device__ __forceinline__ void attend_rows(const typename Elem<T>::vec8 (&kr)[8], typename Elem<T>::vec8 (&vr)[8],
-                                            const typename Elem<T>::vec8 (&qreg)[4], int tok0, int lim, int lim_lo,
-                                            int lim_hi, int lane, float scale_log2, float& m, float& l,
-                                            f32x4 (&o)[8]) {
-  const int g = lane >> 4;
-  f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+// S^T of a tile's 32 tokens: element e of the pair (s[e / 4][e % 4]) is token
+// 16 (e / 4) + 4 g + e % 4 against the lane's column.
+template <typename T>
+__device__ __forceinline__ void tile_scores(const typename Elem<T>::vec8 (&kr)[8],
+                                            const typename Elem<T>::vec8 (&qreg)[4], f32x4 (&s)[2]) {
+  s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     s[0] = mma_16x16x32(kr[x], qreg[x], s[0]);
     s[1] = mma_16x16x32(kr[4 + x], qreg[x], s[1]);
   }
-  const bool edge = tok0 + HC_TILE > lim_lo;
-  if (edge) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (tok0 + 16 * (e >> 2) + 4 * g + (e & 3) >= lim) s[e >> 2][e & 3] = -INFINITY;
-    if (tok0 + HC_TILE > lim_hi) {
-#pragma unroll
-      for (int mt = 0; mt < 8; ++mt) zero_tail<T>(vr[mt], tok0, lim_hi, g);
-    }
-  }
+}
+
+// Probabilities of a tile's scores (already masked) in the input type, the
+// state m, l and, when the reference point moves, O following.  scale_log2 > 0.
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::vec8 tile_probs(const f32x4 (&s)[2], float scale_log2, float& m, float& l,
+                                                             f32x4 (&o)[8]) {
   typename Elem<T>::vec8 pb;
   float ps;
   auto probs = [&](float nm) {
@@ -91,11 +84,25 @@ __device__ __forceinline__ void attend_rows(const typename Elem<T>::vec8 (&kr)[8
     probs(mnew == -INFINITY ? 0.f : -mnew);
   }
   l += ps;
-  if (MIXED && edge && lim_lo < lim_hi) {
+  return pb;
+}
+
+// O += V^T P^T over tokens tok0 + [0, 32).  lim: this lane's column limit;
+// lim_lo <= lim <= lim_hi over the wave's columns (both uniform), and equal
+// unless MIXED.
+template <typename T, bool MIXED>
+__device__ __forceinline__ void tile_values(typename Elem<T>::vec8 (&vr)[8], const typename Elem<T>::vec8& pb, int tok0,
+                                            int lim, int lim_lo, int lim_hi, int g, f32x4 (&o)[8]) {
+  if (tok0 + HC_TILE > lim_hi) {
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) zero_tail<T>(vr[mt], tok0, lim_hi, g);
+  }
+  if (MIXED && tok0 + HC_TILE > lim_lo && lim_lo < lim_hi) {
     // Some columns do not see tokens that others see.  Their probabilities
-    // are zero, but zero times an infinite or NaN value is not: with one
-    // among those tokens each limit takes its own product, over values that
-    // end at it, and only its own columns keep the result.
+    // are zero, but zero times an infinite or NaN value is not: with one in
+    // the tile the finite values take the product, and what the others would
+    // add is told by the weight that their positive and their negative ones
+    // (NaN: both) have in each column.
     bool bad = false;
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt)
@@ -105,13 +112,24 @@ __device__ __forceinline__ void attend_rows(const typename Elem<T>::vec8 (&kr)[8
         bad |= !(x - x == 0.f);
       }
     if (__any(bad)) {
-      for (int end = lim_lo; end <= lim_hi; ++end) {
 #pragma unroll
-        for (int mt = 0; mt < 8; ++mt) {
-          typename Elem<T>::vec8 vz = vr[mt];
-          zero_tail<T>(vz, tok0, end, g);
-          const f32x4 r = mma_16x16x32(vz, pb, o[mt]);
-          if (lim == end) o[mt] = r;
+      for (int mt = 0; mt < 8; ++mt) {
+        typename Elem<T>::vec8 up, down;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = vec8_at<T>(vr[mt], e);
+          const bool odd = !(x - x == 0.f);
+          set8<T>(up, e, odd && !(x < 0.f) ? 1.f : 0.f);
+          set8<T>(down, e, odd && !(x > 0.f) ? 1.f : 0.f);
+          if (odd) set8<T>(vr[mt], e, 0.f);
+        }
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        const f32x4 wu = mma_16x16x32(up, pb, zero), wd = mma_16x16x32(down, pb, zero);
+        o[mt] = mma_16x16x32(vr[mt], pb, o[mt]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (wu[j] > 0.f) o[mt][j] += INFINITY;
+          if (wd[j] > 0.f) o[mt][j] -= INFINITY;
         }
       }
       return;
@@ -121,15 +139,11 @@ __device__ __forceinline__ void attend_rows(const typename Elem<T>::vec8 (&kr)[8
   for (int mt = 0; mt < 8; ++mt) o[mt] = mma_16x16x32(vr[mt], pb, o[mt]);
 }
 
-// K and V operands of the tile that starts at element `at` of both stores.
+// The eight operands of a tile of K or V (8 wave loads of 1 KB in a row).
 template <typename T>
-__device__ __forceinline__ void load_rows_tile(typename Elem<T>::vec8 (&kr)[8], typename Elem<T>::vec8 (&vr)[8],
-                                               const T* kb, const T* vb, int64_t at) {
+__device__ __forceinline__ void load_operands(typename Elem<T>::vec8 (&r)[8], const T* p) {
 #pragma unroll
-  for (int x = 0; x < 8; ++x) {
-    kr[x] = load8_stream<T>(kb + at + x * 512);
-    vr[x] = load8_stream<T>(vb + at + x * 512);
-  }
+  for (int x = 0; x < 8; ++x) r[x] = load8_stream<T>(p + x * 512);
 }
 
 // One output row's weights: the reference M of several (m, l) states and
@@ -142,8 +156,7 @@ __device__ __forceinline__ float state_weight(float m, float M) { return m == -I
 
 namespace hc {
 
-// Attention of a wave's query columns over rows of the store, and the fold of
-// partial results; defined in hc_rows.hip.
+// A launch's jobs over rows of the store (rows_job).
 struct RowsArgs {
   const void* q;
   int64_t q_s[3];  // element strides: batch, head, token
@@ -165,6 +178,153 @@ struct RowsArgs {
   int64_t o_s[3];
 };
 
+constexpr int kRowsWaves = 4;
+constexpr int kRowsPitch = HC_HEAD_DIM + 4;
+// LDS floats of rows_job: the waves' O and (m, l).
+constexpr int kRowsLds = kRowsWaves * 16 * (kRowsPitch + 2);
+
+// Workgroup `wg` of a rows launch (4 waves): one split of one job (qpb queries
+// of one row and its G heads).  The waves take every fourth tile of the split
+// straight into the operand registers and are combined through LDS (lds:
+// kRowsLds floats).  K's registers are refilled once the scores are formed,
+// V's once the values are added, so a wave always has half a tile or more in
+// flight with one tile's registers, and three waves fit a SIMD (a second
+// buffer leaves two).  Bound by HBM: a token's K and V (512 bytes in 16 bits)
+// feed 512 G operations a query.
+template <typename T, bool LIST, bool MIXED>
+__device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds) {
+  typedef typename Elem<T>::vec8 vec8;
+  float(*s_o)[16][kRowsPitch] = reinterpret_cast<float(*)[16][kRowsPitch]>(lds);
+  float(*s_m)[16] = reinterpret_cast<float(*)[16]>(lds + kRowsWaves * 16 * kRowsPitch);
+  float(*s_l)[16] = s_m + kRowsWaves;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, n = lane & 15;
+  const int jobs = a.rows * a.ncb;
+  const int job = wg % jobs, split = wg / jobs;
+  const int row = job / a.ncb, cb = job % a.ncb;
+  const int b = row / a.Hkv, kv = row % a.Hkv;
+  const int len = max(a.row_len[row], 0);
+  const int64_t base = a.row_tile_off[row] * (int64_t)HC_TILE_ELEMS + lane * 8;
+
+  // Column n: query i0 + n / G, head n % G of the row's group.
+  const int i0 = cb * a.qpb, nq = min(a.qpb, a.Q - i0), ncols = nq * a.G;
+  const bool col_ok = n < ncols;
+  const int qi = col_ok ? n / a.G : nq - 1, gi = col_ok ? n % a.G : 0;
+  const int lim_lo = min(max(len - a.Q + 1 + i0, 0), len);
+  const int lim_hi = min(max(len - a.Q + i0 + nq, 0), len);
+  const int lim = min(max(len - a.Q + 1 + i0 + qi, 0), len);
+
+  // Entries of the job, this workgroup's share of them and this wave's: e0 +
+  // wave, e0 + wave + 4, ...
+  const int vis = (lim_hi + HC_TILE - 1) / HC_TILE;
+  const int64_t job_q = (int64_t)row * a.Q + i0;  // LIST: one query a job
+  int entries = vis;
+  bool void_list = false;  // no selection was made: the output is NaN
+  if constexpr (LIST) {
+    const int c = a.counts[job_q];
+    void_list = c < 0;
+    entries = vis > 0 ? min(max(c, 0), a.keep) * a.tpb : 0;
+  }
+  const int e0 = (int)((int64_t)entries * split / a.nsplit), e1 = (int)((int64_t)entries * (split + 1) / a.nsplit);
+  const int cnt = max((e1 - e0 - wave + kRowsWaves - 1) / kRowsWaves, 0);
+
+  vec8 qreg[4];
+  {
+    const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_s[0] + (int64_t)(kv * a.G + gi) * a.q_s[1] +
+                  (int64_t)(i0 + qi) * a.q_s[2] + 8 * g;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) qreg[s] = col_ok ? load8<T>(qp + 32 * s) : zero8<T>();
+  }
+  float m = -INFINITY, l = 0.f;
+  f32x4 o[8];
+#pragma unroll
+  for (int mt = 0; mt < 8; ++mt) o[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const T* kb = reinterpret_cast<const T*>(a.kstore) + base;
+  const T* vb = reinterpret_cast<const T*>(a.vstore) + base;
+  for (int c0 = 0; c0 < cnt; c0 += 64) {
+    const int nt = min(cnt - c0, 64);
+    // LIST: lane x holds the tile of the wave's entry c0 + x, -1 for one that
+    // is not a visible tile of the row (such an entry attends nothing).
+    int mine = 0;
+    if constexpr (LIST) {
+      const int e = e0 + wave + (c0 + min(lane, nt - 1)) * kRowsWaves;
+      const int blk = a.idx[job_q * a.keep + e / a.tpb];
+      const int64_t t = (int64_t)blk * a.tpb + e % a.tpb;
+      mine = blk >= 0 && t < vis ? (int)t : -1;
+    }
+    auto tile_of = [&](int i) {
+      if constexpr (LIST) return __builtin_amdgcn_readlane(mine, i);
+      return e0 + wave + (c0 + i) * kRowsWaves;
+    };
+    vec8 kr[8], vr[8];
+    int tile = tile_of(0);
+    load_operands<T>(kr, kb + (int64_t)max(tile, 0) * HC_TILE_ELEMS);
+    load_operands<T>(vr, vb + (int64_t)max(tile, 0) * HC_TILE_ELEMS);
+    for (int i = 0; i < nt; ++i) {
+      // The next tile's loads are unconditional (the last reads itself
+      // again), so that each wait leaves the younger half tile in flight.
+      const int next = tile_of(min(i + 1, nt - 1));
+      const int64_t at = (int64_t)max(next, 0) * HC_TILE_ELEMS;
+      const bool live = !LIST || tile >= 0;
+      const int tok0 = max(tile, 0) * HC_TILE;
+      f32x4 s[2];
+      tile_scores<T>(kr, qreg, s);
+      __builtin_amdgcn_sched_barrier(0);
+      load_operands<T>(kr, kb + at);
+      __builtin_amdgcn_sched_barrier(0);
+      const int lo = live ? lim_lo : 0, hi = live ? lim_hi : 0, mylim = live ? lim : 0;
+      if (tok0 + HC_TILE > lo) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (tok0 + 16 * (e >> 2) + 4 * g + (e & 3) >= mylim) s[e >> 2][e & 3] = -INFINITY;
+      }
+      const vec8 pb = tile_probs<T>(s, a.scale_log2, m, l, o);
+      tile_values<T, MIXED>(vr, pb, tok0, mylim, lo, hi, g, o);
+      __builtin_amdgcn_sched_barrier(0);
+      load_operands<T>(vr, vb + at);
+      __builtin_amdgcn_sched_barrier(0);
+      tile = next;
+    }
+  }
+  l = rows4_sum(l);
+  if (LIST && void_list) m = 0.f, l = NAN;
+
+  if (col_ok) {
+    if (g == 0) s_m[wave][n] = m, s_l[wave][n] = l;
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) *reinterpret_cast<f32x4*>(&s_o[wave][n][16 * mt + 4 * g]) = o[mt];
+  }
+  __syncthreads();
+  // 32 threads a column, 4 channels each.
+  for (int c = threadIdx.x >> 5; c < ncols; c += kRowsWaves * 2) {
+    const int d0 = 4 * (threadIdx.x & 31);
+    float M = s_m[0][c];
+#pragma unroll
+    for (int w = 1; w < kRowsWaves; ++w) M = fmaxf(M, s_m[w][c]);
+    float L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kRowsWaves; ++w) {
+      const float f = state_weight(s_m[w][c], M);
+      L = fmaf(s_l[w][c], f, L);
+      acc += *reinterpret_cast<const f32x4*>(&s_o[w][c][d0]) * f;
+    }
+    const int i = i0 + c / a.G, hd = c % a.G;
+    if (a.part_o) {
+      const int64_t at = (((int64_t)row * a.Q + i) * a.G + hd) * a.nsplit + split;
+      *reinterpret_cast<f32x4*>(a.part_o + at * kPartO + d0) = acc;
+      if (d0 == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
+    } else {
+      const float inv = M == -INFINITY ? 0.f : 1.f / L;
+      T* op = reinterpret_cast<T*>(a.out) + b * a.o_s[0] + (int64_t)(kv * a.G + hd) * a.o_s[1] +
+              (int64_t)i * a.o_s[2] + d0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) op[e] = Elem<T>::from_f32(M == -INFINITY ? 0.f : acc[e] * inv);
+    }
+  }
+}
+
 struct MergeArgs {
   // Partials of a shared prefix: [part][column][128], column = (b * Q + i) * G
   // + g; info[2 kv] = first part, info[2 kv + 1] = parts of KV head kv.
@@ -184,7 +344,7 @@ struct RowsPlan {
   int qpb, ncb, nsplit;
 };
 RowsPlan rows_plan(int rows, int G, int Q, int64_t max_tiles);
-int launch_rows_attn(int dtype, const RowsArgs& a, hipStream_t s);
+int launch_block_rows(int dtype, const RowsArgs& a, hipStream_t s);
 int launch_merge(int dtype, const MergeArgs& a, int64_t columns, hipStream_t s);
 int device_cus();
 

@@ -7,12 +7,14 @@
 // Both parts lie in ragged tiled stores; the prefix has one row per KV head,
 // of its own length (a document compressed per head, or whole).  Softmax over
 // the union is folded from partial states (m, l, O), so the prefix is read
-// once for all sequences:
-//  * prefix_attn_kernel: the batch * Q * G query rows of a KV head are the
-//    columns of the products S^T = K Q^T and O^T += V^T P^T over a part of
-//    the prefix; a workgroup's 4 waves x NC x 16 columns share every tile
-//    through LDS.
-//  * rows_attn_kernel (hc_rows.hip): each sequence's own rows.
+// once for all sequences.  Two launches:
+//  * shared_attn_kernel, two kinds of workgroups side by side.  Prefix
+//    workgroups: the batch * Q * G query rows of a KV head are the columns of
+//    the products S^T = K Q^T and O^T += V^T P^T over a part of the prefix,
+//    whose tiles 4 waves x NC x 16 columns share through LDS.  Row
+//    workgroups: each sequence's own rows (rows_job).  With many columns the
+//    former are bound by the matrix cores and the latter by HBM, so they run
+//    on the same CUs at once.
 //  * merge_kernel (hc_rows.hip): one fold of a column's partials.
 #include <algorithm>
 #include <cmath>
@@ -24,8 +26,7 @@ namespace {
 
 constexpr int kPreWaves = 4;
 constexpr int kPreThreads = kPreWaves * 64;
-constexpr int kPreTiles = 2;  // tiles an iteration
-constexpr int kPreKeys = kPreTiles * HC_TILE;
+constexpr int kPreRing = 3;  // tiles of K and V held in LDS: one attended, two in flight
 
 struct PrefixArgs {
   const void* q;
@@ -36,48 +37,55 @@ struct PrefixArgs {
   int Hkv, G, Q;
   int64_t M;   // columns: batch * Q * G
   int ncg;     // column groups of 64 * NC
-  int parts;   // workgroups of a column group
+  int parts;   // workgroups of a column group, a multiple of 8 (0: no prefix)
   float scale_log2;
   float *part_o, *part_ml;
   int32_t* info;
 };
 
-// Iterations a part takes so that every row is covered by at most `parts`
-// parts in all: each row's last part may be short, so the shares are cut from
-// the parts left when every row has one.
-__device__ __forceinline__ int part_iterations(int64_t total, int rows, int parts) {
+// Tiles a part takes so that every row is covered by at most `parts` parts in
+// all: each row's last part may be short, so the shares are cut from the
+// parts left when every row has one.
+__device__ __forceinline__ int part_tiles(int64_t total, int rows, int parts) {
   const int64_t n = max(parts - rows, 1);
   return (int)max((total + n - 1) / n, (int64_t)1);
 }
 
-// Lane state of one 16-column block over LDS-staged tiles; see attend_rows.
+__device__ __forceinline__ int tiles_of(int len) { return (max(len, 0) + HC_TILE - 1) / HC_TILE; }
+
+// A barrier that waits for this wave's LDS reads and not for its loads in
+// flight, as __syncthreads does.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 template <typename T, int NC>
-__global__ __launch_bounds__(kPreThreads, sizeof(T) == 4 ? 1 : 3) void prefix_attn_kernel(const PrefixArgs a) {
+__device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
   typedef typename Elem<T>::vec8 vec8;
-  extern __shared__ __attribute__((aligned(16))) unsigned char pre_lds[];
-  T* lds = reinterpret_cast<T*>(pre_lds);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g4 = lane >> 4, n16 = lane & 15;
 
   // Column groups of one part go to one XCD (workgroups are dealt to the 8
   // XCDs in turn), so its L2 serves the tiles after their first read.
-  const int x = blockIdx.x;
   const int part = (x / (8 * a.ncg)) * 8 + x % 8, cg = (x / 8) % a.ncg;
 
   // (row, share) of the part, from the device lengths: rows 64 at a time.
   int64_t total = 0;
   for (int r0 = 0; r0 < a.Hkv; r0 += 64) {
-    int it = r0 + lane < a.Hkv ? (max(a.len[r0 + lane], 0) + kPreKeys - 1) / kPreKeys : 0;
+    int nt = r0 + lane < a.Hkv ? tiles_of(a.len[r0 + lane]) : 0;
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) it += __shfl_xor(it, d, 64);
-    total += it;
+    for (int d = 32; d >= 1; d >>= 1) nt += __shfl_xor(nt, d, 64);
+    total += nt;
   }
-  const int share = part_iterations(total, a.Hkv, a.parts);
-  int kv = -1, it0 = 0, nit = 0, first = 0;
+  const int share = part_tiles(total, a.Hkv, a.parts);
+  int kv = -1, t0 = 0, t1 = 0, first = 0;
   for (int r0 = 0; r0 < a.Hkv; r0 += 64) {
     const int r = r0 + lane;
-    const int it = r < a.Hkv ? (max(a.len[r], 0) + kPreKeys - 1) / kPreKeys : 0;
-    const int np = (it + share - 1) / share;
+    const int nt = r < a.Hkv ? tiles_of(a.len[r]) : 0;
+    const int np = (nt + share - 1) / share;
     int incl = np;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -93,16 +101,45 @@ __global__ __launch_bounds__(kPreThreads, sizeof(T) == 4 ? 1 : 3) void prefix_at
     if (hit && kv < 0) {
       const int src = __builtin_ctzll(hit);
       kv = r0 + src;
-      it0 = (part - __shfl(incl - np, src, 64)) * share;
-      nit = min(it0 + share, __shfl(it, src, 64));
+      t0 = (part - __shfl(incl - np, src, 64)) * share;
+      t1 = min(t0 + share, __shfl(nt, src, 64));
     }
     first = __shfl(incl, 63, 64);
   }
   kv = __builtin_amdgcn_readfirstlane(kv);
   if (kv < 0) return;
-  it0 = __builtin_amdgcn_readfirstlane(it0);
-  nit = __builtin_amdgcn_readfirstlane(nit);
-  const int len = a.len[kv], last_tile = (len - 1) / HC_TILE;
+  t0 = __builtin_amdgcn_readfirstlane(t0);
+  t1 = __builtin_amdgcn_readfirstlane(t1);
+  const int len = a.len[kv];
+
+  // Staging: the tiles lie contiguous in memory and keep their layout in LDS,
+  // so a tile is 16-byte units copied straight into LDS (global_load_lds).
+  constexpr int kTileBytes = HC_TILE_ELEMS * (int)sizeof(T);
+  constexpr int kLoads = kTileBytes / (16 * kPreThreads);  // per thread, of K and of V
+  const int64_t at = (a.tile_off[kv] + t0) * (int64_t)kTileBytes + 16 * tid;
+  const char* kb = reinterpret_cast<const char*>(a.kstore) + at;
+  const char* vb = reinterpret_cast<const char*>(a.vstore) + at;
+  // One column group reads a tile once: streamed past L2 (83 against 95 us for
+  // 16 columns over 131072 tokens of 8 heads; with more column groups the
+  // others' reads come from L2, and 4 of them lose 7 % by the hint).
+  const bool once = a.ncg == 1;
+  auto stage = [&](int slot) {  // the next tile not staged yet
+    char* dst = reinterpret_cast<char*>(lds + slot * 2 * HC_TILE_ELEMS) + 1024 * wave;
+    if (once) {
+#pragma unroll
+      for (int r = 0; r < kLoads; ++r) lds_dma16_stream(kb + 16 * r * kPreThreads, dst + 16 * r * kPreThreads);
+#pragma unroll
+      for (int r = 0; r < kLoads; ++r)
+        lds_dma16_stream(vb + 16 * r * kPreThreads, dst + kTileBytes + 16 * r * kPreThreads);
+    } else {
+#pragma unroll
+      for (int r = 0; r < kLoads; ++r) lds_dma16(kb + 16 * r * kPreThreads, dst + 16 * r * kPreThreads);
+#pragma unroll
+      for (int r = 0; r < kLoads; ++r) lds_dma16(vb + 16 * r * kPreThreads, dst + kTileBytes + 16 * r * kPreThreads);
+    }
+    kb += kTileBytes;
+    vb += kTileBytes;
+  };
 
   // Q^T operands: column col0 + 16j + n16, k-slots = channels 32s + 8*g4 + [0, 8).
   const int64_t col0 = ((int64_t)cg * kPreWaves + wave) * 16 * NC;
@@ -126,127 +163,104 @@ __global__ __launch_bounds__(kPreThreads, sizeof(T) == 4 ? 1 : 3) void prefix_at
 #pragma unroll
     for (int db = 0; db < 8; ++db) o[db][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  // The queries land before the first tile is staged: the loop counts its
+  // loads in flight.
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
+  stage(0);
+  if (t0 + 1 < t1) stage(1);
 
-  // Staging: the tiles lie contiguous in memory and keep their layout in LDS,
-  // so an iteration is 16-byte units copied straight into LDS
-  // (global_load_lds): unit r * 256 + tid.  A tile past the row's last one
-  // reads the last one again; its tokens are masked.
-  constexpr int kUnits = (int)sizeof(T) / 2;       // 16-byte units per 8 elements
-  constexpr int kPerTile = 2 * kUnits;             // units of a tile per thread
-  constexpr int kTileBytes = HC_TILE_ELEMS * (int)sizeof(T);
-  const int64_t row_at = a.tile_off[kv] * (int64_t)kTileBytes + 16 * tid;
-  const char* kb = reinterpret_cast<const char*>(a.kstore) + row_at;
-  const char* vb = reinterpret_cast<const char*>(a.vstore) + row_at;
-  T* const vbuf = lds + 2 * kPreTiles * HC_TILE_ELEMS;
-  auto stage = [&](const char* src, T* dst, int it) {
-#pragma unroll
-    for (int c = 0; c < kPreTiles; ++c) {
-      const char* t = src + (int64_t)min(it * kPreTiles + c, last_tile) * kTileBytes;
-#pragma unroll
-      for (int r = 0; r < kPerTile; ++r)
-        lds_dma16(t + 16 * r * kPreThreads,
-                  reinterpret_cast<char*>(dst) + c * kTileBytes + 16 * (r * kPreThreads + wave * 64));
-    }
-  };
-
-  stage(kb, lds, it0);
-  stage(vb, vbuf, it0);
-  wait_lds_dma();
-  __syncthreads();
-
-  // K is double-buffered; V(it + 1) is fetched behind the P.V step of it and
-  // arrives while the next scores and probabilities are formed.
-  for (int it = it0; it < nit; ++it) {
-    const int cur = (it - it0) & 1;
-    const int t0 = it * kPreKeys;
-    const bool more = it + 1 < nit;
-    if (more) stage(kb, lds + (cur ^ 1) * kPreTiles * HC_TILE_ELEMS, it + 1);
-    vec8 pb[kPreTiles][NC];
-    if (active) {
-      const T* sk = lds + cur * kPreTiles * HC_TILE_ELEMS;
-      f32x4 sacc[4][NC];
-#pragma unroll
-      for (int tb = 0; tb < 4; ++tb)
-#pragma unroll
-        for (int j = 0; j < NC; ++j) sacc[tb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int tb = 0; tb < 4; ++tb) {
-        const T* kt = sk + (tb >> 1) * HC_TILE_ELEMS + (tb & 1) * 4 * 64 * 8;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const vec8 ka = load8<T>(kt + (s * 64 + lane) * 8);
-#pragma unroll
-          for (int j = 0; j < NC; ++j) sacc[tb][j] = mma_16x16x32(ka, qop[j][s], sacc[tb][j]);
-        }
-      }
-      if (t0 + kPreKeys > len) {
-#pragma unroll
-        for (int tb = 0; tb < 4; ++tb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (t0 + 16 * tb + 4 * g4 + r >= len) {
-#pragma unroll
-              for (int j = 0; j < NC; ++j) sacc[tb][j][r] = -INFINITY;
-            }
-      }
-#pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        float ps;
-        auto probs = [&](float nm) {
-          ps = 0.f;
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float pv[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              pv[e] = fast_exp2(fmaf(sacc[2 * c + (e >> 2)][j][e & 3], a.scale_log2, nm));
-              ps += pv[e];
-            }
-            pb[c][j] = pack8<T>(pv);  // at most half a step of the input type per probability
-          }
-        };
-        probs(-m[j]);
-        if (__any(!(ps <= kRowsLazy))) {  // also NaN, as in the first iteration
-          float mx = -INFINITY;
-#pragma unroll
-          for (int tb = 0; tb < 4; ++tb)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sacc[tb][j][r]);
-          const float mnew = fmaxf(m[j], rows4_max(mx) * a.scale_log2);
-          const float alpha = m[j] == -INFINITY ? 0.f : fast_exp2(m[j] - mnew);
-          m[j] = mnew;
-          l[j] *= alpha;
-#pragma unroll
-          for (int db = 0; db < 8; ++db) o[db][j] *= alpha;
-          probs(mnew == -INFINITY ? 0.f : -mnew);
-        }
-        l[j] += ps;
-      }
-    }
-    // V(it) was fetched before K(it + 1).
-    if (more)
-      wait_lds_dma_but<kPreTiles * kPerTile>();
+  int slot = 0;
+  for (int t = t0; t < t1; ++t) {
+    // This wave's loads of tile t have landed, and past the barrier every
+    // wave's have, while tile t + 1 stays in flight; every wave is also done
+    // with tile t - 1, whose slot takes tile t + 2.
+    if (t + 1 < t1)
+      wait_lds_dma_but<2 * kLoads>();
     else
       wait_lds_dma();
-    __syncthreads();
-    if (active) {
-      const bool tail = t0 + kPreKeys > len;
-#pragma unroll
-      for (int c = 0; c < kPreTiles; ++c) {
-        const T* vt = vbuf + c * HC_TILE_ELEMS;
-#pragma unroll
-        for (int db = 0; db < 8; ++db) {
-          vec8 va = load8<T>(vt + (db * 64 + lane) * 8);
-          // Stale slots may hold NaN, which zero probabilities do not silence.
-          if (tail) zero_tail<T>(va, t0 + c * HC_TILE, len, g4);
-#pragma unroll
-          for (int j = 0; j < NC; ++j) o[db][j] = mma_16x16x32(va, pb[c][j], o[db][j]);
-        }
+    lds_barrier();
+    const T* sk = lds + slot * 2 * HC_TILE_ELEMS;
+    const T* sv = sk + HC_TILE_ELEMS;
+    if (t + 2 < t1) stage(slot == 0 ? 2 : slot - 1);
+    slot = slot == kPreRing - 1 ? 0 : slot + 1;
+    const int left = len - t * HC_TILE;  // tokens from this tile on
+    if (left < HC_TILE) {
+      // The row's last tile: its stale slots may hold NaN, which a zero
+      // probability does not silence.  (No load is in flight any more.)
+      T* z = const_cast<T*>(sv);
+      for (int c = tid; c < HC_TILE_ELEMS / 8; c += kPreThreads) {
+        vec8 v = load8<T>(z + 8 * c);
+        zero_tail<T>(v, 0, left, (c >> 4) & 3);
+        *reinterpret_cast<vec8*>(z + 8 * c) = v;
       }
+      lds_barrier();
     }
-    wait_lds_dma();   // K(it + 1) has landed
-    __syncthreads();  // ... and V(it) is no longer read
-    if (more) stage(vb, vbuf, it + 1);
+    if (!active) continue;
+    // All of a tile's K operands are requested before the first product, and
+    // V's before the softmax that they wait behind (left to itself the
+    // compiler requests two and waits for both, sixteen times a tile).
+    vec8 kv8[8];
+#pragma unroll
+    for (int x8 = 0; x8 < 8; ++x8) kv8[x8] = load8<T>(sk + (x8 * 64 + lane) * 8);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 s[2][NC];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) s[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x4 = 0; x4 < 4; ++x4)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < NC; ++j) s[h][j] = mma_16x16x32(kv8[h * 4 + x4], qop[j][x4], s[h][j]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x8 = 0; x8 < 8; ++x8) kv8[x8] = load8<T>(sv + (x8 * 64 + lane) * 8);
+    __builtin_amdgcn_sched_barrier(0);
+    if (left < HC_TILE) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (16 * (e >> 2) + 4 * g4 + (e & 3) >= left) {
+#pragma unroll
+          for (int j = 0; j < NC; ++j) s[e >> 2][j][e & 3] = -INFINITY;
+        }
+    }
+    vec8 pb[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      float ps;
+      auto probs = [&](float nm) {
+        float pv[8];
+        ps = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          pv[e] = fast_exp2(fmaf(s[e >> 2][j][e & 3], a.scale_log2, nm));
+          ps += pv[e];
+        }
+        pb[j] = pack8<T>(pv);  // at most half a step of the input type per probability
+      };
+      probs(-m[j]);
+      if (__any(!(ps <= kRowsLazy))) {  // also NaN, as in the first tile
+        float mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][j][e & 3]);
+        const float mnew = fmaxf(m[j], rows4_max(mx) * a.scale_log2);
+        const float alpha = m[j] == -INFINITY ? 0.f : fast_exp2(m[j] - mnew);
+        m[j] = mnew;
+        l[j] *= alpha;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) o[db][j] *= alpha;
+        probs(mnew == -INFINITY ? 0.f : -mnew);
+      }
+      l[j] += ps;
+    }
+#pragma unroll
+    for (int db = 0; db < 8; ++db) {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) o[db][j] = mma_16x16x32(kv8[db], pb[j], o[db][j]);
+    }
   }
 
   if (!active) return;
@@ -255,12 +269,31 @@ __global__ __launch_bounds__(kPreThreads, sizeof(T) == 4 ? 1 : 3) void prefix_at
     const float lt = rows4_sum(l[j]);
     const int64_t c = col0 + 16 * j + n16;
     if (c >= a.M) continue;
-    const int64_t at = part * a.M + c;
+    const int64_t pa = part * a.M + c;
 #pragma unroll
     for (int db = 0; db < 8; ++db)
-      *reinterpret_cast<f32x4*>(a.part_o + at * kPartO + 16 * db + 4 * g4) = o[db][j];
-    if (g4 == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m[j], lt);
+      *reinterpret_cast<f32x4*>(a.part_o + pa * kPartO + 16 * db + 4 * g4) = o[db][j];
+    if (g4 == 0) *reinterpret_cast<float2*>(a.part_ml + pa * 2) = make_float2(m[j], lt);
   }
+}
+
+// LDS of a workgroup: the prefix ring, or the row waves' states.
+template <typename T>
+constexpr size_t shared_lds() {
+  const size_t ring = (size_t)kPreRing * 2 * HC_TILE_ELEMS * sizeof(T), rows = kRowsLds * sizeof(float);
+  return ring > rows ? ring : rows;
+}
+
+// Prefix workgroups come first: they are the long ones.
+template <typename T, int NC, bool MIXED>
+__global__ __launch_bounds__(kPreThreads, sizeof(T) == 4 ? 1 : 3) void shared_attn_kernel(const PrefixArgs pre,
+                                                                                         const RowsArgs rows) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char shared_raw[];
+  const int npre = pre.parts * pre.ncg;
+  if ((int)blockIdx.x < npre)
+    prefix_job<T, NC>(pre, blockIdx.x, reinterpret_cast<T*>(shared_raw));
+  else
+    rows_job<T, false, MIXED>(rows, blockIdx.x - npre, reinterpret_cast<float*>(shared_raw));
 }
 
 // Sizes of one call: the prefix launch's column blocks and parts, the rows'
@@ -279,13 +312,34 @@ SharedPlan shared_plan(int dtype, int batch, int Hkv, int G, int Q, int64_t pref
   p.nc = dtype != HC_DTYPE_F32 && M > 64 ? 2 : 1;
   const int64_t per = 64 * p.nc;
   p.ncg = (int)((M + per - 1) / per);
-  // Three workgroups a CU (one in fp32), every KV head at least two parts,
-  // and no more parts than iterations.
-  const int64_t slots = (int64_t)device_cus() * (dtype == HC_DTYPE_F32 ? 1 : 3);
-  int64_t parts = std::max<int64_t>(slots / p.ncg, 2 * (int64_t)Hkv);
-  parts = std::min(parts, prefix_tiles + Hkv + 1);
-  p.parts = (int)std::min<int64_t>((parts + 7) / 8 * 8, 1 << 20);  // whole rounds over the 8 XCDs
   p.rows = rows_plan(batch * Hkv, G, Q, row_tiles);
+  // Prefix workgroups a CU: the least estimate of the two launches' time in
+  // us.  A part's tile of 32 tokens takes 0.6 + 0.37 k with k workgroups of
+  // two column blocks a wave on a CU (128, 512 and 768 workgroups over 128K
+  // tokens: 330, 217 and 195 us against 327, 226 and 192), or the stream's
+  // time; a column's partial costs its writing and reading; the rows' stream
+  // hides behind the products while a third workgroup finds room (1024 rows
+  // beside 512 columns over 128K: 260, 253 and 278 us at k = 2, 2.5 and 3).
+  const int cus = device_cus();
+  const bool f32 = dtype == HC_DTYPE_F32;
+  const double stream = 2e6 * HC_TILE_ELEMS * (f32 ? 4. : 2.) / 5.8e12;
+  const double rows_us = 0.75 * (double)batch * Hkv * row_tiles * stream;
+  const double ks[] = {0.125, 0.25, 0.5, 1., 1.5, 2., 2.5, 3.};
+  int64_t parts = 0;
+  double best = 0.;
+  for (const double k : ks) {
+    if (f32 && k > 1.) break;  // LDS holds one workgroup
+    // Every KV head has two parts at least, and there are no more than tiles.
+    int64_t n = std::max<int64_t>((int64_t)(k * cus) / p.ncg, 2 * (int64_t)Hkv);
+    n = std::min(n, prefix_tiles + Hkv + 1);
+    const double kk = std::max((double)n * p.ncg / cus, 1.);
+    const double tile = f32 ? 3. : p.nc == 1 ? 0.5 + 0.2 * kk : 0.6 + 0.37 * kk;
+    const double share = std::ceil((double)prefix_tiles / (double)std::max<int64_t>(n - Hkv / 2, 1));
+    const double t = std::max(share * tile, prefix_tiles * stream) + (double)n * M * 520. * 0.45e-6 +
+                     rows_us * (f32 || kk > 2.75 ? 0.9 : kk > 2.25 ? 0.5 : 0.35);
+    if (parts == 0 || t < best) best = t, parts = n;
+  }
+  p.parts = (int)std::min<int64_t>((parts + 7) / 8 * 8, 1 << 20);  // whole rounds over the 8 XCDs
   const size_t pre = (size_t)p.parts * M, row = (size_t)batch * Hkv * Q * G * p.rows.nsplit;
   p.info_at = 0;
   p.pre_o = up256((size_t)Hkv * 2 * sizeof(int32_t));
@@ -297,18 +351,19 @@ SharedPlan shared_plan(int dtype, int batch, int Hkv, int G, int Q, int64_t pref
 }
 
 template <typename T>
-int launch_prefix(const PrefixArgs& a, int nc, hipStream_t s) {
-  const size_t lds = (size_t)3 * kPreTiles * HC_TILE_ELEMS * sizeof(T);
-  auto fn = prefix_attn_kernel<T, 1>;
+int launch_shared(const PrefixArgs& a, const RowsArgs& r, int nc, hipStream_t s) {
+  const size_t lds = shared_lds<T>();
+  const bool mixed = r.qpb > 1;
+  auto fn = mixed ? shared_attn_kernel<T, 1, true> : shared_attn_kernel<T, 1, false>;
   if constexpr (sizeof(T) == 2)
-    if (nc == 2) fn = prefix_attn_kernel<T, 2>;
+    if (nc == 2) fn = mixed ? shared_attn_kernel<T, 2, true> : shared_attn_kernel<T, 2, false>;
   if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)lds) != hipSuccess)
     return set_error(HC_ERR_HIP, "hc_shared_attn: %s", hipGetErrorString(hipGetLastError()));
-  const int64_t grid = (int64_t)a.parts * a.ncg;
+  const int64_t grid = (int64_t)a.parts * a.ncg + (int64_t)r.rows * r.ncb * r.nsplit;
   if (grid > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_shared_attn: %lld workgroups", (long long)grid);
-  hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(kPreThreads), lds, s, a);
-  return check_launch("hc_shared_attn(prefix)");
+  hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(kPreThreads), lds, s, a, r);
+  return check_launch("hc_shared_attn");
 }
 
 bool bad_sizes(int dtype, int batch, int q_heads, int kv_heads, int queries) {
@@ -369,28 +424,21 @@ extern "C" int hc_shared_attn(int dtype, const void* q, const int64_t* q_strides
   mg.nsplit = row_len ? p.rows.nsplit : 0;
   mg.Hkv = kv_heads, mg.G = G, mg.Q = queries, mg.out = out;
   for (int i = 0; i < 3; ++i) mg.o_s[i] = out_strides[i];
-  if (prefix_len) {
-    PrefixArgs a;
-    a.q = q, a.kstore = kprefix, a.vstore = vprefix, a.tile_off = prefix_tile_off, a.len = prefix_len;
-    for (int i = 0; i < 3; ++i) a.q_s[i] = q_strides[i];
-    a.Hkv = kv_heads, a.G = G, a.Q = queries, a.M = mg.M, a.ncg = p.ncg, a.parts = p.parts;
-    a.scale_log2 = scale_log2;
-    a.part_o = reinterpret_cast<float*>(ws + p.pre_o), a.part_ml = reinterpret_cast<float*>(ws + p.pre_ml);
-    a.info = reinterpret_cast<int32_t*>(ws + p.info_at);
-    const int rc = dtype == HC_DTYPE_BF16  ? launch_prefix<__bf16>(a, p.nc, s)
-                   : dtype == HC_DTYPE_F16 ? launch_prefix<_Float16>(a, p.nc, s)
-                                           : launch_prefix<float>(a, p.nc, s);
-    if (rc) return rc;
-  }
-  if (row_len) {
-    RowsArgs r = {};
-    r.q = q, r.kstore = kstore, r.vstore = vstore, r.row_tile_off = row_tile_off, r.row_len = row_len;
-    for (int i = 0; i < 3; ++i) r.q_s[i] = q_strides[i];
-    r.Hkv = kv_heads, r.G = G, r.Q = queries, r.rows = batch * kv_heads;
-    r.qpb = p.rows.qpb, r.ncb = p.rows.ncb, r.nsplit = p.rows.nsplit, r.scale_log2 = scale_log2;
-    r.part_o = reinterpret_cast<float*>(ws + p.row_o), r.part_ml = reinterpret_cast<float*>(ws + p.row_ml);
-    const int rc = launch_rows_attn(dtype, r, s);
-    if (rc) return rc;
-  }
+  PrefixArgs a = {};
+  a.q = q, a.kstore = kprefix, a.vstore = vprefix, a.tile_off = prefix_tile_off, a.len = prefix_len;
+  a.Hkv = kv_heads, a.G = G, a.Q = queries, a.M = mg.M, a.ncg = p.ncg, a.parts = prefix_len ? p.parts : 0;
+  a.scale_log2 = scale_log2;
+  a.part_o = reinterpret_cast<float*>(ws + p.pre_o), a.part_ml = reinterpret_cast<float*>(ws + p.pre_ml);
+  a.info = reinterpret_cast<int32_t*>(ws + p.info_at);
+  RowsArgs r = {};
+  r.q = q, r.kstore = kstore, r.vstore = vstore, r.row_tile_off = row_tile_off, r.row_len = row_len;
+  r.Hkv = kv_heads, r.G = G, r.Q = queries, r.rows = row_len ? batch * kv_heads : 0;
+  r.qpb = p.rows.qpb, r.ncb = p.rows.ncb, r.nsplit = p.rows.nsplit, r.scale_log2 = scale_log2;
+  r.part_o = reinterpret_cast<float*>(ws + p.row_o), r.part_ml = reinterpret_cast<float*>(ws + p.row_ml);
+  for (int i = 0; i < 3; ++i) a.q_s[i] = r.q_s[i] = q_strides[i];
+  const int rc = dtype == HC_DTYPE_BF16  ? launch_shared<__bf16>(a, r, p.nc, s)
+                 : dtype == HC_DTYPE_F16 ? launch_shared<_Float16>(a, r, p.nc, s)
+                                         : launch_shared<float>(a, r, p.nc, s);
+  if (rc) return rc;
   return launch_merge(dtype, mg, (int64_t)batch * queries * q_heads, s);
 }
