@@ -9,15 +9,16 @@
 //   store[b, h][len + t] = (k'[b, h, t], v[b, h, t]),  t < counts[b].
 //
 // Bound by HBM: each element is read once and written once, and the tables
-// are read once per KV head (from L2: the tokens of a workgroup share them).
+// are read once per KV head (from L2: the workgroups of a token share them).
 // A workgroup takes the new tokens of one row that fall into one 32-token
-// tile, with the queries of the row's head group at the same tokens: a
-// thread keeps the table values of its (token, 8 + 8 channels) in registers
-// over the group's heads and the key, and each 8-token x 8-channel-chunk
+// tile, with the queries of the row's head group at the same tokens: a thread
+// keeps the table values of its (token, 8 + 8 channels) over the group's heads
+// and the key, four heads' loads in flight, and each 8-token x 8-channel-chunk
 // store of a wave fills whole 128-byte lines of the K tile.  V's tile layout
-// keeps 8 tokens of a channel together, so a whole tile goes through LDS;
-// the tokens of a partly covered tile are stored one element at a time (the
-// other tokens of its 16-byte chunks may be older ones, or not yet written).
+// keeps 8 tokens of a channel together, so a whole tile goes through LDS; the
+// tokens of a partly covered tile are stored one element at a time (the other
+// tokens of its 16-byte chunks may be older ones, or not yet written).
+// 32768 tokens of 32 + 2 x 8 heads in bf16: 151 us, 5.4 TB/s read and written.
 #include "hc_common.h"
 #include "hc_internal.h"
 
@@ -37,7 +38,6 @@ struct RotArgs {
   int advance;                 // len_out is written by this launch
 };
 
-constexpr int kRotThreads = 256;
 
 // Eight table values as fp32.
 template <typename C>
@@ -52,23 +52,10 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   *reinterpret_cast<typename Elem<T>::vec8*>(p) = pack8<T>(x);
 }
 
-// Channels c0 + [0, 8) and 64 + c0 + [0, 8) of one token of one head, turned.
-template <typename T>
-__device__ __forceinline__ void turn(const T* src, const float (&c)[2][8], const float (&s)[2][8], float (&lo)[8],
-                                     float (&hi)[8]) {
-  const typename Elem<T>::vec8 a = load8_stream<T>(src), b = load8_stream<T>(src + 64);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float x = vec8_at<T>(a, e), y = vec8_at<T>(b, e);
-    lo[e] = x * c[0][e] - y * s[0][e];
-    hi[e] = y * c[1][e] + x * s[1][e];
-  }
-}
-
-template <typename T, typename C>
-__global__ __launch_bounds__(kRotThreads) void append_rotated_kernel(const RotArgs a) {
+template <typename T, typename C, int NT>
+__global__ __launch_bounds__(NT, sizeof(T) == 4 ? 2 : 4) void append_rotated_kernel(const RotArgs a) {
   typedef typename Elem<T>::vec8 vec8;
-  __shared__ T sv[HC_TILE][HC_HEAD_DIM + 8];
+  __shared__ T sv[NT == 256 ? HC_TILE : 1][HC_HEAD_DIM + 8];
   const int row = blockIdx.x % a.rows;
   const int b = row / a.Hkv, h = row % a.Hkv;
   const int tid = threadIdx.x;
@@ -98,54 +85,79 @@ __global__ __launch_bounds__(kRotThreads) void append_rotated_kernel(const RotAr
     const int slot0 = (first + ta) & (HC_TILE - 1);
     T* kt = reinterpret_cast<T*>(a.kstore) + (tile0 + j) * (int64_t)HC_TILE_ELEMS;
     T* vt = reinterpret_cast<T*>(a.vstore) + (tile0 + j) * (int64_t)HC_TILE_ELEMS;
-    const bool whole = nst == HC_TILE;
+    const bool whole = NT == 256 && nst == HC_TILE;
 
-    // V: chunk x = (token, 8 channels), two per thread.
+    // V: chunk x = (token, 8 channels), two per thread (one token: one, of 16
+    // threads).
     vec8 vr[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int x = tid + u * kRotThreads, t = x >> 4;
+      const int x = tid + u * NT, t = x >> 4;
       if (t < nst) vr[u] = load8_stream<T>(vp + (int64_t)(ta + t) * a.v_s[2] + 8 * (x & 15));
     }
 
-    // Q and K: eight threads a (token, head) pair; head G is the key.
-    const int c8 = tid & 7, c0 = 8 * c8;
-    float cc[2][8], ss[2][8], lo[8], hi[8];
-    int have = -1;  // token whose table values are held
-    const int pairs = n * (a.G + 1);
-    for (int p = tid >> 3; p < pairs; p += kRotThreads / 8) {
-      const int t = p % n, hd = p / n;
-      if (t != have) {
-        const int64_t at = (int64_t)(ta + t) * a.t_st + c0;
-        load_table<C>(cp + at, cc[0]);
-        load_table<C>(cp + at + 64, cc[1]);
-        load_table<C>(sp + at, ss[0]);
-        load_table<C>(sp + at + 64, ss[1]);
-        have = t;
-      }
-      if (hd < a.G) {
-        turn<T>(qp + hd * a.q_s[1] + (int64_t)(ta + t) * a.q_s[2] + c0, cc, ss, lo, hi);
-        T* o = qo + hd * a.qo_s[1] + (int64_t)(ta + t) * a.qo_s[2] + c0;
-        store8<T>(o, lo);
-        store8<T>(o + 64, hi);
-      } else if (t < nst) {
-        turn<T>(kp + (int64_t)(ta + t) * a.k_s[2] + c0, cc, ss, lo, hi);
-        store8<T>(kt + k_tile_offset(slot0 + t, c0), lo);
-        store8<T>(kt + k_tile_offset(slot0 + t, c0 + 64), hi);
+    // Q and K: eight threads a token and head; head G is the key.  A thread
+    // stays with one token, so its 8 + 8 channels' table values are read once,
+    // and takes every hp-th head (hp: how often the tile's tokens fit the
+    // groups of 8 threads), kBatch of them in flight.
+    constexpr int kBatch = 4;
+    const int grp = tid >> 3, c0 = 8 * (tid & 7);
+    const int hp = n > 0 ? NT / 8 / n : 0, h0 = n > 0 ? grp / n : 0;
+    if (h0 < hp) {
+      const int t = grp % n;
+      const int64_t tok = ta + t;
+      const T* const qs = qp + tok * a.q_s[2] + c0;
+      const T* const ks = kp + tok * a.k_s[2] + c0;
+      const C* const cs = cp + tok * a.t_st + c0;
+      const C* const ss = sp + tok * a.t_st + c0;
+      float cc[2][8], sn[2][8];
+      load_table<C>(cs, cc[0]);
+      load_table<C>(cs + 64, cc[1]);
+      load_table<C>(ss, sn[0]);
+      load_table<C>(ss + 64, sn[1]);
+      for (int hb = 0; hb <= a.G; hb += kBatch * hp) {
+        vec8 lo8[kBatch], hi8[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          if (hb + u * hp > a.G) continue;
+          const int hd = hb + u * hp + h0;  // past the key: the key again, not stored
+          const T* src = hd < a.G ? qs + hd * a.q_s[1] : ks;
+          lo8[u] = load8_stream<T>(src), hi8[u] = load8_stream<T>(src + 64);
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          if (hb + u * hp > a.G) continue;
+          const int hd = hb + u * hp + h0;
+          float lo[8], hi[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float x = vec8_at<T>(lo8[u], e), y = vec8_at<T>(hi8[u], e);
+            lo[e] = x * cc[0][e] - y * sn[0][e];
+            hi[e] = y * cc[1][e] + x * sn[1][e];
+          }
+          if (hd < a.G) {
+            T* o = qo + hd * a.qo_s[1] + tok * a.qo_s[2] + c0;
+            store8<T>(o, lo);
+            store8<T>(o + 64, hi);
+          } else if (hd == a.G && t < nst) {
+            store8<T>(kt + k_tile_offset(slot0 + t, c0), lo);
+            store8<T>(kt + k_tile_offset(slot0 + t, c0 + 64), hi);
+          }
+        }
       }
     }
 
     if (whole) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int x = tid + u * kRotThreads;
+        const int x = tid + u * NT;
         *reinterpret_cast<vec8*>(&sv[x >> 4][8 * (x & 15)]) = vr[u];
       }
       __syncthreads();
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         // V chunk x = (mt*4+g)*16+nn: channel 16mt+nn, tokens 16*(i/4)+4g+i%4.
-        const int x = tid + u * kRotThreads;
+        const int x = tid + u * NT;
         const int nn = x & 15, g = (x >> 4) & 3, d = 16 * (x >> 6) + nn;
         float v8[8];
 #pragma unroll
@@ -156,7 +168,7 @@ __global__ __launch_bounds__(kRotThreads) void append_rotated_kernel(const RotAr
     } else {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int x = tid + u * kRotThreads, t = x >> 4;
+        const int x = tid + u * NT, t = x >> 4;
         if (t < nst) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -197,7 +209,13 @@ int launch_rotated(RotArgs& a, hipStream_t s) {
   a.tiles = a.walk ? 1 : (a.T + 2 * HC_TILE - 2) / HC_TILE;
   const int64_t grid = (int64_t)a.tiles * a.rows;
   if (grid > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_append_rotated: %d rows x %d tokens", a.rows, a.T);
-  hipLaunchKernelGGL((append_rotated_kernel<T, C>), dim3((unsigned)grid), dim3(kRotThreads), 0, s, a);
+  // One token of many rows: a wave a row, whose eight groups of threads take the
+  // heads, leaves room for all rows at once (2048 rows 6.4 against 10.2 us; 8
+  // rows 4.8 against 4.4).
+  if (a.T == 1 && a.rows > 512)
+    hipLaunchKernelGGL((append_rotated_kernel<T, C, 64>), dim3((unsigned)grid), dim3(64), 0, s, a);
+  else
+    hipLaunchKernelGGL((append_rotated_kernel<T, C, 256>), dim3((unsigned)grid), dim3(256), 0, s, a);
   int rc = check_launch("hc_append_rotated");
   if (rc || !a.len_out || a.advance) return rc;
   hipLaunchKernelGGL(advance_kernel, dim3((a.rows + 255) / 256), dim3(256), 0, s, a.len_out, a.row_cap, a.counts,

@@ -52,284 +52,409 @@ struct BoundArgs {
   int8_t *bounds, *exps;
   int rows, tpb, span;  // span: blocks a row, the last complete ones
   int fresh;            // > 0: only blocks that the last `fresh` tokens completed
+  int per;              // blocks a workgroup takes
 };
 
-// One workgroup a block.  K chunk c = ((h*4+s)*4+g)*16+m of a tile holds token
-// 16h+m, channels 32s+8g+[0,8): a thread reads both halves h of its (s, g, m),
-// so a wave's load is 1 KB in a row, and the 16 lanes m of a channel group are
-// folded by row rotations.  Bound by the key stream.
-template <typename T>
-__global__ __launch_bounds__(256) void block_bounds_kernel(const BoundArgs a) {
-  __shared__ float s_top[4];
-  const int row = blockIdx.x % a.rows, j0 = blockIdx.x / a.rows;
-  const int len = max(a.row_len[row], 0), S = a.tpb * HC_TILE;
-  const int j = len / S - 1 - j0;
-  if (j < 0) return;
-  if (a.fresh > 0 && (int64_t)(j + 1) * S <= (int64_t)len - a.fresh) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const T* kb = reinterpret_cast<const T*>(a.kstore) + (a.row_tile_off[row] + (int64_t)j * a.tpb) * HC_TILE_ELEMS;
-  float hi[8], lo[8];
+// The greater of two values, the other one where one is NaN: one instruction,
+// where fmaxf first canonicalises operands it cannot prove canonical.
+__device__ __forceinline__ float greater(float x, float y) { return __builtin_amdgcn_fmed3f(x, y, INFINITY); }
+
+// Greatest values over the 16 lanes of each 16-lane row of a wave, for 16
+// values a lane at once: lane l ends with its row's greatest value l % 16 (a
+// reduce-scatter: the values held halve at every step).
+__device__ __forceinline__ float row16_max_scatter(float (&v)[16], int lane) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) hi[e] = -INFINITY, lo[e] = INFINITY;
-  for (int t = 0; t < a.tpb; ++t) {
-    const T* kt = kb + (int64_t)t * HC_TILE_ELEMS + tid * 8;
-    const typename Elem<T>::vec8 x = load8_stream<T>(kt), y = load8_stream<T>(kt + 2048);
+  for (int half = 8, bit = 1; half >= 1; half >>= 1, bit <<= 1) {
+    const bool b = lane & bit;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      hi[e] = fmaxf(hi[e], fmaxf(vec8_at<T>(x, e), vec8_at<T>(y, e)));
-      lo[e] = fminf(lo[e], fminf(vec8_at<T>(x, e), vec8_at<T>(y, e)));
+    for (int j = 0; j < half; ++j) {
+      const float keep = b ? v[2 * j + 1] : v[2 * j], send = b ? v[2 * j] : v[2 * j + 1];
+      const float got = bit == 1   ? dpp_mov<0xB1>(send)    // quad_perm [1,0,3,2]
+                        : bit == 2 ? dpp_mov<0x4E>(send)    // quad_perm [2,3,0,1]
+                        : bit == 4 ? dpp_mov<0x124>(send)   // row_ror:4
+                                   : dpp_mov<0x128>(send);  // row_ror:8
+      v[j] = greater(keep, got);
     }
   }
-  float top = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    hi[e] = fmaxf(hi[e], dpp_mov<0x128>(hi[e])), lo[e] = fminf(lo[e], dpp_mov<0x128>(lo[e]));  // row_ror:8
-    hi[e] = fmaxf(hi[e], dpp_mov<0x124>(hi[e])), lo[e] = fminf(lo[e], dpp_mov<0x124>(lo[e]));  // row_ror:4
-    hi[e] = fmaxf(hi[e], dpp_mov<0x4E>(hi[e])), lo[e] = fminf(lo[e], dpp_mov<0x4E>(lo[e]));    // quad_perm
-    hi[e] = fmaxf(hi[e], dpp_mov<0xB1>(hi[e])), lo[e] = fminf(lo[e], dpp_mov<0xB1>(lo[e]));
-    top = fmaxf(top, fmaxf(fabsf(hi[e]), fabsf(lo[e])));
-  }
-  top = rows4_max(top);
-  if (lane == 0) s_top[wave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  const int ex = least_exp(top);
-  const int64_t blk = a.row_blk_off[row] + j;
-  if ((lane & 15) == 0) {
-    // Channel group tid / 16 = 4s + g: channels 8 * (tid / 16) + [0, 8).
-    const float down = power2(-ex);
-    uint32_t wh[2] = {0, 0}, wl[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      wh[e >> 2] |= (uint32_t)(clamp8(ceilf(hi[e] * down)) & 0xff) << (8 * (e & 3));
-      wl[e >> 2] |= (uint32_t)(clamp8(floorf(lo[e] * down)) & 0xff) << (8 * (e & 3));
-    }
-    int8_t* bp = a.bounds + blk * kBoundBytes + 8 * (tid >> 4);
-    *reinterpret_cast<uint2*>(bp) = make_uint2(wh[0], wh[1]);
-    *reinterpret_cast<uint2*>(bp + HC_HEAD_DIM) = make_uint2(wl[0], wl[1]);
-  }
-  if (tid == 0) a.exps[blk] = (int8_t)ex;
+  return v[0];
 }
 
-// ---- scores ------------------------------------------------------------------
+// K chunk c = ((h*4+s)*4+g)*16+m of a tile holds token 16h+m, channels
+// 32s+8g+[0,8): a thread reads both halves h of its (s, g, m), so a wave's load
+// is 1 KB in a row.  A thread folds the greatest values of its 8 channels and
+// of their negatives, the 16 lanes m of a channel group fold theirs, and each
+// rounds one of the 16 (floor(x) = -ceil(-x)).  Bound by the key stream: a
+// workgroup takes `per` blocks of a row one after another, the next one's
+// first tiles (two; ONE: blocks of one tile) on their way while one is folded
+// and written.
+template <typename T, bool ONE>
+__global__ __launch_bounds__(256) void block_bounds_kernel(const BoundArgs a) {
+  typedef typename Elem<T>::vec8 vec8;
+  __shared__ float s_top[2][4];
+  // Neighbouring workgroups read neighbouring blocks.
+  const int chunks = gridDim.x / a.rows;
+  const int row = blockIdx.x / chunks, j0 = blockIdx.x % chunks * a.per;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row_at = a.row_tile_off[row], blk_at = a.row_blk_off[row];
+  const int len = max(a.row_len[row], 0), S = a.tpb * HC_TILE;
+  // Blocks counted from the last complete one back; those that were complete
+  // before the last `fresh` tokens are left.
+  const int have = len / S;
+  const int old = a.fresh > 0 ? max(len - a.fresh, 0) / S : 0;
+  const int first = have - 1 - j0, last = max(max(first - a.per + 1, old), have - a.span);
+  if (first < last) return;
+  const T* kb = reinterpret_cast<const T*>(a.kstore) + tid * 8;
+  constexpr int kLoads = ONE ? 2 : 4;
+  vec8 x[kLoads];
+  auto fetch = [&](const T* p, bool two) {  // a pair of tiles, or one twice
+    x[0] = load8_stream<T>(p), x[1] = load8_stream<T>(p + 2048);
+    if constexpr (!ONE) {
+      const T* p1 = p + (two ? HC_TILE_ELEMS : 0);
+      x[2] = load8_stream<T>(p1), x[3] = load8_stream<T>(p1 + 2048);
+    }
+  };
+  fetch(kb + (row_at + (int64_t)first * a.tpb) * HC_TILE_ELEMS, a.tpb > 1);
+  for (int j = first; j >= last; --j) {
+    float v[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = -INFINITY;
+    auto fold = [&]() {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = vec8_at<T>(x[u], e);
+          v[e] = greater(v[e], y);
+          v[8 + e] = greater(v[8 + e], -y);
+        }
+    };
+    fold();
+    if constexpr (!ONE)
+      for (int t = 2; t < a.tpb; t += 2) {
+        fetch(kb + (row_at + (int64_t)j * a.tpb + t) * HC_TILE_ELEMS, t + 1 < a.tpb);
+        fold();
+      }
+    fetch(kb + (row_at + (int64_t)max(j - 1, last) * a.tpb) * HC_TILE_ELEMS, a.tpb > 1);  // (at the end the last again)
+    const float mine = row16_max_scatter(v, lane);
+    // The greatest |k| is the greatest of all 16 values of all groups.
+    float top = greater(mine, dpp_mov<0xB1>(mine));
+    top = greater(top, dpp_mov<0x4E>(top));
+    top = greater(top, dpp_mov<0x124>(top));
+    top = greater(top, dpp_mov<0x128>(top));
+    top = rows4_max(top);
+    float* st = s_top[j & 1];
+    if (lane == 0) st[wave] = top;
+    // Only LDS is waited for: the next block's loads stay in flight.
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    top = fmaxf(fmaxf(st[0], st[1]), fmaxf(fmaxf(st[2], st[3]), 0.f));
+    const int ex = least_exp(top);
+    const int64_t blk = blk_at + j;
+    // Value m of channel group tid / 16 = 4s + g: channel 8 (tid / 16) + m % 8,
+    // its maximum (m < 8) or its minimum's negative.
+    const int m = lane & 15, q8 = clamp8(ceilf(mine * power2(-ex)));
+    a.bounds[blk * kBoundBytes + (m >> 3) * HC_HEAD_DIM + 8 * (tid >> 4) + (m & 7)] = (int8_t)(m < 8 ? q8 : -q8);
+    if (tid == 0) a.exps[blk] = (int8_t)ex;
+  }
+}
+
+template <typename T>
+void launch_bounds(const BoundArgs& a, unsigned grid, hipStream_t s) {
+  if (a.tpb == 1)
+    hipLaunchKernelGGL((block_bounds_kernel<T, true>), dim3(grid), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((block_bounds_kernel<T, false>), dim3(grid), dim3(256), 0, s, a);
+}
+
+// ---- scores and selection ------------------------------------------------------
 struct SelectArgs {
   const void* q;
   int64_t q_s[3];
   const int8_t *bounds, *exps;
   const int64_t* row_blk_off;
   const int32_t* row_len;
-  float* scores;  // [row * Q + query][pitch]
+  float* scores;  // [row * Q + query][pitch]; unused where scores stay in LDS
   int64_t pitch;
   int32_t *idx, *counts;
   int Hkv, G, Q, rows, S, keep, sink, local;
-  int qpb, ncb;   // queries of a 16-column block, such blocks of a row
-  int chunks;     // workgroups along the blocks of a row
-  int max_blocks; // visible blocks a row has room for in scores; a row of more selects nothing
+  int chunks;      // score workgroups of a query
+  int max_blocks;  // visible blocks a query has room for; one that sees more selects nothing
 };
 
-// Visible tokens and blocks of query i of a row.
+// Visible tokens of query i of a row.
 __device__ __forceinline__ int visible(int len, int Q, int i) { return min(max(len - Q + 1 + i, 0), len); }
 
-// A wave scores 16 blocks at a time against the 16 columns (query, head):
-// the blocks are the A operand (16 bytes a lane of the 256 of a block, so a
-// wave's four loads read 4 KB in all), the queries' positive and negative
-// parts the B operand.  Bound by the index's bytes.
-constexpr int kScoreWaves = 4;
-template <typename T>
-__global__ __launch_bounds__(kScoreWaves * 64) void block_score_kernel(const SelectArgs a) {
-  __shared__ float s_s[kScoreWaves][16][17];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = lane >> 4, n = lane & 15;
-  const int jobs = a.rows * a.ncb;
-  const int job = blockIdx.x % jobs, chunk = blockIdx.x / jobs;
-  const int row = job / a.ncb, cb = job % a.ncb;
-  const int b = row / a.Hkv, kv = row % a.Hkv;
-  const int i0 = cb * a.qpb, nq = min(a.qpb, a.Q - i0), ncols = nq * a.G;
-  const int len = max(a.row_len[row], 0);
-  // Blocks whose score may decide: those between the first `sink` and the
-  // last `local` of some query that has more blocks than it keeps.
-  const int have = (visible(len, a.Q, i0 + nq - 1) + a.S - 1) / a.S;
-  const int lo = a.sink, hi = have <= a.keep || have > a.max_blocks ? a.sink : have - a.local;
-  const int steps = (hi - lo + 15) / 16;
-  const int st0 = chunk * kScoreWaves + wave;
-  if (steps <= chunk * kScoreWaves) return;  // whole workgroups only: no barrier is missed
+// A job is one query of one row; the queries of a row go to one XCD, whose L2
+// then holds the row's bounds.
+struct SelectJob {
+  int row, i;
+  int have;     // visible blocks
+  int lo, hi;   // scored blocks: those between the first `sink` and the last `local`, if any are left out
+};
+__device__ __forceinline__ bool select_job(const SelectArgs& a, int x, SelectJob& j) {
+  const int rest = x % (8 * a.Q);
+  j.row = x / (8 * a.Q) * 8 + rest % 8;
+  j.i = rest / 8;
+  return j.row < a.rows;
+}
+// Apart from select_job: the query's loads do not wait for the row's length.
+__device__ __forceinline__ void select_range(const SelectArgs& a, SelectJob& j) {
+  j.have = (visible(max(a.row_len[j.row], 0), a.Q, j.i) + a.S - 1) / a.S;
+  j.lo = a.sink;
+  j.hi = j.have <= a.keep || j.have > a.max_blocks ? a.sink : j.have - a.local;
+}
 
-  const bool col_ok = n < ncols;
-  i32x4 qp[4];  // B operands: steps 0, 1 the positive parts, 2, 3 the negative ones
-  float unit;
-  {
-    const T* p = reinterpret_cast<const T*>(a.q) + b * a.q_s[0] + (int64_t)(kv * a.G + (col_ok ? n % a.G : 0)) * a.q_s[1] +
-                 (int64_t)(i0 + (col_ok ? n / a.G : 0)) * a.q_s[2] + 16 * g;
-    float x[2][16];
-    float top = 0.f;
+// A wave's 16 x 64 products: the query's heads in 8 bits are the A operand
+// (lane: head l % 16, 16 bytes of the 256 a block has, steps 0 and 1 the
+// positive parts against the maxima, 2 and 3 the negative ones against the
+// minima), 16 blocks the B operand.
+struct ScoreQuery {
+  i32x4 op[4];
+  float unit[4];  // powers of two of heads 4g .. 4g + 3; 0 heads are told apart by G
+};
+template <typename T>
+__device__ __forceinline__ ScoreQuery score_query(const SelectArgs& a, const SelectJob& j, int lane) {
+  const int g = lane >> 4, n = lane & 15;
+  const int b = j.row / a.Hkv, kv = j.row % a.Hkv;
+  const bool ok = n < a.G;
+  const T* p = reinterpret_cast<const T*>(a.q) + b * a.q_s[0] + (int64_t)(kv * a.G + (ok ? n : 0)) * a.q_s[1] +
+               (int64_t)j.i * a.q_s[2] + 16 * g;
+  float x[2][16];
+  float top = 0.f;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+  for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const typename Elem<T>::vec8 v = load8<T>(p + 64 * s + 8 * u);
+    for (int u = 0; u < 2; ++u) {
+      const typename Elem<T>::vec8 v = load8<T>(p + 64 * s + 8 * u);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = col_ok ? vec8_at<T>(v, e) : 0.f;
-          x[s][8 * u + e] = y;
-          top = fmaxf(top, fabsf(y));
-        }
+      for (int e = 0; e < 8; ++e) {
+        const float y = ok ? vec8_at<T>(v, e) : 0.f;
+        x[s][8 * u + e] = y;
+        top = fmaxf(top, fabsf(y));
       }
-    const int ex = least_exp(rows4_max(top));
-    const float down = power2(-ex);
-    unit = power2(ex);
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t pos = 0, neg = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int v = clamp8(rintf(x[s][4 * w + e] * down));
-          pos |= (uint32_t)(max(v, 0) & 0xff) << (8 * e);
-          neg |= (uint32_t)(min(v, 0) & 0xff) << (8 * e);
-        }
-        qp[s][w] = (int)pos;
-        qp[2 + s][w] = (int)neg;
-      }
-  }
-  const int64_t blk0 = a.row_blk_off[row];
-  for (int st = st0; st < steps; st += kScoreWaves * a.chunks) {
-    const int j0 = lo + 16 * st;
-    const int mine = min(j0 + n, hi - 1);  // past the end: the last block again, not stored
-    const int8_t* bp = a.bounds + (blk0 + mine) * kBoundBytes + 16 * g;
-    i32x4 acc = {0, 0, 0, 0};
-    i32x4 x[4];
-#pragma unroll
-    for (int s = 0; s < 4; ++s) x[s] = *reinterpret_cast<const i32x4*>(bp + 64 * s);
-    const float eu = power2(a.exps[blk0 + mine]);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[s], qp[s], acc, 0, 0, 0);
-    // Lane: blocks j0 + 4g + r, column n.
-#pragma unroll
-    for (int r = 0; r < 4; ++r) s_s[wave][4 * g + r][n] = (float)acc[r] * unit;
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-    __builtin_amdgcn_wave_barrier();
-    for (int y = lane; y < 16 * nq; y += 64) {
-      const int jj = y & 15, i = y >> 4;
-      float best = s_s[wave][jj][i * a.G];
-      for (int h = 1; h < a.G; ++h) best = fmaxf(best, s_s[wave][jj][i * a.G + h]);
-      best *= __shfl(eu, jj, 64);
-      if (j0 + jj < hi) a.scores[((int64_t)row * a.Q + i0 + i) * a.pitch + j0 + jj] = best;
     }
-    __builtin_amdgcn_wave_barrier();
+  const int ex = least_exp(rows4_max(top));
+  const float down = power2(-ex), up = power2(ex);
+  ScoreQuery r;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      uint32_t pos = 0, neg = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int v = clamp8(rintf(x[s][4 * w + e] * down));
+        pos |= (uint32_t)(max(v, 0) & 0xff) << (8 * e);
+        neg |= (uint32_t)(min(v, 0) & 0xff) << (8 * e);
+      }
+      r.op[s][w] = (int)pos;
+      r.op[2 + s][w] = (int)neg;
+    }
+#pragma unroll
+  for (int t = 0; t < 4; ++t) r.unit[t] = __shfl(up, 4 * g + t, 64);
+  return r;
+}
+
+// Scores of U * 16 blocks from blk0 on: f(u, score) with lane l's block u * 16 +
+// l % 16 (all four lanes of it hold it).  last: the last block that may be
+// read; those past it read it again.  The 4 U loads of 1 KB are in flight
+// together.
+template <int U, typename F>
+__device__ __forceinline__ void score_blocks(const SelectArgs& a, const ScoreQuery& q, int64_t blk0, int64_t last,
+                                             int lane, F f) {
+  const int g = lane >> 4, n = lane & 15;
+  i32x4 x[U][4];
+  float unit[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t blk = min(blk0 + 16 * u + n, last);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      x[u][s] = *reinterpret_cast<const i32x4*>(a.bounds + blk * kBoundBytes + 64 * s + 16 * g);
+    unit[u] = power2(a.exps[blk]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    i32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.op[s], x[u][s], acc, 0, 0, 0);
+    // Lane: heads 4g + r of block n.  Whole numbers below 2^24 and powers of
+    // two: every step is exact.
+    float best = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (4 * g + r < a.G) best = fmaxf(best, (float)acc[r] * q.unit[r]);
+    f(u, rows4_max(best) * unit[u]);
   }
 }
 
-// ---- selection ---------------------------------------------------------------
-// One workgroup a query: the threshold score by four 8-bit radix passes over
-// the keys of the middle blocks, then one ordered pass that writes the kept
-// blocks.  The keys live in LDS where they fit (kPickKeys), else each pass
-// reads the scores again.  Bound by the latency of its dependent passes.
-constexpr int kPickThreads = 512;
-constexpr int kPickKeys = 8192;
-__global__ __launch_bounds__(kPickThreads) void block_pick_kernel(const SelectArgs a) {
-  __shared__ uint32_t s_key[kPickKeys];
-  __shared__ int s_hist[256];
-  __shared__ int s_scan[kPickThreads / 64];
-  __shared__ int s_digit, s_need;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t x = blockIdx.x;  // row * Q + query
-  const int row = (int)(x / a.Q), i = (int)(x % a.Q);
-  const int len = max(a.row_len[row], 0);
-  const int have = (visible(len, a.Q, i) + a.S - 1) / a.S;
+// Scores of long rows for few queries: many workgroups a query, through
+// memory.  Bound by the index's bytes.
+constexpr int kScoreWaves = 4;
+template <typename T>
+__global__ __launch_bounds__(kScoreWaves * 64) void block_score_kernel(const SelectArgs a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int jobs = (a.rows + 7) / 8 * 8 * a.Q;
+  SelectJob j;
+  if (!select_job(a, blockIdx.x % jobs, j)) return;
+  const ScoreQuery q = score_query<T>(a, j, lane);
+  const int chunk = blockIdx.x / jobs;
+  select_range(a, j);
+  const int steps = (j.hi - j.lo + 31) / 32;
+  if (steps <= chunk * kScoreWaves) return;
+  const int64_t base = a.row_blk_off[j.row];
+  float* out = a.scores + ((int64_t)j.row * a.Q + j.i) * a.pitch;
+  for (int st = chunk * kScoreWaves + wave; st < steps; st += kScoreWaves * a.chunks) {
+    const int j0 = j.lo + 32 * st;
+    score_blocks<2>(a, q, base + j0, base + j.hi - 1, lane, [&](int u, float s) {
+      const int blk = j0 + 16 * u + (lane & 15);
+      if (lane < 16 && blk < j.hi) out[blk] = s;
+    });
+  }
+}
+
+// One workgroup a query: the scores' keys (from score_blocks itself where
+// SCORED is not set, else from memory) in LDS, the threshold, and one ordered
+// pass that writes the kept blocks.  The threshold is found by counting the
+// keys into 1024 equal steps between the least and the greatest left and going
+// on in the step where the count of kept ones is reached: scores of one query
+// lie within a few powers of two, where fixed digits of the key would pile up
+// in few counters.  Bound by the latency of its dependent steps; a barrier
+// each for scores, range, counts (one or two rounds) and places.
+constexpr int kPickKeys = 12288;  // keys in LDS; a longer row's are read again from memory each time
+constexpr int kPickBins = 1024;
+// Counters are read 16 in a row by each lane: one of padding after each 16
+// keeps the lanes on different banks.
+constexpr int kPickPad = kPickBins / 16 * 17;
+__device__ __forceinline__ int pick_slot(uint32_t bin) { return (int)(bin + (bin >> 4)); }
+template <typename T, bool SCORED, int NT>
+__global__ __launch_bounds__(NT) void block_pick_kernel(const SelectArgs a) {
+  constexpr int kWaves = NT / 64;
+  extern __shared__ uint32_t s_key[];
+  __shared__ int s_hist[2][kPickPad];
+  __shared__ uint32_t s_lo[kWaves], s_hi[kWaves];
+  __shared__ int s_gt[kWaves], s_eq[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  SelectJob j;
+  if (!select_job(a, blockIdx.x, j)) return;
+  ScoreQuery q;
+  if constexpr (!SCORED) q = score_query<T>(a, j, lane);
+  select_range(a, j);
+  const int64_t x = (int64_t)j.row * a.Q + j.i;
   int32_t* out = a.idx + x * a.keep;
-  const bool fits = have <= a.max_blocks;
-  if (tid == 0) a.counts[x] = fits ? min(have, a.keep) : -1;
-  if (!fits) {
-    for (int k = tid; k < a.keep; k += kPickThreads) out[k] = -1;
+  const bool fits = j.have <= a.max_blocks;
+  if (tid == 0) a.counts[x] = fits ? min(j.have, a.keep) : -1;
+  if (!fits || j.have <= a.keep) {
+    for (int k = tid; k < a.keep; k += NT) out[k] = fits && k < j.have ? k : -1;
     return;
   }
-  if (have <= a.keep) {
-    for (int k = tid; k < a.keep; k += kPickThreads) out[k] = k < have ? k : -1;
-    return;
-  }
-  const int lo = a.sink, nmid = have - a.local - lo;
+  const int lo = j.lo, nmid = j.hi - lo;
   int need = a.keep - a.sink - a.local;  // < nmid
-  for (int k = tid; k < a.sink; k += kPickThreads) out[k] = k;
-  for (int k = tid; k < a.local; k += kPickThreads) out[a.keep - a.local + k] = have - a.local + k;
+  for (int k = tid; k < a.sink; k += NT) out[k] = k;
+  for (int k = tid; k < a.local; k += NT) out[a.keep - a.local + k] = j.have - a.local + k;
   if (need == 0) return;
-  const float* sc = a.scores + x * a.pitch + lo;
-  const bool in_lds = nmid <= kPickKeys;
-  if (in_lds) {
-    for (int k = tid; k < nmid; k += kPickThreads) s_key[k] = order_key(sc[k]);
+  for (int k = tid; k < 2 * kPickPad; k += NT) s_hist[0][k] = 0;
+  const float* sc = SCORED ? a.scores + x * a.pitch + lo : nullptr;
+  const bool in_lds = !SCORED || nmid <= kPickKeys;
+  if constexpr (SCORED) {
+    if (in_lds)
+      for (int k = tid; k < nmid; k += NT) s_key[k] = order_key(sc[k]);
+  } else {
+    const int64_t base = a.row_blk_off[j.row] + lo;
+    for (int k0 = 64 * wave; k0 < nmid; k0 += 64 * kWaves)
+      score_blocks<4>(a, q, base + k0, base + nmid - 1, lane, [&](int u, float s) {
+        const int k = k0 + 16 * u + (lane & 15);
+        if (lane < 16 && k < nmid) s_key[k] = order_key(s);
+      });
   }
+  __syncthreads();
   auto key = [&](int k) { return in_lds ? s_key[k] : order_key(sc[k]); };
-  uint32_t prefix = 0, mask = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) s_hist[tid] = 0;
-    __syncthreads();
-    for (int k = tid; k < nmid; k += kPickThreads) {
-      const uint32_t u = key(k);
-      if ((u & mask) == prefix) atomicAdd(&s_hist[(u >> shift) & 255], 1);
-    }
-    __syncthreads();
-    if (wave == 0) {
-      // Lane y: bins 255 - 4y .. 252 - 4y; keys above its first bin, then the
-      // bin in which the need-th highest key lies.
-      int c[4], sum = 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) sum += c[u] = s_hist[255 - 4 * lane - u];
-      int incl = sum;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(incl, d, 64);
-        if (lane >= d) incl += v;
-      }
-      int above = incl - sum;
-      if (above < need && need <= incl) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (above < need && need <= above + c[u]) {
-            s_digit = 255 - 4 * lane - u;
-            s_need = need - above;
-          }
-          above += c[u];
-        }
-      }
-    }
-    __syncthreads();
-    prefix |= (uint32_t)s_digit << shift;
-    mask |= 255u << shift;
-    need = s_need;
-  }
-  // Keys above `prefix` are kept, and the first `need` equal to it.  Every
-  // thread takes a run of blocks; two scans (equal keys, then kept ones) give
-  // the places.
-  const int run = (nmid + kPickThreads - 1) / kPickThreads;
+
+  // Every thread keeps to a run of blocks.
+  const int run = (nmid + NT - 1) / NT;
   const int k0 = min(tid * run, nmid), k1 = min(k0 + run, nmid);
-  int eq = 0, gt = 0;
+  uint32_t least = 0xffffffffu, most = 0u;
   for (int k = k0; k < k1; ++k) {
     const uint32_t u = key(k);
-    eq += u == prefix;
-    gt += u > prefix;
+    least = min(least, u);
+    most = max(most, u);
   }
-  auto scan = [&](int v) {  // exclusive, over the workgroup
-    int incl = v;
+  least = wave_fold(least, [](uint32_t u, uint32_t v) { return min(u, v); });
+  most = wave_fold(most, [](uint32_t u, uint32_t v) { return max(u, v); });
+  if (lane == 0) s_lo[wave] = least, s_hi[wave] = most;
+  __syncthreads();
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int u = __shfl_up(incl, d, 64);
-      if (lane >= d) incl += u;
+  for (int w = 0; w < kWaves; ++w) {
+    least = min(least, s_lo[w]);
+    most = max(most, s_hi[w]);
+  }
+
+  // Kept: the keys above T, and the first `need` equal to it.
+  uint32_t T0 = least;
+  for (int round = 0; least < most; ++round) {
+    const uint32_t span = most - least;
+    const int shift = max(32 - __clz((int)span) - 10, 0);
+    int* hist = s_hist[round & 1];
+    for (int k = k0; k < k1; ++k) {
+      const uint32_t u = key(k);
+      if (u >= least && u <= most) atomicAdd(&hist[pick_slot((u - least) >> shift)], 1);
     }
     __syncthreads();
-    if (lane == 63) s_scan[wave] = incl;
-    __syncthreads();
-    int before = 0;
-    for (int w = 0; w < wave; ++w) before += s_scan[w];
-    return before + incl - v;
-  };
-  const int eq0 = scan(eq);
-  const int take = min(max(need - eq0, 0), eq);
-  int at = a.sink + scan(gt + take);
-  int left = take;
+    // Lane y: bins 1023 - 16 y .. 1008 - 16 y; keys above its first one, then
+    // the bin in which the need-th highest key lies (every wave for itself).
+    int c[16], sum = 0;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) sum += c[u] = hist[kPickPad - 2 - 17 * lane - u];
+    const int incl = wave_scan_add(sum);
+    int above = incl - sum, bin = 0, in_bin = 0, before = 0;
+    const bool mine = above < need && need <= incl;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      if (above < need && need <= above + c[u]) bin = kPickBins - 1 - 16 * lane - u, in_bin = c[u], before = above;
+      above += c[u];
+    }
+    const int src = __builtin_ctzll(__ballot(mine));
+    bin = __builtin_amdgcn_readlane(bin, src);
+    in_bin = __builtin_amdgcn_readlane(in_bin, src);
+    need -= __builtin_amdgcn_readlane(before, src);
+    least += (uint32_t)bin << shift;
+    most = min(most, least + ((1u << shift) - 1u));
+    T0 = least;
+    if (in_bin == need) {  // the whole step is kept
+      T0 = least - 1u;     // (no score's key is 0)
+      need = 0;
+      break;
+    }
+    // The counts of the round after next: zeroed behind the next barrier's
+    // reads of the other ones.
+    int* other = s_hist[(round + 1) & 1];
+    if (round > 0) {
+      for (int k = tid; k < kPickPad; k += NT) other[k] = 0;
+      __syncthreads();
+    }
+  }
+
+  int gt = 0, eq = 0;
   for (int k = k0; k < k1; ++k) {
     const uint32_t u = key(k);
-    if (u > prefix || (u == prefix && left > 0)) {
-      left -= u == prefix;
+    gt += u > T0;
+    eq += u == T0;
+  }
+  const int gt_in = wave_scan_add(gt), eq_in = wave_scan_add(eq);
+  if (lane == 63) s_gt[wave] = gt_in, s_eq[wave] = eq_in;
+  __syncthreads();
+  int gt0 = gt_in - gt, eq0 = eq_in - eq;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+    if (w < wave) gt0 += s_gt[w], eq0 += s_eq[w];
+  int at = a.sink + gt0 + min(eq0, need);
+  int left = max(need - eq0, 0);
+  for (int k = k0; k < k1; ++k) {
+    const uint32_t u = key(k);
+    if (u > T0 || (u == T0 && left > 0)) {
+      left -= u == T0;
       out[at++] = lo + k;
     }
   }
@@ -358,6 +483,30 @@ int check_q(const char* what, int dtype, const void* q, const int64_t* st) {
   return HC_OK;
 }
 
+// Whether scores go through memory: rows whose keys LDS does not hold, and few
+// queries over long rows -- one CU draws some 33 GB/s, so a workgroup that
+// scores its row alone is slow where it has the device almost to itself (8
+// queries of 512, 1024 and 4096 blocks: 10.3, 15.8 and 38 us against 9.4, 10.8
+// and 14.5 through memory; 192 queries: 11.2, 17.4 and 42.6 against 12.3, 18.7
+// and 43.3; 8 of 256 blocks: 7.7 against 8.8).
+constexpr int kSoloBlocks = 256;
+bool select_in_memory(int64_t jobs, int max_blocks) {
+  return max_blocks > kPickKeys || (max_blocks > kSoloBlocks && jobs <= device_cus() / 2);
+}
+// Blocks that four waves pick from, sixteen beyond (8 queries of 512, 1024 and
+// 2048 blocks through memory: 9.4, 10.8 and 13.5 us with four, 10.7, 11.8 and
+// 12.6 with sixteen).
+constexpr int kFewBlocks = 1024;
+
+template <typename T, bool SCORED>
+void launch_pick(const SelectArgs& a, dim3 grid, hipStream_t s) {
+  const size_t lds = (size_t)std::min(std::max(a.max_blocks, 1), kPickKeys) * sizeof(uint32_t);
+  if (a.max_blocks <= kFewBlocks)
+    hipLaunchKernelGGL((block_pick_kernel<T, SCORED, 256>), grid, dim3(256), lds, s, a);
+  else
+    hipLaunchKernelGGL((block_pick_kernel<T, SCORED, 1024>), grid, dim3(1024), lds, s, a);
+}
+
 int64_t score_pitch(int64_t max_blocks) { return (max_blocks + 63) / 64 * 64; }
 
 }  // namespace
@@ -377,22 +526,27 @@ extern "C" int hc_block_bounds(int dtype, const void* kstore, const int64_t* row
     return set_error(HC_ERR_INVALID, "hc_block_bounds: null pointer argument");
   if ((reinterpret_cast<uintptr_t>(kstore) | reinterpret_cast<uintptr_t>(bounds)) & 15)
     return set_error(HC_ERR_INVALID, "hc_block_bounds: the store and the bounds must be 16-byte aligned");
-  const int64_t grid = (int64_t)rows * span;
+  // One resident round of workgroups, each with its share of a row's blocks (16
+  // rows of 1025 blocks of 64 tokens: 71, 60, 53 and 50 us with 1, 2, 4 and 8
+  // blocks a workgroup).
+  const int per = (int)std::min<int64_t>(std::max<int64_t>((int64_t)rows * span / (8 * device_cus()), 1), 64);
+  const int64_t grid = (int64_t)rows * ((span + (int64_t)per - 1) / per);
   if (grid > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_block_bounds: %d rows x %d blocks", rows, span);
-  BoundArgs a = {kstore, row_tile_off, row_block_off, row_len, bounds, exps, rows, block / HC_TILE, span, fresh};
+  BoundArgs a = {kstore, row_tile_off, row_block_off, row_len, bounds, exps, rows, block / HC_TILE, span, fresh, per};
   hipStream_t s = (hipStream_t)stream;
-  const dim3 g((unsigned)grid), t(256);
   switch (dtype) {
-    case HC_DTYPE_BF16: hipLaunchKernelGGL(block_bounds_kernel<__bf16>, g, t, 0, s, a); break;
-    case HC_DTYPE_F16: hipLaunchKernelGGL(block_bounds_kernel<_Float16>, g, t, 0, s, a); break;
-    default: hipLaunchKernelGGL(block_bounds_kernel<float>, g, t, 0, s, a); break;
+    case HC_DTYPE_BF16: launch_bounds<__bf16>(a, (unsigned)grid, s); break;
+    case HC_DTYPE_F16: launch_bounds<_Float16>(a, (unsigned)grid, s); break;
+    default: launch_bounds<float>(a, (unsigned)grid, s); break;
   }
   return check_launch("hc_block_bounds");
 }
 
 extern "C" size_t hc_block_select_scratch_size(int batch, int kv_heads, int queries, int max_blocks) {
   if (batch < 0 || kv_heads < 1 || queries < 0 || max_blocks < 0) return 0;
-  return (size_t)batch * kv_heads * queries * score_pitch(max_blocks) * sizeof(float);
+  const int64_t rows = (int64_t)batch * kv_heads;
+  if (!select_in_memory((rows + 7) / 8 * 8 * queries, max_blocks)) return 0;
+  return (size_t)rows * queries * score_pitch(max_blocks) * sizeof(float);
 }
 
 extern "C" int hc_block_select(int dtype, const void* q, const int64_t* q_strides, const int8_t* bounds,
@@ -423,15 +577,24 @@ extern "C" int hc_block_select(int dtype, const void* q, const int64_t* q_stride
   a.scores = reinterpret_cast<float*>(scratch), a.pitch = score_pitch(max_blocks), a.idx = idx, a.counts = counts;
   a.Hkv = kv_heads, a.G = q_heads / kv_heads, a.Q = queries, a.rows = batch * kv_heads, a.S = block;
   a.keep = keep, a.sink = sink, a.local = local, a.max_blocks = max_blocks;
-  a.qpb = std::max(1, std::min(queries, 16 / a.G)), a.ncb = (queries + a.qpb - 1) / a.qpb;
-  const int64_t jobs = (int64_t)a.rows * a.ncb;
-  const int64_t most = (max_blocks + 16 * kScoreWaves - 1) / (16 * kScoreWaves);
-  a.chunks = (int)std::max<int64_t>(std::min<int64_t>((8 * device_cus() + jobs - 1) / jobs, most), 1);
-  const int64_t grid = jobs * a.chunks;
-  if (grid > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_block_select: %lld workgroups", (long long)grid);
+  const int64_t jobs = ((int64_t)a.rows + 7) / 8 * 8 * queries;
+  if (jobs > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_block_select: %lld queries", (long long)jobs);
   hipStream_t s = (hipStream_t)stream;
+  const dim3 grid((unsigned)jobs);
+  if (!select_in_memory(jobs, max_blocks)) {
+    switch (dtype) {
+      case HC_DTYPE_BF16: launch_pick<__bf16, false>(a, grid, s); break;
+      case HC_DTYPE_F16: launch_pick<_Float16, false>(a, grid, s); break;
+      default: launch_pick<float, false>(a, grid, s); break;
+    }
+    return check_launch("hc_block_select");
+  }
+  const int64_t most = (max_blocks + 32 * kScoreWaves - 1) / (32 * kScoreWaves);
+  a.chunks = (int)std::max<int64_t>(std::min<int64_t>((8 * device_cus() + jobs - 1) / jobs, most), 1);
+  if (jobs * a.chunks > 0x7fffffffLL)
+    return set_error(HC_ERR_INVALID, "hc_block_select: %lld workgroups", (long long)(jobs * a.chunks));
   if (max_blocks > keep) {
-    const dim3 g((unsigned)grid), t(kScoreWaves * 64);
+    const dim3 g((unsigned)(jobs * a.chunks)), t(kScoreWaves * 64);
     switch (dtype) {
       case HC_DTYPE_BF16: hipLaunchKernelGGL(block_score_kernel<__bf16>, g, t, 0, s, a); break;
       case HC_DTYPE_F16: hipLaunchKernelGGL(block_score_kernel<_Float16>, g, t, 0, s, a); break;
@@ -439,19 +602,36 @@ extern "C" int hc_block_select(int dtype, const void* q, const int64_t* q_stride
     }
     if ((rc = check_launch("hc_block_select(scores)"))) return rc;
   }
-  hipLaunchKernelGGL(block_pick_kernel, dim3((unsigned)(a.rows * a.Q)), dim3(kPickThreads), 0, s, a);
+  launch_pick<float, true>(a, grid, s);
   return check_launch("hc_block_select");
 }
 
 namespace {
-// The plan and workspace of hc_block_attn: one query a job.
+// The plan and workspace of hc_block_attn: one query a job, `waves` waves a
+// workgroup, nsplit workgroups a job.
 struct BlockPlan {
-  int nsplit;
+  int waves, nsplit;
   size_t part_o, bytes;
 };
 BlockPlan block_plan(int batch, int kv_heads, int G, int queries, int block, int keep) {
-  BlockPlan p;
-  p.nsplit = rows_plan(batch * kv_heads * queries, G, 1, (int64_t)keep * (block / HC_TILE)).nsplit;
+  // The least estimate in us: a wave's tiles one after another (2.4 each, the
+  // latency of scattered blocks, behind 2.2 of start and end: 7.2, 22.8 and
+  // 32.6 for 2, 8 and 12; more where the tiles of all waves on the device take
+  // longer to stream) in as many rounds as the device needs; a split adds the
+  // launch that folds it.  A CU holds three
+  // workgroups of four waves or one of eight, which have at most 8 columns.
+  BlockPlan p = {4, 1, 0, 0};
+  const int64_t jobs = (int64_t)batch * kv_heads * queries, tiles = (int64_t)keep * (block / HC_TILE);
+  double best = 0.;
+  for (int waves = 4; waves <= (G <= 8 ? 8 : 4); waves += 4)
+    for (int ns = 1; ns <= 64 && (ns == 1 || (int64_t)ns * waves <= tiles); ++ns) {
+      const int64_t slots = (int64_t)device_cus() * (waves == 8 ? 1 : 3);
+      const double rounds = (double)((jobs * ns + slots - 1) / slots);
+      const double load = (double)std::min(jobs * ns, slots) * waves * HC_TILE_ELEMS * 4. / 5.5e6;
+      const double own = 2.2 + std::max(2.4, load) * (double)((tiles + waves * ns - 1) / (waves * ns));
+      const double t = rounds * own + (ns > 1 ? 4.5 : 0.);
+      if (best == 0. || t < best * 0.98) best = t, p.waves = waves, p.nsplit = ns;
+    }
   const size_t cols = (size_t)batch * kv_heads * queries * G * p.nsplit;
   p.part_o = cols * kPartO * sizeof(float);
   p.bytes = p.nsplit > 1 ? p.part_o + cols * 2 * sizeof(float) : 0;
@@ -500,7 +680,7 @@ extern "C" int hc_block_attn(int dtype, const void* q, const int64_t* q_strides,
     r.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + p.part_o);
   }
   hipStream_t s = (hipStream_t)stream;
-  if ((rc = launch_block_rows(dtype, r, s)) || p.nsplit == 1) return rc;
+  if ((rc = launch_block_rows(dtype, r, p.waves, s)) || p.nsplit == 1) return rc;
   MergeArgs mg = {};
   mg.row_o = r.part_o, mg.row_ml = r.part_ml, mg.nsplit = p.nsplit;
   mg.Hkv = kv_heads, mg.G = G, mg.Q = queries, mg.out = out;

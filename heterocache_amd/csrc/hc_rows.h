@@ -178,56 +178,55 @@ struct RowsArgs {
   int64_t o_s[3];
 };
 
-constexpr int kRowsWaves = 4;
 constexpr int kRowsPitch = HC_HEAD_DIM + 4;
-// LDS floats of rows_job: the waves' O and (m, l).
-constexpr int kRowsLds = kRowsWaves * 16 * (kRowsPitch + 2);
+// LDS floats of rows_job: O and (m, l) of NW waves x 64 / NW columns.
+constexpr int kRowsLds = 64 * (kRowsPitch + 2);
 
-// Workgroup `wg` of a rows launch (4 waves): one split of one job (qpb queries
-// of one row and its G heads).  The waves take every fourth tile of the split
-// straight into the operand registers and are combined through LDS (lds:
-// kRowsLds floats).  K's registers are refilled once the scores are formed,
+inline int64_t rows_workgroups(const RowsArgs& a) { return ((int64_t)a.rows + 7) / 8 * 8 * a.ncb * a.nsplit; }
+
+// Workgroup `wg` of a rows launch (NW waves): one split of one job (qpb queries
+// of one row and its G heads, at most 64 / NW columns).  The waves take every
+// NW-th tile of the split straight into the operand registers and are combined
+// through LDS (lds: kRowsLds floats).  K's registers are refilled once the scores are formed,
 // V's once the values are added, so a wave always has half a tile or more in
 // flight with one tile's registers, and three waves fit a SIMD (a second
 // buffer leaves two).  Bound by HBM: a token's K and V (512 bytes in 16 bits)
 // feed 512 G operations a query.
-template <typename T, bool LIST, bool MIXED>
+template <typename T, bool LIST, bool MIXED, int NW>
 __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds) {
   typedef typename Elem<T>::vec8 vec8;
-  float(*s_o)[16][kRowsPitch] = reinterpret_cast<float(*)[16][kRowsPitch]>(lds);
-  float(*s_m)[16] = reinterpret_cast<float(*)[16]>(lds + kRowsWaves * 16 * kRowsPitch);
-  float(*s_l)[16] = s_m + kRowsWaves;
+  constexpr int kCols = 64 / NW;
+  float(*s_o)[kCols][kRowsPitch] = reinterpret_cast<float(*)[kCols][kRowsPitch]>(lds);
+  float(*s_m)[kCols] = reinterpret_cast<float(*)[kCols]>(lds + 64 * kRowsPitch);
+  float(*s_l)[kCols] = s_m + NW;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, n = lane & 15;
-  const int jobs = a.rows * a.ncb;
+  // The jobs of a row (LIST: its queries, which keep many of the same blocks)
+  // go to one XCD, as workgroups are dealt to the 8 XCDs in turn.
+  const int jobs = (a.rows + 7) / 8 * 8 * a.ncb;
   const int job = wg % jobs, split = wg / jobs;
-  const int row = job / a.ncb, cb = job % a.ncb;
+  const int row = job / (8 * a.ncb) * 8 + job % 8, cb = job % (8 * a.ncb) / 8;
+  if (row >= a.rows) return;
   const int b = row / a.Hkv, kv = row % a.Hkv;
-  const int len = max(a.row_len[row], 0);
-  const int64_t base = a.row_tile_off[row] * (int64_t)HC_TILE_ELEMS + lane * 8;
-
   // Column n: query i0 + n / G, head n % G of the row's group.
   const int i0 = cb * a.qpb, nq = min(a.qpb, a.Q - i0), ncols = nq * a.G;
   const bool col_ok = n < ncols;
   const int qi = col_ok ? n / a.G : nq - 1, gi = col_ok ? n % a.G : 0;
-  const int lim_lo = min(max(len - a.Q + 1 + i0, 0), len);
-  const int lim_hi = min(max(len - a.Q + i0 + nq, 0), len);
-  const int lim = min(max(len - a.Q + 1 + i0 + qi, 0), len);
 
-  // Entries of the job, this workgroup's share of them and this wave's: e0 +
-  // wave, e0 + wave + 4, ...
-  const int vis = (lim_hi + HC_TILE - 1) / HC_TILE;
+  // Everything the tiles' addresses and products wait for is requested at
+  // once: the length, the tile offset, the list and the queries.
   const int64_t job_q = (int64_t)row * a.Q + i0;  // LIST: one query a job
-  int entries = vis;
-  bool void_list = false;  // no selection was made: the output is NaN
+  const int32_t* const list = LIST ? a.idx + job_q * a.keep : nullptr;
+  const int row_len = a.row_len[row];
+  const int64_t base = a.row_tile_off[row] * (int64_t)HC_TILE_ELEMS + lane * 8;
+  int kept = 0, spec = 0;
+  // This wave's first 64 entries of a whole list.
+  const int full = LIST ? a.keep * a.tpb : 0;
+  const int f0 = (int)((int64_t)full * split / a.nsplit), f1 = (int)((int64_t)full * (split + 1) / a.nsplit);
   if constexpr (LIST) {
-    const int c = a.counts[job_q];
-    void_list = c < 0;
-    entries = vis > 0 ? min(max(c, 0), a.keep) * a.tpb : 0;
+    kept = a.counts[job_q];
+    spec = list[min(f0 + wave + lane * NW, full - 1) / a.tpb];
   }
-  const int e0 = (int)((int64_t)entries * split / a.nsplit), e1 = (int)((int64_t)entries * (split + 1) / a.nsplit);
-  const int cnt = max((e1 - e0 - wave + kRowsWaves - 1) / kRowsWaves, 0);
-
   vec8 qreg[4];
   {
     const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_s[0] + (int64_t)(kv * a.G + gi) * a.q_s[1] +
@@ -235,6 +234,21 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds) 
 #pragma unroll
     for (int s = 0; s < 4; ++s) qreg[s] = col_ok ? load8<T>(qp + 32 * s) : zero8<T>();
   }
+
+  const int len = max(row_len, 0);
+  const int lim_lo = min(max(len - a.Q + 1 + i0, 0), len);
+  const int lim_hi = min(max(len - a.Q + i0 + nq, 0), len);
+  const int lim = min(max(len - a.Q + 1 + i0 + qi, 0), len);
+  // Entries of the job, this workgroup's share of them and this wave's: e0 +
+  // wave, e0 + wave + NW, ...
+  const int vis = (lim_hi + HC_TILE - 1) / HC_TILE;
+  const bool void_list = LIST && kept < 0;  // no selection was made: the output is NaN
+  int entries = vis;
+  if constexpr (LIST) entries = vis > 0 ? min(max(kept, 0), a.keep) * a.tpb : 0;
+  const int e0 = (int)((int64_t)entries * split / a.nsplit), e1 = (int)((int64_t)entries * (split + 1) / a.nsplit);
+  const int cnt = max((e1 - e0 - wave + NW - 1) / NW, 0);
+  const bool whole = LIST && e0 == f0 && e1 == f1;
+
   float m = -INFINITY, l = 0.f;
   f32x4 o[8];
 #pragma unroll
@@ -248,14 +262,14 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds) 
     // is not a visible tile of the row (such an entry attends nothing).
     int mine = 0;
     if constexpr (LIST) {
-      const int e = e0 + wave + (c0 + min(lane, nt - 1)) * kRowsWaves;
-      const int blk = a.idx[job_q * a.keep + e / a.tpb];
+      const int e = e0 + wave + (c0 + min(lane, nt - 1)) * NW;
+      const int blk = whole && c0 == 0 ? spec : list[e / a.tpb];
       const int64_t t = (int64_t)blk * a.tpb + e % a.tpb;
       mine = blk >= 0 && t < vis ? (int)t : -1;
     }
     auto tile_of = [&](int i) {
       if constexpr (LIST) return __builtin_amdgcn_readlane(mine, i);
-      return e0 + wave + (c0 + i) * kRowsWaves;
+      return e0 + wave + (c0 + i) * NW;
     };
     vec8 kr[8], vr[8];
     int tile = tile_of(0);
@@ -297,15 +311,15 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds) 
   }
   __syncthreads();
   // 32 threads a column, 4 channels each.
-  for (int c = threadIdx.x >> 5; c < ncols; c += kRowsWaves * 2) {
+  for (int c = threadIdx.x >> 5; c < ncols; c += NW * 2) {
     const int d0 = 4 * (threadIdx.x & 31);
     float M = s_m[0][c];
 #pragma unroll
-    for (int w = 1; w < kRowsWaves; ++w) M = fmaxf(M, s_m[w][c]);
+    for (int w = 1; w < NW; ++w) M = fmaxf(M, s_m[w][c]);
     float L = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kRowsWaves; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float f = state_weight(s_m[w][c], M);
       L = fmaf(s_l[w][c], f, L);
       acc += *reinterpret_cast<const f32x4*>(&s_o[w][c][d0]) * f;
@@ -344,7 +358,7 @@ struct RowsPlan {
   int qpb, ncb, nsplit;
 };
 RowsPlan rows_plan(int rows, int G, int Q, int64_t max_tiles);
-int launch_block_rows(int dtype, const RowsArgs& a, hipStream_t s);
+int launch_block_rows(int dtype, const RowsArgs& a, int waves, hipStream_t s);
 int launch_merge(int dtype, const MergeArgs& a, int64_t columns, hipStream_t s);
 int device_cus();
 

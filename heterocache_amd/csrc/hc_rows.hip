@@ -7,10 +7,18 @@
 namespace hc {
 namespace {
 
+template <typename T, int NW>
+__global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : sizeof(T) == 4 ? 2 : 3) void block_rows_kernel(const RowsArgs a) {
+  __shared__ __attribute__((aligned(16))) float lds[kRowsLds];
+  rows_job<T, true, false, NW>(a, blockIdx.x, lds);
+}
+
 template <typename T>
-__global__ __launch_bounds__(kRowsWaves * 64, sizeof(T) == 4 ? 2 : 3) void block_rows_kernel(const RowsArgs a) {
-  __shared__ float lds[kRowsLds];
-  rows_job<T, true, false>(a, blockIdx.x, lds);
+void launch_block_rows_t(const RowsArgs& a, int waves, unsigned n, hipStream_t s) {
+  if (waves == 8)
+    hipLaunchKernelGGL((block_rows_kernel<T, 8>), dim3(n), dim3(512), 0, s, a);
+  else
+    hipLaunchKernelGGL((block_rows_kernel<T, 4>), dim3(n), dim3(256), 0, s, a);
 }
 
 // One workgroup an output row: 8 groups of 32 threads (4 channels each) take
@@ -100,22 +108,21 @@ RowsPlan rows_plan(int rows, int G, int Q, int64_t max_tiles) {
   RowsPlan p;
   p.qpb = std::max(1, std::min(Q, 16 / G));
   p.ncb = (Q + p.qpb - 1) / p.qpb;
-  // Two workgroups a CU; a split keeps a tile for each of its waves.
+  // Two workgroups a CU; a split keeps a tile for each of its four waves.
   const int64_t jobs = std::max<int64_t>((int64_t)rows * p.ncb, 1);
   const int64_t want = (2 * device_cus() + jobs - 1) / jobs;
-  const int64_t most = std::max<int64_t>((max_tiles + kRowsWaves - 1) / kRowsWaves, 1);
+  const int64_t most = std::max<int64_t>((max_tiles + 3) / 4, 1);
   p.nsplit = (int)std::min<int64_t>(std::min(want, most), 1024);
   return p;
 }
 
-int launch_block_rows(int dtype, const RowsArgs& a, hipStream_t s) {
-  const int64_t n = (int64_t)a.rows * a.ncb * a.nsplit;
+int launch_block_rows(int dtype, const RowsArgs& a, int waves, hipStream_t s) {
+  const int64_t n = rows_workgroups(a);
   if (n > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "block attention: %lld workgroups", (long long)n);
-  const dim3 grid((unsigned)n), block(kRowsWaves * 64);
   switch (dtype) {
-    case HC_DTYPE_BF16: hipLaunchKernelGGL(block_rows_kernel<__bf16>, grid, block, 0, s, a); break;
-    case HC_DTYPE_F16: hipLaunchKernelGGL(block_rows_kernel<_Float16>, grid, block, 0, s, a); break;
-    default: hipLaunchKernelGGL(block_rows_kernel<float>, grid, block, 0, s, a); break;
+    case HC_DTYPE_BF16: launch_block_rows_t<__bf16>(a, waves, (unsigned)n, s); break;
+    case HC_DTYPE_F16: launch_block_rows_t<_Float16>(a, waves, (unsigned)n, s); break;
+    default: launch_block_rows_t<float>(a, waves, (unsigned)n, s); break;
   }
   return check_launch("block attention");
 }

@@ -141,6 +141,9 @@ __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
     vb += kTileBytes;
   };
 
+  stage(0);
+  if (t0 + 1 < t1) stage(1);
+
   // Q^T operands: column col0 + 16j + n16, k-slots = channels 32s + 8*g4 + [0, 8).
   const int64_t col0 = ((int64_t)cg * kPreWaves + wave) * 16 * NC;
   const bool active = col0 < a.M;
@@ -163,12 +166,10 @@ __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
 #pragma unroll
     for (int db = 0; db < 8; ++db) o[db][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // The queries land before the first tile is staged: the loop counts its
-  // loads in flight.
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  // The queries and the first tiles travel together; from here on the loop
+  // counts its loads in flight.
+  wait_lds_dma();
   asm volatile("" ::: "memory");
-  stage(0);
-  if (t0 + 1 < t1) stage(1);
 
   int slot = 0;
   for (int t = t0; t < t1; ++t) {
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(kPreThreads, sizeof(T) == 4 ? 1 : 3) void shared_at
   if ((int)blockIdx.x < npre)
     prefix_job<T, NC>(pre, blockIdx.x, reinterpret_cast<T*>(shared_raw));
   else
-    rows_job<T, false, MIXED>(rows, blockIdx.x - npre, reinterpret_cast<float*>(shared_raw));
+    rows_job<T, false, MIXED, kPreWaves>(rows, blockIdx.x - npre, reinterpret_cast<float*>(shared_raw));
 }
 
 // Sizes of one call: the prefix launch's column blocks and parts, the rows'
@@ -360,7 +361,7 @@ int launch_shared(const PrefixArgs& a, const RowsArgs& r, int nc, hipStream_t s)
   if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)lds) != hipSuccess)
     return set_error(HC_ERR_HIP, "hc_shared_attn: %s", hipGetErrorString(hipGetLastError()));
-  const int64_t grid = (int64_t)a.parts * a.ncg + (int64_t)r.rows * r.ncb * r.nsplit;
+  const int64_t grid = (int64_t)a.parts * a.ncg + rows_workgroups(r);
   if (grid > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_shared_attn: %lld workgroups", (long long)grid);
   hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(kPreThreads), lds, s, a, r);
   return check_launch("hc_shared_attn");

@@ -797,67 +797,75 @@ def _on_device(fn):
 
     @functools.wraps(fn)
     def call(*args, stream=None, **kwargs):
-        t = args[0] if args else kwargs[first]
-        if not t.is_cuda:
+        dev = (args[0] if args else kwargs[first]).get_device()
+        if dev < 0:
             raise ValueError("libhc ops need tensors on a ROCm device")
         if stream is not None:
-            if stream.device != t.device:
-                raise ValueError(f"a stream of {stream.device} for tensors on {t.device}")
+            if stream.device.index != dev:
+                raise ValueError(f"a stream of {stream.device} for tensors on device {dev}")
             with torch.cuda.stream(stream):
                 return fn(*args, **kwargs)
-        if t.device.index != torch.cuda.current_device():
-            with torch.cuda.device(t.device):
+        if dev != torch._C._cuda_getDevice():
+            with torch.cuda.device(dev):
                 return fn(*args, **kwargs)
         return fn(*args, **kwargs)
     return call
 
 
-def _meta(device, *specs):
-    """Metadata tensors as the kernels read them: (name, tensor, dtype, entries)."""
-    for name, t, dtype, n in specs:
-        if t.dtype != dtype or t.numel() != n or t.device != device or not t.is_contiguous():
-            raise ValueError(f"{name} must be {n} contiguous entries of {dtype} on {device}, got {tuple(t.shape)} of "
-                             f"{t.dtype} on {t.device}")
+# The serving ops are called once a layer and token, some on a few microseconds
+# of kernels: their checks read each property once, and say what is wrong only
+# once something is.
+def _is(t, dtype, n, dev):
+    """Whether t is n contiguous entries of dtype on device index dev, as the
+    kernels read metadata."""
+    return t.dtype is dtype and t.numel() == n and t.get_device() == dev and t.is_contiguous()
 
 
-def _unit(t):
-    return t.stride(-1) == 1 or t.numel() == 0
+def _need(ok, name, t, dtype, n, dev):
+    if not ok:
+        raise ValueError(f"{name} must be {n} contiguous entries of {dtype} on device {dev}, got {tuple(t.shape)} of "
+                         f"{t.dtype} on {t.device}")
 
 
-def _heads(name, t, batch=None, tokens=None, like=None):
-    if t.dim() != 4 or t.shape[3] != HEAD_DIM or not _unit(t):
-        raise ValueError(f"{name} must be [B, H, T, {HEAD_DIM}] with unit channel stride, got {tuple(t.shape)}")
-    if like is not None:
-        if t.dtype != like.dtype:
-            raise TypeError(f"{name} is {t.dtype}, the queries are {like.dtype}")
-        if t.device != like.device:
-            raise ValueError(f"{name} is on {t.device}, the queries on {like.device}")
-        if t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2]:
-            raise ValueError(f"{name} {tuple(t.shape)} does not match the queries' batch and tokens {tuple(like.shape)}")
+def _meta(dev, name, t, dtype, n):
+    if not _is(t, dtype, n, dev):
+        _need(False, name, t, dtype, n, dev)
 
 
-def _stores(like, *stores):
+def _queries(q):
+    shape = q.shape
+    if len(shape) != 4 or shape[3] != HEAD_DIM or (q.stride(3) != 1 and q.numel()):
+        raise ValueError(f"queries must be [B, H, T, {HEAD_DIM}] with unit channel stride, got {tuple(shape)}")
+    return shape
+
+
+def _stores(dtype, dev, *stores):
     for t in stores:
-        if t.dtype != like.dtype:
-            raise TypeError("q and the store must share a dtype")
-        if t.device != like.device or not t.is_contiguous():
-            raise ValueError(f"the store must be contiguous on {like.device}")
+        if t.dtype is not dtype:
+            raise TypeError(f"q is {dtype}, the store {t.dtype}: they must share a dtype")
+        if t.get_device() != dev or not t.is_contiguous():
+            raise ValueError(f"the store must be contiguous on device {dev}")
 
 
-def _strides3(*ts):
-    """Batch, head and token strides of each [B, H, T, 128] tensor; a dimension
-    of one entry is never stepped over."""
-    return (ctypes.c_int64 * (3 * len(ts)))(*[st if n > 1 else 0 for t in ts for n, st in zip(t.shape[:3], t.stride())])
+@functools.lru_cache(maxsize=256)
+def _strides3(*layouts):
+    """The batch, head and token strides of [B, H, T, 128] tensors given as
+    (shape, strides) pairs, for the C ABI; a dimension of one entry is never
+    stepped over.  Layouts are few: one array each."""
+    return (ctypes.c_int64 * (3 * len(layouts)))(*[s if n > 1 else 0 for shape, strides in layouts
+                                                   for n, s in zip(shape[:3], strides)])
 
 
-def _out_bthd(q, out):
+def _out_bthd(q, out, shape, dev):
     """The [B, T, Hq, 128] output of queries [B, Hq, T, 128], and its strides."""
-    B, Hq, T, D = q.shape
+    B, Hq, T, D = shape
     if out is None:
         out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
-    elif out.shape != (B, T, Hq, D) or out.dtype != q.dtype or out.device != q.device or not _unit(out):
+    elif (out.shape != (B, T, Hq, D) or out.dtype is not q.dtype or out.get_device() != dev
+          or (out.stride(3) != 1 and out.numel())):
         raise ValueError(f"out must be [{B}, {T}, {Hq}, {D}] of {q.dtype} on {q.device} with unit channel stride")
-    return out, (ctypes.c_int64 * 3)(out.stride(0), out.stride(2), out.stride(1))
+    b, t, h, _ = out.stride()
+    return out, _strides3(((2, 2, 2), (b, h, t)))
 
 
 @_on_device
@@ -874,50 +882,48 @@ def append_rotated(q, k, v, cos, sin, kstore, vstore, row_tile_off, row_len, row
     [B]; None: all T) from slot row_len on.  len_out (int32 [rows]) receives
     the new lengths: row_len itself, or another tensor.  A row without room is
     left as it is and sets bit 0 of status (int32 device word; read_status)."""
-    _heads("q", q)
-    _heads("k", k, like=q)
-    _heads("v", v, like=q)
-    B, Hq, T, _ = q.shape
-    Hkv = k.shape[1]
-    if v.shape[1] != Hkv or Hkv == 0 or Hq % Hkv:
-        raise ValueError(f"{Hq} query heads, {Hkv} key heads, {v.shape[1]} value heads")
-    tab = []
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t.dim() == 2:
-            t = t[None]
-        if t.dim() != 3 or t.shape[0] not in (1, B) or t.shape[1:] != (T, HEAD_DIM) or not _unit(t):
-            raise ValueError(f"{name} must be [{B} or 1, {T}, {HEAD_DIM}] with unit channel stride, got {tuple(t.shape)}")
-        if t.dtype not in (q.dtype, torch.float32) or t.device != q.device:
-            raise ValueError(f"{name} must be {q.dtype} or float32 on {q.device}")
-        tab.append(t)
-    cos, sin = tab
-    if cos.dtype != sin.dtype or cos.shape != sin.shape or (cos.stride() != sin.stride() and cos.numel()):
-        raise ValueError("cos and sin must share a dtype, shape and strides")
-    _stores(q, kstore, vstore)
-    rows, dev = B * Hkv, q.device
-    _meta(dev, ("row_tile_off", row_tile_off, torch.int64, rows), ("row_len", row_len, torch.int32, rows),
-          ("row_cap", row_cap, torch.int32, rows))
+    dt, dev = q.dtype, q.get_device()
+    qsh, ksh, vsh = _queries(q), _queries(k), _queries(v)
+    B, Hq, T, _ = qsh
+    Hkv = ksh[1]
+    if k.dtype is not dt or v.dtype is not dt:
+        raise TypeError(f"q is {dt}, k {k.dtype}, v {v.dtype}: they must share a dtype")
+    if ksh != vsh or ksh[0] != B or ksh[2] != T or Hkv == 0 or Hq % Hkv or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"q {tuple(qsh)} on {q.device}, k {tuple(ksh)} on {k.device}, v {tuple(vsh)} on {v.device}: one "
+                         "batch, one token count, one device, query heads a multiple of the KV heads")
+    csh, cst, ct = cos.shape, cos.stride(), cos.dtype
+    if (csh != sin.shape or csh[-2:] != (T, HEAD_DIM) or len(csh) > 3 or (len(csh) == 3 and csh[0] != 1 and csh[0] != B)
+            or ((cst != sin.stride() or cst[-1] != 1) and cos.numel()) or sin.dtype is not ct
+            or (ct is not dt and ct is not torch.float32) or cos.get_device() != dev or sin.get_device() != dev):
+        raise ValueError(f"cos {tuple(csh)} of {ct} and sin {tuple(sin.shape)} of {sin.dtype} must be [{B} or 1, {T}, "
+                         f"{HEAD_DIM}] of {dt} or float32 on {q.device}, with the same strides and unit channel stride")
+    _stores(dt, dev, kstore, vstore)
+    rows = B * Hkv
+    _meta(dev, "row_tile_off", row_tile_off, torch.int64, rows)
+    _meta(dev, "row_len", row_len, torch.int32, rows)
+    _meta(dev, "row_cap", row_cap, torch.int32, rows)
     if counts is not None:
-        _meta(dev, ("counts", counts, torch.int32, B))
+        _meta(dev, "counts", counts, torch.int32, B)
     if status is not None:
-        _meta(dev, ("status", status, torch.int32, 1))
+        _meta(dev, "status", status, torch.int32, 1)
+    len_at, new_at = row_len.data_ptr(), None
     if len_out is not None:
-        _meta(dev, ("len_out", len_out, torch.int32, rows))
-        if 0 < abs(len_out.data_ptr() - row_len.data_ptr()) < 4 * rows:
+        _meta(dev, "len_out", len_out, torch.int32, rows)
+        new_at = len_out.data_ptr()
+        if 0 < abs(new_at - len_at) < 4 * rows:
             raise ValueError("len_out overlaps row_len without being it")
     if out is None:
         out = torch.empty_like(q)
-        if not _unit(out):
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not _unit(out):
-        raise ValueError(f"out must be {tuple(q.shape)} of {q.dtype} on {dev} with unit channel stride")
-    st = _strides3(q, out, k, v)
-    base = ctypes.addressof(st)
+        if out.stride(3) != 1:
+            out = torch.empty(qsh, dtype=dt, device=q.device)
+    elif out.shape != qsh or out.dtype is not dt or out.get_device() != dev or (out.stride(3) != 1 and out.numel()):
+        raise ValueError(f"out must be {tuple(qsh)} of {dt} on {q.device} with unit channel stride")
+    base = ctypes.addressof(_strides3((qsh, q.stride()), (qsh, out.stride()), (ksh, k.stride()), (ksh, v.stride())))
     _lib.check(_lib.load().hc_append_rotated(
-        dtype_code(q.dtype), dtype_code(cos.dtype), q.data_ptr(), base, out.data_ptr(), base + 24, k.data_ptr(),
-        base + 48, v.data_ptr(), base + 72, cos.data_ptr(), sin.data_ptr(), cos.stride(0) if cos.shape[0] > 1 else 0,
-        cos.stride(1) if T > 1 else 0, kstore.data_ptr(), vstore.data_ptr(), row_tile_off.data_ptr(), row_len.data_ptr(),
-        row_cap.data_ptr(), _ptr(len_out), _ptr(counts), B, Hq, Hkv, T, _ptr(status), _stream(None, q)))
+        dtype_code(dt), dtype_code(ct), q.data_ptr(), base, out.data_ptr(), base + 24, k.data_ptr(), base + 48,
+        v.data_ptr(), base + 72, cos.data_ptr(), sin.data_ptr(), cst[0] if len(csh) == 3 and csh[0] > 1 else 0,
+        cst[-2] if T > 1 else 0, kstore.data_ptr(), vstore.data_ptr(), row_tile_off.data_ptr(), len_at,
+        row_cap.data_ptr(), new_at, _ptr(counts), B, Hq, Hkv, T, _ptr(status), torch._C._cuda_getCurrentRawStream(dev)))
     return out
 
 
@@ -931,27 +937,33 @@ def shared_attn(q, prefix, rows, kv_heads, scale, prefix_tiles=0, row_tiles=0, o
     sees the whole prefix and its row's tokens t < row_len - Q + 1 + i.
     prefix_tiles / row_tiles: tiles of all prefix rows, and of the longest own
     row, to cut the call for (sizes, not limits)."""
-    _heads("q", q)
-    B, Hq, Q, _ = q.shape
+    dt, dev = q.dtype, q.get_device()
+    shape = _queries(q)
+    B, Hq, Q, _ = shape
     if kv_heads < 1 or Hq % kv_heads:
         raise ValueError(f"{Hq} query heads are not a multiple of {kv_heads} KV heads")
-    ptrs = []
-    for name, part, n in (("prefix", prefix, kv_heads), ("rows", rows, B * kv_heads)):
-        if part is None:
-            ptrs.append((None,) * 4)
-            continue
-        ks, vs, off, length = part
-        _stores(q, ks, vs)
-        _meta(q.device, (name + " tile offsets", off, torch.int64, n), (name + " lengths", length, torch.int32, n))
-        ptrs.append((ks.data_ptr(), vs.data_ptr(), off.data_ptr(), length.data_ptr()))
-    out, o_st = _out_bthd(q, out)
+    p0 = p1 = p2 = p3 = r0 = r1 = r2 = r3 = None
+    if prefix is not None:
+        ks, vs, off, length = prefix
+        _stores(dt, dev, ks, vs)
+        _meta(dev, "prefix tile offsets", off, torch.int64, kv_heads)
+        _meta(dev, "prefix lengths", length, torch.int32, kv_heads)
+        p0, p1, p2, p3 = ks.data_ptr(), vs.data_ptr(), off.data_ptr(), length.data_ptr()
+    if rows is not None:
+        ks, vs, off, length = rows
+        n = B * kv_heads
+        _stores(dt, dev, ks, vs)
+        _meta(dev, "row tile offsets", off, torch.int64, n)
+        _meta(dev, "row lengths", length, torch.int32, n)
+        r0, r1, r2, r3 = ks.data_ptr(), vs.data_ptr(), off.data_ptr(), length.data_ptr()
+    out, o_st = _out_bthd(q, out, shape, dev)
     lib = _lib.load()
-    code = dtype_code(q.dtype)
-    ws = torch.empty(max(lib.hc_shared_workspace_size(code, B, Hq, kv_heads, Q, prefix_tiles, row_tiles), 16),
-                     dtype=torch.uint8, device=q.device)
-    _lib.check(lib.hc_shared_attn(code, q.data_ptr(), _strides3(q), *ptrs[0], prefix_tiles, *ptrs[1], row_tiles,
-                                  out.data_ptr(), o_st, B, Hq, kv_heads, Q, scale, ws.data_ptr(), ws.numel(),
-                                  _stream(None, q)))
+    code = dtype_code(dt)
+    nbytes = lib.hc_shared_workspace_size(code, B, Hq, kv_heads, Q, prefix_tiles, row_tiles)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _lib.check(lib.hc_shared_attn(code, q.data_ptr(), _strides3((shape, q.stride())), p0, p1, p2, p3, prefix_tiles, r0, r1,
+                                  r2, r3, row_tiles, out.data_ptr(), o_st, B, Hq, kv_heads, Q, scale, _ptr(ws), nbytes,
+                                  torch._C._cuda_getCurrentRawStream(dev)))
     return out
 
 
@@ -961,15 +973,25 @@ def block_bounds(kstore, row_tile_off, row_len, row_block_off, block, bounds, ex
     with fresh > 0 only of those that its last `fresh` tokens completed
     (hc_block_bounds in include/hc.h).  bounds: int8 [blocks, 2, 128]; exps:
     int8 [blocks]; row_block_off: int64 [rows], each row's first block."""
-    n = row_len.numel()
-    _meta(kstore.device, ("row_tile_off", row_tile_off, torch.int64, n), ("row_len", row_len, torch.int32, n),
-          ("row_block_off", row_block_off, torch.int64, n), ("exps", exps, torch.int8, exps.numel()),
-          ("bounds", bounds, torch.int8, exps.numel() * 2 * HEAD_DIM))
+    dev, n, nb = kstore.get_device(), row_len.numel(), exps.numel()
+    _meta(dev, "row_tile_off", row_tile_off, torch.int64, n)
+    _meta(dev, "row_len", row_len, torch.int32, n)
+    _meta(dev, "row_block_off", row_block_off, torch.int64, n)
+    _meta(dev, "exps", exps, torch.int8, nb)
+    _meta(dev, "bounds", bounds, torch.int8, nb * 2 * HEAD_DIM)
     if not kstore.is_contiguous():
         raise ValueError("the store must be contiguous")
     _lib.check(_lib.load().hc_block_bounds(dtype_code(kstore.dtype), kstore.data_ptr(), row_tile_off.data_ptr(),
                                            row_len.data_ptr(), row_block_off.data_ptr(), n, block, span, fresh,
-                                           bounds.data_ptr(), exps.data_ptr(), _stream(None, kstore)))
+                                           bounds.data_ptr(), exps.data_ptr(), torch._C._cuda_getCurrentRawStream(dev)))
+
+
+def _block_rows(q, row_len):
+    shape = _queries(q)
+    rows, B = row_len.numel(), shape[0]
+    if B == 0 or rows % B or rows == 0 or shape[1] % (rows // B):
+        raise ValueError(f"{rows} rows for queries {tuple(shape)}")
+    return shape, rows, rows // B
 
 
 @_on_device
@@ -978,23 +1000,23 @@ def block_select(q, bounds, exps, row_block_off, row_len, block, max_blocks, kee
     [rows, Q, keep], ascending and -1 past the count, counts int32 [rows, Q])
     (hc_block_select in include/hc.h).  max_blocks: at least the blocks of the
     longest row (a capacity will do)."""
-    _heads("q", q)
-    B, Hq, Q, _ = q.shape
-    rows = row_len.numel()
-    if B == 0 or rows % B or rows == 0 or Hq % (rows // B):
-        raise ValueError(f"{rows} rows for queries {tuple(q.shape)}")
-    _meta(q.device, ("row_len", row_len, torch.int32, rows), ("row_block_off", row_block_off, torch.int64, rows),
-          ("exps", exps, torch.int8, exps.numel()), ("bounds", bounds, torch.int8, exps.numel() * 2 * HEAD_DIM))
+    dev, nb = q.get_device(), exps.numel()
+    shape, rows, Hkv = _block_rows(q, row_len)
+    B, Hq, Q, _ = shape
+    _meta(dev, "row_len", row_len, torch.int32, rows)
+    _meta(dev, "row_block_off", row_block_off, torch.int64, rows)
+    _meta(dev, "exps", exps, torch.int8, nb)
+    _meta(dev, "bounds", bounds, torch.int8, nb * 2 * HEAD_DIM)
     lib = _lib.load()
-    Hkv = rows // B
-    idx = torch.empty((rows, Q, max(keep, 0)), dtype=torch.int32, device=q.device)
-    counts = torch.empty((rows, Q), dtype=torch.int32, device=q.device)
-    scratch = torch.empty(max(lib.hc_block_select_scratch_size(B, Hkv, Q, max_blocks), 16), dtype=torch.uint8,
-                          device=q.device)
-    _lib.check(lib.hc_block_select(dtype_code(q.dtype), q.data_ptr(), _strides3(q), bounds.data_ptr(), exps.data_ptr(),
-                                   row_block_off.data_ptr(), row_len.data_ptr(), B, Hq, Hkv, Q, block, max_blocks, keep,
-                                   sink, local, idx.data_ptr(), counts.data_ptr(), scratch.data_ptr(), scratch.numel(),
-                                   _stream(None, q)))
+    device = q.device
+    idx = torch.empty((rows, Q, max(keep, 0)), dtype=torch.int32, device=device)
+    counts = torch.empty((rows, Q), dtype=torch.int32, device=device)
+    nbytes = lib.hc_block_select_scratch_size(B, Hkv, Q, max_blocks)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _lib.check(lib.hc_block_select(dtype_code(q.dtype), q.data_ptr(), _strides3((shape, q.stride())), bounds.data_ptr(),
+                                   exps.data_ptr(), row_block_off.data_ptr(), row_len.data_ptr(), B, Hq, Hkv, Q, block,
+                                   max_blocks, keep, sink, local, idx.data_ptr(), counts.data_ptr(), _ptr(scratch), nbytes,
+                                   torch._C._cuda_getCurrentRawStream(dev)))
     return idx, counts
 
 
@@ -1003,24 +1025,23 @@ def block_attn(q, kstore, vstore, row_tile_off, row_len, idx, counts, block, sca
     """Attention of queries [B, Hq, Q, 128] over the visible tokens of their
     kept blocks idx[row, i, :counts[row, i]]; [B, Q, Hq, 128] (hc_block_attn in
     include/hc.h)."""
-    _heads("q", q)
-    B, Hq, Q, _ = q.shape
-    rows = row_len.numel()
-    if B == 0 or rows % B or rows == 0 or Hq % (rows // B):
-        raise ValueError(f"{rows} rows for queries {tuple(q.shape)}")
-    _stores(q, kstore, vstore)
-    if idx.dim() != 3:
-        raise ValueError(f"idx must be [{rows}, {Q}, keep], got {tuple(idx.shape)}")
-    keep = idx.shape[2]
-    _meta(q.device, ("row_tile_off", row_tile_off, torch.int64, rows), ("row_len", row_len, torch.int32, rows),
-          ("idx", idx, torch.int32, rows * Q * keep), ("counts", counts, torch.int32, rows * Q))
-    out, o_st = _out_bthd(q, out)
+    dt, dev = q.dtype, q.get_device()
+    shape, rows, Hkv = _block_rows(q, row_len)
+    B, Hq, Q, _ = shape
+    _stores(dt, dev, kstore, vstore)
+    keep = idx.shape[2] if idx.dim() == 3 else 0
+    _meta(dev, "row_tile_off", row_tile_off, torch.int64, rows)
+    _meta(dev, "row_len", row_len, torch.int32, rows)
+    _meta(dev, "counts", counts, torch.int32, rows * Q)
+    if idx.shape != (rows, Q, keep) or not _is(idx, torch.int32, rows * Q * keep, dev):
+        raise ValueError(f"idx must be a contiguous int32 [{rows}, {Q}, keep] on device {dev}, got {tuple(idx.shape)} of "
+                         f"{idx.dtype} on {idx.device}")
+    out, o_st = _out_bthd(q, out, shape, dev)
     lib = _lib.load()
-    Hkv = rows // B
     nbytes = lib.hc_block_attn_workspace_size(B, Hq, Hkv, Q, block, keep)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _lib.check(lib.hc_block_attn(dtype_code(q.dtype), q.data_ptr(), _strides3(q), kstore.data_ptr(), vstore.data_ptr(),
-                                 row_tile_off.data_ptr(), row_len.data_ptr(), idx.data_ptr(), counts.data_ptr(), keep,
-                                 block, out.data_ptr(), o_st, B, Hq, Hkv, Q, scale, _ptr(ws), nbytes,
-                                 _stream(None, q)))
+    _lib.check(lib.hc_block_attn(dtype_code(dt), q.data_ptr(), _strides3((shape, q.stride())), kstore.data_ptr(),
+                                 vstore.data_ptr(), row_tile_off.data_ptr(), row_len.data_ptr(), idx.data_ptr(),
+                                 counts.data_ptr(), keep, block, out.data_ptr(), o_st, B, Hq, Hkv, Q, scale, _ptr(ws),
+                                 nbytes, torch._C._cuda_getCurrentRawStream(dev)))
     return out

@@ -83,8 +83,8 @@ def test_shared_attn(lib):
 
 def test_shared_workspace_is_bounded(lib):
     """Partials grow with the work of one round of workgroups, not with the prefix."""
-    a, b = (lib.hc_shared_workspace_size(2, 32, 32, 8, 1, t, 16) for t in (1 << 12, 1 << 22))
-    assert 0 < a == b < 200 << 20
+    for tiles in (1 << 12, 1 << 16, 1 << 22):
+        assert 0 < lib.hc_shared_workspace_size(2, 32, 32, 8, 1, tiles, 16) < 100 << 20
 
 
 def test_block_bounds(lib):
@@ -102,7 +102,7 @@ def test_block_bounds(lib):
 
 
 def test_block_select(lib):
-    def call(dtype=2, q=FAKE, qs=_s(1024, 128, 1024), b=1, hq=8, hkv=2, n=1, block=32, mb=100, keep=8, sink=1, local=2,
+    def call(dtype=2, q=FAKE, qs=_s(1024, 128, 1024), b=1, hq=8, hkv=2, n=1, block=32, mb=20000, keep=8, sink=1, local=2,
              idx=FAKE, scratch=FAKE, sb=None):
         sb = lib.hc_block_select_scratch_size(b, hkv, n, mb) - 1 if sb is None else sb
         return lib.hc_block_select(dtype, q, qs, FAKE, FAKE, FAKE, FAKE, b, hq, hkv, n, block, mb, keep, sink, local, idx,
@@ -120,11 +120,11 @@ def test_block_select(lib):
 
 
 def test_block_attn(lib):
-    def call(dtype=2, q=FAKE, qs=_s(1024, 128, 1024), ks=FAKE, idx=FAKE, keep=8, block=32, b=1, hq=8, hkv=2, n=1,
+    def call(dtype=2, q=FAKE, qs=_s(1024, 128, 1024), ks=FAKE, idx=FAKE, keep=4096, block=32, b=1, hq=8, hkv=2, n=1,
              scale=0.1, ws=FAKE, wb=0):
         return lib.hc_block_attn(dtype, q, qs, ks, FAKE, FAKE, FAKE, idx, FAKE, keep, block, FAKE, _s(1024, 128, 1024), b,
                                  hq, hkv, n, scale, ws, wb, None)
-    assert lib.hc_block_attn_workspace_size(1, 8, 2, 1, 32, 8) > 0
+    assert lib.hc_block_attn_workspace_size(1, 8, 2, 1, 32, 4096) > 0  # the kept blocks are split
     _refused(lib, call(), b"workspace too small")
     _refused(lib, call(hq=34), b"at most 16")
     _refused(lib, call(keep=0), b"keep=0")
