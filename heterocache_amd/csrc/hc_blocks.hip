@@ -210,30 +210,41 @@ __device__ __forceinline__ void select_range(const SelectArgs& a, SelectJob& j) 
 // (lane: head l % 16, 16 bytes of the 256 a block has, steps 0 and 1 the
 // positive parts against the maxima, 2 and 3 the negative ones against the
 // minima), 16 blocks the B operand.
+template <typename T>
+struct RawQuery {
+  typename Elem<T>::vec8 v[2][2];
+};
 struct ScoreQuery {
   i32x4 op[4];
-  float unit[4];  // powers of two of heads 4g .. 4g + 3; 0 heads are told apart by G
+  float unit[4];  // powers of two of heads 4g .. 4g + 3
 };
+// The loads and the rounding apart: the blocks' loads go out in between.
 template <typename T>
-__device__ __forceinline__ ScoreQuery score_query(const SelectArgs& a, const SelectJob& j, int lane) {
+__device__ __forceinline__ RawQuery<T> load_query(const SelectArgs& a, const SelectJob& j, int lane) {
   const int g = lane >> 4, n = lane & 15;
   const int b = j.row / a.Hkv, kv = j.row % a.Hkv;
-  const bool ok = n < a.G;
-  const T* p = reinterpret_cast<const T*>(a.q) + b * a.q_s[0] + (int64_t)(kv * a.G + (ok ? n : 0)) * a.q_s[1] +
+  const T* p = reinterpret_cast<const T*>(a.q) + b * a.q_s[0] + (int64_t)(kv * a.G + (n < a.G ? n : 0)) * a.q_s[1] +
                (int64_t)j.i * a.q_s[2] + 16 * g;
+  RawQuery<T> r;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) r.v[s][u] = load8<T>(p + 64 * s + 8 * u);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ ScoreQuery score_query(const SelectArgs& a, const RawQuery<T>& raw, int lane) {
+  const int g = lane >> 4;
+  const bool ok = (lane & 15) < a.G;
   float x[2][16];
   float top = 0.f;
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const typename Elem<T>::vec8 v = load8<T>(p + 64 * s + 8 * u);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = ok ? vec8_at<T>(v, e) : 0.f;
-        x[s][8 * u + e] = y;
-        top = fmaxf(top, fabsf(y));
-      }
+    for (int e = 0; e < 16; ++e) {
+      const float y = ok ? vec8_at<T>(raw.v[s][e >> 3], e & 7) : 0.f;
+      x[s][e] = y;
+      top = fmaxf(top, fabsf(y));
     }
   const int ex = least_exp(rows4_max(top));
   const float down = power2(-ex), up = power2(ex);
@@ -257,36 +268,43 @@ __device__ __forceinline__ ScoreQuery score_query(const SelectArgs& a, const Sel
   return r;
 }
 
-// Scores of U * 16 blocks from blk0 on: f(u, score) with lane l's block u * 16 +
-// l % 16 (all four lanes of it hold it).  last: the last block that may be
-// read; those past it read it again.  The 4 U loads of 1 KB are in flight
-// together.
-template <int U, typename F>
-__device__ __forceinline__ void score_blocks(const SelectArgs& a, const ScoreQuery& q, int64_t blk0, int64_t last,
-                                             int lane, F f) {
-  const int g = lane >> 4, n = lane & 15;
+// Bounds of U * 16 blocks from blk0 on, 4 U loads of 1 KB in flight together;
+// blocks past `last` read it again.
+template <int U>
+struct ScoreBlocks {
   i32x4 x[U][4];
-  float unit[U];
+  int e[U];
+};
+template <int U>
+__device__ __forceinline__ void load_blocks(const SelectArgs& a, int64_t blk0, int64_t last, int lane, ScoreBlocks<U>& t) {
+  const int g = lane >> 4, n = lane & 15;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t blk = min(blk0 + 16 * u + n, last);
 #pragma unroll
     for (int s = 0; s < 4; ++s)
-      x[u][s] = *reinterpret_cast<const i32x4*>(a.bounds + blk * kBoundBytes + 64 * s + 16 * g);
-    unit[u] = power2(a.exps[blk]);
+      t.x[u][s] = *reinterpret_cast<const i32x4*>(a.bounds + blk * kBoundBytes + 64 * s + 16 * g);
+    t.e[u] = a.exps[blk];
   }
+}
+// Their scores: f(u, score) with lane l's block 16 u + l % 16 (all four lanes of
+// a block hold its score).
+template <int U, typename F>
+__device__ __forceinline__ void score_blocks(const SelectArgs& a, const ScoreQuery& q, const ScoreBlocks<U>& t, int lane,
+                                             F f) {
+  const int g = lane >> 4;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-    for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.op[s], x[u][s], acc, 0, 0, 0);
+    for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.op[s], t.x[u][s], acc, 0, 0, 0);
     // Lane: heads 4g + r of block n.  Whole numbers below 2^24 and powers of
     // two: every step is exact.
     float best = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (4 * g + r < a.G) best = fmaxf(best, (float)acc[r] * q.unit[r]);
-    f(u, rows4_max(best) * unit[u]);
+    f(u, rows4_max(best) * power2(t.e[u]));
   }
 }
 
@@ -299,120 +317,151 @@ __global__ __launch_bounds__(kScoreWaves * 64) void block_score_kernel(const Sel
   const int jobs = (a.rows + 7) / 8 * 8 * a.Q;
   SelectJob j;
   if (!select_job(a, blockIdx.x % jobs, j)) return;
-  const ScoreQuery q = score_query<T>(a, j, lane);
+  const RawQuery<T> raw = load_query<T>(a, j, lane);
+  const int64_t base = a.row_blk_off[j.row];
   const int chunk = blockIdx.x / jobs;
   select_range(a, j);
   const int steps = (j.hi - j.lo + 31) / 32;
-  if (steps <= chunk * kScoreWaves) return;
-  const int64_t base = a.row_blk_off[j.row];
+  int st = chunk * kScoreWaves + wave;
+  if (st >= steps) return;
+  ScoreBlocks<2> t;
+  load_blocks<2>(a, base + j.lo + 32 * st, base + j.hi - 1, lane, t);
+  const ScoreQuery q = score_query<T>(a, raw, lane);
   float* out = a.scores + ((int64_t)j.row * a.Q + j.i) * a.pitch;
-  for (int st = chunk * kScoreWaves + wave; st < steps; st += kScoreWaves * a.chunks) {
+  while (true) {
     const int j0 = j.lo + 32 * st;
-    score_blocks<2>(a, q, base + j0, base + j.hi - 1, lane, [&](int u, float s) {
+    score_blocks<2>(a, q, t, lane, [&](int u, float s) {
       const int blk = j0 + 16 * u + (lane & 15);
       if (lane < 16 && blk < j.hi) out[blk] = s;
     });
+    st += kScoreWaves * a.chunks;
+    if (st >= steps) return;
+    load_blocks<2>(a, base + j.lo + 32 * st, base + j.hi - 1, lane, t);
   }
 }
 
-// One workgroup a query: the scores' keys (from score_blocks itself where
-// SCORED is not set, else from memory) in LDS, the threshold, and one ordered
-// pass that writes the kept blocks.  The threshold is found by counting the
-// keys into 1024 equal steps between the least and the greatest left and going
-// on in the step where the count of kept ones is reached: scores of one query
-// lie within a few powers of two, where fixed digits of the key would pile up
-// in few counters.  Bound by the latency of its dependent steps; a barrier
-// each for scores, range, counts (one or two rounds) and places.
+// The selection of one query by a workgroup of NT threads: the scores' keys (of
+// score_blocks itself where SCORED is not set, else from memory) in LDS, the
+// threshold, and one ordered pass that writes the kept blocks.  The threshold
+// is found by counting the keys into equal steps between the least and the
+// greatest left and going on in the step where the count of kept ones is
+// reached: scores of one query lie within a few powers of two, where fixed
+// digits of the key would pile up in few counters.  Bound by the latency of
+// its dependent steps; a barrier each for the keys, the counts (one or two
+// rounds) and the places.  128 blocks take 1 us of loads, 2 of scores and 2 of
+// selection; 4096 scored ones 2 and 6.
 constexpr int kPickKeys = 12288;  // keys in LDS; a longer row's are read again from memory each time
-constexpr int kPickBins = 1024;
-// Counters are read 16 in a row by each lane: one of padding after each 16
-// keeps the lanes on different banks.
-constexpr int kPickPad = kPickBins / 16 * 17;
-__device__ __forceinline__ int pick_slot(uint32_t bin) { return (int)(bin + (bin >> 4)); }
+template <int NT>
+struct Pick {
+  static constexpr int kWaves = NT / 64;
+  static constexpr int kPer = NT == 1024 ? 16 : 4;  // counters that a lane reads in a row
+  static constexpr int kBins = 64 * kPer;
+  // One of padding after each row of them keeps the lanes on different banks.
+  static constexpr int kSlots = 64 * (kPer + 1);
+  static __device__ __forceinline__ int slot(uint32_t bin) { return (int)(bin + bin / kPer); }
+  int hist[2][kSlots];
+  uint32_t lo[kWaves], hi[kWaves];
+  int gt[kWaves], eq[kWaves];
+};
+
+// Writes the query's counts and list to memory and, where list is not null, to
+// LDS as well (a.keep entries; visible behind the next barrier); returns the
+// count.  s_key: min(a.max_blocks, kPickKeys) words of LDS.
 template <typename T, bool SCORED, int NT>
-__global__ __launch_bounds__(NT) void block_pick_kernel(const SelectArgs a) {
-  constexpr int kWaves = NT / 64;
-  extern __shared__ uint32_t s_key[];
-  __shared__ int s_hist[2][kPickPad];
-  __shared__ uint32_t s_lo[kWaves], s_hi[kWaves];
-  __shared__ int s_gt[kWaves], s_eq[kWaves];
+__device__ __forceinline__ int pick_blocks(const SelectArgs& a, SelectJob& j, Pick<NT>& L, uint32_t* s_key,
+                                           int32_t* list) {
+  typedef Pick<NT> P;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  SelectJob j;
-  if (!select_job(a, blockIdx.x, j)) return;
-  ScoreQuery q;
-  if constexpr (!SCORED) q = score_query<T>(a, j, lane);
+  RawQuery<T> raw;
+  int64_t base = 0;
+  if constexpr (!SCORED) {
+    raw = load_query<T>(a, j, lane);
+    base = a.row_blk_off[j.row] + a.sink;
+  }
   select_range(a, j);
   const int64_t x = (int64_t)j.row * a.Q + j.i;
-  int32_t* out = a.idx + x * a.keep;
+  int32_t* const out = a.idx + x * a.keep;
+  auto put = [&](int at, int blk) {
+    out[at] = blk;
+    if (list) list[at] = blk;
+  };
   const bool fits = j.have <= a.max_blocks;
-  if (tid == 0) a.counts[x] = fits ? min(j.have, a.keep) : -1;
+  const int kept = fits ? min(j.have, a.keep) : -1;
+  if (tid == 0) a.counts[x] = kept;
   if (!fits || j.have <= a.keep) {
-    for (int k = tid; k < a.keep; k += NT) out[k] = fits && k < j.have ? k : -1;
-    return;
+    for (int k = tid; k < a.keep; k += NT) put(k, k < kept ? k : -1);
+    return kept;
   }
   const int lo = j.lo, nmid = j.hi - lo;
   int need = a.keep - a.sink - a.local;  // < nmid
-  for (int k = tid; k < a.sink; k += NT) out[k] = k;
-  for (int k = tid; k < a.local; k += NT) out[a.keep - a.local + k] = j.have - a.local + k;
-  if (need == 0) return;
-  for (int k = tid; k < 2 * kPickPad; k += NT) s_hist[0][k] = 0;
+  for (int k = tid; k < a.sink; k += NT) put(k, k);
+  for (int k = tid; k < a.local; k += NT) put(a.keep - a.local + k, j.have - a.local + k);
+  if (need == 0) return kept;
+  for (int k = tid; k < 2 * P::kSlots; k += NT) L.hist[0][k] = 0;
   const float* sc = SCORED ? a.scores + x * a.pitch + lo : nullptr;
   const bool in_lds = !SCORED || nmid <= kPickKeys;
-  if constexpr (SCORED) {
-    if (in_lds)
-      for (int k = tid; k < nmid; k += NT) s_key[k] = order_key(sc[k]);
-  } else {
-    const int64_t base = a.row_blk_off[j.row] + lo;
-    for (int k0 = 64 * wave; k0 < nmid; k0 += 64 * kWaves)
-      score_blocks<4>(a, q, base + k0, base + nmid - 1, lane, [&](int u, float s) {
-        const int k = k0 + 16 * u + (lane & 15);
-        if (lane < 16 && k < nmid) s_key[k] = order_key(s);
-      });
-  }
-  __syncthreads();
-  auto key = [&](int k) { return in_lds ? s_key[k] : order_key(sc[k]); };
-
-  // Every thread keeps to a run of blocks.
-  const int run = (nmid + NT - 1) / NT;
-  const int k0 = min(tid * run, nmid), k1 = min(k0 + run, nmid);
   uint32_t least = 0xffffffffu, most = 0u;
-  for (int k = k0; k < k1; ++k) {
-    const uint32_t u = key(k);
-    least = min(least, u);
-    most = max(most, u);
+  if constexpr (SCORED) {
+    for (int k = tid; k < nmid; k += NT) {
+      const uint32_t u = order_key(sc[k]);
+      if (in_lds) s_key[k] = u;
+      least = min(least, u);
+      most = max(most, u);
+    }
+  } else if (64 * wave < nmid) {
+    ScoreBlocks<4> t;
+    load_blocks<4>(a, base + 64 * wave, base + nmid - 1, lane, t);
+    const ScoreQuery q = score_query<T>(a, raw, lane);
+    for (int k0 = 64 * wave;;) {
+      score_blocks<4>(a, q, t, lane, [&](int u, float s) {
+        const int k = k0 + 16 * u + (lane & 15);
+        const uint32_t key = order_key(s);
+        if (lane < 16 && k < nmid) s_key[k] = key;
+        least = min(least, key);  // (a block past the end is the last one again)
+        most = max(most, key);
+      });
+      k0 += 64 * P::kWaves;
+      if (k0 >= nmid) break;
+      load_blocks<4>(a, base + k0, base + nmid - 1, lane, t);
+    }
   }
   least = wave_fold(least, [](uint32_t u, uint32_t v) { return min(u, v); });
   most = wave_fold(most, [](uint32_t u, uint32_t v) { return max(u, v); });
-  if (lane == 0) s_lo[wave] = least, s_hi[wave] = most;
+  if (lane == 0) L.lo[wave] = least, L.hi[wave] = most;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    least = min(least, s_lo[w]);
-    most = max(most, s_hi[w]);
+  for (int w = 0; w < P::kWaves; ++w) {
+    least = min(least, L.lo[w]);
+    most = max(most, L.hi[w]);
   }
+  auto key = [&](int k) { return in_lds ? s_key[k] : order_key(sc[k]); };
+  // Every thread keeps to a run of blocks.
+  const int run = (nmid + NT - 1) / NT;
+  const int k0 = min(tid * run, nmid), k1 = min(k0 + run, nmid);
 
-  // Kept: the keys above T, and the first `need` equal to it.
+  // Kept: the keys above T0, and the first `need` equal to it.
   uint32_t T0 = least;
   for (int round = 0; least < most; ++round) {
     const uint32_t span = most - least;
-    const int shift = max(32 - __clz((int)span) - 10, 0);
-    int* hist = s_hist[round & 1];
+    const int shift = max(32 - __clz((int)span) - (NT == 1024 ? 10 : 8), 0);
+    int* hist = L.hist[round & 1];
     for (int k = k0; k < k1; ++k) {
       const uint32_t u = key(k);
-      if (u >= least && u <= most) atomicAdd(&hist[pick_slot((u - least) >> shift)], 1);
+      if (u >= least && u <= most) atomicAdd(&hist[P::slot((u - least) >> shift)], 1);
     }
     __syncthreads();
-    // Lane y: bins 1023 - 16 y .. 1008 - 16 y; keys above its first one, then
-    // the bin in which the need-th highest key lies (every wave for itself).
-    int c[16], sum = 0;
+    // Lane y reads kPer bins in a row from the top down; keys above its first
+    // one, then the bin in which the need-th highest key lies (every wave for
+    // itself).
+    int c[P::kPer], sum = 0;
 #pragma unroll
-    for (int u = 0; u < 16; ++u) sum += c[u] = hist[kPickPad - 2 - 17 * lane - u];
+    for (int u = 0; u < P::kPer; ++u) sum += c[u] = hist[P::kSlots - 2 - (P::kPer + 1) * lane - u];
     const int incl = wave_scan_add(sum);
     int above = incl - sum, bin = 0, in_bin = 0, before = 0;
     const bool mine = above < need && need <= incl;
 #pragma unroll
-    for (int u = 0; u < 16; ++u) {
-      if (above < need && need <= above + c[u]) bin = kPickBins - 1 - 16 * lane - u, in_bin = c[u], before = above;
+    for (int u = 0; u < P::kPer; ++u) {
+      if (above < need && need <= above + c[u]) bin = P::kBins - 1 - P::kPer * lane - u, in_bin = c[u], before = above;
       above += c[u];
     }
     const int src = __builtin_ctzll(__ballot(mine));
@@ -427,11 +476,11 @@ __global__ __launch_bounds__(NT) void block_pick_kernel(const SelectArgs a) {
       need = 0;
       break;
     }
-    // The counts of the round after next: zeroed behind the next barrier's
-    // reads of the other ones.
-    int* other = s_hist[(round + 1) & 1];
+    // The counts of the round after next: their last readers are behind this
+    // round's barrier, their next writers behind the one here.
+    int* other = L.hist[(round + 1) & 1];
     if (round > 0) {
-      for (int k = tid; k < kPickPad; k += NT) other[k] = 0;
+      for (int k = tid; k < P::kSlots; k += NT) other[k] = 0;
       __syncthreads();
     }
   }
@@ -443,21 +492,45 @@ __global__ __launch_bounds__(NT) void block_pick_kernel(const SelectArgs a) {
     eq += u == T0;
   }
   const int gt_in = wave_scan_add(gt), eq_in = wave_scan_add(eq);
-  if (lane == 63) s_gt[wave] = gt_in, s_eq[wave] = eq_in;
+  if (lane == 63) L.gt[wave] = gt_in, L.eq[wave] = eq_in;
   __syncthreads();
   int gt0 = gt_in - gt, eq0 = eq_in - eq;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w)
-    if (w < wave) gt0 += s_gt[w], eq0 += s_eq[w];
+  for (int w = 0; w < P::kWaves; ++w)
+    if (w < wave) gt0 += L.gt[w], eq0 += L.eq[w];
   int at = a.sink + gt0 + min(eq0, need);
   int left = max(need - eq0, 0);
   for (int k = k0; k < k1; ++k) {
     const uint32_t u = key(k);
     if (u > T0 || (u == T0 && left > 0)) {
       left -= u == T0;
-      out[at++] = lo + k;
+      put(at++, lo + k);
     }
   }
+  return kept;
+}
+
+template <typename T, bool SCORED, int NT>
+__global__ __launch_bounds__(NT) void block_pick_kernel(const SelectArgs a) {
+  extern __shared__ uint32_t s_key[];
+  __shared__ Pick<NT> pick;
+  SelectJob j;
+  if (select_job(a, blockIdx.x, j)) pick_blocks<T, SCORED, NT>(a, j, pick, s_key, nullptr);
+}
+
+// Selection and attention of one query in one workgroup of eight waves, for
+// few queries over short rows, where launches count: the list stays in LDS.
+template <typename T>
+__global__ __launch_bounds__(512, 1) void block_step_kernel(const SelectArgs a, const RowsArgs r) {
+  extern __shared__ uint32_t s_key[];  // a.max_blocks keys, then the list
+  __shared__ __attribute__((aligned(16))) float s_rows[kRowsLds];
+  __shared__ Pick<512> pick;
+  SelectJob j;
+  if (!select_job(a, blockIdx.x, j)) return;
+  int32_t* list = reinterpret_cast<int32_t*>(s_key + a.max_blocks);
+  const int kept = pick_blocks<T, false, 512>(a, j, pick, s_key, list);
+  __syncthreads();
+  rows_job<T, kRowsListed, false, 8>(r, blockIdx.x, s_rows, list, kept);
 }
 
 bool known(int dtype) { return dtype == HC_DTYPE_BF16 || dtype == HC_DTYPE_F16 || dtype == HC_DTYPE_F32; }
@@ -549,61 +622,79 @@ extern "C" size_t hc_block_select_scratch_size(int batch, int kv_heads, int quer
   return (size_t)rows * queries * score_pitch(max_blocks) * sizeof(float);
 }
 
-extern "C" int hc_block_select(int dtype, const void* q, const int64_t* q_strides, const int8_t* bounds,
-                               const int8_t* exps, const int64_t* row_block_off, const int32_t* row_len, int batch,
-                               int q_heads, int kv_heads, int queries, int block, int max_blocks, int keep, int sink,
-                               int local, int32_t* idx, int32_t* counts, void* scratch, size_t scratch_bytes,
-                               void* stream) {
-  clear_error();
-  int rc = check_shape("hc_block_select", dtype, batch, q_heads, kv_heads, queries, block);
+namespace {
+// The checks and arguments of a selection.
+int select_args(const char* what, int dtype, const void* q, const int64_t* q_strides, const int8_t* bounds,
+                const int8_t* exps, const int64_t* row_block_off, const int32_t* row_len, int batch, int q_heads,
+                int kv_heads, int queries, int block, int max_blocks, int keep, int sink, int local, int32_t* idx,
+                int32_t* counts, SelectArgs& a) {
+  int rc = check_shape(what, dtype, batch, q_heads, kv_heads, queries, block);
   if (rc) return rc;
   if (sink < 0 || local < 1 || keep < 1 || keep > (1 << 24) || (int64_t)sink + local > keep || max_blocks < 0)
     return set_error(HC_ERR_INVALID,
-                     "hc_block_select: keep=%d sink=%d local=%d max_blocks=%d (local at least 1, sink + local at most "
-                     "keep)",
+                     "%s: keep=%d sink=%d local=%d max_blocks=%d (local at least 1, sink + local at most keep)", what,
                      keep, sink, local, max_blocks);
   if (batch == 0 || queries == 0) return HC_OK;
   if (!q || !q_strides || !bounds || !exps || !row_block_off || !row_len || !idx || !counts)
-    return set_error(HC_ERR_INVALID, "hc_block_select: null pointer argument");
-  if ((rc = check_q("hc_block_select", dtype, q, q_strides))) return rc;
+    return set_error(HC_ERR_INVALID, "%s: null pointer argument", what);
+  if ((rc = check_q(what, dtype, q, q_strides))) return rc;
   if (reinterpret_cast<uintptr_t>(bounds) & 15)
-    return set_error(HC_ERR_INVALID, "hc_block_select: the bounds must be 16-byte aligned");
-  const size_t need = hc_block_select_scratch_size(batch, kv_heads, queries, max_blocks);
-  if (need > 0 && (!scratch || scratch_bytes < need))
-    return set_error(HC_ERR_INVALID, "hc_block_select: scratch too small (%zu < %zu bytes)", scratch_bytes, need);
-  SelectArgs a;
+    return set_error(HC_ERR_INVALID, "%s: the bounds must be 16-byte aligned", what);
+  a = SelectArgs{};
   a.q = q, a.bounds = bounds, a.exps = exps, a.row_blk_off = row_block_off, a.row_len = row_len;
   for (int i = 0; i < 3; ++i) a.q_s[i] = q_strides[i];
-  a.scores = reinterpret_cast<float*>(scratch), a.pitch = score_pitch(max_blocks), a.idx = idx, a.counts = counts;
+  a.pitch = score_pitch(max_blocks), a.idx = idx, a.counts = counts;
   a.Hkv = kv_heads, a.G = q_heads / kv_heads, a.Q = queries, a.rows = batch * kv_heads, a.S = block;
   a.keep = keep, a.sink = sink, a.local = local, a.max_blocks = max_blocks;
-  const int64_t jobs = ((int64_t)a.rows + 7) / 8 * 8 * queries;
-  if (jobs > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_block_select: %lld queries", (long long)jobs);
-  hipStream_t s = (hipStream_t)stream;
+  return HC_OK;
+}
+
+int launch_select(const char* what, int dtype, SelectArgs& a, void* scratch, hipStream_t s) {
+  const int64_t jobs = ((int64_t)a.rows + 7) / 8 * 8 * a.Q;
+  if (jobs > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "%s: %lld queries", what, (long long)jobs);
   const dim3 grid((unsigned)jobs);
-  if (!select_in_memory(jobs, max_blocks)) {
+  if (!select_in_memory(jobs, a.max_blocks)) {
     switch (dtype) {
       case HC_DTYPE_BF16: launch_pick<__bf16, false>(a, grid, s); break;
       case HC_DTYPE_F16: launch_pick<_Float16, false>(a, grid, s); break;
       default: launch_pick<float, false>(a, grid, s); break;
     }
-    return check_launch("hc_block_select");
+    return check_launch(what);
   }
-  const int64_t most = (max_blocks + 32 * kScoreWaves - 1) / (32 * kScoreWaves);
+  a.scores = reinterpret_cast<float*>(scratch);
+  const int64_t most = (a.max_blocks + 32 * kScoreWaves - 1) / (32 * kScoreWaves);
   a.chunks = (int)std::max<int64_t>(std::min<int64_t>((8 * device_cus() + jobs - 1) / jobs, most), 1);
   if (jobs * a.chunks > 0x7fffffffLL)
-    return set_error(HC_ERR_INVALID, "hc_block_select: %lld workgroups", (long long)(jobs * a.chunks));
-  if (max_blocks > keep) {
+    return set_error(HC_ERR_INVALID, "%s: %lld workgroups", what, (long long)(jobs * a.chunks));
+  if (a.max_blocks > a.keep) {
     const dim3 g((unsigned)(jobs * a.chunks)), t(kScoreWaves * 64);
     switch (dtype) {
       case HC_DTYPE_BF16: hipLaunchKernelGGL(block_score_kernel<__bf16>, g, t, 0, s, a); break;
       case HC_DTYPE_F16: hipLaunchKernelGGL(block_score_kernel<_Float16>, g, t, 0, s, a); break;
       default: hipLaunchKernelGGL(block_score_kernel<float>, g, t, 0, s, a); break;
     }
-    if ((rc = check_launch("hc_block_select(scores)"))) return rc;
+    const int rc = check_launch(what);
+    if (rc) return rc;
   }
   launch_pick<float, true>(a, grid, s);
-  return check_launch("hc_block_select");
+  return check_launch(what);
+}
+}  // namespace
+
+extern "C" int hc_block_select(int dtype, const void* q, const int64_t* q_strides, const int8_t* bounds,
+                               const int8_t* exps, const int64_t* row_block_off, const int32_t* row_len, int batch,
+                               int q_heads, int kv_heads, int queries, int block, int max_blocks, int keep, int sink,
+                               int local, int32_t* idx, int32_t* counts, void* scratch, size_t scratch_bytes,
+                               void* stream) {
+  clear_error();
+  SelectArgs a;
+  const int rc = select_args("hc_block_select", dtype, q, q_strides, bounds, exps, row_block_off, row_len, batch, q_heads,
+                             kv_heads, queries, block, max_blocks, keep, sink, local, idx, counts, a);
+  if (rc || batch == 0 || queries == 0) return rc;
+  const size_t need = hc_block_select_scratch_size(batch, kv_heads, queries, max_blocks);
+  if (need > 0 && (!scratch || scratch_bytes < need))
+    return set_error(HC_ERR_INVALID, "hc_block_select: scratch too small (%zu < %zu bytes)", scratch_bytes, need);
+  return launch_select("hc_block_select", dtype, a, scratch, (hipStream_t)stream);
 }
 
 namespace {
@@ -624,7 +715,8 @@ BlockPlan block_plan(int batch, int kv_heads, int G, int queries, int block, int
   const int64_t jobs = (int64_t)batch * kv_heads * queries, tiles = (int64_t)keep * (block / HC_TILE);
   double best = 0.;
   for (int waves = 4; waves <= (G <= 8 ? 8 : 4); waves += 4)
-    for (int ns = 1; ns <= 64 && (ns == 1 || (int64_t)ns * waves <= tiles); ++ns) {
+    for (int ns : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      if (ns > 1 && (int64_t)ns * waves > tiles) break;
       const int64_t slots = (int64_t)device_cus() * (waves == 8 ? 1 : 3);
       const double rounds = (double)((jobs * ns + slots - 1) / slots);
       const double load = (double)std::min(jobs * ns, slots) * waves * HC_TILE_ELEMS * 4. / 5.5e6;
@@ -647,43 +739,119 @@ extern "C" size_t hc_block_attn_workspace_size(int batch, int q_heads, int kv_he
   return block_plan(batch, kv_heads, q_heads / kv_heads, queries, block, keep).bytes;
 }
 
+namespace {
+// The checks and arguments of an attention over listed blocks.
+int attn_args(const char* what, int dtype, const void* q, const int64_t* q_strides, const void* kstore,
+              const void* vstore, const int64_t* row_tile_off, const int32_t* row_len, const int32_t* idx,
+              const int32_t* counts, int keep, int block, void* out, const int64_t* out_strides, int batch,
+              int q_heads, int kv_heads, int queries, float scale, RowsArgs& r) {
+  int rc = check_shape(what, dtype, batch, q_heads, kv_heads, queries, block);
+  if (rc) return rc;
+  if (keep < 1 || keep > (1 << 24) || (int64_t)keep * (block / HC_TILE) > 0x7fffffffLL)
+    return set_error(HC_ERR_INVALID, "%s: keep=%d", what, keep);
+  if (!(scale > 0.f) || std::isinf(scale)) return set_error(HC_ERR_INVALID, "%s: scale=%g", what, (double)scale);
+  if (batch == 0 || queries == 0) return HC_OK;
+  if (!q || !q_strides || !kstore || !vstore || !row_tile_off || !row_len || !idx || !counts || !out || !out_strides)
+    return set_error(HC_ERR_INVALID, "%s: null pointer argument", what);
+  if ((rc = check_q(what, dtype, q, q_strides))) return rc;
+  if ((reinterpret_cast<uintptr_t>(kstore) | reinterpret_cast<uintptr_t>(vstore)) & 15)
+    return set_error(HC_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
+  r = RowsArgs{};
+  r.q = q, r.kstore = kstore, r.vstore = vstore, r.row_tile_off = row_tile_off, r.row_len = row_len;
+  r.idx = idx, r.counts = counts, r.keep = keep, r.tpb = block / HC_TILE;
+  r.Hkv = kv_heads, r.G = q_heads / kv_heads, r.Q = queries, r.rows = batch * kv_heads, r.qpb = 1, r.ncb = queries;
+  r.nsplit = 1, r.scale_log2 = scale * 1.4426950408889634f, r.out = out;
+  for (int i = 0; i < 3; ++i) r.q_s[i] = q_strides[i], r.o_s[i] = out_strides[i];
+  return HC_OK;
+}
+
+int launch_attn(int dtype, RowsArgs& r, const BlockPlan& p, void* workspace, hipStream_t s) {
+  r.nsplit = p.nsplit;
+  if (p.nsplit > 1) {
+    r.part_o = reinterpret_cast<float*>(workspace);
+    r.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + p.part_o);
+  }
+  const int rc = launch_block_rows(dtype, r, p.waves, s);
+  if (rc || p.nsplit == 1) return rc;
+  MergeArgs mg = {};
+  mg.row_o = r.part_o, mg.row_ml = r.part_ml, mg.nsplit = p.nsplit;
+  mg.Hkv = r.Hkv, mg.G = r.G, mg.Q = r.Q, mg.out = r.out;
+  for (int i = 0; i < 3; ++i) mg.o_s[i] = r.o_s[i];
+  return launch_merge(dtype, mg, (int64_t)r.rows * r.Q * r.G, s);
+}
+
+// Whether one launch does it all: few queries, short rows and lists that eight
+// waves attend unsplit.
+constexpr int kStepBlocks = 512;
+bool one_launch(const BlockPlan& p, int64_t queries, int max_blocks, int keep) {
+  return p.waves == 8 && p.nsplit == 1 && queries <= device_cus() && max_blocks <= kStepBlocks && keep <= 2048;
+}
+
+size_t align16(size_t n) { return (n + 15) / 16 * 16; }
+}  // namespace
+
 extern "C" int hc_block_attn(int dtype, const void* q, const int64_t* q_strides, const void* kstore,
                              const void* vstore, const int64_t* row_tile_off, const int32_t* row_len,
                              const int32_t* idx, const int32_t* counts, int keep, int block, void* out,
                              const int64_t* out_strides, int batch, int q_heads, int kv_heads, int queries,
                              float scale, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
-  int rc = check_shape("hc_block_attn", dtype, batch, q_heads, kv_heads, queries, block);
-  if (rc) return rc;
-  if (keep < 1 || keep > (1 << 24) || (int64_t)keep * (block / HC_TILE) > 0x7fffffffLL)
-    return set_error(HC_ERR_INVALID, "hc_block_attn: keep=%d", keep);
-  if (!(scale > 0.f) || std::isinf(scale)) return set_error(HC_ERR_INVALID, "hc_block_attn: scale=%g", (double)scale);
-  if (batch == 0 || queries == 0) return HC_OK;
-  if (!q || !q_strides || !kstore || !vstore || !row_tile_off || !row_len || !idx || !counts || !out || !out_strides)
-    return set_error(HC_ERR_INVALID, "hc_block_attn: null pointer argument");
-  if ((rc = check_q("hc_block_attn", dtype, q, q_strides))) return rc;
-  if ((reinterpret_cast<uintptr_t>(kstore) | reinterpret_cast<uintptr_t>(vstore) |
-       reinterpret_cast<uintptr_t>(workspace)) & 15)
-    return set_error(HC_ERR_INVALID, "hc_block_attn: tensors must be 16-byte aligned");
-  const int G = q_heads / kv_heads;
-  const BlockPlan p = block_plan(batch, kv_heads, G, queries, block, keep);
-  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
-    return set_error(HC_ERR_INVALID, "hc_block_attn: workspace too small (%zu < %zu bytes)", workspace_bytes, p.bytes);
-  RowsArgs r = {};
-  r.q = q, r.kstore = kstore, r.vstore = vstore, r.row_tile_off = row_tile_off, r.row_len = row_len;
-  r.idx = idx, r.counts = counts, r.keep = keep, r.tpb = block / HC_TILE;
-  r.Hkv = kv_heads, r.G = G, r.Q = queries, r.rows = batch * kv_heads, r.qpb = 1, r.ncb = queries;
-  r.nsplit = p.nsplit, r.scale_log2 = scale * 1.4426950408889634f, r.out = out;
-  for (int i = 0; i < 3; ++i) r.q_s[i] = q_strides[i], r.o_s[i] = out_strides[i];
-  if (p.nsplit > 1) {
-    r.part_o = reinterpret_cast<float*>(workspace);
-    r.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + p.part_o);
-  }
+  RowsArgs r;
+  const int rc = attn_args("hc_block_attn", dtype, q, q_strides, kstore, vstore, row_tile_off, row_len, idx, counts, keep,
+                           block, out, out_strides, batch, q_heads, kv_heads, queries, scale, r);
+  if (rc || batch == 0 || queries == 0) return rc;
+  const BlockPlan p = block_plan(batch, kv_heads, r.G, queries, block, keep);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return set_error(HC_ERR_INVALID, "hc_block_attn: workspace too small (%zu < %zu bytes, 16-byte aligned)",
+                     workspace_bytes, p.bytes);
+  return launch_attn(dtype, r, p, workspace, (hipStream_t)stream);
+}
+
+extern "C" size_t hc_block_step_workspace_size(int batch, int q_heads, int kv_heads, int queries, int block,
+                                               int max_blocks, int keep) {
+  if (check_shape("hc_block_step", HC_DTYPE_BF16, batch, q_heads, kv_heads, queries, block) || keep < 1 ||
+      keep > (1 << 24) || max_blocks < 0 || batch == 0 || queries == 0)
+    return 0;
+  const BlockPlan p = block_plan(batch, kv_heads, q_heads / kv_heads, queries, block, keep);
+  if (one_launch(p, (int64_t)batch * kv_heads * queries, max_blocks, keep)) return 0;
+  return align16(hc_block_select_scratch_size(batch, kv_heads, queries, max_blocks)) + p.bytes;
+}
+
+extern "C" int hc_block_step(int dtype, const void* q, const int64_t* q_strides, const void* kstore,
+                             const void* vstore, const int64_t* row_tile_off, const int32_t* row_len,
+                             const int8_t* bounds, const int8_t* exps, const int64_t* row_block_off, int batch,
+                             int q_heads, int kv_heads, int queries, int block, int max_blocks, int keep, int sink,
+                             int local, float scale, int32_t* idx, int32_t* counts, void* out,
+                             const int64_t* out_strides, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  const char* what = "hc_block_step";
+  SelectArgs a;
+  RowsArgs r;
+  int rc = select_args(what, dtype, q, q_strides, bounds, exps, row_block_off, row_len, batch, q_heads, kv_heads, queries,
+                       block, max_blocks, keep, sink, local, idx, counts, a);
+  if (!rc)
+    rc = attn_args(what, dtype, q, q_strides, kstore, vstore, row_tile_off, row_len, idx, counts, keep, block, out,
+                   out_strides, batch, q_heads, kv_heads, queries, scale, r);
+  if (rc || batch == 0 || queries == 0) return rc;
+  const size_t need = hc_block_step_workspace_size(batch, q_heads, kv_heads, queries, block, max_blocks, keep);
+  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return set_error(HC_ERR_INVALID, "hc_block_step: workspace too small (%zu < %zu bytes, 16-byte aligned)",
+                     workspace_bytes, need);
   hipStream_t s = (hipStream_t)stream;
-  if ((rc = launch_block_rows(dtype, r, p.waves, s)) || p.nsplit == 1) return rc;
-  MergeArgs mg = {};
-  mg.row_o = r.part_o, mg.row_ml = r.part_ml, mg.nsplit = p.nsplit;
-  mg.Hkv = kv_heads, mg.G = G, mg.Q = queries, mg.out = out;
-  for (int i = 0; i < 3; ++i) mg.o_s[i] = out_strides[i];
-  return launch_merge(dtype, mg, (int64_t)batch * queries * q_heads, s);
+  const BlockPlan p = block_plan(batch, kv_heads, r.G, queries, block, keep);
+  if (one_launch(p, (int64_t)a.rows * queries, max_blocks, keep)) {
+    const dim3 grid((unsigned)((a.rows + 7) / 8 * 8 * queries)), t(512);
+    const size_t lds = ((size_t)max_blocks + keep) * sizeof(int32_t);
+    switch (dtype) {
+      case HC_DTYPE_BF16: hipLaunchKernelGGL(block_step_kernel<__bf16>, grid, t, lds, s, a, r); break;
+      case HC_DTYPE_F16: hipLaunchKernelGGL(block_step_kernel<_Float16>, grid, t, lds, s, a, r); break;
+      default: hipLaunchKernelGGL(block_step_kernel<float>, grid, t, lds, s, a, r); break;
+    }
+    return check_launch(what);
+  }
+  if ((rc = launch_select(what, dtype, a, workspace, s))) return rc;
+  return launch_attn(dtype, r, p,
+                     reinterpret_cast<char*>(workspace) +
+                         align16(hc_block_select_scratch_size(batch, kv_heads, queries, max_blocks)),
+                     s);
 }

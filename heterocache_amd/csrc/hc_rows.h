@@ -192,8 +192,15 @@ inline int64_t rows_workgroups(const RowsArgs& a) { return ((int64_t)a.rows + 7)
 // flight with one tile's registers, and three waves fit a SIMD (a second
 // buffer leaves two).  Bound by HBM: a token's K and V (512 bytes in 16 bits)
 // feed 512 G operations a query.
-template <typename T, bool LIST, bool MIXED, int NW>
-__device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds) {
+enum RowsMode {
+  kRowsWhole,   // every visible tile of the row
+  kRowsList,    // the blocks of a.idx and a.counts
+  kRowsListed,  // the same in LDS: list and its count, one workgroup a job
+};
+template <typename T, int MODE, bool MIXED, int NW>
+__device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds, const int32_t* listed = nullptr,
+                                         int listed_count = 0) {
+  constexpr bool LIST = MODE != kRowsWhole;
   typedef typename Elem<T>::vec8 vec8;
   constexpr int kCols = 64 / NW;
   float(*s_o)[kCols][kRowsPitch] = reinterpret_cast<float(*)[kCols][kRowsPitch]>(lds);
@@ -216,14 +223,15 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds) 
   // Everything the tiles' addresses and products wait for is requested at
   // once: the length, the tile offset, the list and the queries.
   const int64_t job_q = (int64_t)row * a.Q + i0;  // LIST: one query a job
-  const int32_t* const list = LIST ? a.idx + job_q * a.keep : nullptr;
+  const int32_t* const list = MODE == kRowsList ? a.idx + job_q * a.keep : listed;
   const int row_len = a.row_len[row];
   const int64_t base = a.row_tile_off[row] * (int64_t)HC_TILE_ELEMS + lane * 8;
   int kept = 0, spec = 0;
   // This wave's first 64 entries of a whole list.
   const int full = LIST ? a.keep * a.tpb : 0;
   const int f0 = (int)((int64_t)full * split / a.nsplit), f1 = (int)((int64_t)full * (split + 1) / a.nsplit);
-  if constexpr (LIST) {
+  if constexpr (MODE == kRowsListed) kept = listed_count;
+  if constexpr (MODE == kRowsList) {
     kept = a.counts[job_q];
     spec = list[min(f0 + wave + lane * NW, full - 1) / a.tpb];
   }
@@ -247,7 +255,7 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds) 
   if constexpr (LIST) entries = vis > 0 ? min(max(kept, 0), a.keep) * a.tpb : 0;
   const int e0 = (int)((int64_t)entries * split / a.nsplit), e1 = (int)((int64_t)entries * (split + 1) / a.nsplit);
   const int cnt = max((e1 - e0 - wave + NW - 1) / NW, 0);
-  const bool whole = LIST && e0 == f0 && e1 == f1;
+  const bool whole = MODE == kRowsList && e0 == f0 && e1 == f1;
 
   float m = -INFINITY, l = 0.f;
   f32x4 o[8];

@@ -10,7 +10,7 @@ namespace {
 template <typename T, int NW>
 __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : sizeof(T) == 4 ? 2 : 3) void block_rows_kernel(const RowsArgs a) {
   __shared__ __attribute__((aligned(16))) float lds[kRowsLds];
-  rows_job<T, true, false, NW>(a, blockIdx.x, lds);
+  rows_job<T, kRowsList, false, NW>(a, blockIdx.x, lds);
 }
 
 template <typename T>

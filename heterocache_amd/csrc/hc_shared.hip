@@ -294,7 +294,7 @@ __global__ __launch_bounds__(kPreThreads, sizeof(T) == 4 ? 1 : 3) void shared_at
   if ((int)blockIdx.x < npre)
     prefix_job<T, NC>(pre, blockIdx.x, reinterpret_cast<T*>(shared_raw));
   else
-    rows_job<T, false, MIXED, kPreWaves>(rows, blockIdx.x - npre, reinterpret_cast<float*>(shared_raw));
+    rows_job<T, kRowsWhole, MIXED, kPreWaves>(rows, blockIdx.x - npre, reinterpret_cast<float*>(shared_raw));
 }
 
 // Sizes of one call: the prefix launch's column blocks and parts, the rows'

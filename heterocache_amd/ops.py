@@ -1045,3 +1045,33 @@ def block_attn(q, kstore, vstore, row_tile_off, row_len, idx, counts, block, sca
                                  counts.data_ptr(), keep, block, out.data_ptr(), o_st, B, Hq, Hkv, Q, scale, _ptr(ws),
                                  nbytes, torch._C._cuda_getCurrentRawStream(dev)))
     return out
+
+
+@_on_device
+def block_step(q, kstore, vstore, row_tile_off, row_len, bounds, exps, row_block_off, block, max_blocks, keep, scale,
+               sink=1, local=1, out=None):
+    """block_select and block_attn over its selection in one call: (out
+    [B, Q, Hq, 128], idx [rows, Q, keep], counts [rows, Q]) (hc_block_step in
+    include/hc.h)."""
+    dt, dev, nb = q.dtype, q.get_device(), exps.numel()
+    shape, rows, Hkv = _block_rows(q, row_len)
+    B, Hq, Q, _ = shape
+    _stores(dt, dev, kstore, vstore)
+    _meta(dev, "row_tile_off", row_tile_off, torch.int64, rows)
+    _meta(dev, "row_len", row_len, torch.int32, rows)
+    _meta(dev, "row_block_off", row_block_off, torch.int64, rows)
+    _meta(dev, "exps", exps, torch.int8, nb)
+    _meta(dev, "bounds", bounds, torch.int8, nb * 2 * HEAD_DIM)
+    out, o_st = _out_bthd(q, out, shape, dev)
+    lib = _lib.load()
+    device = q.device
+    idx = torch.empty((rows, Q, max(keep, 0)), dtype=torch.int32, device=device)
+    counts = torch.empty((rows, Q), dtype=torch.int32, device=device)
+    nbytes = lib.hc_block_step_workspace_size(B, Hq, Hkv, Q, block, max_blocks, keep)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _lib.check(lib.hc_block_step(dtype_code(dt), q.data_ptr(), _strides3((shape, q.stride())), kstore.data_ptr(),
+                                 vstore.data_ptr(), row_tile_off.data_ptr(), row_len.data_ptr(), bounds.data_ptr(),
+                                 exps.data_ptr(), row_block_off.data_ptr(), B, Hq, Hkv, Q, block, max_blocks, keep, sink,
+                                 local, scale, idx.data_ptr(), counts.data_ptr(), out.data_ptr(), o_st, _ptr(ws), nbytes,
+                                 torch._C._cuda_getCurrentRawStream(dev)))
+    return out, idx, counts

@@ -351,16 +351,14 @@ class KVStore:
     def attend_blocks(self, q, index, keep, scale, sink=1, local=2, out=None, stream=None):
         """Attention of queries [B, Hq, Q, 128] (the last Q tokens of their
         rows) over `keep` blocks of each row: its first `sink`, last `local`
-        and those that score highest for the query (ops.block_select,
-        ops.block_attn).  Returns (out [B, Q, Hq, 128], idx [rows, Q, keep],
+        and those that score highest for the query (ops.block_step; a selection
+        kept for several calls: ops.block_select, ops.block_attn).  Returns (out [B, Q, Hq, 128], idx [rows, Q, keep],
         counts [rows, Q]).  The index must hold every complete block."""
         if index.store is not self:
             raise ValueError("the index is another store's")
-        idx, counts = ops.block_select(q, index.bounds, index.exps, index.row_block_off, self.row_len, index.block,
-                                       index.max_blocks, keep, sink=sink, local=local, stream=stream)
-        out = ops.block_attn(q, self.k, self.v, self.row_tile_off, self.row_len, idx, counts, index.block, scale,
-                             out=out, stream=stream)
-        return out, idx, counts
+        return ops.block_step(q, self.k, self.v, self.row_tile_off, self.row_len, index.bounds, index.exps,
+                              index.row_block_off, index.block, index.max_blocks, keep, scale, sink=sink, local=local,
+                              out=out, stream=stream)
 
     def _oom(self):
         name = "?" if self.layer_idx is None else self.layer_idx

@@ -605,8 +605,7 @@ size_t hc_shared_workspace_size(int dtype, int batch, int q_heads, int kv_heads,
                                 int64_t row_tiles);
 
 /*
- * Attention over the key blocks that a score selects for each query, in three
- * calls.  A block is `block` tokens (a multiple of 32) of a row.  No
+ * Attention over the key blocks that a score selects for each query.  A block is `block` tokens (a multiple of 32) of a row.  No
  * counterpart in the reference, which reads a kept head whole; for rows that
  * keep their whole prompt (its volatile and pivot heads).
  *
@@ -653,6 +652,19 @@ int hc_block_attn(int dtype, const void* q, const int64_t* q_strides, const void
                   int keep, int block, void* out, const int64_t* out_strides, int batch, int q_heads, int kv_heads,
                   int queries, float scale, void* workspace, size_t workspace_bytes, void* stream);
 size_t hc_block_attn_workspace_size(int batch, int q_heads, int kv_heads, int queries, int block, int keep);
+/*
+ * hc_block_step: hc_block_select and hc_block_attn over its selection in one
+ * call (idx and counts are written as well), in one launch where the queries
+ * are few, their rows short and their lists unsplit.  workspace:
+ * hc_block_step_workspace_size bytes (may be 0).
+ */
+int hc_block_step(int dtype, const void* q, const int64_t* q_strides, const void* kstore, const void* vstore,
+                  const int64_t* row_tile_off, const int32_t* row_len, const int8_t* bounds, const int8_t* exps,
+                  const int64_t* row_block_off, int batch, int q_heads, int kv_heads, int queries, int block,
+                  int max_blocks, int keep, int sink, int local, float scale, int32_t* idx, int32_t* counts, void* out,
+                  const int64_t* out_strides, void* workspace, size_t workspace_bytes, void* stream);
+size_t hc_block_step_workspace_size(int batch, int q_heads, int kv_heads, int queries, int block, int max_blocks,
+                                    int keep);
 
 #ifdef __cplusplus
 }

@@ -134,3 +134,25 @@ def test_block_attn(lib):
     _refused(lib, call(ks=FAKE + 8), b"aligned")
     assert call(b=0) == 0 and call(n=0) == 0
     assert lib.hc_block_attn_workspace_size(1, 8, 2, 1, 33, 8) == 0
+
+
+def test_block_step(lib):
+    def call(dtype=2, q=FAKE, ks=FAKE, bounds=FAKE, b=1, hq=8, hkv=2, n=1, block=32, mb=20000, keep=4096, sink=1, local=2,
+             scale=0.1, idx=FAKE, out=FAKE, ws=FAKE, wb=0):
+        return lib.hc_block_step(dtype, q, _s(1024, 128, 1024), ks, FAKE, FAKE, FAKE, bounds, FAKE, FAKE, b, hq, hkv, n,
+                                 block, mb, keep, sink, local, scale, idx, FAKE, out, _s(1024, 128, 1024), ws, wb, None)
+    size = lib.hc_block_step_workspace_size(1, 8, 2, 1, 32, 20000, 4096)
+    assert size >= lib.hc_block_select_scratch_size(1, 2, 1, 20000) + lib.hc_block_attn_workspace_size(1, 8, 2, 1, 32, 4096)
+    _refused(lib, call(), b"workspace too small")
+    _refused(lib, call(wb=size, ws=FAKE + 8), b"workspace")
+    _refused(lib, call(hq=9), b"q_heads=9")
+    _refused(lib, call(block=31), b"block=31")
+    _refused(lib, call(sink=4095), b"keep=4096")
+    _refused(lib, call(local=0), b"local")
+    _refused(lib, call(scale=0.0), b"scale")
+    _refused(lib, call(idx=None), b"null")
+    _refused(lib, call(out=None), b"null")
+    _refused(lib, call(ks=FAKE + 8), b"aligned")
+    _refused(lib, call(bounds=FAKE + 8), b"aligned")
+    assert call(b=0) == 0 and call(n=0) == 0
+    assert lib.hc_block_step_workspace_size(1, 8, 2, 1, 32, 128, 16) == 0  # one launch
