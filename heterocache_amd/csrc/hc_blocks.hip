@@ -569,7 +569,7 @@ bool select_in_memory(int64_t jobs, int max_blocks) {
 // Blocks that four waves pick from, sixteen beyond (8 queries of 512, 1024 and
 // 2048 blocks through memory: 9.4, 10.8 and 13.5 us with four, 10.7, 11.8 and
 // 12.6 with sixteen).
-constexpr int kFewBlocks = 1024;
+constexpr int kFewBlocks = 1536;
 
 template <typename T, bool SCORED>
 void launch_pick(const SelectArgs& a, dim3 grid, hipStream_t s) {

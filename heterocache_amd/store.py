@@ -64,6 +64,8 @@ class KVStore:
         self.host_tile_off = off
         self.host_len = np.zeros(self.rows, dtype=np.int32)
         self._headroom = int(self.host_cap.min()) if self.rows else 0  # min over rows of cap - len
+        self._longest = 0   # a bound of the longest row, and the tokens of all rows; None until asked for
+        self._tokens = 0
         if meta is not None:
             # Device metadata prepared by the owner of the arena (one transfer
             # for every store): views holding these rows' tile offsets
@@ -96,6 +98,25 @@ class KVStore:
         return int(((caps + TILE - 1) // TILE).sum())
 
     # -- bookkeeping -------------------------------------------------------
+    def _grown(self, tokens):
+        """The lengths advanced by at most `tokens` a row (None: any way)."""
+        self._tokens = None
+        if tokens is None:
+            self._longest = None
+        elif self._longest is not None:
+            self._longest += tokens
+
+    def longest_row(self):
+        """A bound of the longest row's tokens."""
+        if self._longest is None:
+            self._longest = int(self.host_len.max(initial=0))
+        return self._longest
+
+    def total_tokens(self):
+        if self._tokens is None:
+            self._tokens = int(self.host_len.sum())
+        return self._tokens
+
     def bytes_per_token(self):
         return 2 * HEAD_DIM * self.k.element_size()
 
@@ -109,6 +130,7 @@ class KVStore:
         if (lens > self.host_cap[rows]).any() or (lens < 0).any():
             raise RuntimeError("row length outside its capacity")
         self.host_len[rows] = lens
+        self._grown(None)
         idx = ops.to_device(rows, self.device, torch.int64)
         self.row_len.index_copy_(0, idx, ops.to_device(lens, self.device, torch.int32))
         # Longest rows are scheduled first; appends keep this order.
@@ -132,6 +154,7 @@ class KVStore:
         if (lens > self.host_cap[rows]).any() or (lens < 0).any():
             raise RuntimeError("row length outside its capacity")
         self.host_len[rows] = lens
+        self._grown(None)
         if not on_device:
             self.row_len.index_copy_(0, dev_rows, dev_lens)
         if dev_order is not None:
@@ -148,6 +171,7 @@ class KVStore:
         if lens.shape != (self.rows,) or (lens > self.host_cap).any() or (lens < 0).any():
             raise RuntimeError("row lengths outside their capacity")
         self.host_len[:] = lens
+        self._grown(None)
         self._headroom = int((self.host_cap - self.host_len).min()) if self.rows else 0
 
     # -- writers -----------------------------------------------------------
@@ -253,6 +277,7 @@ class KVStore:
                    stream=stream)
         self.host_len += 1
         self._headroom -= 1
+        self._grown(1)
 
     def append_rotated(self, q, k, v, cos, sin, counts=None, out=None, stream=None):
         """Turn new queries [B, Hq, T, 128] and keys [B, Hkv, T, 128] by their
@@ -288,9 +313,11 @@ class KVStore:
         if add is None:
             self.host_len += np.int32(T)
             self._headroom -= T
+            self._grown(T)
         else:
             self.host_len += add
             self._headroom = int((self.host_cap - self.host_len).min()) if self.rows else 0
+            self._grown(None)
         return out
 
     # -- readers -----------------------------------------------------------
@@ -321,6 +348,7 @@ class KVStore:
         if k_new is not None:
             self.host_len += 1
             self._headroom -= 1
+            self._grown(1)
         return out
 
     def attend_shared(self, q, prefix, scale, out=None, stream=None):
@@ -333,15 +361,9 @@ class KVStore:
         if B == 0 or self.rows % B:
             raise ValueError(f"{self.rows} rows for {B} sequences")
         kv = self.rows // B
-        pre = None
-        ptiles = 0
-        if prefix is not None:
-            if prefix.rows != kv:
-                raise ValueError(f"a prefix of {prefix.rows} rows for {kv} KV heads")
-            pre = (prefix.k, prefix.v, prefix.row_tile_off, prefix.row_len)
-            ptiles = int(prefix.host_len.sum()) // TILE + kv
-        return ops.shared_attn(q, pre, (self.k, self.v, self.row_tile_off, self.row_len), kv, scale, prefix_tiles=ptiles,
-                               row_tiles=int(self.host_len.max(initial=0)) // TILE + 1, out=out, stream=stream)
+        if prefix is not None and prefix.rows != kv:
+            raise ValueError(f"a prefix of {prefix.rows} rows for {kv} KV heads")
+        return ops.shared_attn_stores(q, prefix, self, kv, scale, out=out, stream=stream)
 
     def block_index(self, block=64):
         """An index of this store's key blocks of `block` tokens for
@@ -356,9 +378,7 @@ class KVStore:
         counts [rows, Q]).  The index must hold every complete block."""
         if index.store is not self:
             raise ValueError("the index is another store's")
-        return ops.block_step(q, self.k, self.v, self.row_tile_off, self.row_len, index.bounds, index.exps,
-                              index.row_block_off, index.block, index.max_blocks, keep, scale, sink=sink, local=local,
-                              out=out, stream=stream)
+        return ops.block_step_store(q, self, index, keep, scale, sink=sink, local=local, out=out, stream=stream)
 
     def _oom(self):
         name = "?" if self.layer_idx is None else self.layer_idx
