@@ -248,8 +248,12 @@ extern "C" int hc_append_rotated(int dtype, int table_dtype, const void* q, cons
     return set_error(HC_ERR_INVALID, "hc_append_rotated: the tables' dtype %d is neither float32 nor %d", table_dtype,
                      dtype);
   if (batch == 0) return HC_OK;
-  if (!row_len || (len_out && !row_cap)) return set_error(HC_ERR_INVALID, "hc_append_rotated: null pointer argument");
+  if (!row_len || (len_out && (!row_cap || !row_tile_off))) return set_error(HC_ERR_INVALID, "hc_append_rotated: null pointer argument");
   if (tokens == 0 && (!len_out || len_out == row_len)) return HC_OK;
+  const int64_t gap = 4 * (int64_t)batch * kv_heads;
+  const intptr_t apart = reinterpret_cast<intptr_t>(len_out) - reinterpret_cast<intptr_t>(row_len);
+  if (len_out && apart != 0 && apart > -gap && apart < gap)
+    return set_error(HC_ERR_INVALID, "hc_append_rotated: len_out overlaps row_len without being it");
   if (!q_strides || !q_out_strides || !k_strides || !v_strides)
     return set_error(HC_ERR_INVALID, "hc_append_rotated: null strides");
   if (tokens > 0 && (!q || !q_out || !k || !v || !cos || !sin || !kstore || !vstore || !row_tile_off || !row_cap))

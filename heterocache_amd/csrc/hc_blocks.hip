@@ -174,7 +174,7 @@ struct SelectArgs {
   int64_t q_s[3];
   const int8_t *bounds, *exps;
   const int64_t* row_blk_off;
-  const int32_t* row_len;
+  const int32_t *row_len, *query_counts;
   float* scores;  // [row * Q + query][pitch]; unused where scores stay in LDS
   int64_t pitch;
   int32_t *idx, *counts;
@@ -182,9 +182,6 @@ struct SelectArgs {
   int chunks;      // score workgroups of a query
   int max_blocks;  // visible blocks a query has room for; one that sees more selects nothing
 };
-
-// Visible tokens of query i of a row.
-__device__ __forceinline__ int visible(int len, int Q, int i) { return min(max(len - Q + 1 + i, 0), len); }
 
 // A job is one query of one row; the queries of a row go to one XCD, whose L2
 // then holds the row's bounds.
@@ -201,7 +198,8 @@ __device__ __forceinline__ bool select_job(const SelectArgs& a, int x, SelectJob
 }
 // Apart from select_job: the query's loads do not wait for the row's length.
 __device__ __forceinline__ void select_range(const SelectArgs& a, SelectJob& j) {
-  j.have = (visible(max(a.row_len[j.row], 0), a.Q, j.i) + a.S - 1) / a.S;
+  const int len = max(a.row_len[j.row], 0), nqt = query_tokens(a.query_counts, j.row / a.Hkv, a.Q);
+  j.have = (min(max(len - nqt + 1 + j.i, 0), len) + a.S - 1) / a.S;
   j.lo = a.sink;
   j.hi = j.have <= a.keep || j.have > a.max_blocks ? a.sink : j.have - a.local;
 }
@@ -625,9 +623,9 @@ extern "C" size_t hc_block_select_scratch_size(int batch, int kv_heads, int quer
 namespace {
 // The checks and arguments of a selection.
 int select_args(const char* what, int dtype, const void* q, const int64_t* q_strides, const int8_t* bounds,
-                const int8_t* exps, const int64_t* row_block_off, const int32_t* row_len, int batch, int q_heads,
-                int kv_heads, int queries, int block, int max_blocks, int keep, int sink, int local, int32_t* idx,
-                int32_t* counts, SelectArgs& a) {
+                const int8_t* exps, const int64_t* row_block_off, const int32_t* row_len, const int32_t* query_counts,
+                int batch, int q_heads, int kv_heads, int queries, int block, int max_blocks, int keep, int sink,
+                int local, int32_t* idx, int32_t* counts, SelectArgs& a) {
   int rc = check_shape(what, dtype, batch, q_heads, kv_heads, queries, block);
   if (rc) return rc;
   if (sink < 0 || local < 1 || keep < 1 || keep > (1 << 24) || (int64_t)sink + local > keep || max_blocks < 0)
@@ -641,7 +639,7 @@ int select_args(const char* what, int dtype, const void* q, const int64_t* q_str
   if (reinterpret_cast<uintptr_t>(bounds) & 15)
     return set_error(HC_ERR_INVALID, "%s: the bounds must be 16-byte aligned", what);
   a = SelectArgs{};
-  a.q = q, a.bounds = bounds, a.exps = exps, a.row_blk_off = row_block_off, a.row_len = row_len;
+  a.q = q, a.bounds = bounds, a.exps = exps, a.row_blk_off = row_block_off, a.row_len = row_len, a.query_counts = query_counts;
   for (int i = 0; i < 3; ++i) a.q_s[i] = q_strides[i];
   a.pitch = score_pitch(max_blocks), a.idx = idx, a.counts = counts;
   a.Hkv = kv_heads, a.G = q_heads / kv_heads, a.Q = queries, a.rows = batch * kv_heads, a.S = block;
@@ -682,14 +680,14 @@ int launch_select(const char* what, int dtype, SelectArgs& a, void* scratch, hip
 }  // namespace
 
 extern "C" int hc_block_select(int dtype, const void* q, const int64_t* q_strides, const int8_t* bounds,
-                               const int8_t* exps, const int64_t* row_block_off, const int32_t* row_len, int batch,
-                               int q_heads, int kv_heads, int queries, int block, int max_blocks, int keep, int sink,
-                               int local, int32_t* idx, int32_t* counts, void* scratch, size_t scratch_bytes,
-                               void* stream) {
+                               const int8_t* exps, const int64_t* row_block_off, const int32_t* row_len,
+                               const int32_t* query_counts, int batch, int q_heads, int kv_heads, int queries, int block,
+                               int max_blocks, int keep, int sink, int local, int32_t* idx, int32_t* counts,
+                               void* scratch, size_t scratch_bytes, void* stream) {
   clear_error();
   SelectArgs a;
-  const int rc = select_args("hc_block_select", dtype, q, q_strides, bounds, exps, row_block_off, row_len, batch, q_heads,
-                             kv_heads, queries, block, max_blocks, keep, sink, local, idx, counts, a);
+  const int rc = select_args("hc_block_select", dtype, q, q_strides, bounds, exps, row_block_off, row_len, query_counts,
+                             batch, q_heads, kv_heads, queries, block, max_blocks, keep, sink, local, idx, counts, a);
   if (rc || batch == 0 || queries == 0) return rc;
   const size_t need = hc_block_select_scratch_size(batch, kv_heads, queries, max_blocks);
   if (need > 0 && (!scratch || scratch_bytes < need))
@@ -742,12 +740,12 @@ extern "C" size_t hc_block_attn_workspace_size(int batch, int q_heads, int kv_he
 namespace {
 // The checks and arguments of an attention over listed blocks.
 int attn_args(const char* what, int dtype, const void* q, const int64_t* q_strides, const void* kstore,
-              const void* vstore, const int64_t* row_tile_off, const int32_t* row_len, const int32_t* idx,
-              const int32_t* counts, int keep, int block, void* out, const int64_t* out_strides, int batch,
-              int q_heads, int kv_heads, int queries, float scale, RowsArgs& r) {
+              const void* vstore, const int64_t* row_tile_off, const int32_t* row_len, const int32_t* query_counts,
+              const int32_t* idx, const int32_t* counts, int keep, int block, void* out, const int64_t* out_strides,
+              int batch, int q_heads, int kv_heads, int queries, float scale, RowsArgs& r) {
   int rc = check_shape(what, dtype, batch, q_heads, kv_heads, queries, block);
   if (rc) return rc;
-  if (keep < 1 || keep > (1 << 24) || (int64_t)keep * (block / HC_TILE) > 0x7fffffffLL)
+  if (keep < 1 || keep > (1 << 24) || (int64_t)keep * (block / HC_TILE) > (1 << 30))
     return set_error(HC_ERR_INVALID, "%s: keep=%d", what, keep);
   if (!(scale > 0.f) || std::isinf(scale)) return set_error(HC_ERR_INVALID, "%s: scale=%g", what, (double)scale);
   if (batch == 0 || queries == 0) return HC_OK;
@@ -758,7 +756,7 @@ int attn_args(const char* what, int dtype, const void* q, const int64_t* q_strid
     return set_error(HC_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
   r = RowsArgs{};
   r.q = q, r.kstore = kstore, r.vstore = vstore, r.row_tile_off = row_tile_off, r.row_len = row_len;
-  r.idx = idx, r.counts = counts, r.keep = keep, r.tpb = block / HC_TILE;
+  r.query_counts = query_counts, r.idx = idx, r.counts = counts, r.keep = keep, r.tpb = block / HC_TILE;
   r.Hkv = kv_heads, r.G = q_heads / kv_heads, r.Q = queries, r.rows = batch * kv_heads, r.qpb = 1, r.ncb = queries;
   r.nsplit = 1, r.scale_log2 = scale * 1.4426950408889634f, r.out = out;
   for (int i = 0; i < 3; ++i) r.q_s[i] = q_strides[i], r.o_s[i] = out_strides[i];
@@ -792,13 +790,13 @@ size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
 extern "C" int hc_block_attn(int dtype, const void* q, const int64_t* q_strides, const void* kstore,
                              const void* vstore, const int64_t* row_tile_off, const int32_t* row_len,
-                             const int32_t* idx, const int32_t* counts, int keep, int block, void* out,
-                             const int64_t* out_strides, int batch, int q_heads, int kv_heads, int queries,
+                             const int32_t* query_counts, const int32_t* idx, const int32_t* counts, int keep, int block,
+                             void* out, const int64_t* out_strides, int batch, int q_heads, int kv_heads, int queries,
                              float scale, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   RowsArgs r;
-  const int rc = attn_args("hc_block_attn", dtype, q, q_strides, kstore, vstore, row_tile_off, row_len, idx, counts, keep,
-                           block, out, out_strides, batch, q_heads, kv_heads, queries, scale, r);
+  const int rc = attn_args("hc_block_attn", dtype, q, q_strides, kstore, vstore, row_tile_off, row_len, query_counts, idx,
+                           counts, keep, block, out, out_strides, batch, q_heads, kv_heads, queries, scale, r);
   if (rc || batch == 0 || queries == 0) return rc;
   const BlockPlan p = block_plan(batch, kv_heads, r.G, queries, block, keep);
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)))
@@ -819,19 +817,19 @@ extern "C" size_t hc_block_step_workspace_size(int batch, int q_heads, int kv_he
 
 extern "C" int hc_block_step(int dtype, const void* q, const int64_t* q_strides, const void* kstore,
                              const void* vstore, const int64_t* row_tile_off, const int32_t* row_len,
-                             const int8_t* bounds, const int8_t* exps, const int64_t* row_block_off, int batch,
-                             int q_heads, int kv_heads, int queries, int block, int max_blocks, int keep, int sink,
-                             int local, float scale, int32_t* idx, int32_t* counts, void* out,
+                             const int32_t* query_counts, const int8_t* bounds, const int8_t* exps,
+                             const int64_t* row_block_off, int batch, int q_heads, int kv_heads, int queries, int block,
+                             int max_blocks, int keep, int sink, int local, float scale, int32_t* idx, int32_t* counts, void* out,
                              const int64_t* out_strides, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   const char* what = "hc_block_step";
   SelectArgs a;
   RowsArgs r;
-  int rc = select_args(what, dtype, q, q_strides, bounds, exps, row_block_off, row_len, batch, q_heads, kv_heads, queries,
-                       block, max_blocks, keep, sink, local, idx, counts, a);
+  int rc = select_args(what, dtype, q, q_strides, bounds, exps, row_block_off, row_len, query_counts, batch, q_heads,
+                       kv_heads, queries, block, max_blocks, keep, sink, local, idx, counts, a);
   if (!rc)
-    rc = attn_args(what, dtype, q, q_strides, kstore, vstore, row_tile_off, row_len, idx, counts, keep, block, out,
-                   out_strides, batch, q_heads, kv_heads, queries, scale, r);
+    rc = attn_args(what, dtype, q, q_strides, kstore, vstore, row_tile_off, row_len, query_counts, idx, counts, keep,
+                   block, out, out_strides, batch, q_heads, kv_heads, queries, scale, r);
   if (rc || batch == 0 || queries == 0) return rc;
   const size_t need = hc_block_step_workspace_size(batch, q_heads, kv_heads, queries, block, max_blocks, keep);
   if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))

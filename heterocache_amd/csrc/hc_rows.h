@@ -87,17 +87,16 @@ __device__ __forceinline__ typename Elem<T>::vec8 tile_probs(const f32x4 (&s)[2]
   return pb;
 }
 
-// O += V^T P^T over tokens tok0 + [0, 32).  lim: this lane's column limit;
-// lim_lo <= lim <= lim_hi over the wave's columns (both uniform), and equal
-// unless MIXED.
+// O += V^T P^T over tokens tok0 + [0, 32), of which those from `end` on are
+// seen by no column.
 template <typename T, bool MIXED>
 __device__ __forceinline__ void tile_values(typename Elem<T>::vec8 (&vr)[8], const typename Elem<T>::vec8& pb, int tok0,
-                                            int lim, int lim_lo, int lim_hi, int g, f32x4 (&o)[8]) {
-  if (tok0 + HC_TILE > lim_hi) {
+                                            int end, int g, f32x4 (&o)[8]) {
+  if (tok0 + HC_TILE > end) {
 #pragma unroll
-    for (int mt = 0; mt < 8; ++mt) zero_tail<T>(vr[mt], tok0, lim_hi, g);
+    for (int mt = 0; mt < 8; ++mt) zero_tail<T>(vr[mt], tok0, end, g);
   }
-  if (MIXED && tok0 + HC_TILE > lim_lo && lim_lo < lim_hi) {
+  if constexpr (MIXED) {
     // Some columns do not see tokens that others see.  Their probabilities
     // are zero, but zero times an infinite or NaN value is not: with one in
     // the tile the finite values take the product, and what the others would
@@ -163,6 +162,7 @@ struct RowsArgs {
   const void *kstore, *vstore;
   const int64_t* row_tile_off;
   const int32_t* row_len;
+  const int32_t* query_counts;  // per sequence, or null: all Q
   // Kept blocks of each (row, query): keep entries of tpb tiles, the first
   // counts of them used; null: every visible tile of the row.
   const int32_t *idx, *counts;
@@ -177,6 +177,12 @@ struct RowsArgs {
   void* out;
   int64_t o_s[3];
 };
+
+// How many of the Q queries of sequence b are tokens of its rows (the others,
+// behind them, are padding).
+__device__ __forceinline__ int query_tokens(const int32_t* counts, int b, int Q) {
+  return counts ? min(max(counts[b], 0), Q) : Q;
+}
 
 constexpr int kRowsPitch = HC_HEAD_DIM + 4;
 // LDS floats of rows_job: O and (m, l) of NW waves x 64 / NW columns.
@@ -224,7 +230,7 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds, 
   // once: the length, the tile offset, the list and the queries.
   const int64_t job_q = (int64_t)row * a.Q + i0;  // LIST: one query a job
   const int32_t* const list = MODE == kRowsList ? a.idx + job_q * a.keep : listed;
-  const int row_len = a.row_len[row];
+  const int row_len = a.row_len[row], nqt = query_tokens(a.query_counts, b, a.Q);
   const int64_t base = a.row_tile_off[row] * (int64_t)HC_TILE_ELEMS + lane * 8;
   int kept = 0, spec = 0;
   // This wave's first 64 entries of a whole list.
@@ -244,9 +250,9 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds, 
   }
 
   const int len = max(row_len, 0);
-  const int lim_lo = min(max(len - a.Q + 1 + i0, 0), len);
-  const int lim_hi = min(max(len - a.Q + i0 + nq, 0), len);
-  const int lim = min(max(len - a.Q + 1 + i0 + qi, 0), len);
+  const int lim_lo = min(max(len - nqt + 1 + i0, 0), len);
+  const int lim_hi = min(max(len - nqt + i0 + nq, 0), len);
+  const int lim = min(max(len - nqt + 1 + i0 + qi, 0), len);
   // Entries of the job, this workgroup's share of them and this wave's: e0 +
   // wave, e0 + wave + NW, ...
   const int vis = (lim_hi + HC_TILE - 1) / HC_TILE;
@@ -290,19 +296,27 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds, 
       const int64_t at = (int64_t)max(next, 0) * HC_TILE_ELEMS;
       const bool live = !LIST || tile >= 0;
       const int tok0 = max(tile, 0) * HC_TILE;
+      const int lo = live ? lim_lo : 0, hi = live ? lim_hi : 0, mylim = live ? lim : 0;
+      // A tile that some columns see more of than others (a row's last one or
+      // two): the next one's keys wait, which leaves it their registers.
+      const bool mixed = MIXED && tok0 + HC_TILE > lo && lo < hi;
       f32x4 s[2];
       tile_scores<T>(kr, qreg, s);
       __builtin_amdgcn_sched_barrier(0);
-      load_operands<T>(kr, kb + at);
+      if (!mixed) load_operands<T>(kr, kb + at);
       __builtin_amdgcn_sched_barrier(0);
-      const int lo = live ? lim_lo : 0, hi = live ? lim_hi : 0, mylim = live ? lim : 0;
       if (tok0 + HC_TILE > lo) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (tok0 + 16 * (e >> 2) + 4 * g + (e & 3) >= mylim) s[e >> 2][e & 3] = -INFINITY;
       }
       const vec8 pb = tile_probs<T>(s, a.scale_log2, m, l, o);
-      tile_values<T, MIXED>(vr, pb, tok0, mylim, lo, hi, g, o);
+      if (mixed) {
+        tile_values<T, true>(vr, pb, tok0, hi, g, o);
+        load_operands<T>(kr, kb + at);
+      } else {
+        tile_values<T, false>(vr, pb, tok0, hi, g, o);
+      }
       __builtin_amdgcn_sched_barrier(0);
       load_operands<T>(vr, vb + at);
       __builtin_amdgcn_sched_barrier(0);

@@ -1,8 +1,9 @@
 // Attention of a batch over one shared prefix and each sequence's own rows.
 //
 //   out[b, i, h] = softmax over the tokens of prefix row kv(h) and the visible
-//   tokens of row (b, kv(h)), times their values; query i of Q sees the
-//   row's tokens t < len - Q + 1 + i.
+//   tokens of row (b, kv(h)), times their values; query i sees the row's
+//   tokens t < len - n + 1 + i, n the new tokens of the sequence (all Q
+//   queries, or a count of its own behind which queries are padding).
 //
 // Both parts lie in ragged tiled stores; the prefix has one row per KV head,
 // of its own length (a document compressed per head, or whole).  Softmax over
@@ -388,9 +389,10 @@ extern "C" size_t hc_shared_workspace_size(int dtype, int batch, int q_heads, in
 extern "C" int hc_shared_attn(int dtype, const void* q, const int64_t* q_strides, const void* kprefix,
                               const void* vprefix, const int64_t* prefix_tile_off, const int32_t* prefix_len,
                               int64_t prefix_tiles, const void* kstore, const void* vstore,
-                              const int64_t* row_tile_off, const int32_t* row_len, int64_t row_tiles, void* out,
-                              const int64_t* out_strides, int batch, int q_heads, int kv_heads, int queries,
-                              float scale, void* workspace, size_t workspace_bytes, void* stream) {
+                              const int64_t* row_tile_off, const int32_t* row_len, const int32_t* query_counts,
+                              int64_t row_tiles, void* out, const int64_t* out_strides, int batch,
+                              int q_heads, int kv_heads, int queries, float scale, void* workspace,
+                              size_t workspace_bytes, void* stream) {
   clear_error();
   if (bad_sizes(dtype, batch, q_heads, kv_heads, queries) || prefix_tiles < 0 || row_tiles < 0)
     return set_error(HC_ERR_INVALID,
@@ -432,7 +434,7 @@ extern "C" int hc_shared_attn(int dtype, const void* q, const int64_t* q_strides
   a.part_o = reinterpret_cast<float*>(ws + p.pre_o), a.part_ml = reinterpret_cast<float*>(ws + p.pre_ml);
   a.info = reinterpret_cast<int32_t*>(ws + p.info_at);
   RowsArgs r = {};
-  r.q = q, r.kstore = kstore, r.vstore = vstore, r.row_tile_off = row_tile_off, r.row_len = row_len;
+  r.q = q, r.kstore = kstore, r.vstore = vstore, r.row_tile_off = row_tile_off, r.row_len = row_len, r.query_counts = query_counts;
   r.Hkv = kv_heads, r.G = G, r.Q = queries, r.rows = row_len ? batch * kv_heads : 0;
   r.qpb = p.rows.qpb, r.ncb = p.rows.ncb, r.nsplit = p.rows.nsplit, r.scale_log2 = scale_log2;
   r.part_o = reinterpret_cast<float*>(ws + p.row_o), r.part_ml = reinterpret_cast<float*>(ws + p.row_ml);

@@ -286,8 +286,10 @@ class KVStore:
         queries.
 
         counts: tokens of each sequence to append (host integers, at most T;
-        None: all T): the rest is padding.  Raises the reference's "Layer i
-        OOM." when a row has no room.
+        None: all T): the rest is padding.  They are copied to the device, so
+        a call with counts is refused while a graph is captured
+        (ops.append_rotated takes them there).  Raises the reference's "Layer
+        i OOM." when a row has no room.
         """
         rows, T = k.shape[0] * k.shape[1], k.shape[2]
         if rows != self.rows:
@@ -303,11 +305,8 @@ class KVStore:
             add = np.repeat(counts, k.shape[1]).astype(np.int32)
             if (self.host_len + add > self.host_cap).any():
                 raise self._oom()
-            if stream is not None:
-                with torch.cuda.stream(stream):
-                    dev_counts = ops.to_device(counts, self.device, torch.int32)
-            else:
-                dev_counts = ops.to_device(counts, self.device, torch.int32)
+            with torch.cuda.stream(stream):  # (None: the current one)
+                dev_counts = ops.host_counts("counts", counts, self.device)
         out = ops.append_rotated(q, k, v, cos, sin, self.k, self.v, self.row_tile_off, self.row_len, self.row_cap,
                                  counts=dev_counts, out=out, len_out=self.row_len, status=self.status, stream=stream)
         if add is None:
@@ -351,34 +350,34 @@ class KVStore:
             self._grown(1)
         return out
 
-    def attend_shared(self, q, prefix, scale, out=None, stream=None):
+    def attend_shared(self, q, prefix, scale, out=None, query_counts=None, stream=None):
         """Attention of queries [B, Hq, Q, 128] (the last Q tokens of these
         rows) over the shared `prefix`, a KVStore of Hkv rows or None, and
         over this store's rows b * Hkv + h: [B, Q, Hq, 128]
-        (ops.shared_attn).  Lengths are read on the device: a captured call
-        replays while the rows grow."""
+        (ops.shared_attn).  query_counts: where append_rotated took counts,
+        the same, as an int32 device tensor or host integers.  Lengths are
+        read on the device: a captured call replays while the rows grow."""
         B = q.shape[0]
         if B == 0 or self.rows % B:
             raise ValueError(f"{self.rows} rows for {B} sequences")
         kv = self.rows // B
-        if prefix is not None and prefix.rows != kv:
-            raise ValueError(f"a prefix of {prefix.rows} rows for {kv} KV heads")
-        return ops.shared_attn_stores(q, prefix, self, kv, scale, out=out, stream=stream)
+        return ops.shared_attn_stores(q, prefix, self, kv, scale, out=out, query_counts=query_counts, stream=stream)
 
     def block_index(self, block=64):
         """An index of this store's key blocks of `block` tokens for
         attend_blocks (empty until its update)."""
         return BlockIndex(self, block)
 
-    def attend_blocks(self, q, index, keep, scale, sink=1, local=2, out=None, stream=None):
+    def attend_blocks(self, q, index, keep, scale, sink=1, local=2, out=None, query_counts=None, stream=None):
         """Attention of queries [B, Hq, Q, 128] (the last Q tokens of their
-        rows) over `keep` blocks of each row: its first `sink`, last `local`
-        and those that score highest for the query (ops.block_step; a selection
-        kept for several calls: ops.block_select, ops.block_attn).  Returns (out [B, Q, Hq, 128], idx [rows, Q, keep],
-        counts [rows, Q]).  The index must hold every complete block."""
-        if index.store is not self:
-            raise ValueError("the index is another store's")
-        return ops.block_step_store(q, self, index, keep, scale, sink=sink, local=local, out=out, stream=stream)
+        rows; query_counts as in attend_shared) over `keep` blocks of each
+        row: its first `sink`, last `local` and those that score highest for
+        the query (ops.block_step; a selection kept for several calls:
+        ops.block_select, ops.block_attn).  Returns (out [B, Q, Hq, 128], idx
+        [rows, Q, keep], counts [rows, Q]).  The index must hold every
+        complete block."""
+        return ops.block_step_store(q, self, index, keep, scale, sink=sink, local=local, out=out,
+                                    query_counts=query_counts, stream=stream)
 
     def _oom(self):
         name = "?" if self.layer_idx is None else self.layer_idx
@@ -434,7 +433,9 @@ class BlockIndex:
         those that each row's last new_tokens tokens completed."""
         s = self.store
         if new_tokens is None:
-            span, fresh = int(s.host_len.max(initial=0)) // self.block, 0
+            # A graph's replays find other lengths than the capture's.
+            longest = s.host_cap if torch.cuda.is_current_stream_capturing() else s.host_len
+            span, fresh = int(longest.max(initial=0)) // self.block, 0
         else:
             fresh = int(new_tokens)
             if fresh < 0:

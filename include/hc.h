@@ -577,10 +577,12 @@ int hc_append_rotated(int dtype, int table_dtype, const void* q, const int64_t* 
 /*
  * Attention of a batch over one shared prefix and each sequence's own rows:
  *   out[b, h, i] = softmax over {prefix row kv, tokens t < prefix_len[kv]} and
- *                  {row b * kv_heads + kv, tokens t < row_len - queries + 1 + i}
+ *                  {row b * kv_heads + kv, tokens t < row_len - n + 1 + i}
  * of scale * q[b, h, i] . k_t, times their values; kv = h / (q_heads /
- * kv_heads).  The queries are the last `queries` tokens of the rows (1: a
- * decode step); zeros where nothing is visible.  The prefix is a store of
+ * kv_heads).  The first n queries of sequence b are the last n tokens of its
+ * rows: n = query_counts[b], clamped to [0, queries] (NULL: all queries; 1: a
+ * decode step).  The others are padding and see the whole row.  Zeros where
+ * nothing is visible.  The prefix is a store of
  * kv_heads rows, each of its own length (a prompt kept whole or compressed
  * per head), and is read once for all sequences.  prefix_len NULL: no prefix;
  * row_len NULL: no rows of their own.  prefix_tiles, row_tiles: tiles of all
@@ -589,7 +591,7 @@ int hc_append_rotated(int dtype, int table_dtype, const void* q, const int64_t* 
  * any device lengths are attended whole whatever they are, so a captured
  * call replays while the rows grow).
  * q, out: base + b*strides[0] + h*strides[1] + i*strides[2] + c, q's strides
- * 16-byte multiples; at most 16 query heads a KV head and 2^24 query rows;
+ * 16-byte multiples; out shares no memory with q; at most 16 query heads a KV head and 2^24 query rows;
  * scale finite and positive.  workspace: hc_shared_workspace_size bytes,
  * 16-byte aligned, no initialisation; calls that overlap in time need their
  * own.  Matrix products on the input type, softmax and sums in float32.
@@ -598,16 +600,17 @@ int hc_append_rotated(int dtype, int table_dtype, const void* q, const int64_t* 
  */
 int hc_shared_attn(int dtype, const void* q, const int64_t* q_strides, const void* kprefix, const void* vprefix,
                    const int64_t* prefix_tile_off, const int32_t* prefix_len, int64_t prefix_tiles, const void* kstore,
-                   const void* vstore, const int64_t* row_tile_off, const int32_t* row_len, int64_t row_tiles,
-                   void* out, const int64_t* out_strides, int batch, int q_heads, int kv_heads, int queries,
+                   const void* vstore, const int64_t* row_tile_off, const int32_t* row_len,
+                   const int32_t* query_counts, int64_t row_tiles, void* out, const int64_t* out_strides, int batch, int q_heads, int kv_heads, int queries,
                    float scale, void* workspace, size_t workspace_bytes, void* stream);
 size_t hc_shared_workspace_size(int dtype, int batch, int q_heads, int kv_heads, int queries, int64_t prefix_tiles,
                                 int64_t row_tiles);
 
 /*
- * Attention over the key blocks that a score selects for each query.  A block is `block` tokens (a multiple of 32) of a row.  No
- * counterpart in the reference, which reads a kept head whole; for rows that
- * keep their whole prompt (its volatile and pivot heads).
+ * Attention over the key blocks that a score selects for each query.  A block
+ * is `block` tokens (a multiple of 32) of a row.  No counterpart in the
+ * reference, which reads a kept head whole; for rows that keep their whole
+ * prompt (its volatile and pivot heads).
  *
  * hc_block_bounds: of complete blocks, bounds int8 [block][2][128] (channel
  * maxima, then minima, of the keys) and exps int8 [block]:
@@ -626,19 +629,19 @@ int hc_block_bounds(int dtype, const void* kstore, const int64_t* row_tile_off, 
  * rint(q / 2^eq) (eq found as e above) a block scores
  *   max over the row's query heads of 2^(eq + e) * sum_d max(q8_d hi_d, q8_d lo_d),
  * a sum of whole numbers, so the score is exact and the selection does not
- * depend on batch, grid or order.  Query i sees row_len - queries + 1 + i
- * tokens; of its visible blocks it keeps the first `sink`, the last `local`
+ * depend on batch, grid or order.  Query i sees row_len - n + 1 + i tokens (n
+ * of query_counts, as in hc_shared_attn); of its visible blocks it keeps the first `sink`, the last `local`
  * (at least 1: the unfinished block is never scored) and the best of the
  * others, equal scores to the lower block: `keep` in all, or every block if
  * there are no more.  idx int32 [rows][queries][keep]: ascending, -1 past
- * counts int32 [rows][queries].  max_blocks: visible blocks that scratch
+ * the count; counts int32 [rows][queries].  max_blocks: visible blocks that scratch
  * (hc_block_select_scratch_size bytes, no initialisation) has room for; a
  * query that sees more gets counts -1 and no block.
  */
 int hc_block_select(int dtype, const void* q, const int64_t* q_strides, const int8_t* bounds, const int8_t* exps,
-                    const int64_t* row_block_off, const int32_t* row_len, int batch, int q_heads, int kv_heads,
-                    int queries, int block, int max_blocks, int keep, int sink, int local, int32_t* idx,
-                    int32_t* counts, void* scratch, size_t scratch_bytes, void* stream);
+                    const int64_t* row_block_off, const int32_t* row_len, const int32_t* query_counts, int batch,
+                    int q_heads, int kv_heads, int queries, int block, int max_blocks, int keep, int sink, int local,
+                    int32_t* idx, int32_t* counts, void* scratch, size_t scratch_bytes, void* stream);
 size_t hc_block_select_scratch_size(int batch, int kv_heads, int queries, int max_blocks);
 /*
  * hc_block_attn: out[b, h, i] = softmax(scale * q . k_t) v_t over the visible
@@ -648,9 +651,10 @@ size_t hc_block_select_scratch_size(int batch, int kv_heads, int queries, int ma
  * hc_block_attn_workspace_size bytes (may be 0).
  */
 int hc_block_attn(int dtype, const void* q, const int64_t* q_strides, const void* kstore, const void* vstore,
-                  const int64_t* row_tile_off, const int32_t* row_len, const int32_t* idx, const int32_t* counts,
-                  int keep, int block, void* out, const int64_t* out_strides, int batch, int q_heads, int kv_heads,
-                  int queries, float scale, void* workspace, size_t workspace_bytes, void* stream);
+                  const int64_t* row_tile_off, const int32_t* row_len, const int32_t* query_counts,
+                  const int32_t* idx, const int32_t* counts, int keep, int block, void* out,
+                  const int64_t* out_strides, int batch, int q_heads, int kv_heads, int queries, float scale,
+                  void* workspace, size_t workspace_bytes, void* stream);
 size_t hc_block_attn_workspace_size(int batch, int q_heads, int kv_heads, int queries, int block, int keep);
 /*
  * hc_block_step: hc_block_select and hc_block_attn over its selection in one
@@ -659,10 +663,11 @@ size_t hc_block_attn_workspace_size(int batch, int q_heads, int kv_heads, int qu
  * hc_block_step_workspace_size bytes (may be 0).
  */
 int hc_block_step(int dtype, const void* q, const int64_t* q_strides, const void* kstore, const void* vstore,
-                  const int64_t* row_tile_off, const int32_t* row_len, const int8_t* bounds, const int8_t* exps,
-                  const int64_t* row_block_off, int batch, int q_heads, int kv_heads, int queries, int block,
-                  int max_blocks, int keep, int sink, int local, float scale, int32_t* idx, int32_t* counts, void* out,
-                  const int64_t* out_strides, void* workspace, size_t workspace_bytes, void* stream);
+                  const int64_t* row_tile_off, const int32_t* row_len, const int32_t* query_counts,
+                  const int8_t* bounds, const int8_t* exps, const int64_t* row_block_off, int batch, int q_heads,
+                  int kv_heads, int queries, int block, int max_blocks, int keep, int sink, int local, float scale,
+                  int32_t* idx, int32_t* counts, void* out, const int64_t* out_strides, void* workspace,
+                  size_t workspace_bytes, void* stream);
 size_t hc_block_step_workspace_size(int batch, int q_heads, int kv_heads, int queries, int block, int max_blocks,
                                     int keep);
 

@@ -49,6 +49,9 @@ def test_append_rotated(lib):
     _refused(lib, _append(lib, tt=132), b"table strides")
     _refused(lib, _append(lib, v=FAKE + 2), b"aligned")
     _refused(lib, _append(lib, b=1 << 20, t=1 << 20), b"rows")
+    _refused(lib, _append(lib, off=None, t=0, lo=FAKE + 64), b"null")
+    _refused(lib, _append(lib, lo=FAKE + 4), b"overlaps")
+    _refused(lib, _append(lib, lo=FAKE - 4), b"overlaps")
     assert _append(lib, b=0) == 0 and _append(lib, t=0, q=None, lo=None) == 0
 
 
@@ -57,7 +60,7 @@ def _shared(lib, **kw):
              len=FAKE, rt=4, out=FAKE, os=_s(1024, 128, 1024), b=1, hq=8, hkv=2, n=1, scale=0.1, ws=FAKE, wb=0)
     a.update(kw)
     return lib.hc_shared_attn(a["dtype"], a["q"], a["qs"], a["pk"], a["pv"], a["po"], a["pl"], a["pt"], a["k"], a["v"],
-                              a["off"], a["len"], a["rt"], a["out"], a["os"], a["b"], a["hq"], a["hkv"], a["n"],
+                              a["off"], a["len"], None, a["rt"], a["out"], a["os"], a["b"], a["hq"], a["hkv"], a["n"],
                               a["scale"], a["ws"], a["wb"], None)
 
 
@@ -105,7 +108,7 @@ def test_block_select(lib):
     def call(dtype=2, q=FAKE, qs=_s(1024, 128, 1024), b=1, hq=8, hkv=2, n=1, block=32, mb=20000, keep=8, sink=1, local=2,
              idx=FAKE, scratch=FAKE, sb=None):
         sb = lib.hc_block_select_scratch_size(b, hkv, n, mb) - 1 if sb is None else sb
-        return lib.hc_block_select(dtype, q, qs, FAKE, FAKE, FAKE, FAKE, b, hq, hkv, n, block, mb, keep, sink, local, idx,
+        return lib.hc_block_select(dtype, q, qs, FAKE, FAKE, FAKE, FAKE, None, b, hq, hkv, n, block, mb, keep, sink, local, idx,
                                    FAKE, scratch, sb, None)
     _refused(lib, call(), b"scratch too small")
     _refused(lib, call(scratch=None, sb=1 << 30), b"scratch too small")
@@ -122,14 +125,15 @@ def test_block_select(lib):
 def test_block_attn(lib):
     def call(dtype=2, q=FAKE, qs=_s(1024, 128, 1024), ks=FAKE, idx=FAKE, keep=4096, block=32, b=1, hq=8, hkv=2, n=1,
              scale=0.1, ws=FAKE, wb=0):
-        return lib.hc_block_attn(dtype, q, qs, ks, FAKE, FAKE, FAKE, idx, FAKE, keep, block, FAKE, _s(1024, 128, 1024), b,
-                                 hq, hkv, n, scale, ws, wb, None)
+        return lib.hc_block_attn(dtype, q, qs, ks, FAKE, FAKE, FAKE, None, idx, FAKE, keep, block, FAKE,
+                                 _s(1024, 128, 1024), b, hq, hkv, n, scale, ws, wb, None)
     assert lib.hc_block_attn_workspace_size(1, 8, 2, 1, 32, 4096) > 0  # the kept blocks are split
     _refused(lib, call(), b"workspace too small")
     _refused(lib, call(hq=34), b"at most 16")
     _refused(lib, call(keep=0), b"keep=0")
     _refused(lib, call(block=48), b"block=48")
     _refused(lib, call(scale=-0.5), b"scale")
+    _refused(lib, call(keep=1 << 24, block=1 << 12), b"keep=")
     _refused(lib, call(idx=None), b"null")
     _refused(lib, call(ks=FAKE + 8), b"aligned")
     assert call(b=0) == 0 and call(n=0) == 0
@@ -139,8 +143,8 @@ def test_block_attn(lib):
 def test_block_step(lib):
     def call(dtype=2, q=FAKE, ks=FAKE, bounds=FAKE, b=1, hq=8, hkv=2, n=1, block=32, mb=20000, keep=4096, sink=1, local=2,
              scale=0.1, idx=FAKE, out=FAKE, ws=FAKE, wb=0):
-        return lib.hc_block_step(dtype, q, _s(1024, 128, 1024), ks, FAKE, FAKE, FAKE, bounds, FAKE, FAKE, b, hq, hkv, n,
-                                 block, mb, keep, sink, local, scale, idx, FAKE, out, _s(1024, 128, 1024), ws, wb, None)
+        return lib.hc_block_step(dtype, q, _s(1024, 128, 1024), ks, FAKE, FAKE, FAKE, None, bounds, FAKE, FAKE, b, hq,
+                                 hkv, n, block, mb, keep, sink, local, scale, idx, FAKE, out, _s(1024, 128, 1024), ws, wb, None)
     size = lib.hc_block_step_workspace_size(1, 8, 2, 1, 32, 20000, 4096)
     assert size >= lib.hc_block_select_scratch_size(1, 2, 1, 20000) + lib.hc_block_attn_workspace_size(1, 8, 2, 1, 32, 4096)
     _refused(lib, call(), b"workspace too small")
