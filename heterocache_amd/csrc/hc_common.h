@@ -321,8 +321,8 @@ __device__ __forceinline__ void wait_lds_dma() { __builtin_amdgcn_s_waitcnt(0x0f
 // landed (loads complete in order).
 template <int N>
 __device__ __forceinline__ void wait_lds_dma_but() {
-  static_assert(N >= 0 && N < 16, "vmcnt field");
-  __builtin_amdgcn_s_waitcnt(0x0f70 | N);
+  static_assert(N >= 0 && N < 64, "vmcnt field");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
 }
 
 // Order-preserving uint32 key of a float score (larger float, larger key;

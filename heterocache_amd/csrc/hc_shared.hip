@@ -19,6 +19,7 @@
 //  * merge_kernel (hc_rows.hip): one fold of a column's partials.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "hc_rows.h"
 
@@ -27,7 +28,9 @@ namespace {
 
 constexpr int kPreWaves = 4;
 constexpr int kPreThreads = kPreWaves * 64;
-constexpr int kPreRing = 3;  // tiles of K and V held in LDS: one attended, two in flight
+// Slots of a tile's keys in LDS; of its values there is one less.  (One more
+// slot changes no time by more than 2 %.)
+constexpr int kRing = 4;
 
 struct PrefixArgs {
   const void* q;
@@ -47,9 +50,9 @@ struct PrefixArgs {
 // Tiles a part takes so that every row is covered by at most `parts` parts in
 // all: each row's last part may be short, so the shares are cut from the
 // parts left when every row has one.
-__device__ __forceinline__ int part_tiles(int64_t total, int rows, int parts) {
-  const int64_t n = max(parts - rows, 1);
-  return (int)max((total + n - 1) / n, (int64_t)1);
+__device__ __forceinline__ int part_tiles(uint32_t total, int rows, int parts) {
+  const uint32_t n = max(parts - rows, 1);
+  return (int)max((total + n - 1) / n, 1u);
 }
 
 __device__ __forceinline__ int tiles_of(int len) { return (max(len, 0) + HC_TILE - 1) / HC_TILE; }
@@ -63,7 +66,21 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
-template <typename T, int NC>
+// Waits until at most `units` (0 .. U) times LOADS of this wave's loads are in
+// flight.
+template <int U, int LOADS>
+__device__ __forceinline__ void wait_dma_units(int units) {
+  if constexpr (U == 0) {
+    wait_lds_dma();
+  } else {
+    if (units >= U)
+      wait_lds_dma_but<U * LOADS>();
+    else
+      wait_dma_units<U - 1, LOADS>(units);
+  }
+}
+
+template <typename T, int NC, bool ONCE>
 __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
   typedef typename Elem<T>::vec8 vec8;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -73,77 +90,53 @@ __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
   // XCDs in turn), so its L2 serves the tiles after their first read.
   const int part = (x / (8 * a.ncg)) * 8 + x % 8, cg = (x / 8) % a.ncg;
 
-  // (row, share) of the part, from the device lengths: rows 64 at a time.
-  int64_t total = 0;
-  for (int r0 = 0; r0 < a.Hkv; r0 += 64) {
-    int nt = r0 + lane < a.Hkv ? tiles_of(a.len[r0 + lane]) : 0;
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) nt += __shfl_xor(nt, d, 64);
-    total += nt;
+  // (row, share) of the part, from the device lengths: rows 64 at a time,
+  // their tile offsets requested along with the lengths.
+  int row_n = 0, nt = 0;
+  int64_t row_off = 0;
+  auto load_rows = [&](int r0) {
+    const int r = min(r0 + lane, a.Hkv - 1);
+    row_off = a.tile_off[r];
+    row_n = max(a.len[r], 0);
+    row_n = r0 + lane < a.Hkv ? row_n : 0;
+    // Opaque: knowing which lanes hold zero, the compiler would run them apart
+    // and the wave's sums over the others alone; and it would move the offsets'
+    // load behind the sums.
+    asm("" : "+v"(row_n), "+v"(row_off));
+    nt = tiles_of(row_n);
+  };
+  load_rows(0);
+  uint32_t total = 0;  // (2^31 tiles are 35 TB)
+  for (int r0 = 0;;) {
+    total += __builtin_amdgcn_readlane(wave_scan_add(nt), 63);
+    r0 += 64;
+    if (r0 >= a.Hkv) break;
+    load_rows(r0);
   }
   const int share = part_tiles(total, a.Hkv, a.parts);
-  int kv = -1, t0 = 0, t1 = 0, first = 0;
+  int kv = -1, t0 = 0, t1 = 0, len = 0, first = 0;
+  int64_t tile0 = 0;
   for (int r0 = 0; r0 < a.Hkv; r0 += 64) {
-    const int r = r0 + lane;
-    const int nt = r < a.Hkv ? tiles_of(a.len[r]) : 0;
+    if (a.Hkv > 64) load_rows(r0);
     const int np = (nt + share - 1) / share;
-    int incl = np;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int u = __shfl_up(incl, d, 64);
-      if (lane >= d) incl += u;
-    }
-    incl += first;
-    if (x == 0 && wave == 0 && r < a.Hkv) {
-      a.info[2 * r] = incl - np;
-      a.info[2 * r + 1] = np;
+    const int incl = wave_scan_add(np) + first;
+    if (x == 0 && wave == 0 && r0 + lane < a.Hkv) {
+      a.info[2 * (r0 + lane)] = incl - np;
+      a.info[2 * (r0 + lane) + 1] = np;
     }
     const uint64_t hit = __ballot(part >= incl - np && part < incl);
     if (hit && kv < 0) {
       const int src = __builtin_ctzll(hit);
       kv = r0 + src;
-      t0 = (part - __shfl(incl - np, src, 64)) * share;
-      t1 = min(t0 + share, __shfl(nt, src, 64));
+      t0 = (part - __builtin_amdgcn_readlane(incl - np, src)) * share;
+      t1 = min(t0 + share, __builtin_amdgcn_readlane(nt, src));
+      len = __builtin_amdgcn_readlane(row_n, src);
+      tile0 = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)row_off, src) |
+              (int64_t)__builtin_amdgcn_readlane((int)(row_off >> 32), src) << 32;
     }
-    first = __shfl(incl, 63, 64);
+    first = __builtin_amdgcn_readlane(incl, 63);
   }
-  kv = __builtin_amdgcn_readfirstlane(kv);
   if (kv < 0) return;
-  t0 = __builtin_amdgcn_readfirstlane(t0);
-  t1 = __builtin_amdgcn_readfirstlane(t1);
-  const int len = a.len[kv];
-
-  // Staging: the tiles lie contiguous in memory and keep their layout in LDS,
-  // so a tile is 16-byte units copied straight into LDS (global_load_lds).
-  constexpr int kTileBytes = HC_TILE_ELEMS * (int)sizeof(T);
-  constexpr int kLoads = kTileBytes / (16 * kPreThreads);  // per thread, of K and of V
-  const int64_t at = (a.tile_off[kv] + t0) * (int64_t)kTileBytes + 16 * tid;
-  const char* kb = reinterpret_cast<const char*>(a.kstore) + at;
-  const char* vb = reinterpret_cast<const char*>(a.vstore) + at;
-  // One column group reads a tile once: streamed past L2 (83 against 95 us for
-  // 16 columns over 131072 tokens of 8 heads; with more column groups the
-  // others' reads come from L2, and 4 of them lose 7 % by the hint).
-  const bool once = a.ncg == 1;
-  auto stage = [&](int slot) {  // the next tile not staged yet
-    char* dst = reinterpret_cast<char*>(lds + slot * 2 * HC_TILE_ELEMS) + 1024 * wave;
-    if (once) {
-#pragma unroll
-      for (int r = 0; r < kLoads; ++r) lds_dma16_stream(kb + 16 * r * kPreThreads, dst + 16 * r * kPreThreads);
-#pragma unroll
-      for (int r = 0; r < kLoads; ++r)
-        lds_dma16_stream(vb + 16 * r * kPreThreads, dst + kTileBytes + 16 * r * kPreThreads);
-    } else {
-#pragma unroll
-      for (int r = 0; r < kLoads; ++r) lds_dma16(kb + 16 * r * kPreThreads, dst + 16 * r * kPreThreads);
-#pragma unroll
-      for (int r = 0; r < kLoads; ++r) lds_dma16(vb + 16 * r * kPreThreads, dst + kTileBytes + 16 * r * kPreThreads);
-    }
-    kb += kTileBytes;
-    vb += kTileBytes;
-  };
-
-  stage(0);
-  if (t0 + 1 < t1) stage(1);
 
   // Q^T operands: column col0 + 16j + n16, k-slots = channels 32s + 8*g4 + [0, 8).
   const int64_t col0 = ((int64_t)cg * kPreWaves + wave) * 16 * NC;
@@ -159,143 +152,245 @@ __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) qop[j][s] = ok ? load8<T>(qp + 32 * s) : zero8<T>();
   }
-  f32x4 o[8][NC];
+  __builtin_amdgcn_sched_barrier(0);
+
+  // Staging: the tiles lie contiguous in memory and keep their layout in LDS,
+  // so a tile is 16-byte units copied straight into LDS (global_load_lds).
+  // Batch i holds the keys of tile i + 2 and the values of tile i.
+  constexpr int kTileBytes = HC_TILE_ELEMS * (int)sizeof(T);
+  constexpr int kLoads = kTileBytes / (16 * kPreThreads);  // per thread, of K and of V
+  const int n = t1 - t0;
+  const char* kb = reinterpret_cast<const char*>(a.kstore) + (tile0 + t0) * (int64_t)kTileBytes;
+  const char* vb = reinterpret_cast<const char*>(a.vstore) + (tile0 + t0) * (int64_t)kTileBytes;
+  char* const ring = reinterpret_cast<char*>(lds) + 1024 * wave;
+  const float scale_log2 = a.scale_log2;
+  auto copy = [&](const char* src, char* dst) {
+#pragma unroll
+    for (int r = 0; r < kLoads; ++r) {
+      // A 32-bit offset from a scalar base, which the compiler forgets once it
+      // has widened it outside of the loop.
+      uint32_t own = 16 * tid;
+      asm volatile("" : "+v"(own));
+      const char* p = src + 16 * r * kPreThreads + own;
+      if constexpr (ONCE)
+        lds_dma16_stream(p, dst + 16 * r * kPreThreads);
+      else
+        lds_dma16(p, dst + 16 * r * kPreThreads);
+    }
+  };
+  auto after = [](int s, int slots) { return s == slots - 1 ? 0 : s + 1; };
+  int kin = 0, vin = 0;  // slots of the next keys and values to stage
+  auto stage_k = [&]() {
+    copy(kb, ring + kin * kTileBytes);
+    kb += kTileBytes, kin = after(kin, kRing);
+  };
+  auto stage_v = [&]() {
+    copy(vb, ring + (kRing + vin) * kTileBytes);
+    vb += kTileBytes, vin = after(vin, kRing - 1);
+  };
+  stage_k();
+  if (1 < n) stage_k();
+#pragma unroll
+  for (int i = 0; i < kRing - 2; ++i) {
+    if (i + 2 < n) stage_k();
+    if (i < n) stage_v();
+  }
+
+  f32x4 o[8][NC], s[2][2][NC];  // s: of the tile attended, and of the next one, in turn
+  vec8 pb[NC], vr[8];
   float m[NC], l[NC];
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
     m[j] = -INFINITY, l[j] = 0.f;
+    pb[j] = zero8<T>();
 #pragma unroll
     for (int db = 0; db < 8; ++db) o[db][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) s[0][h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // The queries and the first tiles travel together; from here on the loop
-  // counts its loads in flight.
-  wait_lds_dma();
-  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int x = 0; x < 8; ++x) vr[x] = zero8<T>();
+  // The queries and the first two tiles' keys are here, the batches in flight.
+  if (kRing <= n)
+    wait_lds_dma_but<(kRing - 2) * 2 * kLoads>();
+  else
+    wait_lds_dma();
+  lds_barrier();
+  vec8 kr[8];  // keys in the order of the products: half h = x & 1, channels 32 (x / 2) + [0, 32)
+  auto key_at = [&](const T* p, int x) { return load8<T>(p + ((x & 1) * 4 + (x >> 1)) * 512 + lane * 8); };
+  if (active) {
+#pragma unroll
+    for (int x = 0; x < 8; ++x) kr[x] = key_at(lds, x);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) s[0][x & 1][j] = mma_16x16x32(kr[x], qop[j][x >> 1], s[0][x & 1][j]);
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) kr[x] = key_at(lds + HC_TILE_ELEMS, x);
+  }
 
-  int slot = 0;
-  for (int t = t0; t < t1; ++t) {
-    // This wave's loads of tile t have landed, and past the barrier every
-    // wave's have, while tile t + 1 stays in flight; every wave is also done
-    // with tile t - 1, whose slot takes tile t + 2.
-    if (t + 1 < t1)
-      wait_lds_dma_but<2 * kLoads>();
-    else
-      wait_lds_dma();
+  int kout = after(1, kRing), vout = 0;
+  // One tile, i, with tile i + 1's scores and the product of tile i - 1's
+  // values on the matrix cores while the vector unit forms the probabilities
+  // between them: kr holds the keys of tile i + 1, vr and pb the values and
+  // probabilities of tile i - 1, and each operand is read from LDS again, for
+  // the next step, once it is used.  STEADY: kRing tiles or more follow.
+  // (Behind the last tile: products of stale slots, which nothing reads.)
+  auto step = [&](auto steady, int i, f32x4(&sc)[2][NC], f32x4(&sn)[2][NC]) {
+    constexpr bool STEADY = decltype(steady)::value;
+    // This wave's loads of batch i have landed, and past the barrier every
+    // wave's have, while the younger ones stay in flight; every wave is also
+    // done with the keys of tile i + 1 and the values of tile i - 1: batch
+    // i + kRing - 2 takes the slots of the keys of tile i and of those values.
+    if constexpr (STEADY)
+      wait_lds_dma_but<(kRing - 3) * 2 * kLoads>();
+    else  // younger values, and keys
+      wait_dma_units<2 * (kRing - 3), kLoads>(min(n - 1 - i, kRing - 3) + max(min(n - 3 - i, kRing - 3), 0));
     lds_barrier();
-    const T* sk = lds + slot * 2 * HC_TILE_ELEMS;
-    const T* sv = sk + HC_TILE_ELEMS;
-    if (t + 2 < t1) stage(slot == 0 ? 2 : slot - 1);
-    slot = slot == kPreRing - 1 ? 0 : slot + 1;
-    const int left = len - t * HC_TILE;  // tokens from this tile on
-    if (left < HC_TILE) {
-      // The row's last tile: its stale slots may hold NaN, which a zero
-      // probability does not silence.  (No load is in flight any more.)
-      T* z = const_cast<T*>(sv);
-      for (int c = tid; c < HC_TILE_ELEMS / 8; c += kPreThreads) {
-        vec8 v = load8<T>(z + 8 * c);
-        zero_tail<T>(v, 0, left, (c >> 4) & 3);
-        *reinterpret_cast<vec8*>(z + 8 * c) = v;
+    if (STEADY || i + kRing < n) stage_k();
+    if (STEADY || i + kRing - 2 < n) stage_v();
+    const T* sk = lds + kout * HC_TILE_ELEMS;
+    const T* sv = lds + (kRing + vout) * HC_TILE_ELEMS + lane * 8;
+    kout = after(kout, kRing), vout = after(vout, kRing - 1);
+    if (!active) return;
+    if constexpr (!STEADY) {
+      const int left = len - (t0 + i) * HC_TILE;  // tokens from this tile on
+      if (left < HC_TILE) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (16 * (e >> 2) + 4 * g4 + (e & 3) >= left) {
+#pragma unroll
+            for (int j = 0; j < NC; ++j) sc[e >> 2][j][e & 3] = -INFINITY;
+          }
       }
-      lds_barrier();
     }
-    if (!active) continue;
-    // All of a tile's K operands are requested before the first product, and
-    // V's before the softmax that they wait behind (left to itself the
-    // compiler requests two and waits for both, sixteen times a tile).
-    vec8 kv8[8];
-#pragma unroll
-    for (int x8 = 0; x8 < 8; ++x8) kv8[x8] = load8<T>(sk + (x8 * 64 + lane) * 8);
-    __builtin_amdgcn_sched_barrier(0);
-    f32x4 s[2][NC];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int j = 0; j < NC; ++j) s[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int x4 = 0; x4 < 4; ++x4)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < NC; ++j) s[h][j] = mma_16x16x32(kv8[h * 4 + x4], qop[j][x4], s[h][j]);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int x8 = 0; x8 < 8; ++x8) kv8[x8] = load8<T>(sv + (x8 * 64 + lane) * 8);
-    __builtin_amdgcn_sched_barrier(0);
-    if (left < HC_TILE) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (16 * (e >> 2) + 4 * g4 + (e & 3) >= left) {
-#pragma unroll
-          for (int j = 0; j < NC; ++j) s[e >> 2][j][e & 3] = -INFINITY;
-        }
-    }
-    vec8 pb[NC];
+    float pv[NC][8], ps[NC];
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      float ps;
-      auto probs = [&](float nm) {
-        float pv[8];
-        ps = 0.f;
+      ps[j] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          pv[e] = fast_exp2(fmaf(s[e >> 2][j][e & 3], a.scale_log2, nm));
-          ps += pv[e];
-        }
-        pb[j] = pack8<T>(pv);  // at most half a step of the input type per probability
-      };
-      probs(-m[j]);
-      if (__any(!(ps <= kRowsLazy))) {  // also NaN, as in the first tile
+      for (int h = 0; h < 2; ++h) sn[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        sn[x & 1][j] = mma_16x16x32(kr[x], qop[j][x >> 1], sn[x & 1][j]);
+        o[x][j] = mma_16x16x32(vr[x], pb[j], o[x][j]);
+        pv[j][x] = fast_exp2(fmaf(sc[x >> 2][j][x & 3], scale_log2, -m[j]));
+        ps[j] += pv[j][x];
+      }
+      kr[x] = key_at(sk, x);
+      vr[x] = load8<T>(sv + x * 512);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    bool fine = ps[0] <= kRowsLazy;
+#pragma unroll
+    for (int j = 1; j < NC; ++j) fine = fine && ps[j] <= kRowsLazy;
+    if (__any(!fine)) {  // also NaN, as in the first tile
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
         float mx = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][j][e & 3]);
-        const float mnew = fmaxf(m[j], rows4_max(mx) * a.scale_log2);
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, sc[e >> 2][j][e & 3]);
+        const float mnew = fmaxf(m[j], rows4_max(mx) * scale_log2);
         const float alpha = m[j] == -INFINITY ? 0.f : fast_exp2(m[j] - mnew);
         m[j] = mnew;
         l[j] *= alpha;
 #pragma unroll
         for (int db = 0; db < 8; ++db) o[db][j] *= alpha;
-        probs(mnew == -INFINITY ? 0.f : -mnew);
+        const float nm = mnew == -INFINITY ? 0.f : -mnew;
+        ps[j] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          pv[j][e] = fast_exp2(fmaf(sc[e >> 2][j][e & 3], scale_log2, nm));
+          ps[j] += pv[j][e];
+        }
       }
-      l[j] += ps;
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      l[j] += ps[j];
+      pb[j] = pack8<T>(pv[j]);  // at most half a step of the input type per probability
+    }
+  };
+  int i = 0;
+  for (; i + kRing + 1 < n; i += 2) {
+    step(std::true_type{}, i, s[0], s[1]);
+    step(std::true_type{}, i + 1, s[1], s[0]);
+  }
+  for (; i < n; ++i) {
+    step(std::false_type{}, i, s[0], s[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) s[0][h][j] = s[1][h][j];
+  }
+  if (active) {
+    const int left = len - (t1 - 1) * HC_TILE;
+    if (left < HC_TILE) {
+      // The row's last tile: its stale slots may hold NaN, which a zero
+      // probability does not silence.
+#pragma unroll
+      for (int x = 0; x < 8; ++x) zero_tail<T>(vr[x], 0, left, g4);
     }
 #pragma unroll
     for (int db = 0; db < 8; ++db) {
 #pragma unroll
-      for (int j = 0; j < NC; ++j) o[db][j] = mma_16x16x32(kv8[db], pb[j], o[db][j]);
+      for (int j = 0; j < NC; ++j) o[db][j] = mma_16x16x32(vr[db], pb[j], o[db][j]);
     }
   }
 
+  // The partials leave through LDS: a wave stores 1 KB in a row, two columns,
+  // where its registers hold 64 bytes of each of 16.
+  wait_lds_dma();
+  lds_barrier();
   if (!active) return;
+  float(*so)[kRowsPitch] = reinterpret_cast<float(*)[kRowsPitch]>(lds) + 16 * wave;
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
     const float lt = rows4_sum(l[j]);
-    const int64_t c = col0 + 16 * j + n16;
-    if (c >= a.M) continue;
-    const int64_t pa = part * a.M + c;
+    const int64_t c0 = col0 + 16 * j;
+    float* po = a.part_o + ((int64_t)part * a.M + c0) * kPartO;
 #pragma unroll
-    for (int db = 0; db < 8; ++db)
-      *reinterpret_cast<f32x4*>(a.part_o + pa * kPartO + 16 * db + 4 * g4) = o[db][j];
-    if (g4 == 0) *reinterpret_cast<float2*>(a.part_ml + pa * 2) = make_float2(m[j], lt);
+    for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4*>(&so[n16][16 * db + 4 * g4]) = o[db][j];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int c = 2 * r + (lane >> 5), d = 4 * (lane & 31);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(&so[c][d]);
+      if (c0 + c < a.M) *reinterpret_cast<f32x4*>(po + c * kPartO + d) = v;
+    }
+    if (g4 == 0 && c0 + n16 < a.M)
+      *reinterpret_cast<float2*>(a.part_ml + ((int64_t)part * a.M + c0 + n16) * 2) = make_float2(m[j], lt);
   }
 }
 
 // LDS of a workgroup: the prefix ring, or the row waves' states.
 template <typename T>
-constexpr size_t shared_lds() {
-  const size_t ring = (size_t)kPreRing * 2 * HC_TILE_ELEMS * sizeof(T), rows = kRowsLds * sizeof(float);
-  return ring > rows ? ring : rows;
+constexpr size_t shared_lds(bool prefix) {
+  const size_t ring = (size_t)(2 * kRing - 1) * HC_TILE_ELEMS * sizeof(T), rows = kRowsLds * sizeof(float);
+  return prefix && ring > rows ? ring : rows;
 }
 
-// Prefix workgroups come first: they are the long ones.
+// Prefix workgroups come first: they are the long ones.  (One round of them,
+// then the rows', then the rest: 282 us against 265 for 512 columns over 756K
+// tokens beside rows of 1.06M.)
 template <typename T, int NC, bool MIXED>
-__global__ __launch_bounds__(kPreThreads, sizeof(T) == 4 ? 1 : 3) void shared_attn_kernel(const PrefixArgs pre,
-                                                                                         const RowsArgs rows) {
+__global__ __launch_bounds__(kPreThreads, sizeof(T) == 4 ? 1 : NC == 2 ? 2 : 3) void shared_attn_kernel(
+    const PrefixArgs pre, const RowsArgs rows) {
   extern __shared__ __attribute__((aligned(16))) unsigned char shared_raw[];
   const int npre = pre.parts * pre.ncg;
-  if ((int)blockIdx.x < npre)
-    prefix_job<T, NC>(pre, blockIdx.x, reinterpret_cast<T*>(shared_raw));
-  else
+  T* const lds = reinterpret_cast<T*>(shared_raw);
+  // One column group reads a tile once: streamed past L2 (83 against 95 us for
+  // 16 columns over 131072 tokens of 8 heads; with more column groups the
+  // others' reads come from L2, and 4 of them lose 7 % by the hint).
+  if ((int)blockIdx.x >= npre)
     rows_job<T, kRowsWhole, MIXED, kPreWaves>(rows, blockIdx.x - npre, reinterpret_cast<float*>(shared_raw));
+  else if (pre.ncg == 1)
+    prefix_job<T, NC, true>(pre, blockIdx.x, lds);
+  else
+    prefix_job<T, NC, false>(pre, blockIdx.x, lds);
 }
 
 // Sizes of one call: the prefix launch's column blocks and parts, the rows'
@@ -311,37 +406,38 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 SharedPlan shared_plan(int dtype, int batch, int Hkv, int G, int Q, int64_t prefix_tiles, int64_t row_tiles) {
   SharedPlan p;
   const int64_t M = (int64_t)batch * Q * G;
-  p.nc = dtype != HC_DTYPE_F32 && M > 64 ? 2 : 1;
-  const int64_t per = 64 * p.nc;
-  p.ncg = (int)((M + per - 1) / per);
   p.rows = rows_plan(batch * Hkv, G, Q, row_tiles);
-  // Prefix workgroups a CU: the least estimate of the two launches' time in
-  // us.  A part's tile of 32 tokens takes 0.6 + 0.37 k with k workgroups of
-  // two column blocks a wave on a CU (128, 512 and 768 workgroups over 128K
-  // tokens: 330, 217 and 195 us against 327, 226 and 192), or the stream's
-  // time; a column's partial costs its writing and reading; the rows' stream
-  // hides behind the products while a third workgroup finds room (1024 rows
-  // beside 512 columns over 128K: 260, 253 and 278 us at k = 2, 2.5 and 3).
+  // Column blocks a wave (nc) and prefix workgroups a CU (k): the least
+  // estimate of the call's time in us, fitted to 300 timings of 15 shapes (a
+  // few columns to 512, prefixes of 1K to 128K tokens, own rows of 64 to 16K)
+  // and within 5 % of their best.  A part's tile of 32 tokens takes `tile` on a
+  // CU of its own and 0.65 more for each further workgroup there; the prefix
+  // is streamed at 6.5 TB/s at best; a column's partial costs its writing and
+  // reading; the rows' stream hides a third behind the products while a CU has
+  // room for a row workgroup beside them.  128 columns over 178K tokens: 36.2
+  // us with nc = 1, 38.2 with 2, whose partials are twice as many; 448 over
+  // 49K, bound by the products: 34.6 and 32.1.
   const int cus = device_cus();
   const bool f32 = dtype == HC_DTYPE_F32;
-  const double stream = 2e6 * HC_TILE_ELEMS * (f32 ? 4. : 2.) / 5.8e12;
-  const double rows_us = 0.75 * (double)batch * Hkv * row_tiles * stream;
-  const double ks[] = {0.125, 0.25, 0.5, 1., 1.5, 2., 2.5, 3.};
-  int64_t parts = 0;
+  const double stream = 1e6 * 2 * HC_TILE_ELEMS * (f32 ? 4. : 2.) / 6.5e12;
+  // (Of rows only the longest's length is known: 0.6 of it stands for the mean.)
+  const double pre_us = prefix_tiles * stream, rows_us = 0.6 * (double)batch * Hkv * row_tiles * stream;
   double best = 0.;
-  for (const double k : ks) {
-    if (f32 && k > 1.) break;  // LDS holds one workgroup
-    // Every KV head has two parts at least, and there are no more than tiles.
-    int64_t n = std::max<int64_t>((int64_t)(k * cus) / p.ncg, 2 * (int64_t)Hkv);
-    n = std::min(n, prefix_tiles + Hkv + 1);
-    const double kk = std::max((double)n * p.ncg / cus, 1.);
-    const double tile = f32 ? 3. : p.nc == 1 ? 0.5 + 0.2 * kk : 0.6 + 0.37 * kk;
-    const double share = std::ceil((double)prefix_tiles / (double)std::max<int64_t>(n - Hkv / 2, 1));
-    const double t = std::max(share * tile, prefix_tiles * stream) + (double)n * M * 520. * 0.45e-6 +
-                     rows_us * (f32 || kk > 2.75 ? 0.9 : kk > 2.25 ? 0.5 : 0.35);
-    if (parts == 0 || t < best) best = t, parts = n;
+  for (int nc = 1; nc <= (f32 || M <= 64 ? 1 : 2); ++nc) {
+    const int ncg = (int)((M + 64 * nc - 1) / (64 * nc));
+    const double tile = f32 ? 1.2 : nc == 1 ? 0.35 : 0.5;
+    for (const double k : {0.25, 0.5, 0.75, 1., 1.25, 1.5, 1.75, 2.}) {
+      // Every KV head has four parts at least, and there are no more than tiles.
+      int64_t n = std::max<int64_t>((int64_t)(k * cus) / ncg, 4 * (int64_t)Hkv);
+      n = (std::min(n, prefix_tiles + Hkv + 1) + 7) / 8 * 8;  // whole rounds over the 8 XCDs
+      const double kk = (double)n * ncg / cus;
+      const double share = std::ceil((double)prefix_tiles / (double)std::max<int64_t>(n - Hkv / 2, 1));
+      const double work = share * tile * (1. + 0.65 * (std::max(std::ceil(kk), 1.) - 1.));
+      const double t = std::max(std::max(work, pre_us) + rows_us * (kk < (f32 ? 1. : 2.) ? 0.67 : 1.), pre_us + rows_us) +
+                       (double)n * M * 0.2e-3;
+      if (best == 0. || t < best) best = t, p.nc = nc, p.ncg = ncg, p.parts = (int)n;
+    }
   }
-  p.parts = (int)std::min<int64_t>((parts + 7) / 8 * 8, 1 << 20);  // whole rounds over the 8 XCDs
   const size_t pre = (size_t)p.parts * M, row = (size_t)batch * Hkv * Q * G * p.rows.nsplit;
   p.info_at = 0;
   p.pre_o = up256((size_t)Hkv * 2 * sizeof(int32_t));
@@ -354,7 +450,7 @@ SharedPlan shared_plan(int dtype, int batch, int Hkv, int G, int Q, int64_t pref
 
 template <typename T>
 int launch_shared(const PrefixArgs& a, const RowsArgs& r, int nc, hipStream_t s) {
-  const size_t lds = shared_lds<T>();
+  const size_t lds = shared_lds<T>(a.parts > 0);
   const bool mixed = r.qpb > 1;
   auto fn = mixed ? shared_attn_kernel<T, 1, true> : shared_attn_kernel<T, 1, false>;
   if constexpr (sizeof(T) == 2)

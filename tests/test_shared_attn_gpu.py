@@ -211,3 +211,27 @@ def test_refusals(dev):
     with pytest.raises(_lib.HCError, match="16 of it|at most 16"):
         ops.shared_attn(_q(rng, 2, 34, 1, BF, dev), (prefix.k, prefix.v, prefix.row_tile_off, prefix.row_len), None, 2,
                         SCALE)
+
+
+@pytest.mark.parametrize("B,Hkv,G,Q,dtype", [(2, 2, 4, 1, BF), (40, 2, 4, 1, BF), (9, 1, 8, 3, FP), (3, 2, 2, 1, FL),
+                                             (70, 1, 2, 1, FL)])
+@pytest.mark.parametrize("tail", [0, 1, 17])
+def test_long_parts(dev, B, Hkv, G, Q, dtype, tail):
+    """Parts of many tiles (cut for a short prefix), of every number of tiles at their end."""
+    rng = np.random.default_rng(13 + tail)
+    for tiles in (33, 36, 39, 42):
+        prefix, pre = make_rows(rng, [32 * tiles + tail] + [32 * tiles * 3] * (Hkv - 1), dtype, dev)
+        rows, kv = make_rows(rng, [7 + r % 5 for r in range(B * Hkv)], dtype, dev)
+        q = _q(rng, B, Hkv * G, Q, dtype, dev)
+        meta = lambda s: (s.k, s.v, s.row_tile_off, s.row_len)
+        got = ops.shared_attn(q, meta(prefix), meta(rows), Hkv, SCALE, prefix_tiles=0, row_tiles=1)
+        _check(got, q, pre, kv, G, SCALE, dtype)
+
+
+@pytest.mark.parametrize("B,Hkv,G,dtype", [(1, 64, 1, BF), (2, 65, 2, BF), (1, 130, 1, FP), (1, 200, 3, FL)])
+def test_many_kv_heads(dev, B, Hkv, G, dtype):
+    rng = np.random.default_rng(14)
+    prefix, pre = make_rows(rng, [(37 * h) % 300 for h in range(Hkv)], dtype, dev)
+    rows, kv = make_rows(rng, [(11 * r) % 70 for r in range(B * Hkv)], dtype, dev)
+    q = _q(rng, B, Hkv * G, 1, dtype, dev)
+    _check(rows.attend_shared(q, prefix, SCALE), q, pre, kv, G, SCALE, dtype)
