@@ -339,21 +339,26 @@ __global__ __launch_bounds__(kScoreWaves * 64) void block_score_kernel(const Sel
 }
 
 // The selection of one query by a workgroup of NT threads: the scores' keys (of
-// score_blocks itself where SCORED is not set, else from memory) in LDS, the
-// threshold, and one ordered pass that writes the kept blocks.  The threshold
+// score_blocks itself where SCORED is not set, by way of LDS, else from
+// memory) in registers, the threshold, and one ordered pass that writes the
+// kept blocks.  The threshold
 // is found by counting the keys into equal steps between the least and the
 // greatest left and going on in the step where the count of kept ones is
 // reached: scores of one query lie within a few powers of two, where fixed
 // digits of the key would pile up in few counters.  Bound by the latency of
 // its dependent steps; a barrier each for the keys, the counts (one or two
 // rounds) and the places.  128 blocks take 1 us of loads, 2 of scores and 2 of
-// selection; 4096 scored ones 2 and 6.
-constexpr int kPickKeys = 12288;  // keys in LDS; a longer row's are read again from memory each time
+// selection; 1000 scored ones a launch of 4.4, 4096 of 7.1.
+constexpr int kPickKeys = 12288;  // keys in LDS, of rows scored by the same workgroup
 template <int NT>
 struct Pick {
   static constexpr int kWaves = NT / 64;
-  static constexpr int kPer = NT == 1024 ? 16 : 4;  // counters that a lane reads in a row
+  static constexpr int kPer = NT / 64;  // counters that a lane reads in a row
   static constexpr int kBins = 64 * kPer;
+  // Keys that a thread keeps in registers; a longer row's scores are read
+  // again each time.
+  static constexpr int kHeld = NT == 1024 ? 32 : 12;
+  static constexpr int kBits = NT == 1024 ? 10 : NT == 512 ? 9 : 8;
   // One of padding after each row of them keeps the lanes on different banks.
   static constexpr int kSlots = 64 * (kPer + 1);
   static __device__ __forceinline__ int slot(uint32_t bin) { return (int)(bin + bin / kPer); }
@@ -364,7 +369,7 @@ struct Pick {
 
 // Writes the query's counts and list to memory and, where list is not null, to
 // LDS as well (a.keep entries; visible behind the next barrier); returns the
-// count.  s_key: min(a.max_blocks, kPickKeys) words of LDS.
+// count.  s_key: a.max_blocks words of LDS (SCORED: none).
 template <typename T, bool SCORED, int NT>
 __device__ __forceinline__ int pick_blocks(const SelectArgs& a, SelectJob& j, Pick<NT>& L, uint32_t* s_key,
                                            int32_t* list) {
@@ -397,14 +402,28 @@ __device__ __forceinline__ int pick_blocks(const SelectArgs& a, SelectJob& j, Pi
   if (need == 0) return kept;
   for (int k = tid; k < 2 * P::kSlots; k += NT) L.hist[0][k] = 0;
   const float* sc = SCORED ? a.scores + x * a.pitch + lo : nullptr;
-  const bool in_lds = !SCORED || nmid <= kPickKeys;
   uint32_t least = 0xffffffffu, most = 0u;
+  // Every thread keeps to a run of blocks; the keys of a short one stay in its
+  // registers.
+  const int run = (nmid + NT - 1) / NT;
+  const int k0 = min(tid * run, nmid), k1 = min(k0 + run, nmid);
+  const bool held = !SCORED || run <= P::kHeld;  // (launch_pick: rows scored here are short enough)
+  uint32_t mine[P::kHeld];
   if constexpr (SCORED) {
-    for (int k = tid; k < nmid; k += NT) {
-      const uint32_t u = order_key(sc[k]);
-      if (in_lds) s_key[k] = u;
-      least = min(least, u);
-      most = max(most, u);
+    if (held) {
+#pragma unroll
+      for (int e = 0; e < P::kHeld; ++e) {
+        if (e > 0 && e >= run) break;
+        mine[e] = order_key(sc[min(k0 + e, nmid - 1)]);
+        least = min(least, mine[e]);  // (a block past the end is the last one again)
+        most = max(most, mine[e]);
+      }
+    } else {
+      for (int k = tid; k < nmid; k += NT) {
+        const uint32_t u = order_key(sc[k]);
+        least = min(least, u);
+        most = max(most, u);
+      }
     }
   } else if (64 * wave < nmid) {
     ScoreBlocks<4> t;
@@ -432,21 +451,36 @@ __device__ __forceinline__ int pick_blocks(const SelectArgs& a, SelectJob& j, Pi
     least = min(least, L.lo[w]);
     most = max(most, L.hi[w]);
   }
-  auto key = [&](int k) { return in_lds ? s_key[k] : order_key(sc[k]); };
-  // Every thread keeps to a run of blocks.
-  const int run = (nmid + NT - 1) / NT;
-  const int k0 = min(tid * run, nmid), k1 = min(k0 + run, nmid);
+  if constexpr (!SCORED) {
+    if (held) {
+#pragma unroll
+      for (int e = 0; e < P::kHeld; ++e) {
+        if (e > 0 && e >= run) break;
+        mine[e] = s_key[min(k0 + e, nmid - 1)];
+      }
+    }
+  }
+  auto each = [&](auto f) {  // of the thread's run, in order: f(block, key)
+    if (held) {
+#pragma unroll
+      for (int e = 0; e < P::kHeld; ++e) {
+        if (e > 0 && e >= run) break;
+        if (k0 + e < k1) f(k0 + e, mine[e]);
+      }
+    } else {
+      for (int k = k0; k < k1; ++k) f(k, order_key(sc[k]));
+    }
+  };
 
   // Kept: the keys above T0, and the first `need` equal to it.
   uint32_t T0 = least;
   for (int round = 0; least < most; ++round) {
     const uint32_t span = most - least;
-    const int shift = max(32 - __clz((int)span) - (NT == 1024 ? 10 : 8), 0);
+    const int shift = max(32 - __clz((int)span) - P::kBits, 0);
     int* hist = L.hist[round & 1];
-    for (int k = k0; k < k1; ++k) {
-      const uint32_t u = key(k);
+    each([&](int, uint32_t u) {
       if (u >= least && u <= most) atomicAdd(&hist[P::slot((u - least) >> shift)], 1);
-    }
+    });
     __syncthreads();
     // Lane y reads kPer bins in a row from the top down; keys above its first
     // one, then the bin in which the need-th highest key lies (every wave for
@@ -484,11 +518,10 @@ __device__ __forceinline__ int pick_blocks(const SelectArgs& a, SelectJob& j, Pi
   }
 
   int gt = 0, eq = 0;
-  for (int k = k0; k < k1; ++k) {
-    const uint32_t u = key(k);
+  each([&](int, uint32_t u) {
     gt += u > T0;
     eq += u == T0;
-  }
+  });
   const int gt_in = wave_scan_add(gt), eq_in = wave_scan_add(eq);
   if (lane == 63) L.gt[wave] = gt_in, L.eq[wave] = eq_in;
   __syncthreads();
@@ -498,13 +531,12 @@ __device__ __forceinline__ int pick_blocks(const SelectArgs& a, SelectJob& j, Pi
     if (w < wave) gt0 += L.gt[w], eq0 += L.eq[w];
   int at = a.sink + gt0 + min(eq0, need);
   int left = max(need - eq0, 0);
-  for (int k = k0; k < k1; ++k) {
-    const uint32_t u = key(k);
+  each([&](int k, uint32_t u) {
     if (u > T0 || (u == T0 && left > 0)) {
       left -= u == T0;
       put(at++, lo + k);
     }
-  }
+  });
   return kept;
 }
 
@@ -564,16 +596,20 @@ constexpr int kSoloBlocks = 256;
 bool select_in_memory(int64_t jobs, int max_blocks) {
   return max_blocks > kPickKeys || (max_blocks > kSoloBlocks && jobs <= device_cus() / 2);
 }
-// Blocks that four waves pick from, sixteen beyond (8 queries of 512, 1024 and
-// 2048 blocks through memory: 9.4, 10.8 and 13.5 us with four, 10.7, 11.8 and
-// 12.6 with sixteen).
-constexpr int kFewBlocks = 1536;
+// Blocks that four waves pick from, and eight, sixteen beyond: keys that fit
+// the threads' registers, by as few waves as that takes (8 queries of 1024,
+// 2048, 4096 and 8192 blocks through memory: 8.9, 10.2, 21.5 and 29.8 us with
+// four, 9.0, 9.7, 12.7 and 20.6 with eight, 11.4, 11.7, 14.2 and 17.0 with
+// sixteen).
+constexpr int kFewBlocks = 1024, kMoreBlocks = 512 * Pick<512>::kHeld;
 
 template <typename T, bool SCORED>
 void launch_pick(const SelectArgs& a, dim3 grid, hipStream_t s) {
-  const size_t lds = (size_t)std::min(std::max(a.max_blocks, 1), kPickKeys) * sizeof(uint32_t);
+  const size_t lds = SCORED ? 0 : (size_t)std::max(a.max_blocks, 1) * sizeof(uint32_t);
   if (a.max_blocks <= kFewBlocks)
     hipLaunchKernelGGL((block_pick_kernel<T, SCORED, 256>), grid, dim3(256), lds, s, a);
+  else if (a.max_blocks <= kMoreBlocks)
+    hipLaunchKernelGGL((block_pick_kernel<T, SCORED, 512>), grid, dim3(512), lds, s, a);
   else
     hipLaunchKernelGGL((block_pick_kernel<T, SCORED, 1024>), grid, dim3(1024), lds, s, a);
 }

@@ -185,6 +185,9 @@ __device__ __forceinline__ float dpp_mov(float v) {
 // every lane, by DPP moves (a __shfl step is a round trip through the LDS
 // crossbar).
 __device__ __forceinline__ int wave_scan_add(int v) {
+  // Opaque: where the compiler knows some lanes' values it may run those lanes
+  // apart, and the moves would miss them.
+  asm("" : "+v"(v));
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
   v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);  // row_shr:2
   v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);  // row_shr:4

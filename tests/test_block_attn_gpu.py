@@ -7,7 +7,7 @@ import torch
 
 from heterocache_amd import _lib, ops
 from heterocache_amd.store import KVStore
-from tests.serving_util import D, attend, bounds, close, make_rows, select
+from tests.serving_util import D, attend, bounds, close, exponent, make_rows, select
 
 pytestmark = pytest.mark.gpu
 BF, FP, FL = torch.bfloat16, torch.float16, torch.float32
@@ -290,3 +290,35 @@ def test_refusals(dev):
         ops.block_attn(q, rows.k, rows.v, rows.row_tile_off, rows.row_len, idx[:1], counts, 32, SCALE)
     with pytest.raises(_lib.HCError, match="block"):
         ops.block_attn(q, rows.k, rows.v, rows.row_tile_off, rows.row_len, idx, counts, 40, SCALE)
+
+
+@pytest.mark.parametrize("blocks", [255, 256, 257, 1023, 1026, 2051, 6140, 6148, 12290, 32765, 32780])
+def test_every_way_to_hold_the_keys(dev, blocks):
+    """Row lengths around each change of the selection's launch, with many equal scores, against sorting."""
+    rng = np.random.default_rng(blocks)
+    B, Hkv, G, keep = 2, 2, 3, 40
+    lens = [32 * blocks - 7, 32 * (blocks // 2) + 1, 32 * 41, 32 * (blocks - 1) + 1]
+    hi = rng.integers(-127, 128, (B * Hkv * blocks, D)).astype(np.int8)
+    hi[1::3] = hi[::3][:len(hi[1::3])]  # pairs of equal blocks
+    lo = np.minimum(hi, rng.integers(-127, 128, hi.shape)).astype(np.int8)
+    lo[1::3] = lo[::3][:len(lo[1::3])]
+    ex = np.full(len(hi), -5, np.int8)
+    table = torch.as_tensor(np.stack([hi, lo], 1)).to(dev)
+    off = torch.arange(B * Hkv, device=dev) * blocks
+    q = _q(rng, B, Hkv * G, 1, BF, dev)
+    idx, counts = ops.block_select(q, table, torch.as_tensor(ex).to(dev), off,
+                                   torch.tensor(lens, dtype=torch.int32, device=dev), 32, blocks, keep, sink=1, local=2)
+    hi, lo = hi.astype(np.int64), lo.astype(np.int64)
+    for r in range(B * Hkv):
+        b, h = divmod(r, Hkv)
+        have = -(-lens[r] // 32)
+        score = np.full(have, -np.inf)
+        at = slice(r * blocks + 1, r * blocks + have - 2)
+        for row in q[b, h * G:(h + 1) * G, 0].double().cpu().numpy():
+            eq = exponent(np.abs(row).max())
+            q8 = np.clip(np.rint(row / 2.0 ** eq), -127, 127).astype(np.int64)
+            s = np.maximum(q8 * hi[at], q8 * lo[at]).sum(1) * 2.0 ** (eq - 5)
+            score[1:have - 2] = np.maximum(score[1:have - 2], s)
+        score[:1] = score[have - 2:] = np.inf
+        want = np.sort(np.lexsort((np.arange(have), -score))[:keep])
+        assert int(counts[r, 0]) == keep and np.array_equal(idx[r, 0].cpu().numpy(), want), r
