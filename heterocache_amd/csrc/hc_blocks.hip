@@ -52,7 +52,6 @@ struct BoundArgs {
   int8_t *bounds, *exps;
   int rows, tpb, span;  // span: blocks a row, the last complete ones
   int fresh;            // > 0: only blocks that the last `fresh` tokens completed
-  int per;              // blocks a workgroup takes
 };
 
 // The greater of two values, the other one where one is NaN: one instruction,
@@ -84,16 +83,16 @@ __device__ __forceinline__ float row16_max_scatter(float (&v)[16], int lane) {
 // is 1 KB in a row.  A thread folds the greatest values of its 8 channels and
 // of their negatives, the 16 lanes m of a channel group fold theirs, and each
 // rounds one of the 16 (floor(x) = -ceil(-x)).  Bound by the key stream: a
-// workgroup takes `per` blocks of a row one after another, the next one's
-// first tiles (two; ONE: blocks of one tile) on their way while one is folded
-// and written.
+// workgroup takes every chunks-th block of a row one after another, so that
+// neighbouring workgroups read neighbouring blocks (runs of blocks each: 46.4
+// us against 41.6 for 258 MB), the next one's first tiles (two; ONE: blocks of
+// one tile) on their way while one is folded and written.
 template <typename T, bool ONE>
 __global__ __launch_bounds__(256) void block_bounds_kernel(const BoundArgs a) {
   typedef typename Elem<T>::vec8 vec8;
   __shared__ float s_top[2][4];
-  // Neighbouring workgroups read neighbouring blocks.
   const int chunks = gridDim.x / a.rows;
-  const int row = blockIdx.x / chunks, j0 = blockIdx.x % chunks * a.per;
+  const int row = blockIdx.x / chunks, j0 = blockIdx.x % chunks;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row_at = a.row_tile_off[row], blk_at = a.row_blk_off[row];
   const int len = max(a.row_len[row], 0), S = a.tpb * HC_TILE;
@@ -101,7 +100,7 @@ __global__ __launch_bounds__(256) void block_bounds_kernel(const BoundArgs a) {
   // before the last `fresh` tokens are left.
   const int have = len / S;
   const int old = a.fresh > 0 ? max(len - a.fresh, 0) / S : 0;
-  const int first = have - 1 - j0, last = max(max(first - a.per + 1, old), have - a.span);
+  const int first = have - 1 - j0, last = max(old, have - a.span);
   if (first < last) return;
   const T* kb = reinterpret_cast<const T*>(a.kstore) + tid * 8;
   constexpr int kLoads = ONE ? 2 : 4;
@@ -114,7 +113,8 @@ __global__ __launch_bounds__(256) void block_bounds_kernel(const BoundArgs a) {
     }
   };
   fetch(kb + (row_at + (int64_t)first * a.tpb) * HC_TILE_ELEMS, a.tpb > 1);
-  for (int j = first; j >= last; --j) {
+  int turn = 0;
+  for (int j = first; j >= last; j -= chunks) {
     float v[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = -INFINITY;
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(256) void block_bounds_kernel(const BoundArgs a) {
         fetch(kb + (row_at + (int64_t)j * a.tpb + t) * HC_TILE_ELEMS, t + 1 < a.tpb);
         fold();
       }
-    fetch(kb + (row_at + (int64_t)max(j - 1, last) * a.tpb) * HC_TILE_ELEMS, a.tpb > 1);  // (at the end the last again)
+    fetch(kb + (row_at + (int64_t)max(j - chunks, last) * a.tpb) * HC_TILE_ELEMS, a.tpb > 1);  // (at the end the last again)
     const float mine = row16_max_scatter(v, lane);
     // The greatest |k| is the greatest of all 16 values of all groups.
     float top = greater(mine, dpp_mov<0xB1>(mine));
@@ -142,7 +142,8 @@ __global__ __launch_bounds__(256) void block_bounds_kernel(const BoundArgs a) {
     top = greater(top, dpp_mov<0x124>(top));
     top = greater(top, dpp_mov<0x128>(top));
     top = rows4_max(top);
-    float* st = s_top[j & 1];
+    float* st = s_top[turn];
+    turn ^= 1;
     if (lane == 0) st[wave] = top;
     // Only LDS is waited for: the next block's loads stay in flight.
     asm volatile("" ::: "memory");
@@ -634,12 +635,12 @@ extern "C" int hc_block_bounds(int dtype, const void* kstore, const int64_t* row
   if ((reinterpret_cast<uintptr_t>(kstore) | reinterpret_cast<uintptr_t>(bounds)) & 15)
     return set_error(HC_ERR_INVALID, "hc_block_bounds: the store and the bounds must be 16-byte aligned");
   // One resident round of workgroups, each with its share of a row's blocks (16
-  // rows of 1025 blocks of 64 tokens: 71, 60, 53 and 50 us with 1, 2, 4 and 8
-  // blocks a workgroup).
+  // rows of 1023 blocks of 64 tokens: 48.8, 47.3, 44.0 and 42.8 us with 3, 4, 8
+  // and 16 workgroups a CU; 256 rows of 32: 24.0, 24.1, 28.3 and 31.1).
   const int per = (int)std::min<int64_t>(std::max<int64_t>((int64_t)rows * span / (8 * device_cus()), 1), 64);
   const int64_t grid = (int64_t)rows * ((span + (int64_t)per - 1) / per);
   if (grid > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_block_bounds: %d rows x %d blocks", rows, span);
-  BoundArgs a = {kstore, row_tile_off, row_block_off, row_len, bounds, exps, rows, block / HC_TILE, span, fresh, per};
+  BoundArgs a = {kstore, row_tile_off, row_block_off, row_len, bounds, exps, rows, block / HC_TILE, span, fresh};
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
     case HC_DTYPE_BF16: launch_bounds<__bf16>(a, (unsigned)grid, s); break;
