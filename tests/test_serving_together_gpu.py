@@ -320,3 +320,20 @@ def test_refusals(dev):
     g.replay()
     torch.cuda.synchronize()
     assert mark.item() == 1.0 and (rows.host_len == lens).all()
+
+
+@pytest.mark.parametrize("dtype", [FP, FL])
+def test_captured_prefix_of_every_type(dev, dtype):
+    """attend_shared captured before the rows grow: replays see the device's lengths."""
+    feed = Feed(9, 2, 4, dtype, dev)
+    prefix, rows = KVStore([500] * 2, dtype, dev), KVStore([120] * 4, dtype, dev)
+    _append(prefix, feed([0], 437))
+    q = _append(rows, feed([437] * 2, 9))[:, :, -2:].contiguous()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = rows.attend_shared(q, prefix, SCALE)
+    for n in (0, 1, 60, 40):
+        if n:
+            q.copy_(_append(rows, feed([446] * 2, max(n, 2)), [n, n])[:, :, :2])
+        g.replay()
+        _check_shared(out, q, prefix, rows)
