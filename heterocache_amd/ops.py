@@ -856,6 +856,13 @@ def _strides3(*layouts):
                                                    for n, s in zip(shape[:3], strides)])
 
 
+@functools.lru_cache(maxsize=256)
+def _append_strides(qsh, qst, ost, ksh, kst, vst):
+    """The four stride triples of an append, and their address."""
+    a = (ctypes.c_int64 * 12)(*_strides3((qsh, qst), (qsh, ost), (ksh, kst), (ksh, vst)))
+    return a, ctypes.addressof(a)
+
+
 def _out_bthd(q, out, shape, dev):
     """The [B, T, Hq, 128] output of queries [B, Hq, T, 128], and its strides."""
     B, Hq, T, D = shape
@@ -907,7 +914,10 @@ def append_rotated(q, k, v, cos, sin, kstore, vstore, row_tile_off, row_len, row
     the new lengths: row_len itself, or another tensor.  A row without room is
     left as it is and sets bit 0 of status (int32 device word; read_status)."""
     dt, dev = q.dtype, q.get_device()
-    qsh, ksh, vsh = _queries(q), _queries(k), _queries(v)
+    qsh, qst, ksh, kst, vsh, vst = q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride()
+    if (len(qsh) != 4 or len(ksh) != 4 or vsh != ksh or qsh[3] != HEAD_DIM or ksh[3] != HEAD_DIM
+            or not qst[3] == kst[3] == vst[3] == 1):
+        _queries(q), _queries(k), _queries(v)
     B, Hq, T, _ = qsh
     Hkv = ksh[1]
     if k.dtype is not dt or v.dtype is not dt:
@@ -942,13 +952,17 @@ def append_rotated(q, k, v, cos, sin, kstore, vstore, row_tile_off, row_len, row
             raise ValueError("len_out overlaps row_len without being it")
     if out is None:
         out = torch.empty_like(q)
-        if out.stride(3) != 1:
+        ost = out.stride()
+        if ost[3] != 1:
             out = torch.empty(qsh, dtype=dt, device=q.device)
+            ost = out.stride()
     elif out.shape != qsh or out.dtype is not dt or out.get_device() != dev or (out.stride(3) != 1 and out.numel()):
         raise ValueError(f"out must be {tuple(qsh)} of {dt} on {q.device} with unit channel stride")
-    elif any(n > 1 and s == 0 for n, s in zip(qsh, out.stride())):
-        raise ValueError("out is an expanded tensor, whose entries share memory")
-    base = ctypes.addressof(_strides3((qsh, q.stride()), (qsh, out.stride()), (ksh, k.stride()), (ksh, v.stride())))
+    else:
+        ost = out.stride()
+        if any(n > 1 and s == 0 for n, s in zip(qsh, ost)):
+            raise ValueError("out is an expanded tensor, whose entries share memory")
+    strides, base = _append_strides(qsh, qst, ost, ksh, kst, vst)  # (held until the call is made)
     _lib.check(_lib.load().hc_append_rotated(
         dtype_code(dt), dtype_code(ct), q.data_ptr(), base, out.data_ptr(), base + 24, k.data_ptr(), base + 48,
         v.data_ptr(), base + 72, cos.data_ptr(), sin.data_ptr(), cst[0] if len(csh) == 3 and csh[0] > 1 else 0,
