@@ -314,9 +314,16 @@ __device__ __forceinline__ void rows4_transpose(float (&e)[4]) {
 __device__ __forceinline__ void lds_dma16(const void* src, void* lds) {
   __builtin_amdgcn_global_load_lds(src, lds, 16, 0, 0);
 }
-// lds_dma16 with the nontemporal hint, for data that one workgroup reads.
-__device__ __forceinline__ void lds_dma16_stream(const void* src, void* lds) {
-  __builtin_amdgcn_global_load_lds(src, lds, 16, 0, 2);
+// N of them in a row, 1 KB apart on both sides (the instruction's own offset,
+// which it adds to both); STREAM: with the nontemporal hint, for data that one
+// workgroup reads.
+template <int N, bool STREAM, int I = 0>
+__device__ __forceinline__ void lds_dma16_run(const void* src, void* lds) {
+  static_assert(N <= 4, "the offset field ends at 4095");
+  if constexpr (I < N) {
+    __builtin_amdgcn_global_load_lds(src, lds, 16, 1024 * I, STREAM ? 2 : 0);
+    lds_dma16_run<N, STREAM, I + 1>(src, lds);
+  }
 }
 // s_waitcnt vmcnt(0): every LDS-DMA load of this wave has landed.
 __device__ __forceinline__ void wait_lds_dma() { __builtin_amdgcn_s_waitcnt(0x0f70); }

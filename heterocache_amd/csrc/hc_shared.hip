@@ -17,6 +17,11 @@
 //    former are bound by the matrix cores and the latter by HBM, so they run
 //    on the same CUs at once.
 //  * merge_kernel (hc_rows.hip): one fold of a column's partials.
+// In bf16: 32 sequences x 32 heads behind 178K prefix tokens of 8 heads, own
+// rows of up to 512: 32 + 4.3 us, of which the bytes (128 MB) need 18 and a
+// workgroup's start and end 8 to 10; 128 sequences behind 756K tokens, 1.06M of
+// their own: 250 + 9 us, the prefix alone 190 (1.04 PFLOP/s, 68 % of the issue
+// slots taken), the rows alone 100 (5.4 TB/s).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -28,8 +33,8 @@ namespace {
 
 constexpr int kPreWaves = 4;
 constexpr int kPreThreads = kPreWaves * 64;
-// Slots of a tile's keys in LDS; of its values there is one less.  (One more
-// slot changes no time by more than 2 %.)
+// Slots of tiles in LDS, of keys and of values (one more or less changes no
+// time by more than 2 %).
 constexpr int kRing = 4;
 
 struct PrefixArgs {
@@ -140,7 +145,7 @@ __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
 
   // Q^T operands: column col0 + 16j + n16, k-slots = channels 32s + 8*g4 + [0, 8).
   const int64_t col0 = ((int64_t)cg * kPreWaves + wave) * 16 * NC;
-  const bool active = col0 < a.M;
+  const int active = __builtin_amdgcn_readfirstlane(col0 < a.M);
   vec8 qop[NC][4];
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
@@ -162,38 +167,30 @@ __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
   const int n = t1 - t0;
   const char* kb = reinterpret_cast<const char*>(a.kstore) + (tile0 + t0) * (int64_t)kTileBytes;
   const char* vb = reinterpret_cast<const char*>(a.vstore) + (tile0 + t0) * (int64_t)kTileBytes;
-  char* const ring = reinterpret_cast<char*>(lds) + 1024 * wave;
+  char* const ring = reinterpret_cast<char*>(lds) + 1024 * kLoads * wave;
   const float scale_log2 = a.scale_log2;
-  auto copy = [&](const char* src, char* dst) {
+  auto copy = [&](const char* src, int slot) {  // slots: kRing of keys, then kRing of values
+    // A 32-bit offset from a scalar base, which the compiler forgets once it
+    // has widened it outside of the loop.
+    uint32_t own = 1024 * kLoads * wave + 16 * lane;
+    asm volatile("" : "+v"(own));
+    lds_dma16_run<kLoads, ONCE>(src + own, ring + slot * kTileBytes);
+  };
+  auto stage_k = [&](int slot) {  // the next keys, the next values
+    copy(kb, slot);
+    kb += kTileBytes;
+  };
+  auto stage_v = [&](int slot) {
+    copy(vb, kRing + slot);
+    vb += kTileBytes;
+  };
+  static_assert(kRing == 4, "slots i % 4 and their neighbours by ^ 2");
+  stage_k(0);
+  if (1 < n) stage_k(1);
 #pragma unroll
-    for (int r = 0; r < kLoads; ++r) {
-      // A 32-bit offset from a scalar base, which the compiler forgets once it
-      // has widened it outside of the loop.
-      uint32_t own = 16 * tid;
-      asm volatile("" : "+v"(own));
-      const char* p = src + 16 * r * kPreThreads + own;
-      if constexpr (ONCE)
-        lds_dma16_stream(p, dst + 16 * r * kPreThreads);
-      else
-        lds_dma16(p, dst + 16 * r * kPreThreads);
-    }
-  };
-  auto after = [](int s, int slots) { return s == slots - 1 ? 0 : s + 1; };
-  int kin = 0, vin = 0;  // slots of the next keys and values to stage
-  auto stage_k = [&]() {
-    copy(kb, ring + kin * kTileBytes);
-    kb += kTileBytes, kin = after(kin, kRing);
-  };
-  auto stage_v = [&]() {
-    copy(vb, ring + (kRing + vin) * kTileBytes);
-    vb += kTileBytes, vin = after(vin, kRing - 1);
-  };
-  stage_k();
-  if (1 < n) stage_k();
-#pragma unroll
-  for (int i = 0; i < kRing - 2; ++i) {
-    if (i + 2 < n) stage_k();
-    if (i < n) stage_v();
+  for (int i = 0; i < 2; ++i) {
+    if (i + 2 < n) stage_k(i + 2);
+    if (i < n) stage_v(i);
   }
 
   f32x4 o[8][NC], s[2][2][NC];  // s: of the tile attended, and of the next one, in turn
@@ -230,29 +227,29 @@ __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
     for (int x = 0; x < 8; ++x) kr[x] = key_at(lds + HC_TILE_ELEMS, x);
   }
 
-  int kout = after(1, kRing), vout = 0;
+  int slot = 0;  // i % kRing
   // One tile, i, with tile i + 1's scores and the product of tile i - 1's
   // values on the matrix cores while the vector unit forms the probabilities
   // between them: kr holds the keys of tile i + 1, vr and pb the values and
   // probabilities of tile i - 1, and each operand is read from LDS again, for
-  // the next step, once it is used.  STEADY: kRing tiles or more follow.
+  // the next step, once it is used.  STEADY: four tiles or more follow.
   // (Behind the last tile: products of stale slots, which nothing reads.)
   auto step = [&](auto steady, int i, f32x4(&sc)[2][NC], f32x4(&sn)[2][NC]) {
     constexpr bool STEADY = decltype(steady)::value;
     // This wave's loads of batch i have landed, and past the barrier every
     // wave's have, while the younger ones stay in flight; every wave is also
-    // done with the keys of tile i + 1 and the values of tile i - 1: batch
-    // i + kRing - 2 takes the slots of the keys of tile i and of those values.
+    // done with the keys of tile i + 1 and the values of tile i - 1: batch i + 2
+    // takes the slots of the keys of tile i and of the values of tile i - 2.
     if constexpr (STEADY)
-      wait_lds_dma_but<(kRing - 3) * 2 * kLoads>();
+      wait_lds_dma_but<2 * kLoads>();
     else  // younger values, and keys
-      wait_dma_units<2 * (kRing - 3), kLoads>(min(n - 1 - i, kRing - 3) + max(min(n - 3 - i, kRing - 3), 0));
+      wait_dma_units<2, kLoads>((i + 1 < n) + (i + 3 < n));
     lds_barrier();
-    if (STEADY || i + kRing < n) stage_k();
-    if (STEADY || i + kRing - 2 < n) stage_v();
-    const T* sk = lds + kout * HC_TILE_ELEMS;
-    const T* sv = lds + (kRing + vout) * HC_TILE_ELEMS + lane * 8;
-    kout = after(kout, kRing), vout = after(vout, kRing - 1);
+    if (STEADY || i + 4 < n) stage_k(slot);
+    if (STEADY || i + 2 < n) stage_v(slot ^ 2);
+    const T* sk = lds + (slot ^ 2) * HC_TILE_ELEMS;
+    const T* sv = lds + (kRing + slot) * HC_TILE_ELEMS + lane * 8;
+    slot = (slot + 1) & 3;
     if (!active) return;
     if constexpr (!STEADY) {
       const int left = len - (t0 + i) * HC_TILE;  // tokens from this tile on
@@ -369,7 +366,7 @@ __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
 // LDS of a workgroup: the prefix ring, or the row waves' states.
 template <typename T>
 constexpr size_t shared_lds(bool prefix) {
-  const size_t ring = (size_t)(2 * kRing - 1) * HC_TILE_ELEMS * sizeof(T), rows = kRowsLds * sizeof(float);
+  const size_t ring = (size_t)2 * kRing * HC_TILE_ELEMS * sizeof(T), rows = kRowsLds * sizeof(float);
   return prefix && ring > rows ? ring : rows;
 }
 
