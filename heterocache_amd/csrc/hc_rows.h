@@ -8,6 +8,8 @@
 // (at most log2(kRowsLazy) below their maximum), l, its share of the sum of
 // exp2(score - m), and o[mt][j] = O^T[16 mt + 4 g + j][column].
 #pragma once
+#include <type_traits>
+
 #include "hc_common.h"
 
 namespace hc {
@@ -289,11 +291,11 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds, 
     int tile = tile_of(0);
     load_operands<T>(kr, kb + (int64_t)max(tile, 0) * HC_TILE_ELEMS);
     load_operands<T>(vr, vb + (int64_t)max(tile, 0) * HC_TILE_ELEMS);
-    for (int i = 0; i < nt; ++i) {
-      // The next tile's loads are unconditional (the last reads itself
-      // again), so that each wait leaves the younger half tile in flight.
-      const int next = tile_of(min(i + 1, nt - 1));
-      const int64_t at = (int64_t)max(next, 0) * HC_TILE_ELEMS;
+    // One tile, and the loads of the next one (LAST: there is none), so that
+    // each wait leaves the younger half tile in flight.
+    auto step = [&](auto last, int next) {
+      constexpr bool LAST = decltype(last)::value;
+      const int64_t at = LAST ? 0 : (int64_t)max(next, 0) * HC_TILE_ELEMS;
       const bool live = !LIST || tile >= 0;
       const int tok0 = max(tile, 0) * HC_TILE;
       const int lo = live ? lim_lo : 0, hi = live ? lim_hi : 0, mylim = live ? lim : 0;
@@ -303,7 +305,7 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds, 
       f32x4 s[2];
       tile_scores<T>(kr, qreg, s);
       __builtin_amdgcn_sched_barrier(0);
-      if (!mixed) load_operands<T>(kr, kb + at);
+      if (!LAST && !mixed) load_operands<T>(kr, kb + at);
       __builtin_amdgcn_sched_barrier(0);
       if (tok0 + HC_TILE > lo) {
 #pragma unroll
@@ -313,15 +315,18 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds, 
       const vec8 pb = tile_probs<T>(s, a.scale_log2, m, l, o);
       if (mixed) {
         tile_values<T, true>(vr, pb, tok0, hi, g, o);
-        load_operands<T>(kr, kb + at);
+        if (!LAST) load_operands<T>(kr, kb + at);
       } else {
         tile_values<T, false>(vr, pb, tok0, hi, g, o);
       }
+      if (LAST) return;
       __builtin_amdgcn_sched_barrier(0);
       load_operands<T>(vr, vb + at);
       __builtin_amdgcn_sched_barrier(0);
       tile = next;
-    }
+    };
+    for (int i = 1; i < nt; ++i) step(std::false_type{}, tile_of(i));
+    step(std::true_type{}, 0);
   }
   l = rows4_sum(l);
   if (LIST && void_list) m = 0.f, l = NAN;
