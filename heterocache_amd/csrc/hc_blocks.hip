@@ -741,11 +741,13 @@ struct BlockPlan {
 };
 BlockPlan block_plan(int batch, int kv_heads, int G, int queries, int block, int keep) {
   // The least estimate in us: a wave's tiles one after another (2.4 each, the
-  // latency of scattered blocks, behind 2.2 of start and end: 7.2, 22.8 and
-  // 32.6 for 2, 8 and 12; more where the tiles of all waves on the device take
-  // longer to stream) in as many rounds as the device needs; a split adds the
-  // launch that folds it.  A CU holds three
-  // workgroups of four waves or one of eight, which have at most 8 columns.
+  // latency of scattered blocks, behind 3.3 of start and end: 5.7, 8.6, 13.5,
+  // 23.1 and 42.4 for 1, 2, 4, 8 and 16; more where the tiles of all waves on
+  // the device take longer to stream) in as many rounds as the device needs; a
+  // split adds the launch that folds it.  A CU holds three workgroups of four
+  // waves or one of eight, which have at most 8 columns.  (8 to 512 queries of
+  // 4 to 256 tiles: within 8 % of the best of twenty choices, but for 1.23 at 64
+  // queries of 32 and 1.13 at 128 of 128.)
   BlockPlan p = {4, 1, 0, 0};
   const int64_t jobs = (int64_t)batch * kv_heads * queries, tiles = (int64_t)keep * (block / HC_TILE);
   double best = 0.;
@@ -755,8 +757,8 @@ BlockPlan block_plan(int batch, int kv_heads, int G, int queries, int block, int
       const int64_t slots = (int64_t)device_cus() * (waves == 8 ? 1 : 3);
       const double rounds = (double)((jobs * ns + slots - 1) / slots);
       const double load = (double)std::min(jobs * ns, slots) * waves * HC_TILE_ELEMS * 4. / 5.5e6;
-      const double own = 2.2 + std::max(2.4, load) * (double)((tiles + waves * ns - 1) / (waves * ns));
-      const double t = rounds * own + (ns > 1 ? 4.5 : 0.);
+      const double own = 3.3 + std::max(2.4, load) * (double)((tiles + waves * ns - 1) / (waves * ns));
+      const double t = rounds * own + (ns > 1 ? 4. : 0.);
       if (best == 0. || t < best * 0.98) best = t, p.waves = waves, p.nsplit = ns;
     }
   const size_t cols = (size_t)batch * kv_heads * queries * G * p.nsplit;
