@@ -18,10 +18,10 @@
 //    on the same CUs at once.
 //  * merge_kernel (hc_rows.hip): one fold of a column's partials.
 // In bf16: 32 sequences x 32 heads behind 178K prefix tokens of 8 heads, own
-// rows of up to 512: 32 + 4.3 us, of which the bytes (128 MB) need 18 and a
+// rows of up to 512: 27 to 31 + 4 us, of which the bytes (128 MB) need 18 and a
 // workgroup's start and end 8 to 10; 128 sequences behind 756K tokens, 1.06M of
-// their own: 250 + 9 us, the prefix alone 190 (1.04 PFLOP/s, 68 % of the issue
-// slots taken), the rows alone 100 (5.4 TB/s).
+// their own: 240 to 255 + 9 us, the prefix alone 190 (1.04 PFLOP/s, 68 % of the
+// issue slots taken), the rows alone 92 (5.9 TB/s).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
