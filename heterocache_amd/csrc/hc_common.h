@@ -198,6 +198,7 @@ __device__ __forceinline__ int wave_scan_add(int v) {
 }
 template <typename F>
 __device__ __forceinline__ uint32_t wave_fold(uint32_t v, F f) {
+  asm("" : "+v"(v));  // (as above)
   v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));   // quad_perm [1,0,3,2]
   v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));   // quad_perm [2,3,0,1]
   v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x124, 0xF, 0xF, false));  // row_ror:4

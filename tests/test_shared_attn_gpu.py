@@ -235,3 +235,18 @@ def test_many_kv_heads(dev, B, Hkv, G, dtype):
     rows, kv = make_rows(rng, [(11 * r) % 70 for r in range(B * Hkv)], dtype, dev)
     q = _q(rng, B, Hkv * G, 1, dtype, dev)
     _check(rows.attend_shared(q, prefix, SCALE), q, pre, kv, G, SCALE, dtype)
+
+
+@pytest.mark.parametrize("B,Hkv,G,Q,dtype,tiles", [
+    (20, 8, 4, 1, BF, 8192), (32, 2, 16, 1, FP, 24000), (32, 8, 4, 1, BF, 5558), (16, 4, 7, 4, FP, 1537),
+    (33, 2, 4, 1, BF, 300000), (6, 3, 5, 2, FP, 20000),
+])
+def test_cut_for_other_sizes(dev, B, Hkv, G, Q, dtype, tiles):
+    """Column blocks and parts as they are chosen for long prefixes, over short ones."""
+    rng = np.random.default_rng(tiles)
+    prefix, pre = make_rows(rng, [(1500, 40, 0, 701, 32, 33, 1, 900)[h] for h in range(Hkv)], dtype, dev)
+    rows, kv = make_rows(rng, [(5, 40, 64)[r % 3] + Q for r in range(B * Hkv)], dtype, dev)
+    q = _q(rng, B, Hkv * G, Q, dtype, dev)
+    meta = lambda s: (s.k, s.v, s.row_tile_off, s.row_len)
+    got = ops.shared_attn(q, meta(prefix), meta(rows), Hkv, SCALE, prefix_tiles=tiles, row_tiles=4)
+    _check(got, q, pre, kv, G, SCALE, dtype)
