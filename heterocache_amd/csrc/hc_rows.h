@@ -41,15 +41,28 @@ __device__ __forceinline__ void zero_tail(typename Elem<T>::vec8& v, int tok0, i
 }
 
 // S^T of a tile's 32 tokens: element e of the pair (s[e / 4][e % 4]) is token
-// 16 (e / 4) + 4 g + e % 4 against the lane's column.
+// 16 (e / 4) + 4 g + e % 4 against the lane's column.  In fp32, where these sums
+// are the largest error, four of 32 channels each are formed apart: a rounding
+// is half a step of the partial sum that it falls on.
 template <typename T>
 __device__ __forceinline__ void tile_scores(const typename Elem<T>::vec8 (&kr)[8],
                                             const typename Elem<T>::vec8 (&qreg)[4], f32x4 (&s)[2]) {
-  s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    s[0] = mma_16x16x32(kr[x], qreg[x], s[0]);
-    s[1] = mma_16x16x32(kr[4 + x], qreg[x], s[1]);
+    for (int h = 0; h < 2; ++h) {
+      f32x4 part[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) part[x] = mma_16x16x32(kr[4 * h + x], qreg[x], zero);
+      s[h] = (part[0] + part[1]) + (part[2] + part[3]);
+    }
+  } else {
+    s[0] = s[1] = zero;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      s[0] = mma_16x16x32(kr[x], qreg[x], s[0]);
+      s[1] = mma_16x16x32(kr[4 + x], qreg[x], s[1]);
+    }
   }
 }
 

@@ -263,17 +263,19 @@ __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
       }
     }
     float pv[NC][8], ps[NC];
+    f32x4 upper[2][NC];  // fp32: the sums over the upper 64 channels apart (see tile_scores)
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
       ps[j] = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) sn[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int h = 0; h < 2; ++h) sn[h][j] = upper[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
-        sn[x & 1][j] = mma_16x16x32(kr[x], qop[j][x >> 1], sn[x & 1][j]);
+        f32x4& acc = sizeof(T) == 4 && x >= 4 ? upper[x & 1][j] : sn[x & 1][j];
+        acc = mma_16x16x32(kr[x], qop[j][x >> 1], acc);
         o[x][j] = mma_16x16x32(vr[x], pb[j], o[x][j]);
         pv[j][x] = fast_exp2(fmaf(sc[x >> 2][j][x & 3], scale_log2, -m[j]));
         ps[j] += pv[j][x];
@@ -281,6 +283,12 @@ __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
       kr[x] = key_at(sk, x);
       vr[x] = load8<T>(sv + x * 512);
       __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) sn[h][j] += upper[h][j];
     }
     bool fine = ps[0] <= kRowsLazy;
 #pragma unroll
