@@ -404,20 +404,30 @@ __device__ __forceinline__ int pick_blocks(const SelectArgs& a, SelectJob& j, Pi
   for (int k = tid; k < 2 * P::kSlots; k += NT) L.hist[0][k] = 0;
   const float* sc = SCORED ? a.scores + x * a.pitch + lo : nullptr;
   uint32_t least = 0xffffffffu, most = 0u;
-  // Every thread keeps to a run of blocks; the keys of a short one stay in its
-  // registers.
-  const int run = (nmid + NT - 1) / NT;
-  const int k0 = min(tid * run, nmid), k1 = min(k0 + run, nmid);
+  // Every thread keeps to a run of blocks, the keys of a short one in its
+  // registers.  SCORED: a run starts at a multiple of four blocks of the row, for
+  // 16-byte loads (what lies in front of the first scored block and behind the
+  // last is not used).
+  const int span = SCORED ? j.hi : nmid, skip = SCORED ? lo : 0;
+  const int run = SCORED ? ((span + NT - 1) / NT + 3) / 4 * 4 : (span + NT - 1) / NT;
+  const int k0 = min(tid * run, span) - skip, k1 = min(tid * run + run, span) - skip;
   const bool held = !SCORED || run <= P::kHeld;  // (launch_pick: rows scored here are short enough)
   uint32_t mine[P::kHeld];
   if constexpr (SCORED) {
     if (held) {
+      const float* row = sc - lo;
 #pragma unroll
-      for (int e = 0; e < P::kHeld; ++e) {
+      for (int e = 0; e < P::kHeld; e += 4) {
         if (e > 0 && e >= run) break;
-        mine[e] = order_key(sc[min(k0 + e, nmid - 1)]);
-        least = min(least, mine[e]);  // (a block past the end is the last one again)
-        most = max(most, mine[e]);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(row + min((int64_t)tid * run + e, a.pitch - 4));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          mine[e + u] = order_key(v[u]);
+          if (k0 + e + u >= 0 && k0 + e + u < k1) {
+            least = min(least, mine[e + u]);
+            most = max(most, mine[e + u]);
+          }
+        }
       }
     } else {
       for (int k = tid; k < nmid; k += NT) {
@@ -466,10 +476,10 @@ __device__ __forceinline__ int pick_blocks(const SelectArgs& a, SelectJob& j, Pi
 #pragma unroll
       for (int e = 0; e < P::kHeld; ++e) {
         if (e > 0 && e >= run) break;
-        if (k0 + e < k1) f(k0 + e, mine[e]);
+        if (k0 + e >= 0 && k0 + e < k1) f(k0 + e, mine[e]);
       }
     } else {
-      for (int k = k0; k < k1; ++k) f(k, order_key(sc[k]));
+      for (int k = max(k0, 0); k < k1; ++k) f(k, order_key(sc[k]));
     }
   };
 
@@ -727,8 +737,9 @@ extern "C" int hc_block_select(int dtype, const void* q, const int64_t* q_stride
                              batch, q_heads, kv_heads, queries, block, max_blocks, keep, sink, local, idx, counts, a);
   if (rc || batch == 0 || queries == 0) return rc;
   const size_t need = hc_block_select_scratch_size(batch, kv_heads, queries, max_blocks);
-  if (need > 0 && (!scratch || scratch_bytes < need))
-    return set_error(HC_ERR_INVALID, "hc_block_select: scratch too small (%zu < %zu bytes)", scratch_bytes, need);
+  if (need > 0 && (!scratch || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15)))
+    return set_error(HC_ERR_INVALID, "hc_block_select: scratch too small (%zu < %zu bytes, 16-byte aligned)", scratch_bytes,
+                     need);
   return launch_select("hc_block_select", dtype, a, scratch, (hipStream_t)stream);
 }
 
