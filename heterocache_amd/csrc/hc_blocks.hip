@@ -342,14 +342,13 @@ __global__ __launch_bounds__(kScoreWaves * 64) void block_score_kernel(const Sel
 // The selection of one query by a workgroup of NT threads: the scores' keys (of
 // score_blocks itself where SCORED is not set, by way of LDS, else from
 // memory) in registers, the threshold, and one ordered pass that writes the
-// kept blocks.  The threshold
-// is found by counting the keys into equal steps between the least and the
-// greatest left and going on in the step where the count of kept ones is
-// reached: scores of one query lie within a few powers of two, where fixed
+// kept blocks.  The threshold is found by counting the keys into equal steps
+// between the least and the greatest left and going on in the step where the
+// count of kept ones is reached: scores of one query lie within a few powers of two, where fixed
 // digits of the key would pile up in few counters.  Bound by the latency of
 // its dependent steps; a barrier each for the keys, the counts (one or two
 // rounds) and the places.  128 blocks take 1 us of loads, 2 of scores and 2 of
-// selection; 1000 scored ones a launch of 4.4, 4096 of 7.1.
+// selection; 1000 scored ones a launch of 4.3, 4096 of 5.9.
 constexpr int kPickKeys = 12288;  // keys in LDS, of rows scored by the same workgroup
 template <int NT>
 struct Pick {
@@ -609,9 +608,9 @@ bool select_in_memory(int64_t jobs, int max_blocks) {
 }
 // Blocks that four waves pick from, and eight, sixteen beyond: keys that fit
 // the threads' registers, by as few waves as that takes (8 queries of 1024,
-// 2048, 4096 and 8192 blocks through memory: 8.9, 10.2, 21.5 and 29.8 us with
-// four, 9.0, 9.7, 12.7 and 20.6 with eight, 11.4, 11.7, 14.2 and 17.0 with
-// sixteen).
+// 2048, 4096 and 8192 blocks through memory, scores and all: 8.9, 10.2, 21.5
+// and 29.8 us with four, 9.0, 9.7, 12.7 and 20.6 with eight, 11.4, 11.7, 14.2
+// and 17.0 with sixteen; since then 8.8, 9.6, 10.7 and 15.5 as chosen).
 constexpr int kFewBlocks = 1024, kMoreBlocks = 512 * Pick<512>::kHeld;
 
 template <typename T, bool SCORED>
