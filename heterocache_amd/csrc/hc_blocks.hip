@@ -28,6 +28,7 @@ namespace hc {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMinExp = -48, kMaxExp = 48;
 constexpr int kBoundBytes = 2 * HC_HEAD_DIM;  // 128 maxima, then 128 minima
@@ -344,11 +345,12 @@ __global__ __launch_bounds__(kScoreWaves * 64) void block_score_kernel(const Sel
 // memory) in registers, the threshold, and one ordered pass that writes the
 // kept blocks.  The threshold is found by counting the keys into equal steps
 // between the least and the greatest left and going on in the step where the
-// count of kept ones is reached: scores of one query lie within a few powers of two, where fixed
-// digits of the key would pile up in few counters.  Bound by the latency of
+// count of kept ones is reached: scores of one query lie within a few powers of
+// two, where fixed digits of the key would pile up in few counters.  Bound by the latency of
 // its dependent steps; a barrier each for the keys, the counts (one or two
 // rounds) and the places.  128 blocks take 1 us of loads, 2 of scores and 2 of
 // selection; 1000 scored ones a launch of 4.3, 4096 of 5.9.
+__host__ __device__ constexpr int key_words(int blocks) { return (blocks + 15) / 16 * 16; }
 constexpr int kPickKeys = 12288;  // keys in LDS, of rows scored by the same workgroup
 template <int NT>
 struct Pick {
@@ -369,7 +371,7 @@ struct Pick {
 
 // Writes the query's counts and list to memory and, where list is not null, to
 // LDS as well (a.keep entries; visible behind the next barrier); returns the
-// count.  s_key: a.max_blocks words of LDS (SCORED: none).
+// count.  s_key: key_words(a.max_blocks) words of LDS (SCORED: none).
 template <typename T, bool SCORED, int NT>
 __device__ __forceinline__ int pick_blocks(const SelectArgs& a, SelectJob& j, Pick<NT>& L, uint32_t* s_key,
                                            int32_t* list) {
@@ -435,21 +437,58 @@ __device__ __forceinline__ int pick_blocks(const SelectArgs& a, SelectJob& j, Pi
         most = max(most, u);
       }
     }
-  } else if (64 * wave < nmid) {
-    ScoreBlocks<4> t;
-    load_blocks<4>(a, base + 64 * wave, base + nmid - 1, lane, t);
-    const ScoreQuery q = score_query<T>(a, raw, lane);
-    for (int k0 = 64 * wave;;) {
-      score_blocks<4>(a, q, t, lane, [&](int u, float s) {
-        const int k = k0 + 16 * u + (lane & 15);
-        const uint32_t key = order_key(s);
-        if (lane < 16 && k < nmid) s_key[k] = key;
-        least = min(least, key);  // (a block past the end is the last one again)
-        most = max(most, key);
-      });
-      k0 += 64 * P::kWaves;
-      if (k0 >= nmid) break;
-      load_blocks<4>(a, base + k0, base + nmid - 1, lane, t);
+  } else {
+    // As few blocks a wave at a time as that all waves take part in.
+    auto scored = [&](auto u_c) {
+      constexpr int U = decltype(u_c)::value;
+      if (16 * U * wave >= nmid) return;
+      ScoreBlocks<U> t;
+      load_blocks<U>(a, base + 16 * U * wave, base + nmid - 1, lane, t);
+      const ScoreQuery q = score_query<T>(a, raw, lane);
+      for (int k0 = 16 * U * wave;;) {
+        score_blocks<U>(a, q, t, lane, [&](int u, float s) {
+          const int k = k0 + 16 * u + (lane & 15);
+          const uint32_t key = order_key(s);
+          if (lane < 16 && k < nmid) s_key[k] = key;
+          least = min(least, key);  // (a block past the end is the last one again)
+          most = max(most, key);
+        });
+        k0 += 16 * U * P::kWaves;
+        if (k0 >= nmid) break;
+        load_blocks<U>(a, base + k0, base + nmid - 1, lane, t);
+      }
+    };
+    if (nmid <= 16 * P::kWaves)
+      scored(std::integral_constant<int, 1>{});
+    else
+      scored(std::integral_constant<int, 4>{});
+    if (nmid <= NT / 4) {
+      // Few keys: four lanes a key count the keys that go before it, a quarter
+      // of them each, and no threshold is needed (with the spread of the scores
+      // over the waves, 128 blocks selected and 16 attended: 12.4 to 11.9 us).
+      const int words = key_words(nmid);
+      for (int k = nmid + tid; k < words; k += NT) s_key[k] = 0;  // (no score's key)
+      __syncthreads();
+      const int kk = tid >> 2;
+      const uint32_t mine = kk < nmid ? s_key[kk] : 0xffffffffu;
+      int before = 0;
+      for (int k = 4 * (tid & 3); k < words; k += 16) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(s_key + k);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) before += v[u] > mine || (v[u] == mine && k + u < kk);
+      }
+      before += __builtin_amdgcn_mov_dpp(before, 0xB1, 0xF, 0xF, false);  // quad_perm [1,0,3,2]
+      before += __builtin_amdgcn_mov_dpp(before, 0x4E, 0xF, 0xF, false);  // quad_perm [2,3,0,1]
+      const bool take = (tid & 3) == 0 && kk < nmid && before < need;
+      const uint64_t taken = __ballot(take);
+      if (lane == 0) L.gt[wave] = __builtin_popcountll(taken);
+      __syncthreads();
+      int at = a.sink + __builtin_popcountll(taken & ((1ull << lane) - 1));
+#pragma unroll
+      for (int w = 0; w < P::kWaves; ++w)
+        if (w < wave) at += L.gt[w];
+      if (take) put(at, lo + kk);
+      return kept;
     }
   }
   least = wave_fold(least, [](uint32_t u, uint32_t v) { return min(u, v); });
@@ -552,7 +591,7 @@ __device__ __forceinline__ int pick_blocks(const SelectArgs& a, SelectJob& j, Pi
 
 template <typename T, bool SCORED, int NT>
 __global__ __launch_bounds__(NT) void block_pick_kernel(const SelectArgs a) {
-  extern __shared__ uint32_t s_key[];
+  extern __shared__ __attribute__((aligned(16))) uint32_t s_key[];
   __shared__ Pick<NT> pick;
   SelectJob j;
   if (select_job(a, blockIdx.x, j)) pick_blocks<T, SCORED, NT>(a, j, pick, s_key, nullptr);
@@ -562,12 +601,12 @@ __global__ __launch_bounds__(NT) void block_pick_kernel(const SelectArgs a) {
 // few queries over short rows, where launches count: the list stays in LDS.
 template <typename T>
 __global__ __launch_bounds__(512, 1) void block_step_kernel(const SelectArgs a, const RowsArgs r) {
-  extern __shared__ uint32_t s_key[];  // a.max_blocks keys, then the list
+  extern __shared__ __attribute__((aligned(16))) uint32_t s_key[];  // key_words(a.max_blocks), then the list
   __shared__ __attribute__((aligned(16))) float s_rows[kRowsLds];
   __shared__ Pick<512> pick;
   SelectJob j;
   if (!select_job(a, blockIdx.x, j)) return;
-  int32_t* list = reinterpret_cast<int32_t*>(s_key + a.max_blocks);
+  int32_t* list = reinterpret_cast<int32_t*>(s_key + key_words(a.max_blocks));
   const int kept = pick_blocks<T, false, 512>(a, j, pick, s_key, list);
   __syncthreads();
   rows_job<T, kRowsListed, false, 8>(r, blockIdx.x, s_rows, list, kept);
@@ -615,7 +654,7 @@ constexpr int kFewBlocks = 1024, kMoreBlocks = 512 * Pick<512>::kHeld;
 
 template <typename T, bool SCORED>
 void launch_pick(const SelectArgs& a, dim3 grid, hipStream_t s) {
-  const size_t lds = SCORED ? 0 : (size_t)std::max(a.max_blocks, 1) * sizeof(uint32_t);
+  const size_t lds = SCORED ? 0 : (size_t)std::max(key_words(a.max_blocks), 1) * sizeof(uint32_t);
   if (a.max_blocks <= kFewBlocks)
     hipLaunchKernelGGL((block_pick_kernel<T, SCORED, 256>), grid, dim3(256), lds, s, a);
   else if (a.max_blocks <= kMoreBlocks)
@@ -760,11 +799,12 @@ BlockPlan block_plan(int batch, int kv_heads, int G, int queries, int block, int
   // queries of 32 and 1.13 at 128 of 128.)
   BlockPlan p = {4, 1, 0, 0};
   const int64_t jobs = (int64_t)batch * kv_heads * queries, tiles = (int64_t)keep * (block / HC_TILE);
+  const int64_t cus = device_cus();
   double best = 0.;
   for (int waves = 4; waves <= (G <= 8 ? 8 : 4); waves += 4)
     for (int ns : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
       if (ns > 1 && (int64_t)ns * waves > tiles) break;
-      const int64_t slots = (int64_t)device_cus() * (waves == 8 ? 1 : 3);
+      const int64_t slots = cus * (waves == 8 ? 1 : 3);
       const double rounds = (double)((jobs * ns + slots - 1) / slots);
       const double load = (double)std::min(jobs * ns, slots) * waves * HC_TILE_ELEMS * 4. / 5.5e6;
       const double own = 3.3 + std::max(2.4, load) * (double)((tiles + waves * ns - 1) / (waves * ns));
@@ -888,7 +928,7 @@ extern "C" int hc_block_step(int dtype, const void* q, const int64_t* q_strides,
   const BlockPlan p = block_plan(batch, kv_heads, r.G, queries, block, keep);
   if (one_launch(p, (int64_t)a.rows * queries, max_blocks, keep)) {
     const dim3 grid((unsigned)((a.rows + 7) / 8 * 8 * queries)), t(512);
-    const size_t lds = ((size_t)max_blocks + keep) * sizeof(int32_t);
+    const size_t lds = ((size_t)key_words(max_blocks) + keep) * sizeof(int32_t);
     switch (dtype) {
       case HC_DTYPE_BF16: hipLaunchKernelGGL(block_step_kernel<__bf16>, grid, t, lds, s, a, r); break;
       case HC_DTYPE_F16: hipLaunchKernelGGL(block_step_kernel<_Float16>, grid, t, lds, s, a, r); break;

@@ -1,6 +1,7 @@
 // Attention over the rows of the ragged store for a few queries a row, and
 // the fold of partial results (see hc_rows.h).
 #include <algorithm>
+#include <atomic>
 
 #include "hc_rows.h"
 
@@ -95,12 +96,20 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const MergeArgs a)
 }  // namespace
 
 int device_cus() {
+  // Asked for once a device: the plans of a call read it some twenty times.
+  static std::atomic<int> known[64];
   int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1) {
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) {
     (void)hipGetLastError();
     return 256;
   }
+  cus = known[dev].load(std::memory_order_relaxed);
+  if (cus > 0) return cus;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1) {
+    (void)hipGetLastError();
+    return 256;
+  }
+  known[dev].store(cus, std::memory_order_relaxed);
   return cus;
 }
 

@@ -292,12 +292,13 @@ def test_refusals(dev):
         ops.block_attn(q, rows.k, rows.v, rows.row_tile_off, rows.row_len, idx, counts, 40, SCALE)
 
 
-@pytest.mark.parametrize("blocks", [255, 256, 257, 1023, 1026, 2051, 6140, 6148, 12290, 32765, 32780])
-def test_every_way_to_hold_the_keys(dev, blocks):
+@pytest.mark.parametrize("blocks,keep", [(n, 40) for n in (255, 256, 257, 1023, 1026, 2051, 6140, 6148, 12290, 32765, 32780)]
+                         + [(n, 9) for n in (30, 63, 66, 67, 68, 127, 130, 131, 132, 150)])
+def test_every_way_to_hold_the_keys(dev, blocks, keep):
     """Row lengths around each change of the selection's launch, with many equal scores, against sorting."""
     rng = np.random.default_rng(blocks)
-    B, Hkv, G, keep = 2, 2, 3, 40
-    lens = [32 * blocks - 7, 32 * (blocks // 2) + 1, 32 * 41, 32 * (blocks - 1) + 1]
+    B, Hkv, G = 2, 2, 3
+    lens = [32 * blocks - 7, 32 * (blocks // 2) + 1, 32 * (keep + 1), 32 * (blocks - 1) + 1]
     hi = rng.integers(-127, 128, (B * Hkv * blocks, D)).astype(np.int8)
     hi[1::3] = hi[::3][:len(hi[1::3])]  # pairs of equal blocks
     lo = np.minimum(hi, rng.integers(-127, 128, hi.shape)).astype(np.int8)
@@ -322,3 +323,28 @@ def test_every_way_to_hold_the_keys(dev, blocks):
         score[:1] = score[have - 2:] = np.inf
         want = np.sort(np.lexsort((np.arange(have), -score))[:keep])
         assert int(counts[r, 0]) == keep and np.array_equal(idx[r, 0].cpu().numpy(), want), r
+
+
+@pytest.mark.parametrize("blocks", [12, 66, 67, 127, 130, 131, 132, 300])
+def test_equal_blocks_go_by_their_place(dev, blocks):
+    """Rows of three blocks over and over: most scores are equal, and the lower block wins, in one call as in two."""
+    rng = np.random.default_rng(blocks)
+    lens, block, keep = [32 * blocks - 3, 32 * (blocks // 2)], 32, 10
+    rows, _ = make_rows(rng, lens, BF, dev, room=5)
+    kv = []
+    src = torch.zeros((2, 1, 2, lens[0], D), dtype=BF, device=dev)
+    for r, n in enumerate(lens):
+        three = torch.as_tensor(rng.standard_normal((96, D)), dtype=torch.float32).to(BF).to(dev)
+        k = three.repeat(-(-n // 96), 1)[:n]
+        v = torch.as_tensor(rng.standard_normal((n, D)), dtype=torch.float32).to(BF).to(dev)
+        src[0, 0, r, :n], src[1, 0, r, :n] = k, v
+        kv.append((k, v))
+    rows.write_rows(src[0], src[1], [(0, 0), (0, 1)], [0, 1], lens)
+    index = rows.block_index(block)
+    index.update()
+    q = _q(rng, 1, 8, 1, BF, dev)
+    got = rows.attend_blocks(q, index, keep, SCALE)
+    _check(got, q, kv, 4, block, keep, 1, 2, BF)
+    idx, counts = ops.block_select(q, index.bounds, index.exps, index.row_block_off, rows.row_len, block,
+                                   index.max_blocks, keep, sink=1, local=2)
+    assert torch.equal(idx, got[1]) and torch.equal(counts, got[2])
