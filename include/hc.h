@@ -634,9 +634,10 @@ int hc_block_bounds(int dtype, const void* kstore, const int64_t* row_tile_off, 
  * (at least 1: the unfinished block is never scored) and the best of the
  * others, equal scores to the lower block: `keep` in all, or every block if
  * there are no more.  idx int32 [rows][queries][keep]: ascending, -1 past
- * the count; counts int32 [rows][queries].  max_blocks: visible blocks that scratch
- * (hc_block_select_scratch_size bytes, no initialisation) has room for; a
- * query that sees more gets counts -1 and no block.
+ * the count; counts int32 [rows][queries].  max_blocks: visible blocks that
+ * scratch (hc_block_select_scratch_size bytes, 16-byte aligned, no
+ * initialisation) has room for; a query that sees more gets counts -1 and no
+ * block.
  */
 int hc_block_select(int dtype, const void* q, const int64_t* q_strides, const int8_t* bounds, const int8_t* exps,
                     const int64_t* row_block_off, const int32_t* row_len, const int32_t* query_counts, int batch,

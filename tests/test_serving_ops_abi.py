@@ -112,6 +112,7 @@ def test_block_select(lib):
                                    FAKE, scratch, sb, None)
     _refused(lib, call(), b"scratch too small")
     _refused(lib, call(scratch=None, sb=1 << 30), b"scratch too small")
+    _refused(lib, call(scratch=FAKE + 8, sb=1 << 30), b"aligned")
     _refused(lib, call(hq=9), b"q_heads=9")
     _refused(lib, call(block=40), b"block=40")
     for kw in (dict(keep=0), dict(local=0), dict(sink=-1), dict(keep=2), dict(sink=7), dict(mb=-1), dict(keep=1 << 25)):
