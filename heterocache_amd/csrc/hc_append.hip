@@ -248,7 +248,8 @@ extern "C" int hc_append_rotated(int dtype, int table_dtype, const void* q, cons
     return set_error(HC_ERR_INVALID, "hc_append_rotated: the tables' dtype %d is neither float32 nor %d", table_dtype,
                      dtype);
   if (batch == 0) return HC_OK;
-  if (!row_len || (len_out && (!row_cap || !row_tile_off))) return set_error(HC_ERR_INVALID, "hc_append_rotated: null pointer argument");
+  if (!row_len || (len_out && (!row_cap || !row_tile_off)))
+    return set_error(HC_ERR_INVALID, "hc_append_rotated: null pointer argument");
   if (tokens == 0 && (!len_out || len_out == row_len)) return HC_OK;
   const int64_t gap = 4 * (int64_t)batch * kv_heads;
   const intptr_t apart = reinterpret_cast<intptr_t>(len_out) - reinterpret_cast<intptr_t>(row_len);

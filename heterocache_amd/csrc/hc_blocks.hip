@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256) void block_bounds_kernel(const BoundArgs a) {
         fetch(kb + (row_at + (int64_t)j * a.tpb + t) * HC_TILE_ELEMS, t + 1 < a.tpb);
         fold();
       }
-    fetch(kb + (row_at + (int64_t)max(j - chunks, last) * a.tpb) * HC_TILE_ELEMS, a.tpb > 1);  // (at the end the last again)
+    if (j - chunks >= last) fetch(kb + (row_at + (int64_t)(j - chunks) * a.tpb) * HC_TILE_ELEMS, a.tpb > 1);
     const float mine = row16_max_scatter(v, lane);
     // The greatest |k| is the greatest of all 16 values of all groups.
     float top = greater(mine, dpp_mov<0xB1>(mine));
@@ -724,7 +724,8 @@ int select_args(const char* what, int dtype, const void* q, const int64_t* q_str
   if (reinterpret_cast<uintptr_t>(bounds) & 15)
     return set_error(HC_ERR_INVALID, "%s: the bounds must be 16-byte aligned", what);
   a = SelectArgs{};
-  a.q = q, a.bounds = bounds, a.exps = exps, a.row_blk_off = row_block_off, a.row_len = row_len, a.query_counts = query_counts;
+  a.q = q, a.bounds = bounds, a.exps = exps, a.row_blk_off = row_block_off;
+  a.row_len = row_len, a.query_counts = query_counts;
   for (int i = 0; i < 3; ++i) a.q_s[i] = q_strides[i];
   a.pitch = score_pitch(max_blocks), a.idx = idx, a.counts = counts;
   a.Hkv = kv_heads, a.G = q_heads / kv_heads, a.Q = queries, a.rows = batch * kv_heads, a.S = block;

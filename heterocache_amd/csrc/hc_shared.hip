@@ -438,8 +438,8 @@ SharedPlan shared_plan(int dtype, int batch, int Hkv, int G, int Q, int64_t pref
       const double kk = (double)n * ncg / cus;
       const double share = std::ceil((double)prefix_tiles / (double)std::max<int64_t>(n - Hkv / 2, 1));
       const double work = share * tile * (1. + 0.65 * (std::max(std::ceil(kk), 1.) - 1.));
-      const double t = std::max(std::max(work, pre_us) + rows_us * (kk < (f32 ? 1. : 2.) ? 0.67 : 1.), pre_us + rows_us) +
-                       (double)n * M * 0.2e-3;
+      const double rows_seen = rows_us * (kk < (f32 ? 1. : 2.) ? 0.67 : 1.);
+      const double t = std::max(std::max(work, pre_us) + rows_seen, pre_us + rows_us) + (double)n * M * 0.2e-3;
       if (best == 0. || t < best) best = t, p.nc = nc, p.ncg = ncg, p.parts = (int)n;
     }
   }
@@ -535,7 +535,8 @@ extern "C" int hc_shared_attn(int dtype, const void* q, const int64_t* q_strides
   a.part_o = reinterpret_cast<float*>(ws + p.pre_o), a.part_ml = reinterpret_cast<float*>(ws + p.pre_ml);
   a.info = reinterpret_cast<int32_t*>(ws + p.info_at);
   RowsArgs r = {};
-  r.q = q, r.kstore = kstore, r.vstore = vstore, r.row_tile_off = row_tile_off, r.row_len = row_len, r.query_counts = query_counts;
+  r.q = q, r.kstore = kstore, r.vstore = vstore, r.row_tile_off = row_tile_off, r.row_len = row_len;
+  r.query_counts = query_counts;
   r.Hkv = kv_heads, r.G = G, r.Q = queries, r.rows = row_len ? batch * kv_heads : 0;
   r.qpb = p.rows.qpb, r.ncb = p.rows.ncb, r.nsplit = p.rows.nsplit, r.scale_log2 = scale_log2;
   r.part_o = reinterpret_cast<float*>(ws + p.row_o), r.part_ml = reinterpret_cast<float*>(ws + p.row_ml);

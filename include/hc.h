@@ -601,8 +601,8 @@ int hc_append_rotated(int dtype, int table_dtype, const void* q, const int64_t* 
 int hc_shared_attn(int dtype, const void* q, const int64_t* q_strides, const void* kprefix, const void* vprefix,
                    const int64_t* prefix_tile_off, const int32_t* prefix_len, int64_t prefix_tiles, const void* kstore,
                    const void* vstore, const int64_t* row_tile_off, const int32_t* row_len,
-                   const int32_t* query_counts, int64_t row_tiles, void* out, const int64_t* out_strides, int batch, int q_heads, int kv_heads, int queries,
-                   float scale, void* workspace, size_t workspace_bytes, void* stream);
+                   const int32_t* query_counts, int64_t row_tiles, void* out, const int64_t* out_strides, int batch,
+                   int q_heads, int kv_heads, int queries, float scale, void* workspace, size_t workspace_bytes, void* stream);
 size_t hc_shared_workspace_size(int dtype, int batch, int q_heads, int kv_heads, int queries, int64_t prefix_tiles,
                                 int64_t row_tiles);
 
