@@ -6,7 +6,9 @@
 // k-group l / 16.  Each column has a limit, the first token it does not see.
 // State per lane: m, the reference point of its column's scaled base-2 scores
 // (at most log2(kRowsLazy) below their maximum), l, its share of the sum of
-// exp2(score - m), and o[mt][j] = O^T[16 mt + 4 g + j][column].
+// exp2(score - m), and o[mt][j] = O^T[16 mt + 4 g + j][column].  m stays -inf
+// while no score is a number above it; l then tells why: zero where there was
+// no token, positive where the tokens all score -inf, NaN where one scores NaN.
 #pragma once
 #include <type_traits>
 
@@ -66,11 +68,12 @@ __device__ __forceinline__ void tile_scores(const typename Elem<T>::vec8 (&kr)[8
   }
 }
 
-// Probabilities of a tile's scores (already masked) in the input type, the
-// state m, l and, when the reference point moves, O following.  scale_log2 > 0.
+// Probabilities of a tile's scores (already masked; seen: the column sees one
+// of its tokens) in the input type, the state m, l and, when the reference
+// point moves, O following.  scale_log2 > 0.
 template <typename T>
-__device__ __forceinline__ typename Elem<T>::vec8 tile_probs(const f32x4 (&s)[2], float scale_log2, float& m, float& l,
-                                                             f32x4 (&o)[8]) {
+__device__ __forceinline__ typename Elem<T>::vec8 tile_probs(const f32x4 (&s)[2], bool seen, float scale_log2, float& m,
+                                                             float& l, f32x4 (&o)[8]) {
   typename Elem<T>::vec8 pb;
   float ps;
   auto probs = [&](float nm) {
@@ -97,6 +100,7 @@ __device__ __forceinline__ typename Elem<T>::vec8 tile_probs(const f32x4 (&s)[2]
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) o[mt] *= alpha;
     probs(mnew == -INFINITY ? 0.f : -mnew);
+    if (mnew == -INFINITY && seen) ps += 1.f;
   }
   l += ps;
   return pb;
@@ -160,9 +164,17 @@ __device__ __forceinline__ void load_operands(typename Elem<T>::vec8 (&r)[8], co
   for (int x = 0; x < 8; ++x) r[x] = load8_stream<T>(p + x * 512);
 }
 
-// One output row's weights: the reference M of several (m, l) states and
-// exp2(m - M), zero for a state without tokens.
-__device__ __forceinline__ float state_weight(float m, float M) { return m == -INFINITY ? 0.f : fast_exp2(m - M); }
+// The weight exp2(m - M) of a state (m, l) under the reference M of several:
+// one that holds no number above -inf adds nothing to one that does (but a NaN
+// l, which zero does not silence).
+__device__ __forceinline__ float state_weight(float m, float M) {
+  return m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : fast_exp2(m - M);
+}
+// An output channel of the folded state (M, L): zero without tokens, NaN where
+// their scores have no softmax.
+__device__ __forceinline__ float state_output(float acc, float M, float L) {
+  return M == -INFINITY ? (L == 0.f ? 0.f : NAN) : acc * (1.f / L);
+}
 
 }  // namespace hc
 
@@ -327,7 +339,7 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds, 
         for (int e = 0; e < 8; ++e)
           if (tok0 + 16 * (e >> 2) + 4 * g + (e & 3) >= mylim) s[e >> 2][e & 3] = -INFINITY;
       }
-      const vec8 pb = tile_probs<T>(s, a.scale_log2, m, l, o);
+      const vec8 pb = tile_probs<T>(s, tok0 < mylim, a.scale_log2, m, l, o);
       if (mixed) {
         tile_values<T, true>(vr, pb, tok0, hi, g, o);
         if (!LAST) load_operands<T>(kr, kb + at);
@@ -372,11 +384,10 @@ __device__ __forceinline__ void rows_job(const RowsArgs& a, int wg, float* lds, 
       *reinterpret_cast<f32x4*>(a.part_o + at * kPartO + d0) = acc;
       if (d0 == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
     } else {
-      const float inv = M == -INFINITY ? 0.f : 1.f / L;
       T* op = reinterpret_cast<T*>(a.out) + b * a.o_s[0] + (int64_t)(kv * a.G + hd) * a.o_s[1] +
               (int64_t)i * a.o_s[2] + d0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) op[e] = Elem<T>::from_f32(M == -INFINITY ? 0.f : acc[e] * inv);
+      for (int e = 0; e < 4; ++e) op[e] = Elem<T>::from_f32(state_output(acc[e], M, L));
     }
   }
 }

@@ -57,18 +57,17 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const MergeArgs a)
     float mn = m;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      if (t0 + k * kGroups >= n) ml[k].x = -INFINITY;
+      if (t0 + k * kGroups >= n) ml[k] = make_float2(-INFINITY, 0.f);
       mn = fmaxf(mn, ml[k].x);
     }
-    if (mn == -INFINITY) continue;
     const float f = state_weight(m, mn);
     l *= f;
     acc *= f;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      if (ml[k].x == -INFINITY) continue;  // a partial without tokens: its channels add nothing
-      const float e = fast_exp2(ml[k].x - mn);
+      const float e = state_weight(ml[k].x, mn);
       l = fmaf(ml[k].y, e, l);
+      if (ml[k].x == -INFINITY) continue;  // no number among its scores: its channels add nothing
       acc += ov[k] * e;
     }
     m = mn;
@@ -87,10 +86,9 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const MergeArgs a)
     L = fmaf(s_l[g], e, L);
     r += s_o[g][lane] * e;
   }
-  const float inv = M == -INFINITY ? 0.f : 1.f / L;  // no token at all: zeros
   T* op = reinterpret_cast<T*>(a.out) + b * a.o_s[0] + (int64_t)hq * a.o_s[1] + (int64_t)i * a.o_s[2] + 4 * lane;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) op[e] = Elem<T>::from_f32(M == -INFINITY ? 0.f : r[e] * inv);
+  for (int e = 0; e < 4; ++e) op[e] = Elem<T>::from_f32(state_output(r[e], M, L));
 }
 
 }  // namespace

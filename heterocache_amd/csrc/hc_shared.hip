@@ -312,6 +312,7 @@ __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
           pv[j][e] = fast_exp2(fmaf(sc[e >> 2][j][e & 3], scale_log2, nm));
           ps[j] += pv[j][e];
         }
+        if (mnew == -INFINITY) ps[j] += 1.f;  // tokens, but none above -inf (see hc_rows.h)
       }
     }
 #pragma unroll

@@ -1,0 +1,99 @@
+"""The serving operators where their arithmetic has nothing ordinary to fold: scores without a number, weights far below
+the largest, lengths that only the device knows."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from heterocache_amd import ops
+from tests.serving_util import D, attend, close, make_rows
+
+pytestmark = pytest.mark.gpu
+BF, FP, FL = torch.bfloat16, torch.float16, torch.float32
+SCALE = 1 / math.sqrt(D)
+
+
+def _q(rng, B, Hq, Q, dtype, dev):
+    q = torch.as_tensor(rng.standard_normal((B, Q, Hq, D)), dtype=torch.float32)
+    return q.to(dtype).to(dev).transpose(1, 2)
+
+
+def _meta(s):
+    return s.k, s.v, s.row_tile_off, s.row_len
+
+
+def _every_way(q, prefix, rows, scale=SCALE):
+    """(name, output, tokens of row 0's KV head from) of each way to attend all of a row or prefix: one workgroup a
+    row, split rows, few and many prefix parts, both, all blocks in one launch and split."""
+    index = rows.block_index(32)
+    index.update()
+    keep = index.max_blocks
+    idx, counts = ops.block_select(q, index.bounds, index.exps, index.row_block_off, rows.row_len, 32, keep, keep)
+    kv = prefix.rows
+    return [
+        ("rows", ops.shared_attn(q, None, _meta(rows), kv, scale, row_tiles=1), False, True),
+        ("split rows", ops.shared_attn(q, None, _meta(rows), kv, scale, row_tiles=64), False, True),
+        ("prefix", ops.shared_attn(q, _meta(prefix), None, kv, scale, prefix_tiles=0), True, False),
+        ("parts", ops.shared_attn(q, _meta(prefix), None, kv, scale, prefix_tiles=64), True, False),
+        ("both", rows.attend_shared(q, prefix, scale), True, True),
+        ("step", rows.attend_blocks(q, index, keep, scale)[0], False, True),
+        ("listed", ops.block_attn(q, rows.k, rows.v, rows.row_tile_off, rows.row_len, idx, counts, 32, scale), False,
+         True),
+    ]
+
+
+def _cat(pre, own, use_pre, use_own):
+    """Keys and values of a row as one way attends them."""
+    parts = ([pre] if use_pre else []) + ([own] if use_own else [])
+    return torch.cat([k for k, _ in parts]), torch.cat([v for _, v in parts])
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, FL])
+@pytest.mark.parametrize("n", [5, 700])
+def test_nan_queries_give_nan(dev, dtype, n):
+    """A query with a NaN has no finite score: its output is NaN, not the zeros of a query that sees nothing; the
+    other heads of its group keep their results."""
+    rng = np.random.default_rng(n)
+    prefix, pre = make_rows(rng, [n, n + 1], dtype, dev)
+    rows, kv = make_rows(rng, [n + 2, n, 3, n + 70], dtype, dev, room=6)
+    q = _q(rng, 2, 8, 1, dtype, dev).contiguous()
+    q[0, 1] = math.nan
+    q[1, 6, 0, 77] = math.nan
+    for name, out, use_pre, use_own in _every_way(q, prefix, rows):
+        for b in range(2):
+            for h in range(8):
+                if (b, h) in ((0, 1), (1, 6)):
+                    assert torch.isnan(out[b, 0, h]).all(), (name, b, h)
+                    continue
+                want, tol = attend(q[b, h, 0], *_cat(pre[h // 4], kv[2 * b + h // 4], use_pre, use_own), SCALE, dtype)
+                close(out[b, 0, h], want, tol, f"{name} {b} {h}")
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, FL])
+def test_scores_of_minus_infinity(dev, dtype):
+    """Tokens that score -inf weigh nothing beside others; a query that sees only such tokens has no softmax (NaN); one
+    that sees no token gets zeros."""
+    rng = np.random.default_rng(3)
+    prefix, pre = make_rows(rng, [300, 90], dtype, dev)
+    rows, kv = make_rows(rng, [400, 0, 200, 64], dtype, dev, room=6)
+    q = _q(rng, 2, 2, 1, dtype, dev).abs().contiguous()
+    for r, cut in ((0, 300), (2, 200), (3, 0)):  # (3: every token -inf but the last ten of its first tile)
+        k, v = kv[r]
+        if r == 3:
+            k[:22, 5] = k[32:, 5] = -math.inf
+        else:
+            k[:cut, 5] = -math.inf
+        rows.write_rows(k[None, None], v[None, None], [(0, 0)], [r], [len(k)])
+    for name, out, use_pre, use_own in _every_way(q, prefix, rows):
+        for r in range(4):
+            b, h = divmod(r, 2)
+            k, v = _cat(pre[h], kv[r], use_pre, use_own)
+            live = torch.isfinite(k[:, 5])
+            if len(k) and not live.any():
+                assert torch.isnan(out[b, 0, h]).all(), (name, r)
+                continue
+            want, tol = attend(q[b, h, 0], k[live], v[live], SCALE, dtype)
+            close(out[b, 0, h], want, tol, f"{name} row {r}")
+            if len(k) == 0:
+                assert not out[b, 0, h].any(), (name, r)
