@@ -433,9 +433,9 @@ class BlockIndex:
         those that each row's last new_tokens tokens completed."""
         s = self.store
         if new_tokens is None:
-            # A graph's replays find other lengths than the capture's.
-            longest = s.host_cap if torch.cuda.is_current_stream_capturing() else s.host_len
-            span, fresh = int(longest.max(initial=0)) // self.block, 0
+            # By the capacities: replays of captured appends advance the
+            # lengths on the device alone, and workgroups past them end.
+            span, fresh = int(s.host_cap.max(initial=0)) // self.block, 0
         else:
             fresh = int(new_tokens)
             if fresh < 0:

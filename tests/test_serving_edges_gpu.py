@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from heterocache_amd import ops
-from tests.serving_util import D, attend, close, make_rows
+from tests.serving_util import D, attend, bounds, close, make_rows
 
 pytestmark = pytest.mark.gpu
 BF, FP, FL = torch.bfloat16, torch.float16, torch.float32
@@ -97,3 +97,39 @@ def test_scores_of_minus_infinity(dev, dtype):
             close(out[b, 0, h], want, tol, f"{name} row {r}")
             if len(k) == 0:
                 assert not out[b, 0, h].any(), (name, r)
+
+
+def test_whole_update_after_replayed_appends(dev):
+    """Captured appends advance the lengths on the device and not the host's mirror: an update() outside of the graph, on
+    the current stream or on another, still takes every complete block."""
+    rng = np.random.default_rng(4)
+    rows, kv = make_rows(rng, [40, 95, 0], BF, dev, room=400, stale=0.0)
+    index = rows.block_index(32)
+    T = 50
+    q, k, v = (torch.zeros((1, 3, T, D), dtype=BF, device=dev) for _ in range(3))
+    one, zero = torch.ones((T, D), device=dev), torch.zeros((T, D), device=dev)
+    ops.append_rotated(q, k, v, one, zero, *_meta(rows), rows.row_cap)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.append_rotated(q, k, v, one, zero, *_meta(rows), rows.row_cap, len_out=rows.row_len)
+    side = torch.cuda.Stream(dev)
+    for step in range(4):
+        for t in (k, v):
+            t.copy_(torch.as_tensor(rng.standard_normal(t.shape), dtype=torch.float32))
+        kv = [(torch.cat([a, k[0, r]]), torch.cat([b, v[0, r]])) for r, (a, b) in enumerate(kv)]
+        g.replay()
+        index.bounds.fill_(5)
+        index.exps.fill_(77)
+        if step % 2:
+            side.wait_stream(torch.cuda.current_stream(dev))
+            index.update(stream=side)
+            torch.cuda.current_stream(dev).wait_stream(side)
+        else:
+            index.update()
+        assert rows.host_len.tolist() == [40, 95, 0]
+        off = index.row_block_off.tolist()
+        for r, (a, _) in enumerate(kv):
+            hi, lo, ex = bounds(a, 32)
+            got = index.bounds[off[r]:off[r] + len(ex)].cpu().numpy()
+            assert np.array_equal(got[:, 0], hi) and np.array_equal(got[:, 1], lo), (step, r)
+            assert np.array_equal(index.exps[off[r]:off[r] + len(ex)].cpu().numpy(), ex), (step, r)
