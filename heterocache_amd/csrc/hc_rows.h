@@ -5,10 +5,11 @@
 // A wave holds up to 16 query columns: lane l serves column l % 16 and the
 // k-group l / 16.  Each column has a limit, the first token it does not see.
 // State per lane: m, the reference point of its column's scaled base-2 scores
-// (at most log2(kRowsLazy) below their maximum), l, its share of the sum of
-// exp2(score - m), and o[mt][j] = O^T[16 mt + 4 g + j][column].  m stays -inf
-// while no score is a number above it; l then tells why: zero where there was
-// no token, positive where the tokens all score -inf, NaN where one scores NaN.
+// (at most log2(Weights::kLazy) below their maximum), l, its share of the sum
+// of exp2(score - m), and o[mt][j] = O^T[16 mt + 4 g + j][column].  m stays
+// -inf while no score is a number above it; l then tells why: zero where there
+// was no token, positive where the tokens all score -inf, NaN where one scores
+// NaN.
 #pragma once
 #include <type_traits>
 
@@ -17,9 +18,30 @@
 namespace hc {
 
 // The reference point moves when a lane's sum of a tile's probabilities
-// exceeds this: they stay inside every input type's range, and most tiles
-// take no maximum and rescale nothing.
-constexpr float kRowsLazy = 256.f;
+// exceeds kLazy, to kAbove below the maximum: they stay inside the input type's
+// range, and most tiles take no maximum and rescale nothing.  fp16's range is
+// used whole: with the reference at the maximum a weight below 2^-25 of it
+// leaves the product with V but not the sum, and a tail of e^-17.4 a token
+// behind a dominant one lost what a wave or part held of it beside that one (a
+// quarter of 6000 tokens, 0.5 % of 131072).  2^10 above, weights down to 2^-24
+// keep their 11 bits and those down to 2^-35 count, and the reference moves as
+// seldom (16 sequences of 4 queries behind 12289 fp16 tokens of 4 heads: 31.0
+// us before, 30.4, 30.7 and 31.8 with 8, 10 and 12).
+template <typename T>
+struct Weights {
+  static constexpr float kAbove = 0.f, kLazy = 256.f;
+};
+template <>
+struct Weights<_Float16> {
+  static constexpr float kAbove = 10.f, kLazy = 65504.f;
+};
+// The reference point behind m, for a greatest scaled score of top.  (Beyond 2^26
+// a step of fp32 is 8, and its rounding alone takes the room above.)
+template <typename T>
+__device__ __forceinline__ float next_reference(float m, float top) {
+  if constexpr (Weights<T>::kAbove > 0.f) top = fabsf(top) < 0x1p26f ? top - Weights<T>::kAbove : top;
+  return fmaxf(m, top);
+}
 
 // Floats of one partial: 128 unnormalised channels; (m, l) lie apart.
 constexpr int kPartO = HC_HEAD_DIM;
@@ -89,11 +111,11 @@ __device__ __forceinline__ typename Elem<T>::vec8 tile_probs(const f32x4 (&s)[2]
     pb = pack8<T>(p);
   };
   probs(-m);
-  if (__any(!(ps <= kRowsLazy))) {  // also NaN, as while m = -inf
+  if (__any(!(ps <= Weights<T>::kLazy))) {  // also NaN, as while m = -inf
     float mx = s[0][0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
-    const float mnew = fmaxf(m, rows4_max(mx) * scale_log2);
+    const float mnew = next_reference<T>(m, rows4_max(mx) * scale_log2);
     const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mnew);
     m = mnew;
     l *= alpha;

@@ -290,16 +290,16 @@ __device__ __forceinline__ void prefix_job(const PrefixArgs& a, int x, T* lds) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) sn[h][j] += upper[h][j];
     }
-    bool fine = ps[0] <= kRowsLazy;
+    bool fine = ps[0] <= Weights<T>::kLazy;
 #pragma unroll
-    for (int j = 1; j < NC; ++j) fine = fine && ps[j] <= kRowsLazy;
+    for (int j = 1; j < NC; ++j) fine = fine && ps[j] <= Weights<T>::kLazy;
     if (__any(!fine)) {  // also NaN, as in the first tile
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
         float mx = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 8; ++e) mx = fmaxf(mx, sc[e >> 2][j][e & 3]);
-        const float mnew = fmaxf(m[j], rows4_max(mx) * scale_log2);
+        const float mnew = next_reference<T>(m[j], rows4_max(mx) * scale_log2);
         const float alpha = m[j] == -INFINITY ? 0.f : fast_exp2(m[j] - mnew);
         m[j] = mnew;
         l[j] *= alpha;

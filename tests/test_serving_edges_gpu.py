@@ -133,3 +133,55 @@ def test_whole_update_after_replayed_appends(dev):
             got = index.bounds[off[r]:off[r] + len(ex)].cpu().numpy()
             assert np.array_equal(got[:, 0], hi) and np.array_equal(got[:, 1], lo), (step, r)
             assert np.array_equal(index.exps[off[r]:off[r] + len(ex)].cpu().numpy(), ex), (step, r)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, FL])
+@pytest.mark.parametrize("drop", [9.0, 17.4, 20.0, 24.0])
+def test_flat_tail_behind_a_dominant_token(dev, dtype, drop):
+    """One token whose value is zero outweighs each of the others by e^drop: the output is what they weigh together."""
+    rng = np.random.default_rng(5)
+    n = 6000
+    prefix, rows = (make_rows(rng, [n], dtype, dev, room=3)[0] for _ in range(2))
+    k = torch.zeros((n, D), dtype=dtype, device=dev)
+    v = (1 + 0.25 * torch.as_tensor(rng.random((n, D)), dtype=torch.float32)).to(dtype).to(dev)
+    q = torch.zeros((1, 1, 1, D), dtype=dtype, device=dev)
+    q[..., 0] = 16.0
+    k[3, 0], v[3] = drop / SCALE / 16, 0.0
+    for store in (prefix, rows):
+        store.write_rows(k[None, None], v[None, None], [(0, 0)], [0], [n])
+    # Scores are one exact product each.  An exponent is off by 4 roundings of a
+    # number up to 1.45 drop + 10, exp2 by 2 steps; a weight's rounding to the input type
+    # is half a step, in fp16 (whose smallest steps are 2^-24, the greatest weight 2^10 or
+    # more) at least 2^-35 of the greatest; sums of n terms.
+    for name, out, use_pre, use_own in _every_way(q, prefix, rows):
+        copies = int(use_pre) + int(use_own)
+        s = (q[0, 0].double() @ k.double().t() * SCALE)[0]
+        w = torch.exp(s - s.max())
+        mass = copies * w.sum()
+        want = copies * (w @ v.double()) / mass
+        slip = 2.0 ** -24 * (4 * (1.45 * drop + 10) * math.log(2) + 4 + 2 * copies * n + 64)
+        step = w * torch.finfo(dtype).eps / 2
+        if dtype == FP:
+            step = step.clamp(min=2.0 ** -35)
+        tol = copies * (step @ v.double().abs()) / mass + 2 * slip * want + want * torch.finfo(dtype).eps / 2 * 1.01
+        close(out[0, 0, 0], want, tol * 1.02 + torch.finfo(dtype).tiny * torch.finfo(dtype).eps, f"{name} e^-{drop}")
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, FL])
+@pytest.mark.parametrize("size", [64.0, 700.0, 1024.0, 2048.0])
+def test_scores_far_beyond_the_exponent(dev, dtype, size):
+    """Scores up to 2^26, whose steps in fp32 are several powers of two: the best token's value comes out."""
+    rng = np.random.default_rng(6)
+    n = 300
+    prefix, rows = (make_rows(rng, [n], dtype, dev, room=3)[0] for _ in range(2))
+    sign = torch.as_tensor(rng.choice([-1.0, 1.0], (n, D)), dtype=torch.float32).to(dev)
+    v = torch.as_tensor(rng.standard_normal((n, D)), dtype=torch.float32).to(dtype).to(dev)
+    k = (sign * size).to(dtype)
+    q = k[170].clone().view(1, 1, 1, D)
+    for store in (prefix, rows):
+        store.write_rows(k[None, None], v[None, None], [(0, 0)], [0], [n])
+    want = v[170].double()
+    # The others are e^-1000 or less of it.  Its weight is off by half a step of the type, the output by another.
+    tol = want.abs() * (torch.finfo(dtype).eps * 1.01 + 64 * 2.0 ** -24)
+    for name, out, _, _ in _every_way(q, prefix, rows):
+        close(out[0, 0, 0], want, tol, name)
