@@ -746,7 +746,7 @@ int launch_select(const char* what, int dtype, SelectArgs& a, void* scratch, hip
     return check_launch(what);
   }
   a.scores = reinterpret_cast<float*>(scratch);
-  const int64_t most = (a.max_blocks + 32 * kScoreWaves - 1) / (32 * kScoreWaves);
+  const int64_t most = ((int64_t)a.max_blocks + 32 * kScoreWaves - 1) / (32 * kScoreWaves);
   a.chunks = (int)std::max<int64_t>(std::min<int64_t>((8 * device_cus() + jobs - 1) / jobs, most), 1);
   if (jobs * a.chunks > 0x7fffffffLL)
     return set_error(HC_ERR_INVALID, "%s: %lld workgroups", what, (long long)(jobs * a.chunks));

@@ -411,6 +411,9 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 SharedPlan shared_plan(int dtype, int batch, int Hkv, int G, int Q, int64_t prefix_tiles, int64_t row_tiles) {
   SharedPlan p;
+  // Sizes to cut for: beyond what a device holds they change nothing (and the
+  // sums below stay in range).
+  prefix_tiles = std::min<int64_t>(prefix_tiles, 1LL << 40), row_tiles = std::min<int64_t>(row_tiles, 1LL << 40);
   const int64_t M = (int64_t)batch * Q * G;
   p.rows = rows_plan(batch * Hkv, G, Q, row_tiles);
   // Column blocks a wave (nc) and prefix workgroups a CU (k): the least

@@ -185,3 +185,22 @@ def test_scores_far_beyond_the_exponent(dev, dtype, size):
     tol = want.abs() * (torch.finfo(dtype).eps * 1.01 + 64 * 2.0 ** -24)
     for name, out, _, _ in _every_way(q, prefix, rows):
         close(out[0, 0, 0], want, tol, name)
+
+
+def test_room_without_end(dev):
+    """Tile counts and max_blocks of the types' largest values: nothing more is read or kept than of fitting ones."""
+    rng = np.random.default_rng(7)
+    prefix, pre = make_rows(rng, [700], BF, dev)
+    rows, kv = make_rows(rng, [900], BF, dev, room=5)
+    q = _q(rng, 1, 4, 1, BF, dev)
+    most = (1 << 63) - 1
+    for pt, rt in ((most, 30), (22, most), (most, most)):
+        got = ops.shared_attn(q, _meta(prefix), _meta(rows), 1, SCALE, prefix_tiles=pt, row_tiles=rt)
+        for h in range(4):
+            want, tol = attend(q[0, h, 0], *_cat(pre[0], kv[0], True, True), SCALE, BF)
+            close(got[0, 0, h], want, tol, f"{pt} {rt}")
+    index = rows.block_index(32)
+    index.update()
+    a, b = (ops.block_select(q, index.bounds, index.exps, index.row_block_off, rows.row_len, 32, n, 9, 1, 2)
+            for n in (index.max_blocks, (1 << 31) - 1))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
