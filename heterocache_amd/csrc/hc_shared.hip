@@ -400,22 +400,27 @@ __global__ __launch_bounds__(kPreThreads, sizeof(T) == 4 ? 1 : NC == 2 ? 2 : 3) 
 }
 
 // Sizes of one call: the prefix launch's column blocks and parts, the rows'
-// plan, and the workspace in bytes.
+// plan, and the workspace in bytes.  Rows alone whose jobs are whole write the
+// output themselves.
 struct SharedPlan {
   int nc, ncg, parts;
   RowsPlan rows;
+  bool direct;
   size_t info_at, pre_o, pre_ml, row_o, row_ml, bytes;
 };
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
+// Negative tile counts: no prefix, no rows.
 SharedPlan shared_plan(int dtype, int batch, int Hkv, int G, int Q, int64_t prefix_tiles, int64_t row_tiles) {
-  SharedPlan p;
+  SharedPlan p = {1, 1, 0};
+  const bool with_prefix = prefix_tiles >= 0, with_rows = row_tiles >= 0;
   // Sizes to cut for: beyond what a device holds they change nothing (and the
   // sums below stay in range).
   prefix_tiles = std::min<int64_t>(prefix_tiles, 1LL << 40), row_tiles = std::min<int64_t>(row_tiles, 1LL << 40);
   const int64_t M = (int64_t)batch * Q * G;
-  p.rows = rows_plan(batch * Hkv, G, Q, row_tiles);
+  p.rows = rows_plan(batch * Hkv, G, Q, std::max<int64_t>(row_tiles, 0));
+  p.direct = !with_prefix && p.rows.nsplit == 1;
   // Column blocks a wave (nc) and prefix workgroups a CU (k): the least
   // estimate of the call's time in us, fitted to 300 timings of 15 shapes (a
   // few columns to 512, prefixes of 1K to 128K tokens, own rows of 64 to 16K)
@@ -430,9 +435,9 @@ SharedPlan shared_plan(int dtype, int batch, int Hkv, int G, int Q, int64_t pref
   const bool f32 = dtype == HC_DTYPE_F32;
   const double stream = 1e6 * 2 * HC_TILE_ELEMS * (f32 ? 4. : 2.) / 6.5e12;
   // (Of rows only the longest's length is known: 0.6 of it stands for the mean.)
-  const double pre_us = prefix_tiles * stream, rows_us = 0.6 * (double)batch * Hkv * row_tiles * stream;
+  const double pre_us = prefix_tiles * stream, rows_us = 0.6 * (double)batch * Hkv * std::max<int64_t>(row_tiles, 0) * stream;
   double best = 0.;
-  for (int nc = 1; nc <= (f32 || M <= 64 ? 1 : 2); ++nc) {
+  for (int nc = 1; with_prefix && nc <= (f32 || M <= 64 ? 1 : 2); ++nc) {
     const int ncg = (int)((M + 64 * nc - 1) / (64 * nc));
     const double tile = f32 ? 1.2 : nc == 1 ? 0.35 : 0.5;
     for (const double k : {0.25, 0.5, 0.75, 1., 1.25, 1.5, 1.75, 2.}) {
@@ -447,9 +452,10 @@ SharedPlan shared_plan(int dtype, int batch, int Hkv, int G, int Q, int64_t pref
       if (best == 0. || t < best) best = t, p.nc = nc, p.ncg = ncg, p.parts = (int)n;
     }
   }
-  const size_t pre = (size_t)p.parts * M, row = (size_t)batch * Hkv * Q * G * p.rows.nsplit;
+  const size_t pre = (size_t)p.parts * M;
+  const size_t row = with_rows && !p.direct ? (size_t)batch * Hkv * Q * G * p.rows.nsplit : 0;
   p.info_at = 0;
-  p.pre_o = up256((size_t)Hkv * 2 * sizeof(int32_t));
+  p.pre_o = with_prefix ? up256((size_t)Hkv * 2 * sizeof(int32_t)) : 0;
   p.pre_ml = p.pre_o + up256(pre * kPartO * sizeof(float));
   p.row_o = p.pre_ml + up256(pre * 2 * sizeof(float));
   p.row_ml = p.row_o + up256(row * kPartO * sizeof(float));
@@ -486,7 +492,7 @@ using namespace hc;
 
 extern "C" size_t hc_shared_workspace_size(int dtype, int batch, int q_heads, int kv_heads, int queries,
                                            int64_t prefix_tiles, int64_t row_tiles) {
-  if (bad_sizes(dtype, batch, q_heads, kv_heads, queries) || prefix_tiles < 0 || row_tiles < 0) return 0;
+  if (bad_sizes(dtype, batch, q_heads, kv_heads, queries)) return 0;
   if (batch == 0 || queries == 0) return 0;
   return shared_plan(dtype, batch, kv_heads, q_heads / kv_heads, queries, prefix_tiles, row_tiles).bytes;
 }
@@ -499,11 +505,14 @@ extern "C" int hc_shared_attn(int dtype, const void* q, const int64_t* q_strides
                               int q_heads, int kv_heads, int queries, float scale, void* workspace,
                               size_t workspace_bytes, void* stream) {
   clear_error();
-  if (bad_sizes(dtype, batch, q_heads, kv_heads, queries) || prefix_tiles < 0 || row_tiles < 0)
+  if (bad_sizes(dtype, batch, q_heads, kv_heads, queries))
     return set_error(HC_ERR_INVALID,
                      "hc_shared_attn: dtype=%d batch=%d q_heads=%d kv_heads=%d queries=%d (q_heads a multiple of "
                      "kv_heads, at most 16 of it, at most 2^24 query rows)",
                      dtype, batch, q_heads, kv_heads, queries);
+  if ((prefix_len && prefix_tiles < 0) || (row_len && row_tiles < 0))
+    return set_error(HC_ERR_INVALID, "hc_shared_attn: prefix_tiles=%lld row_tiles=%lld", (long long)prefix_tiles,
+                     (long long)row_tiles);
   if (!(scale > 0.f) || std::isinf(scale)) return set_error(HC_ERR_INVALID, "hc_shared_attn: scale=%g", (double)scale);
   if (batch == 0 || queries == 0) return HC_OK;
   if (!q || !q_strides || !out || !out_strides || (prefix_len && (!kprefix || !vprefix || !prefix_tile_off)) ||
@@ -518,8 +527,9 @@ extern "C" int hc_shared_attn(int dtype, const void* q, const int64_t* q_strides
        reinterpret_cast<uintptr_t>(workspace)) & 15)
     return set_error(HC_ERR_INVALID, "hc_shared_attn: tensors must be 16-byte aligned");
   const int G = q_heads / kv_heads;
-  const SharedPlan p = shared_plan(dtype, batch, kv_heads, G, queries, prefix_tiles, row_tiles);
-  if (!workspace || workspace_bytes < p.bytes)
+  const SharedPlan p =
+      shared_plan(dtype, batch, kv_heads, G, queries, prefix_len ? prefix_tiles : -1, row_len ? row_tiles : -1);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
     return set_error(HC_ERR_INVALID, "hc_shared_attn: workspace too small (%zu < %zu bytes)", workspace_bytes, p.bytes);
   char* ws = reinterpret_cast<char*>(workspace);
   const float scale_log2 = scale * 1.4426950408889634f;
@@ -543,11 +553,12 @@ extern "C" int hc_shared_attn(int dtype, const void* q, const int64_t* q_strides
   r.query_counts = query_counts;
   r.Hkv = kv_heads, r.G = G, r.Q = queries, r.rows = row_len ? batch * kv_heads : 0;
   r.qpb = p.rows.qpb, r.ncb = p.rows.ncb, r.nsplit = p.rows.nsplit, r.scale_log2 = scale_log2;
-  r.part_o = reinterpret_cast<float*>(ws + p.row_o), r.part_ml = reinterpret_cast<float*>(ws + p.row_ml);
-  for (int i = 0; i < 3; ++i) a.q_s[i] = r.q_s[i] = q_strides[i];
+  if (!p.direct) r.part_o = reinterpret_cast<float*>(ws + p.row_o), r.part_ml = reinterpret_cast<float*>(ws + p.row_ml);
+  r.out = out;
+  for (int i = 0; i < 3; ++i) a.q_s[i] = r.q_s[i] = q_strides[i], r.o_s[i] = out_strides[i];
   const int rc = dtype == HC_DTYPE_BF16  ? launch_shared<__bf16>(a, r, p.nc, s)
                  : dtype == HC_DTYPE_F16 ? launch_shared<_Float16>(a, r, p.nc, s)
                                          : launch_shared<float>(a, r, p.nc, s);
-  if (rc) return rc;
+  if (rc || p.direct) return rc;
   return launch_merge(dtype, mg, (int64_t)batch * queries * q_heads, s);
 }

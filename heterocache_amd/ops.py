@@ -1004,6 +1004,10 @@ def _shared_attn(q, dt, dev, prefix, rows, kv_heads, scale, prefix_tiles, row_ti
         raise ValueError(f"{Hq} query heads are not a multiple of {kv_heads} KV heads")
     out, o_st = _out_bthd(q, out, shape, dev)
     code = dtype_code(dt)
+    if prefix[3] is None:
+        prefix_tiles = -1
+    if rows[3] is None:
+        row_tiles = -1
     nbytes = _bytes("hc_shared_workspace_size", dev, code, B, Hq, kv_heads, Q, prefix_tiles, row_tiles)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     qc = _query_counts(query_counts, B, dev)

@@ -591,10 +591,11 @@ int hc_append_rotated(int dtype, int table_dtype, const void* q, const int64_t* 
  * any device lengths are attended whole whatever they are, so a captured
  * call replays while the rows grow).
  * q, out: base + b*strides[0] + h*strides[1] + i*strides[2] + c, q's strides
- * 16-byte multiples; out shares no memory with q; at most 16 query heads a KV head and 2^24 query rows;
- * scale finite and positive.  workspace: hc_shared_workspace_size bytes,
- * 16-byte aligned, no initialisation; calls that overlap in time need their
- * own.  Matrix products on the input type, softmax and sums in float32.
+ * 16-byte multiples; out shares no memory with q; at most 16 query heads a KV
+ * head and 2^24 query rows; scale finite and positive.  workspace:
+ * hc_shared_workspace_size bytes (asked with prefix_tiles -1 for a call with
+ * no prefix and row_tiles -1 for one with no rows; may be 0), 16-byte aligned,
+ * no initialisation; calls that overlap in time need their own.  Matrix products on the input type, softmax and sums in float32.
  * Stands beside hc_decode_attn, which would read the prefix once a sequence;
  * no counterpart in the reference, whose cache serves one sequence.
  */

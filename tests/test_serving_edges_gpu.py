@@ -204,3 +204,26 @@ def test_room_without_end(dev):
     a, b = (ops.block_select(q, index.bounds, index.exps, index.row_block_off, rows.row_len, 32, n, 9, 1, 2)
             for n in (index.max_blocks, (1 << 31) - 1))
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("B,Hkv,G,Q,lens,dtype", [(1, 2, 4, 300, [500, 300], BF), (2, 1, 16, 70, [90, 70], FP),
+                                                 (1, 1, 5, 129, [129], FL), (2, 2, 3, 33, [4000, 2, 33, 600], BF)])
+def test_chunks_of_queries_over_their_own_rows(dev, B, Hkv, G, Q, lens, dtype):
+    """A chunk that attends itself, without a prefix: into a view, without partials where the rows are not split."""
+    rng = np.random.default_rng(Q)
+    rows, kv = make_rows(rng, lens, dtype, dev, room=4)
+    q = _q(rng, B, Hkv * G, Q, dtype, dev)
+    wide = torch.full((B, Q + 1, Hkv * G + 1, D), 7.0, dtype=dtype, device=dev)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats(dev)
+    held = torch.cuda.memory_allocated(dev)
+    rows.attend_shared(q, None, SCALE, out=wide[:, 1:, 1:])
+    if max(lens) <= 128:  # four tiles a row are not split
+        assert torch.cuda.max_memory_allocated(dev) == held
+    assert (wide[:, 0] == 7).all() and (wide[:, :, 0] == 7).all()
+    for r, (k, v) in enumerate(kv):
+        b, h = divmod(r, Hkv)
+        for i in range(Q):
+            n = max(len(k) - Q + 1 + i, 0)
+            want, tol = attend(q[b, h * G:(h + 1) * G, i], k[:n], v[:n], SCALE, dtype)
+            close(wide[b, 1 + i, 1 + h * G:1 + (h + 1) * G], want, tol, f"row {r} query {i}")
