@@ -6,8 +6,9 @@ import numpy as np
 import pytest
 import torch
 
-from heterocache_amd import ops
-from tests.serving_util import D, attend, bounds, close, make_rows
+from heterocache_amd import _lib, ops
+from heterocache_amd.store import KVStore
+from tests.serving_util import D, attend, bounds, close, make_rows, rotate, rounding, select, unpack
 
 pytestmark = pytest.mark.gpu
 BF, FP, FL = torch.bfloat16, torch.float16, torch.float32
@@ -227,3 +228,200 @@ def test_chunks_of_queries_over_their_own_rows(dev, B, Hkv, G, Q, lens, dtype):
             n = max(len(k) - Q + 1 + i, 0)
             want, tol = attend(q[b, h * G:(h + 1) * G, i], k[:n], v[:n], SCALE, dtype)
             close(wide[b, 1 + i, 1 + h * G:1 + (h + 1) * G], want, tol, f"row {r} query {i}")
+
+
+def _turned(x, cos, sin):
+    """rotate with one table a sequence, and the bound of its result in the type of x."""
+    want, tol = rotate(x, cos, sin)
+    return want, tol + rounding(want, x.dtype)
+
+
+@pytest.mark.parametrize("dtype,tdt", [(BF, BF), (BF, FL), (FP, FP), (FP, FL), (FL, FL)])
+@pytest.mark.parametrize("B,Hkv,G", [(65, 8, 4), (129, 4, 16), (600, 1, 1), (86, 6, 7)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_one_token_of_many_rows(dev, dtype, tdt, B, Hkv, G, in_place):
+    """More than 512 rows of one token each: some at a tile's last slot, some full, some sequences with a count of 0."""
+    rng = np.random.default_rng(B)
+    R = B * Hkv
+    draw = lambda *s: torch.as_tensor(rng.standard_normal(s), dtype=torch.float32)
+    q, k, v = (draw(B, 1, h, D).to(dtype).to(dev).transpose(1, 2) for h in (Hkv * G, Hkv, Hkv))
+    ang = rng.uniform(-3, 3, (B, 1, D))
+    cos, sin = (torch.as_tensor(f(ang), dtype=torch.float32).to(tdt).to(dev) for f in (np.cos, np.sin))
+    start = rng.integers(0, 64, R)
+    start[::7] = 31
+    start[3::11] = 64  # full
+    counts = (rng.random(B) < 0.8).astype(np.int32)
+    counts[0], counts[1] = 1, 0
+    store = KVStore([64] * R, dtype, dev)
+    store.k.copy_(draw(store.k.numel()).to(dtype))
+    store.v.copy_(draw(store.v.numel()).to(dtype))
+    store.set_lengths(start)
+    before = [x.clone() for x in unpack(store.k, store.v)]
+    lens = store.row_len if in_place else torch.full_like(store.row_len, -7)
+    got = ops.append_rotated(q, k, v, cos, sin, *_meta(store), store.row_cap, len_out=lens, status=store.status,
+                             counts=torch.as_tensor(counts).to(dev))
+    want, tol = _turned(q, cos, sin)
+    close(got, want, tol, "queries")
+    per_row = np.repeat(counts, Hkv)
+    stored = torch.as_tensor((per_row > 0) & (start < 64)).to(dev)
+    assert lens.tolist() == (start + stored.cpu().numpy()).tolist()
+    assert bool(store.status) == bool(((per_row > 0) & (start == 64)).any())
+    at = (store.row_tile_off * 32 + torch.as_tensor(start).to(dev))[stored]
+    want, tol = _turned(k, cos, sin)
+    kn, vn = unpack(store.k, store.v)
+    close(kn[at], want.reshape(R, D)[stored], tol.reshape(R, D)[stored], "keys")
+    assert torch.equal(vn[at], v.reshape(R, D)[stored])
+    rest = torch.ones(len(kn), dtype=torch.bool, device=dev)
+    rest[at] = False
+    assert torch.equal(kn[rest], before[0][rest]) and torch.equal(vn[rest], before[1][rest])
+
+
+@pytest.mark.parametrize("Q,dtype", [(1, BF), (3, FP), (5, FL)])
+def test_waves_of_many_tiles(dev, Q, dtype):
+    """Rows cut for one tile: each of four waves walks more than 64 tiles, and more than 128."""
+    rng = np.random.default_rng(Q)
+    rows, kv = make_rows(rng, [9001, 17003, 8192, 8193], dtype, dev, room=5)
+    q = _q(rng, 2, 6, Q, dtype, dev)
+    got = ops.shared_attn(q, None, _meta(rows), 2, SCALE, row_tiles=1)
+    for r, (k, v) in enumerate(kv):
+        b, h = divmod(r, 2)
+        for i in range(Q):
+            n = len(k) - Q + 1 + i
+            want, tol = attend(q[b, 3 * h:3 * h + 3, i], k[:n], v[:n], SCALE, dtype)
+            close(got[b, i, 3 * h:3 * h + 3], want, tol, f"row {r} query {i}")
+
+
+@pytest.mark.parametrize("G,dtype", [(4, BF), (9, FP), (2, FL)])
+def test_lists_of_many_tiles(dev, G, dtype):
+    """So many queries that no list is split, each of more than 64 tiles a wave: whole lists, shorter ones, entries in any
+    order and some that are no block of the row."""
+    rng = np.random.default_rng(G)
+    B, Q, block, keep = 2, 260, 64, 400
+    n = 64 * 500 - 9
+    rows, kv = make_rows(rng, [n, 64 * 300 + 5], dtype, dev)
+    q = _q(rng, B, G, Q, dtype, dev)
+    idx = np.stack([[rng.permutation(520)[:keep] for _ in range(Q)] for _ in range(B)]).astype(np.int32)
+    counts = rng.choice([keep, keep, 399, 130, 129, 128, 1], (B, Q)).astype(np.int32)
+    assert _lib.load().hc_block_attn_workspace_size(B, G, 1, Q, block, keep) == 0
+    got = ops.block_attn(q, rows.k, rows.v, rows.row_tile_off, rows.row_len, torch.as_tensor(idx).to(dev),
+                         torch.as_tensor(counts).to(dev), block, SCALE)
+    for r, (k, v) in enumerate(kv):
+        for i in list(range(0, Q, 37)) + [Q - 1]:
+            seen = len(k) - Q + 1 + i
+            pos = (np.sort(idx[r, i, :counts[r, i]])[:, None] * block + np.arange(block)).reshape(-1)
+            pos = torch.as_tensor(pos[pos < seen], dtype=torch.int64).to(dev)
+            want, tol = attend(q[r, :, i], k[pos], v[pos], SCALE, dtype)
+            close(got[r, i], want, tol, f"row {r} query {i}")
+
+
+@pytest.mark.parametrize("block,dtype", [(64, BF), (96, FP), (128, FL), (32, BF)])
+def test_bounds_of_many_blocks(dev, block, dtype):
+    """So many blocks that a workgroup takes several of a row, the next one's first tiles on their way: all entries, and no
+    others."""
+    rng = np.random.default_rng(block)
+    lens = [block * 300 + 7, block * 299, 5, block * 150 + block - 1] * 8
+    store = KVStore([n + 40 for n in lens], dtype, dev)
+    gen = torch.Generator(device=dev).manual_seed(block)
+    store.k.copy_(torch.randn(store.k.numel(), generator=gen, device=dev).to(dtype))
+    store.set_lengths(lens)
+    index = store.block_index(block)
+    assert len(lens) * (max(lens) // block) > 2 * 8 * torch.cuda.get_device_properties(dev).multi_processor_count
+    index.bounds.fill_(5)
+    index.exps.fill_(77)
+    index.update()
+    kn, _ = unpack(store.k, store.v)
+    filled = torch.zeros(len(index.exps), dtype=torch.bool, device=dev)
+    for r, n in enumerate(lens):
+        j, at, off = n // block, int(store.host_tile_off[r]) * 32, int(index.row_block_off[r])
+        cut = kn[at:at + j * block].double().view(j, block, D)
+        hi, lo = cut.amax(1), cut.amin(1)
+        e = torch.ceil(torch.log2(torch.maximum(hi.abs(), lo.abs()).amax(1) / 127))  # (64 bits: no top is on a border)
+        unit = torch.exp2(e)[:, None]
+        assert torch.equal(index.exps[off:off + j].double(), e), r
+        assert torch.equal(index.bounds[off:off + j, 0].double(), torch.ceil(hi / unit)), r
+        assert torch.equal(index.bounds[off:off + j, 1].double(), torch.floor(lo / unit)), r
+        filled[off:off + j] = True
+    assert (index.exps[~filled] == 77).all() and (index.bounds[~filled] == 5).all()
+
+
+@pytest.mark.parametrize("blocks,keep", [(n, 40) for n in (257, 258, 1023, 1024, 1026, 2051, 4099, 6143, 6146, 12287, 12288)]
+                         + [(300, 150), (5000, 2500)])
+@pytest.mark.parametrize("B,Hkv,Q", [(20, 8, 1), (3, 2, 22)])
+def test_selection_that_scores_its_own_rows(dev, blocks, keep, B, Hkv, Q):
+    """So many queries that each row is scored where it is picked from, however long (keys in LDS): lengths around each
+    change of its workgroups, many equal scores, against sorting."""
+    rng = np.random.default_rng(blocks + Q)
+    G, R = 2, B * Hkv
+    assert _lib.load().hc_block_select_scratch_size(B, Hkv, Q, blocks) == 0
+    assert _lib.load().hc_block_select_scratch_size(B, Hkv, Q, 12289) > 0
+    lens = [(32 * blocks, 32 * blocks - 7, 32 * (blocks // 2) + Q, 32 * (keep + 1) + Q, 32 * (blocks - 1) + Q)[r % 5]
+            for r in range(R)]
+    # One table for all rows: pairs of equal blocks in it.
+    hi = rng.integers(-127, 128, (blocks, D)).astype(np.int8)
+    hi[1::3] = hi[::3][:len(hi[1::3])]
+    lo = np.minimum(hi, rng.integers(-127, 128, hi.shape)).astype(np.int8)
+    lo[1::3] = lo[::3][:len(lo[1::3])]
+    ex = np.full(blocks, -5, np.int8)
+    q = _q(rng, B, Hkv * G, Q, BF, dev)
+    table = torch.as_tensor(np.stack([hi, lo], 1)).to(dev)
+    idx, counts = ops.block_select(q, table, torch.as_tensor(ex).to(dev), torch.zeros(R, dtype=torch.int64, device=dev),
+                                   torch.tensor(lens, dtype=torch.int32, device=dev), 32, blocks, keep, sink=1, local=2)
+    # Whole numbers below 2^24 times powers of two: exact in 64 bits.
+    hd, ld = (torch.as_tensor(x).to(dev).double().t().contiguous() for x in (hi, lo))
+    qd = q.double().view(B, Hkv, G, Q, D)
+    top = qd.abs().amax(-1, keepdim=True)
+    eq = torch.ceil(torch.log2(top / 127)).clamp(-48, 48)
+    q8 = torch.round(qd / torch.exp2(eq)).clamp(-127, 127).reshape(-1, D)
+    s = (q8.clamp(min=0) @ hd + q8.clamp(max=0) @ ld).view(B, Hkv, G, Q, blocks) * torch.exp2(eq - 5)
+    s = s.amax(2).reshape(R, Q, blocks)
+    seen = torch.tensor(lens, device=dev)[:, None] - Q + 1 + torch.arange(Q, device=dev)
+    have = ((seen + 31) // 32)[..., None]
+    j = torch.arange(blocks, device=dev)
+    s = torch.where((j < 1) | (j >= have - 2), torch.full_like(s, math.inf), s)
+    s = torch.where(j < have, s, torch.full_like(s, -math.inf))
+    want = torch.sort(s, dim=-1, descending=True, stable=True).indices[..., :keep].sort(-1).values
+    assert (have > keep).all() and (counts == keep).all()
+    assert torch.equal(idx.long(), want)
+
+
+@pytest.mark.parametrize("B,Hkv,G,Q,blocks,keep,dtype", [
+    (2, 2, 4, 1, 60, 8, BF), (1, 2, 9, 1, 60, 8, FP), (2, 1, 4, 3, 700, 6, BF), (1, 1, 2, 1, 100, 80, FL),
+    (5, 4, 1, 1, 300, 6, BF),
+])
+def test_block_step_of_plain_tensors(dev, B, Hkv, G, Q, blocks, keep, dtype):
+    """ops.block_step, on tensors of its own: its output, list and counts against the plain form, with query counts."""
+    rng = np.random.default_rng(blocks)
+    n = 32 * blocks
+    rows, kv = make_rows(rng, [(n - 5, n // 2, 40, n)[r % 4] for r in range(B * Hkv)], dtype, dev, room=6)
+    index = rows.block_index(32)
+    index.update()
+    q = _q(rng, B, Hkv * G, Q, dtype, dev)
+    part = torch.as_tensor(rng.integers(0, Q + 1, B), dtype=torch.int32).to(dev)
+    for qc in (None, part):
+        out, idx, counts = ops.block_step(q, *_meta(rows), index.bounds, index.exps, index.row_block_off, 32,
+                                          index.max_blocks, keep, SCALE, sink=1, local=2, query_counts=qc)
+        for r in ([0, 1, len(kv) - 1] if len(kv) > 8 else range(len(kv))):
+            k, v = kv[r]
+            b, h = divmod(r, Hkv)
+            table = bounds(k, 32)
+            for i in range(Q):
+                c = Q if qc is None else int(qc[b])
+                seen = min(max(len(k) - c + 1 + i, 0), len(k))
+                head = q[b, h * G:(h + 1) * G, i]
+                want = select(head, *table, seen, 32, keep, 1, 2)
+                assert int(counts[r, i]) == len(want) and idx[r, i, :len(want)].tolist() == want.tolist(), (r, i)
+                pos = (want[:, None] * 32 + np.arange(32)).reshape(-1)
+                pos = torch.as_tensor(pos[pos < seen], dtype=torch.int64).to(dev)
+                ref, tol = attend(head, k[pos], v[pos], SCALE, dtype)
+                close(out[b, i, h * G:(h + 1) * G], ref, tol, f"row {r} query {i}")
+    meta = (index.bounds, index.exps, index.row_block_off)
+    for bad in (dict(bounds=index.bounds[:1]), dict(exps=index.exps.int()), dict(off=index.row_block_off.int())):
+        a = dict(bounds=meta[0], exps=meta[1], off=meta[2])
+        a.update(bad)
+        with pytest.raises(ValueError):
+            ops.block_step(q, *_meta(rows), a["bounds"], a["exps"], a["off"], 32, index.max_blocks, keep, SCALE)
+    with pytest.raises(TypeError):
+        ops.block_step(q, rows.k.to(torch.int16), rows.v, rows.row_tile_off, rows.row_len, *meta, 32, index.max_blocks, keep,
+                       SCALE)
+    with pytest.raises(_lib.HCError, match="block=40"):
+        ops.block_step(q, *_meta(rows), *meta, 40, index.max_blocks, keep, SCALE)
