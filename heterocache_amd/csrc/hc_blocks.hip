@@ -869,7 +869,12 @@ int launch_attn(int dtype, RowsArgs& r, const BlockPlan& p, void* workspace, hip
 }
 
 // Whether one launch does it all: few queries, short rows and lists that eight
-// waves attend unsplit.
+// waves attend unsplit.  16 of 384, 512, 640, 768 and 1024 blocks kept for 8
+// queries: 13.3, 14.9, 16.5, 16.9 and 18.8 us in one launch, 15.6, 16.5, 16.3,
+// 16.3 and 16.2 as selection (scores through memory) and attention; 64 queries
+// 16.6 against 17.8 at 512 and 20.1 against 18.6 at 1024; with 192, which score
+// their own rows either way, one launch stays 2 to 3 us ahead.  The list lies in
+// LDS: 2048 entries beside the waves' states and the keys take 49 KB.
 constexpr int kStepBlocks = 512;
 bool one_launch(const BlockPlan& p, int64_t queries, int max_blocks, int keep) {
   return p.waves == 8 && p.nsplit == 1 && queries <= device_cus() && max_blocks <= kStepBlocks && keep <= 2048;

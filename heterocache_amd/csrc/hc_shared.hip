@@ -381,7 +381,8 @@ constexpr size_t shared_lds(bool prefix) {
 
 // Prefix workgroups come first: they are the long ones.  (One round of them,
 // then the rows', then the rest: 282 us against 265 for 512 columns over 756K
-// tokens beside rows of 1.06M.)
+// tokens beside rows of 1.06M.)  Registers for three workgroups a CU serve calls
+// of rows alone; beside a prefix the ring's 64 KB of LDS leave two.
 template <typename T, int NC, bool MIXED>
 __global__ __launch_bounds__(kPreThreads, sizeof(T) == 4 ? 1 : NC == 2 ? 2 : 3) void shared_attn_kernel(
     const PrefixArgs pre, const RowsArgs rows) {
@@ -435,7 +436,8 @@ SharedPlan shared_plan(int dtype, int batch, int Hkv, int G, int Q, int64_t pref
   const bool f32 = dtype == HC_DTYPE_F32;
   const double stream = 1e6 * 2 * HC_TILE_ELEMS * (f32 ? 4. : 2.) / 6.5e12;
   // (Of rows only the longest's length is known: 0.6 of it stands for the mean.)
-  const double pre_us = prefix_tiles * stream, rows_us = 0.6 * (double)batch * Hkv * std::max<int64_t>(row_tiles, 0) * stream;
+  const double pre_us = prefix_tiles * stream;
+  const double rows_us = 0.6 * (double)batch * Hkv * std::max<int64_t>(row_tiles, 0) * stream;
   double best = 0.;
   for (int nc = 1; with_prefix && nc <= (f32 || M <= 64 ? 1 : 2); ++nc) {
     const int ncg = (int)((M + 64 * nc - 1) / (64 * nc));

@@ -133,7 +133,9 @@ class KVStore:
         self._grown(None)
         idx = ops.to_device(rows, self.device, torch.int64)
         self.row_len.index_copy_(0, idx, ops.to_device(lens, self.device, torch.int32))
-        # Longest rows are scheduled first; appends keep this order.
+        # Longest rows are scheduled first.  Appends leave the order as it is
+        # (append_rotated with counts may make others the longest: results do
+        # not depend on it, set_lengths orders anew).
         order = np.argsort(-self.host_len.astype(np.int64), kind="stable").astype(np.int32)
         self._headroom = int((self.host_cap - self.host_len).min()) if self.rows else 0
         self.row_order = ops.to_device(order, self.device)

@@ -44,6 +44,6 @@ def test_negative_tile_counts(lib):
     st = (ctypes.c_int64 * 3)(1024, 128, 1024)
     fake = 4096
     for pre, rows, pt, rt in ((fake, fake, -1, 4), (fake, fake, 4, -1), (None, fake, 4, -2), (fake, None, -1, 4)):
-        rc = lib.hc_shared_attn(2, fake, st, fake, fake, fake, pre, pt, fake, fake, fake, rows, None, rt, fake, st, 1, 8, 2,
-                                1, 0.1, fake, 1 << 40, None)
+        rc = lib.hc_shared_attn(2, fake, st, fake, fake, fake, pre, pt, fake, fake, fake, rows, None, rt, fake, st, 1,
+                                8, 2, 1, 0.1, fake, 1 << 40, None)
         assert rc == _lib.HC_ERR_INVALID and b"tiles=-" in lib.hc_last_error()

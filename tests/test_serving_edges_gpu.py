@@ -101,8 +101,8 @@ def test_scores_of_minus_infinity(dev, dtype):
 
 
 def test_whole_update_after_replayed_appends(dev):
-    """Captured appends advance the lengths on the device and not the host's mirror: an update() outside of the graph, on
-    the current stream or on another, still takes every complete block."""
+    """Captured appends advance the lengths on the device and not the host's mirror: an update() outside of the graph,
+    on the current stream or on another, still takes every complete block."""
     rng = np.random.default_rng(4)
     rows, kv = make_rows(rng, [40, 95, 0], BF, dev, room=400, stale=0.0)
     index = rows.block_index(32)
@@ -293,8 +293,8 @@ def test_waves_of_many_tiles(dev, Q, dtype):
 
 @pytest.mark.parametrize("G,dtype", [(4, BF), (9, FP), (2, FL)])
 def test_lists_of_many_tiles(dev, G, dtype):
-    """So many queries that no list is split, each of more than 64 tiles a wave: whole lists, shorter ones, entries in any
-    order and some that are no block of the row."""
+    """So many queries that no list is split, each of more than 64 tiles a wave: whole lists, shorter ones, entries in
+    any order and some that are no block of the row."""
     rng = np.random.default_rng(G)
     B, Q, block, keep = 2, 260, 64, 400
     n = 64 * 500 - 9
@@ -316,8 +316,8 @@ def test_lists_of_many_tiles(dev, G, dtype):
 
 @pytest.mark.parametrize("block,dtype", [(64, BF), (96, FP), (128, FL), (32, BF)])
 def test_bounds_of_many_blocks(dev, block, dtype):
-    """So many blocks that a workgroup takes several of a row, the next one's first tiles on their way: all entries, and no
-    others."""
+    """So many blocks that a workgroup takes several of a row, the next one's first tiles on their way: all entries, and
+    no others."""
     rng = np.random.default_rng(block)
     lens = [block * 300 + 7, block * 299, 5, block * 150 + block - 1] * 8
     store = KVStore([n + 40 for n in lens], dtype, dev)
@@ -344,8 +344,8 @@ def test_bounds_of_many_blocks(dev, block, dtype):
     assert (index.exps[~filled] == 77).all() and (index.bounds[~filled] == 5).all()
 
 
-@pytest.mark.parametrize("blocks,keep", [(n, 40) for n in (257, 258, 1023, 1024, 1026, 2051, 4099, 6143, 6146, 12287, 12288)]
-                         + [(300, 150), (5000, 2500)])
+@pytest.mark.parametrize("blocks,keep", [(n, 40) for n in (257, 258, 1023, 1024, 1026, 2051, 4099, 6143, 6146, 12287,
+                                                                     12288)] + [(300, 150), (5000, 2500)])
 @pytest.mark.parametrize("B,Hkv,Q", [(20, 8, 1), (3, 2, 22)])
 def test_selection_that_scores_its_own_rows(dev, blocks, keep, B, Hkv, Q):
     """So many queries that each row is scored where it is picked from, however long (keys in LDS): lengths around each
@@ -421,7 +421,7 @@ def test_block_step_of_plain_tensors(dev, B, Hkv, G, Q, blocks, keep, dtype):
         with pytest.raises(ValueError):
             ops.block_step(q, *_meta(rows), a["bounds"], a["exps"], a["off"], 32, index.max_blocks, keep, SCALE)
     with pytest.raises(TypeError):
-        ops.block_step(q, rows.k.to(torch.int16), rows.v, rows.row_tile_off, rows.row_len, *meta, 32, index.max_blocks, keep,
-                       SCALE)
+        ops.block_step(q, rows.k.to(torch.int16), rows.v, rows.row_tile_off, rows.row_len, *meta, 32, index.max_blocks,
+                       keep, SCALE)
     with pytest.raises(_lib.HCError, match="block=40"):
         ops.block_step(q, *_meta(rows), *meta, 40, index.max_blocks, keep, SCALE)
