@@ -584,9 +584,10 @@ int hc_append_rotated(int dtype, int table_dtype, const void* q, const int64_t* 
  * decode step).  The others are padding and see the whole row.  Zeros where
  * nothing is visible; NaN where a visible score is NaN or all are -inf.  The
  * prefix is a store of kv_heads rows, each of its own length (a prompt kept
- * whole or compressed per head), and is read once for all sequences.  prefix_len NULL: no prefix;
- * row_len NULL: no rows of their own.  prefix_tiles, row_tiles: tiles of all
- * prefix rows and of the longest own row that the call should be cut for
+ * whole or compressed per head), and is read once for all sequences.
+ * prefix_len NULL: no prefix; row_len NULL: no rows of their own.
+ * prefix_tiles, row_tiles: tiles of all prefix rows and of the longest own row
+ * that the call should be cut for
  * (bounds such as the capacities; they set the grid and the workspace, and
  * any device lengths are attended whole whatever they are, so a captured
  * call replays while the rows grow).

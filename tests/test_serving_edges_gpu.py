@@ -168,6 +168,29 @@ def test_flat_tail_behind_a_dominant_token(dev, dtype, drop):
         close(out[0, 0, 0], want, tol * 1.02 + torch.finfo(dtype).tiny * torch.finfo(dtype).eps, f"{name} e^-{drop}")
 
 
+@pytest.mark.parametrize("what", ["peaked", "huge", "rising", "falling"])
+@pytest.mark.parametrize("n", [70, 3000])
+def test_fp16_scores_far_apart(dev, what, n):
+    """One dominant key late, scores in the thousands, a steady rise or fall over many reference points."""
+    rng = np.random.default_rng(n)
+    prefix, rows = (make_rows(rng, [n], FP, dev, room=3)[0] for _ in range(2))
+    k, v = (torch.as_tensor(rng.standard_normal((n, D)), dtype=torch.float32).to(FP).to(dev) for _ in range(2))
+    q = _q(rng, 1, 4, 1, FP, dev)
+    if what == "peaked":
+        k[n - 5] = 12 * q[0, 0, 0]
+    elif what == "huge":
+        k *= 60
+    else:
+        ends = (-4, 4) if what == "rising" else (4, -4)
+        k[:] = q[0, 0, 0] * torch.linspace(*ends, n, device=dev)[:, None].to(FP)
+    for store in (prefix, rows):
+        store.write_rows(k[None, None], v[None, None], [(0, 0)], [0], [n])
+    for name, out, use_pre, use_own in _every_way(q, prefix, rows):
+        want, tol = attend(q[0, :, 0], *_cat((k, v), (k, v), use_pre, use_own), SCALE, FP)
+        # Weights below 2^-24 of the greatest: half of fp16's smallest step, 2^-35 of it, each.
+        close(out[0, 0], want, tol + 2 * n * 2.0 ** -35 * v.double().abs().amax(0), f"{name} {what}")
+
+
 @pytest.mark.parametrize("dtype", [BF, FP, FL])
 @pytest.mark.parametrize("size", [64.0, 700.0, 1024.0, 2048.0])
 def test_scores_far_beyond_the_exponent(dev, dtype, size):
