@@ -28,6 +28,18 @@ c_int, c_int32, c_int64, c_size_t, c_float, c_void_p, c_char_p = (
     ctypes.c_int, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t, ctypes.c_float, ctypes.c_void_p,
     ctypes.c_char_p)
 
+
+class PagedCache(ctypes.Structure):
+    """hc_paged_cache of include/hc.h."""
+
+    _fields_ = [("dtype", c_int32), ("batch", c_int32), ("kv_heads", c_int32), ("heads", c_int32),
+                ("pages", c_int32), ("page_tokens", c_int32), ("table_pages", c_int32), ("reserved", c_int32),
+                ("k", c_void_p), ("v", c_void_p), ("k_strides", c_int64 * 3), ("v_strides", c_int64 * 3),
+                ("table", c_void_p), ("table_stride", c_int64), ("row_len", c_void_p),
+                ("weights", c_void_p), ("weight_stride", c_int64), ("pos", c_void_p), ("pos_stride", c_int64),
+                ("dropped", c_void_p), ("status", c_void_p)]
+
+
 # name -> (restype, argtypes); the single Python mirror of include/hc.h.
 SIGNATURES = {
     "hc_last_error": (c_char_p, []),
@@ -125,6 +137,14 @@ SIGNATURES = {
                               c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                               c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "hc_block_step_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "hc_paged_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "hc_paged_attn": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                              c_void_p, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                              c_void_p]),
+    "hc_paged_workspace_size": (c_size_t, [c_void_p, c_int, c_int, c_int, c_int]),
+    "hc_paged_evict": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                               c_void_p, c_size_t, c_void_p]),
+    "hc_paged_evict_scratch_size": (c_size_t, [c_void_p]),
     "hc_store_read": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p,
                               c_void_p]),
 }

@@ -1,0 +1,625 @@
+// Attention of a chunk of new tokens over a paged cache: more than 16 (query,
+// head) columns of a row.
+//
+//   out[c] = sum_t softmax_t(scale q_c . k_t) v_t,   c = i * G + g,
+//   t < base + i + 1
+//
+// A workgroup of four waves takes 128 columns, 32 a wave: the queries of all
+// heads of a group lie beside each other, so a key is read once for 128 / G
+// queries of every head, and the causal edge is as steep as it can be.  Keys
+// advance 64 tokens at a time through LDS, copied straight from the pages
+// (keys double-buffered, values once, as the next ones are requested behind
+// the product that reads them); the values' operand is a transposed LDS read,
+// so pages keep the order in which tokens arrive.  Scores, softmax and O stay
+// in registers.
+//
+// Where page sizes are multiples of 16, the 16 tokens of a copy lie in one page
+// and its address is scalar; other sizes pay an address a lane.
+#include <algorithm>
+#include <mutex>
+
+#include "hc_paged.h"
+
+namespace hc {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kWaveCols = 32;
+constexpr int kCols = kWaves * kWaveCols;
+constexpr int kKeys = 64;  // tokens an iteration
+constexpr int kTiles = kKeys / HC_TILE;
+
+template <typename T>
+constexpr int chunk_lds() {
+  return 3 * kTiles * Tile<T>::kBytes;
+}
+
+// Copies of 64 tokens of keys or values by a workgroup: load r of a thread is
+// chunk tid % kChunks of token r * kPer + tid / kChunks.
+template <typename T, bool UNIFORM>
+struct Stage {
+  static constexpr int kPer = kThreads / Tile<T>::kChunks;  // tokens of one load of all threads: 16 or 8
+  static constexpr int kLoads = kKeys / kPer;
+  const Pool& p;
+  const int32_t* tab;
+  int total, tok, wave;
+  uint32_t chunk;
+  __device__ __forceinline__ Stage(const Pool& pool, int row, int total_tok) : p(pool), total(total_tok) {
+    tab = p.table + table_row(p, row) * p.table_stride;
+    tok = threadIdx.x / Tile<T>::kChunks;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    chunk = 16 * ((threadIdx.x % Tile<T>::kChunks) ^ Tile<T>::swizzle(tok));
+  }
+  // Pages of the tokens t0 + [0, 64): of each 16 of them, or of this thread's.
+  static constexpr int kEntries = UNIFORM ? kKeys / 16 : kLoads;
+  __device__ __forceinline__ int token(int t0, int r) const {
+    return UNIFORM ? min(t0 + 16 * r, (total - 1) & ~15) : min(t0 + r * kPer + tok, total - 1);
+  }
+  __device__ __forceinline__ void entries(int t0, int (&e)[kEntries]) const {
+#pragma unroll
+    for (int r = 0; r < kEntries; ++r) e[r] = tab[page_of(p, token(t0, r))];
+  }
+  __device__ __forceinline__ void copy(int t0, const int (&e)[kEntries], const char* pool, int64_t s_page, int64_t s_tok,
+                                       char* lds, bool& bad) const {
+#pragma unroll
+    for (int r = 0; r < kLoads; ++r) {
+      constexpr int kSame = UNIFORM ? 16 / kPer : 1;  // loads of one entry
+      int pg = e[r / kSame];
+      if ((uint32_t)pg >= (uint32_t)p.pages) bad = true, pg = 0;
+      const int t = token(t0, r / kSame);
+      const int at = t - page_of(p, t) * p.page_tokens;
+      const char* src = pool + pg * s_page + at * s_tok;
+      // (The swizzle is linear in the token's bits.)
+      src += chunk ^ (uint32_t)(16 * Tile<T>::swizzle(r * kPer & 15));
+      if constexpr (UNIFORM) src += (uint32_t)((r % kSame * kPer + tok) * (int)s_tok);
+      lds_dma16(src, lds + r * kThreads * 16 + wave * 1024);
+    }
+  }
+};
+
+// The product of 16 channels of values with a tile's probabilities where some
+// column does not see some token: what lies behind `end`, which no column sees,
+// becomes zero, and an infinite or NaN value reaches the columns that give it a
+// weight and no others (see tile_values in hc_rows.h).
+template <typename T>
+__device__ __forceinline__ void edge_values(typename Elem<T>::vec8 va, const typename Elem<T>::vec8 (&pb)[2], int tok0, int end,
+                                            int g, f32x4 (&o)[2]) {
+  if (tok0 + HC_TILE > end) zero_tail<T>(va, tok0, end, g);
+  bool odd = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = vec8_at<T>(va, e);
+    odd |= !(x - x == 0.f);
+  }
+  if (__any(odd)) {
+    typename Elem<T>::vec8 up, down;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = vec8_at<T>(va, e);
+      const bool is = !(x - x == 0.f);
+      set8<T>(up, e, is && !(x < 0.f) ? 1.f : 0.f);
+      set8<T>(down, e, is && !(x > 0.f) ? 1.f : 0.f);
+      if (is) set8<T>(va, e, 0.f);
+    }
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f32x4 wu = mma_16x16x32(up, pb[j], zero), wd = mma_16x16x32(down, pb[j], zero);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (wu[r] > 0.f) o[j][r] += INFINITY;
+        if (wd[r] > 0.f) o[j][r] -= INFINITY;
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) o[j] = mma_16x16x32(va, pb[j], o[j]);
+}
+
+template <typename T, bool UNIFORM, bool SPLIT>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_kernel(const PagedAttn a) {
+  typedef typename Elem<T>::vec8 vec8;
+  typedef Tile<T> Tl;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const Pool& p = a.pool;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g4 = lane >> 4, n16 = lane & 15;
+  // Workgroup -> (row, part, block of columns), the blocks with the most keys first.
+  const int row = blockIdx.x % p.rows, rest = blockIdx.x / p.rows;
+  const int part = SPLIT ? rest % a.parts : 0;
+  const int cb = a.blocks - 1 - (SPLIT ? rest / a.parts : rest);
+  const int b = row / p.Hkv, h = row % p.Hkv;
+  const int hd = p.heads == 1 ? 0 : h;
+  const RowSpan span = row_span(p, row);
+  // An append ahead of this launch has left the rows' tokens behind.
+  const int info = a.info ? a.info[table_row(p, row)].y : span.total;
+  const bool room = info >= 0;
+  const int total = room ? info : -1 - info, nq = span.n, ncols = nq * a.G;
+  const int base = total - nq;
+  if (a.len_out && rest == 0 && tid == 0 && (p.heads == 1 || h == 0)) a.len_out[table_row(p, row)] = total;
+  const int c_first = cb * kCols, c_wave = c_first + wave * kWaveCols;
+  if (SPLIT && c_first >= ncols) return;  // (padding: the fold writes it)
+  // The last query of the workgroup, and of the wave, that is a token.
+  const int i_last = min(c_first + kCols, ncols) - 1;
+  const int seen = !room || c_first >= ncols ? 0 : min(max(base + i_last / a.G + 1, 0), total);
+  const int its_all = (seen + kKeys - 1) / kKeys;
+  const int share = SPLIT ? (its_all + a.parts - 1) / a.parts : its_all;
+  const int it0 = SPLIT ? min(part * share, its_all) : 0, it1 = SPLIT ? min(it0 + share, its_all) : its_all;
+  const bool active = c_wave < ncols && room;
+  const int w_lo = min(max(base + c_wave / a.G + 1, 0), total);  // tokens that all columns of the wave see
+  const int w_hi = active ? min(max(base + (min(c_wave + kWaveCols, ncols) - 1) / a.G + 1, 0), total) : 0;
+
+  // Q^T operands: column c_wave + 16 j + n16, k-slots = channels 32 s + 8 g4 + [0, 8).
+  vec8 qop[2][4];
+  int lim[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int c = c_wave + 16 * j + n16;
+    const bool ok = c < ncols;
+    const int i = ok ? c / a.G : 0, gi = ok ? c % a.G : 0;
+    lim[j] = ok ? min(max(base + i + 1, 0), total) : w_hi;  // (padding beside tokens sees what the last does)
+    const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_s[0] + (int64_t)(h * a.G + gi) * a.q_s[1] + i * a.q_s[2] + 8 * g4;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) qop[j][s] = ok ? load8<T>(qp + 32 * s) : zero8<T>();
+  }
+
+  f32x4 o[8][2];
+#pragma unroll
+  for (int db = 0; db < 8; ++db)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) o[db][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  bool bad = false;
+
+  typedef Stage<T, UNIFORM> St;
+  const St st(p, row, max(total, 1));
+  const char* const kp = p.k + hd * p.k_head;
+  const char* const vp = p.v + hd * p.v_head;
+  constexpr int kSet = kTiles * Tl::kBytes;
+  char* const sv = lds + 2 * kSet;
+  int e0[St::kEntries], e1[St::kEntries];  // pages of this iteration's tokens, and of the next one's
+  if (it0 < it1) {
+    st.entries(it0 * kKeys, e0);
+    st.copy(it0 * kKeys, e0, kp, p.k_page, p.k_tok, lds, bad);
+    st.copy(it0 * kKeys, e0, vp, p.v_page, p.v_tok, sv, bad);
+    if (it0 + 1 < it1) st.entries((it0 + 1) * kKeys, e1);
+  }
+  wait_lds_dma();
+  __syncthreads();
+
+  for (int it = it0; it < it1; ++it) {
+    const int t0 = it * kKeys;
+    const bool more = it + 1 < it1;
+    if (more) st.copy(t0 + kKeys, e1, kp, p.k_page, p.k_tok, lds + ((it - it0 + 1) & 1) * kSet, bad);
+    const bool work = active && t0 < w_hi;
+    const bool edge = t0 + kKeys > w_lo;  // some column does not see all of these tokens
+    vec8 pb[2][2];
+    if (work) {
+      __builtin_amdgcn_s_setprio(0);
+      const char* sk = lds + ((it - it0) & 1) * kSet;
+      // S^T blocks: rows = tokens 16 tb + 4 g4 + r, column = c_wave + 16 j + n16.
+      f32x4 sacc[4][2];
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) sacc[tb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb) {
+        if constexpr (sizeof(T) == 4) {
+          // Sums of 32 channels apart: a rounding is half a step of the partial
+          // sum that it falls on.
+          f32x4 sum[4][2];
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const vec8 ka = key_operand<T>(sk + (tb >> 1) * Tl::kBytes, g4, n16, tb & 1, s);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) sum[s][j] = mma_16x16x32(ka, qop[j][s], f32x4{0.f, 0.f, 0.f, 0.f});
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) sacc[tb][j] = (sum[0][j] + sum[1][j]) + (sum[2][j] + sum[3][j]);
+        } else {
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const vec8 ka = key_operand<T>(sk + (tb >> 1) * Tl::kBytes, g4, n16, tb & 1, s);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) sacc[tb][j] = mma_16x16x32(ka, qop[j][s], sacc[tb][j]);
+          }
+        }
+      }
+      // The softmax runs at raised wave priority: the other waves of the SIMD
+      // fill the matrix pipe meanwhile.
+      __builtin_amdgcn_s_setprio(1);
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (t0 + 16 * tb + 4 * g4 + r >= lim[j]) sacc[tb][j][r] = -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float ps;
+        auto probs = [&](float nm) {
+          ps = 0.f;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float pv[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              pv[e] = fast_exp2(fmaf(sacc[2 * c + (e >> 2)][j][e & 3], a.scale_log2, nm));
+              ps += pv[e];
+            }
+            pb[c][j] = pack8<T>(pv);  // at most half a step of the input type per probability
+          }
+        };
+        probs(-m[j]);
+        // The reference point moves, and O with it, only when a lane's sum says
+        // so (see hc_rows.h).
+        if (__any(!(ps <= Weights<T>::kLazy))) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sacc[tb][j][r]);
+          const float mnew = next_reference<T>(m[j], rows4_max(mx) * a.scale_log2);
+          const float alpha = m[j] == -INFINITY ? 0.f : fast_exp2(m[j] - mnew);
+          m[j] = mnew;
+          l[j] *= alpha;
+#pragma unroll
+          for (int db = 0; db < 8; ++db) o[db][j] *= alpha;
+          probs(mnew == -INFINITY ? 0.f : -mnew);
+          if (mnew == -INFINITY && t0 < lim[j]) ps += 1.f;
+        }
+        l[j] += ps;
+      }
+      __builtin_amdgcn_s_setprio(0);
+    }
+    wait_lds_dma();  // the values, and the next keys, which were requested before the scores
+    __syncthreads();
+    if (work) {
+      if (edge) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int db = 0; db < 8; ++db) {
+            vec8 va = value_operand<T>(sv + c * Tl::kBytes, g4, n16, db);
+            edge_values<T>(va, pb[c], t0 + c * HC_TILE, w_hi, g4, o[db]);
+          }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int db = 0; db < 8; ++db) {
+            const vec8 va = value_operand<T>(sv + c * Tl::kBytes, g4, n16, db);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) o[db][j] = mma_16x16x32(va, pb[c][j], o[db][j]);
+          }
+      }
+    }
+    __syncthreads();  // the values are no longer read
+    if (more) {
+      st.copy(t0 + kKeys, e1, vp, p.v_page, p.v_tok, sv, bad);
+      if (it + 2 < it1) st.entries(t0 + 2 * kKeys, e1);
+    }
+  }
+
+  // A page outside of the pool: NaN for all columns, and the status word.
+  const bool any_bad = __syncthreads_or(bad);
+  if (any_bad && tid == 0 && p.status) atomicOr(p.status, kStatusPage);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    float lt = rows4_sum(l[j]);
+    const int c = c_wave + 16 * j + n16;
+    if (c >= a.cols) continue;
+    if (c < ncols && (any_bad || !room)) m[j] = -INFINITY, lt = NAN;
+    if (c >= ncols) m[j] = -INFINITY, lt = 0.f;
+    const int64_t col = (int64_t)row * a.cols + c;
+    if constexpr (SPLIT) {
+      float* pp = a.part_o + (col * a.parts + part) * HC_HEAD_DIM + 4 * g4;
+#pragma unroll
+      for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4*>(pp + 16 * db) = o[db][j];
+      if (g4 == 0) *reinterpret_cast<float2*>(a.part_ml + (col * a.parts + part) * 2) = make_float2(m[j], lt);
+    } else {
+      if (a.ml && g4 == 0) *reinterpret_cast<float2*>(a.ml + col * 2) = make_float2(m[j], lt);
+      typedef T quad __attribute__((ext_vector_type(4)));
+      T* op = reinterpret_cast<T*>(a.out) + b * a.o_s[0] + (int64_t)(h * a.G + c % a.G) * a.o_s[1] + (c / a.G) * a.o_s[2] + 4 * g4;
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        quad r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = Elem<T>::from_f32(state_output(o[db][j][e], m[j], lt));
+        *reinterpret_cast<quad*>(op + 16 * db) = r;
+      }
+    }
+  }
+}
+
+// A column's partials folded: 32 threads a column, 4 channels each.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_chunk_fold_kernel(const PagedAttn a) {
+  const Pool& p = a.pool;
+  const int64_t col = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (col >= (int64_t)p.rows * a.cols) return;
+  const int d0 = 4 * (threadIdx.x & 31);
+  const int row = (int)(col / a.cols), c = (int)(col % a.cols);
+  const int b = row / p.Hkv, h = row % p.Hkv;
+  float M = -INFINITY, L = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  if (c < query_tokens(p.counts, b, p.Q) * a.G) {
+    const float* po = a.part_o + col * a.parts * HC_HEAD_DIM + d0;
+    const float* ml = a.part_ml + col * a.parts * 2;
+    for (int s0 = 0; s0 < a.parts; s0 += 4) {
+      f32x4 o4[4];
+      float2 m4[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int s = min(s0 + u, a.parts - 1);
+        o4[u] = *reinterpret_cast<const f32x4*>(po + s * HC_HEAD_DIM);
+        m4[u] = *reinterpret_cast<const float2*>(ml + 2 * s);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (s0 + u >= a.parts) continue;
+        const float mn = fmaxf(M, m4[u].x), f = state_weight(M, mn), e = state_weight(m4[u].x, mn);
+        L = L * f + m4[u].y * e;
+        acc = acc * f + o4[u] * e;
+        M = mn;
+      }
+    }
+  }
+  if (a.ml && d0 == 0) *reinterpret_cast<float2*>(a.ml + col * 2) = make_float2(M, L);
+  typedef T quad __attribute__((ext_vector_type(4)));
+  T* op = reinterpret_cast<T*>(a.out) + b * a.o_s[0] + (int64_t)(h * a.G + c % a.G) * a.o_s[1] + (c / a.G) * a.o_s[2] + d0;
+  quad r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = Elem<T>::from_f32(state_output(acc[e], M, L));
+  *reinterpret_cast<quad*>(op) = r;
+}
+
+// Every token's share of the chunk's attention,
+//
+//   weights_out[t] = weights[t] + sum_c exp2(s_ct - M_c) / L_c,
+//
+// from the columns' folded (M, L): the scores are formed again, tokens as the
+// columns of the matrix product (their operands stay in registers), queries
+// streamed through LDS 64 at a time, so a token's sum stays in its lane.
+template <typename T>
+constexpr int weigh_lds() {
+  return 2 * (64 * Tile<T>::kRow + 64 * 8);
+}
+
+template <typename T, int NC>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : NC == 4 ? 3 : 4) void paged_weigh_kernel(const PagedAttn a) {
+  typedef typename Elem<T>::vec8 vec8;
+  typedef Tile<T> Tl;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const Pool& p = a.pool;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g4 = lane >> 4, n16 = lane & 15;
+  const int row = blockIdx.x % p.rows, tb = blockIdx.x / p.rows;
+  const int b = row / p.Hkv, h = row % p.Hkv;
+  const int hd = p.heads == 1 ? 0 : h;
+  const RowSpan span = row_span(p, row);
+  const int info = a.info ? a.info[table_row(p, row)].y : span.total;
+  const bool room = info >= 0;
+  const int total = room ? info : -1 - info, ncols = room ? span.n * a.G : 0, base = total - span.n;
+  const int old = p.fresh && room ? base : total;
+  const int t_block = tb * kWaves * 16 * NC;
+  if (t_block >= total) return;
+  const int t_wave = t_block + wave * 16 * NC;
+  const int32_t* const tab = p.table + table_row(p, row) * p.table_stride;
+
+  // Key operands: token t_wave + 16 c + n16 (those behind the last repeat it and
+  // are not stored), channels 32 s + 8 g4 + [0, 8).
+  vec8 kop[NC][4];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int t = min(t_wave + 16 * c + n16, total - 1);
+    const int pi = page_of(p, t);
+    int pg = tab[pi];
+    if ((uint32_t)pg >= (uint32_t)p.pages) pg = 0;  // (the columns' sums are NaN)
+    const T* kp = reinterpret_cast<const T*>(p.k + hd * p.k_head + pg * p.k_page + (t - pi * p.page_tokens) * p.k_tok) + 8 * g4;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) kop[c][s] = load8<T>(kp + 32 * s);
+  }
+
+  // Columns of the chunk, 64 an iteration, from the first that sees a token of
+  // the workgroup on: unit u = r * 256 + tid is chunk u % kChunks of column u /
+  // kChunks.  Columns behind the last repeat it, with 1 / L = 0.
+  constexpr int kSet = 64 * Tl::kRow + 64 * 8;
+  constexpr int kPer = kThreads / Tl::kChunks, kLoads = 64 / kPer;
+  const int c0 = max(t_block - base, 0) * a.G / 64 * 64;
+  auto stage = [&](int set, int col) {
+    char* s = lds + set * kSet;
+#pragma unroll
+    for (int r = 0; r < kLoads; ++r) {
+      const int u = r * kPer + tid / Tl::kChunks, c = min(col + u, ncols - 1);
+      const int i = c / a.G, gi = c % a.G;
+      const char* src = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.q) + b * a.q_s[0] +
+                                                      (int64_t)(h * a.G + gi) * a.q_s[1] + i * a.q_s[2]);
+      lds_dma16(src + 16 * ((tid % Tl::kChunks) ^ Tl::swizzle(u)), s + r * kThreads * 16 + wave * 1024);
+    }
+    if (tid < 64) {
+      const int c = min(col + tid, ncols - 1);
+      const float2 ml = *reinterpret_cast<const float2*>(a.ml + ((int64_t)row * a.cols + c) * 2);
+      // No number among the scores: NaN for each token; no token: nothing.
+      const float inv = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : NAN) : 1.f / ml.y;
+      *reinterpret_cast<float2*>(s + 64 * Tl::kRow + 8 * tid) =
+          make_float2(ml.x == -INFINITY ? 0.f : ml.x, col + tid < ncols ? inv : 0.f);
+    }
+  };
+  float sum[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) sum[c] = 0.f;
+  if (c0 < ncols) stage(0, c0);
+  for (int col = c0, it = 0; col < ncols; col += 64, ++it) {
+    wait_lds_dma();
+    __syncthreads();
+    if (col + 64 < ncols) stage((it + 1) & 1, col + 64);
+    const char* s = lds + (it & 1) * kSet;
+    const float2* const ml = reinterpret_cast<const float2*>(s + 64 * Tl::kRow);
+    // Some of these columns may not see some of the wave's tokens.
+    const bool edge = t_wave + 16 * NC > base + col / a.G + 1 || col + 64 > ncols;
+    float part[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) part[c] = 0.f;
+#pragma unroll
+    for (int qb = 0; qb < 4; ++qb) {
+      f32x4 acc[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const vec8 qa = key_operand<T>(s + (qb >> 1) * Tl::kBytes, g4, n16, qb & 1, x);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) acc[c] = mma_16x16x32(qa, kop[c][x], acc[c]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int u = 16 * qb + 4 * g4 + r;
+        const float2 y = ml[u];
+        if (edge) {
+          const bool live = col + u < ncols;
+          const int lim = live ? base + (col + u) / a.G + 1 : 0;
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            if (t_wave + 16 * c + n16 < lim) part[c] = fmaf(fast_exp2(fmaf(acc[c][r], a.scale_log2, -y.x)), y.y, part[c]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) part[c] = fmaf(fast_exp2(fmaf(acc[c][r], a.scale_log2, -y.x)), y.y, part[c]);
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) sum[c] += part[c];
+  }
+  const float* const in = a.weights + row * a.weight_stride;
+  float* const outw = a.weights_out + row * a.weight_stride;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const float w = rows4_sum(sum[c]);
+    const int t = t_wave + 16 * c + n16;
+    if (g4 == 0 && t < total) outw[t] = t < old ? in[t] + w : w;
+  }
+}
+
+template <typename T, bool UNIFORM, bool SPLIT>
+int launch_attn(const PagedAttn& a, hipStream_t s) {
+  static std::once_flag once;
+  static hipError_t attr = hipSuccess;
+  std::call_once(once, [] {
+    attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_chunk_kernel<T, UNIFORM, SPLIT>),
+                               hipFuncAttributeMaxDynamicSharedMemorySize, chunk_lds<T>());
+  });
+  if (attr != hipSuccess) return set_error(HC_ERR_HIP, "hc_paged_attn: %s", hipGetErrorString(attr));
+  hipLaunchKernelGGL((paged_chunk_kernel<T, UNIFORM, SPLIT>), dim3((unsigned)((int64_t)a.pool.rows * a.blocks * a.parts)),
+                     dim3(kThreads), chunk_lds<T>(), s, a);
+  return check_launch("hc_paged_attn(chunk)");
+}
+
+template <typename T, int NC>
+int launch_weigh(const PagedAttn& a, hipStream_t s) {
+  static std::once_flag once;
+  static hipError_t attr = hipSuccess;
+  std::call_once(once, [] {
+    attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_weigh_kernel<T, NC>),
+                               hipFuncAttributeMaxDynamicSharedMemorySize, weigh_lds<T>());
+  });
+  if (attr != hipSuccess) return set_error(HC_ERR_HIP, "hc_paged_attn: %s", hipGetErrorString(attr));
+  const int block = kWaves * 16 * NC;
+  const int64_t grid = (int64_t)a.pool.rows * ((a.pool.capacity + block - 1) / block);
+  hipLaunchKernelGGL((paged_weigh_kernel<T, NC>), dim3((unsigned)grid), dim3(kThreads), weigh_lds<T>(), s, a);
+  return check_launch("hc_paged_attn(weights)");
+}
+
+template <typename T>
+int launch(const PagedAttn& a, hipStream_t s) {
+  const bool uniform = a.pool.page_tokens % 16 == 0;
+  int rc;
+  if (a.parts > 1) {
+    rc = uniform ? launch_attn<T, true, true>(a, s) : launch_attn<T, false, true>(a, s);
+    if (rc) return rc;
+    const int64_t cols = (int64_t)a.pool.rows * a.cols;
+    hipLaunchKernelGGL((paged_chunk_fold_kernel<T>), dim3((unsigned)((cols + 7) / 8)), dim3(256), 0, s, a);
+    rc = check_launch("hc_paged_attn(fold)");
+  } else {
+    rc = uniform ? launch_attn<T, true, false>(a, s) : launch_attn<T, false, false>(a, s);
+  }
+  if (rc || !a.weights_out) return rc;
+  // 64 tokens a wave halve the reads of the queries against 16, once there are workgroups enough.
+  const int64_t wide = (int64_t)a.pool.rows * ((a.pool.capacity + 255) / 256);
+  if (sizeof(T) == 2 && wide >= 512) return launch_weigh<T, 4>(a, s);
+  return launch_weigh<T, 1>(a, s);
+}
+
+// The call's new tokens into their pages, ahead of the chunk's attention:
+// workgroups of 16 tokens of a row.  16 bytes a thread and token, K and V.
+__global__ __launch_bounds__(256) void paged_append_kernel(const PagedAttn a, int chunks, int blocks) {
+  const Pool& p = a.pool;
+  const int row = blockIdx.x / blocks, blk = blockIdx.x % blocks;
+  const int b = row / p.Hkv, h = row % p.Hkv;
+  const int trow = table_row(p, row), hd = p.heads == 1 ? 0 : h;
+  const RowSpan s = row_span(p, row);
+  const bool first = p.heads == 1 || h == 0;
+  if (blk == 0 && threadIdx.x == 0 && first) {
+    if (a.info) a.info[trow] = make_int2(0, s.room ? s.total : -1 - s.len);
+    if (a.len_out) a.len_out[trow] = s.total;
+    if (!s.room && p.status) atomicOr(p.status, kStatusCapacity);
+  }
+  if (!s.room) return;
+  const int32_t* const tab = p.table + trow * p.table_stride;
+  const int i0 = blk * 16, n = min(s.n - i0, 16);
+  for (int u = threadIdx.x; u < n * chunks; u += 256) {
+    const int i = i0 + u / chunks, off = 16 * (u % chunks), t = s.len + i;
+    const int pi = page_of(p, t), pg = tab[pi], at = t - pi * p.page_tokens;
+    if ((uint32_t)pg >= (uint32_t)p.pages) {
+      if (p.status) atomicOr(p.status, kStatusPage);
+      continue;
+    }
+    const u32x4 k = *reinterpret_cast<const u32x4*>(a.fresh.k + b * a.fresh.k_s[0] + h * a.fresh.k_s[1] + i * a.fresh.k_s[2] + off);
+    const u32x4 v = *reinterpret_cast<const u32x4*>(a.fresh.v + b * a.fresh.v_s[0] + h * a.fresh.v_s[1] + i * a.fresh.v_s[2] + off);
+    *reinterpret_cast<u32x4*>(const_cast<char*>(p.k) + pg * p.k_page + hd * p.k_head + at * p.k_tok + off) = k;
+    *reinterpret_cast<u32x4*>(const_cast<char*>(p.v) + pg * p.v_page + hd * p.v_head + at * p.v_tok + off) = v;
+  }
+  if ((int)threadIdx.x < n) {
+    const int t = s.len + i0 + threadIdx.x;
+    if (a.pos && first) a.pos[trow * a.pos_stride + t] = t + a.dropped[trow];
+    if (a.zeroed) a.zeroed[row * a.weight_stride + t] = 0.f;
+  }
+}
+
+// Lengths advanced in place, once an append without attention has read them.
+__global__ __launch_bounds__(256) void paged_advance_kernel(const PagedAttn a, int table_rows) {
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r >= table_rows) return;
+  const RowSpan s = row_span(a.pool, a.pool.heads == 1 ? r : r * a.pool.Hkv);
+  a.len_out[r] = s.total;
+}
+
+}  // namespace
+
+int launch_paged_chunk(int dtype, const PagedAttn& a, hipStream_t s) {
+  switch (dtype) {
+    case HC_DTYPE_BF16: return launch<__bf16>(a, s);
+    case HC_DTYPE_F16: return launch<_Float16>(a, s);
+    default: return launch<float>(a, s);
+  }
+}
+
+int launch_paged_append(int dtype, const PagedAttn& a, hipStream_t s) {
+  const int chunks = dtype == HC_DTYPE_F32 ? 32 : 16, blocks = std::max(1, (a.pool.Q + 15) / 16);
+  PagedAttn first = a;
+  const bool in_place = a.len_out && a.len_out == a.pool.row_len;
+  if (in_place) first.len_out = nullptr;
+  hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)((int64_t)a.pool.rows * blocks)), dim3(256), 0, s, first, chunks, blocks);
+  int rc = check_launch("hc_paged_append");
+  if (rc || !in_place) return rc;
+  const int table_rows = a.pool.heads == 1 ? a.pool.rows : a.pool.rows / a.pool.Hkv;
+  hipLaunchKernelGGL(paged_advance_kernel, dim3((table_rows + 255) / 256), dim3(256), 0, s, a, table_rows);
+  return check_launch("hc_paged_append(lengths)");
+}
+
+}  // namespace hc

@@ -1185,3 +1185,187 @@ def block_step_store(q, store, index, keep, scale, sink=1, local=1, out=None, qu
     return _block_step(q, dt, dev, store.rows, (store.k, store.v, store.row_tile_off, store.row_len),
                        (index.bounds, index.exps, index.row_block_off), index.block, index.max_blocks, keep, scale, sink,
                        local, out, query_counts)
+
+
+class Pages:
+    """A paged cache on plain tensors, checked once: pools k and v [pages,
+    page_tokens, heads, 128] of any strides of whole 16 bytes with unit channel
+    stride, table int32 [rows, entries] and row_len int32 [rows], reached as
+    hc_paged_cache in include/hc.h says.  heads is 1 with rows = batch *
+    kv_heads (a table a head, as the reference's pools), or kv_heads with rows =
+    batch (a table a sequence).
+
+    weights (float32 [batch * kv_heads, at least entries * page_tokens]), pos
+    (int32 [rows, the same]) and dropped (int32 [rows]): what paged_attn(weigh=
+    True) accumulates and paged_evict goes by; all or none.  status: int32
+    device word (read_status)."""
+
+    def __init__(self, k, v, table, row_len, kv_heads, weights=None, pos=None, dropped=None, status=None):
+        dev = k.get_device()
+        if dev < 0:
+            raise ValueError("libhc ops need tensors on a ROCm device")
+        dt = k.dtype
+        code = dtype_code(dt)
+        if k.dim() != 4 or k.shape[3] != HEAD_DIM or v.shape != k.shape or k.numel() == 0 or k.stride(3) != 1 or v.stride(3) != 1:
+            raise ValueError(f"the pools must be two [pages, page tokens, heads, {HEAD_DIM}] with unit channel stride, got "
+                             f"{tuple(k.shape)} and {tuple(v.shape)}")
+        if v.dtype is not dt or v.get_device() != dev:
+            raise TypeError(f"the pools must share a dtype and a device: {dt} on {k.device}, {v.dtype} on {v.device}")
+        for name, t in (("k", k), ("v", v)):
+            if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+                raise ValueError(f"{name} is an expanded tensor, whose entries share memory")
+        pages, size, heads, _ = k.shape
+        kv_heads = int(kv_heads)
+        if kv_heads < 1 or heads not in (1, kv_heads):
+            raise ValueError(f"pools of {heads} heads for {kv_heads} KV heads: 1 or as many")
+        if (table.dim() != 2 or table.dtype is not torch.int32 or table.get_device() != dev or table.shape[1] == 0
+                or (table.stride(1) != 1 and table.shape[1] > 1) or table.shape[0] * heads % kv_heads
+                or (table.stride(0) < table.shape[1] and table.shape[0] > 1)):
+            raise ValueError(f"table must be int32 [rows, entries] with unit column stride on {k.device}, rows a multiple of "
+                             f"{kv_heads // heads}, got {tuple(table.shape)} of {table.dtype} on {table.device}")
+        rows, entries = table.shape
+        _meta(dev, "row_len", row_len, torch.int32, rows)
+        if status is not None:
+            _meta(dev, "status", status, torch.int32, 1)
+        self.k, self.v, self.table, self.row_len, self.status = k, v, table, row_len, status
+        self.weights, self.pos, self.dropped = weights, pos, dropped
+        self.dtype, self.device, self.dev, self.heads, self.kv_heads = dt, k.device, dev, heads, kv_heads
+        self.rows, self.batch = rows, rows * heads // kv_heads
+        self.page_tokens, self.capacity = size, entries * size
+        given = [x is not None for x in (weights, pos, dropped)]
+        if any(given) and not all(given):
+            raise ValueError("weights, pos and dropped come together")
+        wide = lambda n: 0 if n is None else n.stride(0) if n.shape[0] > 1 else n.shape[1]
+        if weights is not None:
+            self._ledger("weights", weights, torch.float32, self.batch * kv_heads)
+            self._ledger("pos", pos, torch.int32, rows)
+            _meta(dev, "dropped", dropped, torch.int32, rows)
+        strides = lambda t: (ctypes.c_int64 * 3)(*[s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride())])
+        self.struct = _lib.PagedCache(
+            dtype=code, batch=self.batch, kv_heads=kv_heads, heads=heads, pages=pages, page_tokens=size, table_pages=entries,
+            k=k.data_ptr(), v=v.data_ptr(), k_strides=strides(k), v_strides=strides(v), table=table.data_ptr(),
+            table_stride=table.stride(0) if rows > 1 else entries, row_len=row_len.data_ptr(), weights=_ptr(weights),
+            weight_stride=wide(weights), pos=_ptr(pos), pos_stride=wide(pos), dropped=_ptr(dropped), status=_ptr(status))
+        self.ref = ctypes.addressof(self.struct)
+        self._sizes = {}
+
+    def _ledger(self, name, t, dtype, rows, like=None):
+        if (t.dim() != 2 or t.dtype is not dtype or t.get_device() != self.dev or t.shape[0] != rows
+                or t.shape[1] < self.capacity or (t.stride(1) != 1 and t.shape[1] > 1)
+                or (rows > 1 and t.stride(0) < self.capacity) or (like is not None and rows > 1 and t.stride(0) != like.stride(0))):
+            raise ValueError(f"{name} must be {dtype} [{rows}, {self.capacity} or more] with unit column stride on {self.device}"
+                             f"{'' if like is None else ' and the row stride of the old'}, got {tuple(t.shape)} of {t.dtype} on "
+                             f"{t.device}")
+
+    def _workspace(self, fn, *sizes):
+        """Scratch of a call; the bytes depend on its sizes and the device alone."""
+        n = self._sizes.get((fn, sizes))
+        if n is None:
+            with torch.cuda.device(self.dev):
+                n = self._sizes[fn, sizes] = getattr(_lib.load(), fn)(self.ref, *sizes)
+        return torch.empty(n, dtype=torch.uint8, device=self.device), n
+
+
+def _new_tokens(pages, k, v, what):
+    ksh = k.shape
+    if len(ksh) != 4 or ksh[3] != HEAD_DIM or (k.numel() and (k.stride(3) != 1 or v.stride(3) != 1)):
+        raise ValueError(f"{what} must be [B, H, T, {HEAD_DIM}] with unit channel stride, got {tuple(ksh)}")
+    if v.shape != ksh or ksh[0] != pages.batch or ksh[1] != pages.kv_heads:
+        raise ValueError(f"{what} {tuple(ksh)} and {tuple(v.shape)} for {pages.batch} sequences of {pages.kv_heads} KV heads")
+    if k.dtype is not pages.dtype or v.dtype is not pages.dtype:
+        raise TypeError(f"the pools are {pages.dtype}, {what} {k.dtype} and {v.dtype}: they must share a dtype")
+    if k.get_device() != pages.dev or v.get_device() != pages.dev:
+        raise ValueError(f"{what} on {k.device} and {v.device} for pools on {pages.device}")
+
+
+@_on_device
+def paged_append(k, v, pages, counts=None, len_out=None):
+    """New keys and values [B, Hkv, T, 128] at the ends of their rows
+    (hc_paged_append in include/hc.h).  counts: int32 device tensor [B] or host
+    integers of the tokens that each sequence appends (None: T); len_out: the
+    new lengths, int32 [rows] (default: in place)."""
+    _new_tokens(pages, k, v, "new keys and values")
+    dev, T = pages.dev, k.shape[2]
+    counts = _query_counts(counts, pages.batch, dev)
+    if len_out is not None:
+        _meta(dev, "len_out", len_out, torch.int32, pages.rows)
+    _lib.check(_lib.load().hc_paged_append(pages.ref, k.data_ptr(), _strides3((k.shape, k.stride())), v.data_ptr(),
+                                           _strides3((v.shape, v.stride())), _ptr(counts), T, _ptr(len_out),
+                                           torch._C._cuda_getCurrentRawStream(dev)))
+
+
+@_on_device
+def paged_attn(q, pages, scale, k_new=None, v_new=None, counts=None, weigh=False, out=None, len_out=None, weights_out=None):
+    """Attention of queries [B, Hq, T, 128], the last counts[b] (None: T) tokens
+    of their sequences, over a paged cache; [B, T, Hq, 128], zeros behind a
+    sequence's count (hc_paged_attn in include/hc.h).
+
+    k_new, v_new [B, Hkv, T, 128]: the tokens' keys and values, appended by this
+    call (None: the pages hold them).  counts: int32 device tensor [B] or host
+    integers.  weigh: every token's share of the attention is added to the
+    cache's weights.  out: not q's memory; len_out, weights_out: receive the new
+    lengths and weights (default: in place)."""
+    dt, dev = q.dtype, q.get_device()
+    shape = _queries(q)
+    B, Hq, T, _ = shape
+    if dt is not pages.dtype:
+        raise TypeError(f"q is {dt}, the pools {pages.dtype}: they must share a dtype")
+    if dev != pages.dev:
+        raise ValueError(f"q on {q.device} for pools on {pages.device}")
+    if B != pages.batch or Hq == 0 or Hq % pages.kv_heads:
+        raise ValueError(f"queries {tuple(shape)} for {pages.batch} sequences of {pages.kv_heads} KV heads")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("new keys and values come together")
+    kp = ks = vp = vs = None
+    if k_new is not None:
+        _new_tokens(pages, k_new, v_new, "new keys and values")
+        if k_new.shape[2] != T:
+            raise ValueError(f"{k_new.shape[2]} new tokens for {T} queries")
+        kp, ks, vp, vs = (k_new.data_ptr(), _strides3((k_new.shape, k_new.stride())), v_new.data_ptr(),
+                          _strides3((v_new.shape, v_new.stride())))
+    counts = _query_counts(counts, B, dev)
+    if len_out is not None:
+        _meta(dev, "len_out", len_out, torch.int32, pages.rows)
+    if weights_out is not None:
+        if not weigh or pages.weights is None:
+            raise ValueError("weights_out without weigh, or for a cache without weights")
+        pages._ledger("weights_out", weights_out, torch.float32, B * pages.kv_heads, like=pages.weights)
+    out, o_st = _out_bthd(q, out, shape, dev)
+    ws, nbytes = pages._workspace("hc_paged_workspace_size", Hq, T, k_new is not None, bool(weigh))
+    _lib.check(_lib.load().hc_paged_attn(pages.ref, q.data_ptr(), _strides3((shape, q.stride())), Hq, T, kp, ks, vp, vs,
+                                         _ptr(counts), scale, bool(weigh), _ptr(weights_out), _ptr(len_out), out.data_ptr(),
+                                         o_st, ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(dev)))
+    return out
+
+
+def paged_evict(pages, keep, sink=0, recent=0, len_out=None, weights_out=None, pos_out=None, dropped_out=None, stream=None):
+    """Every row of more than `keep` tokens (an integer, or int32 [rows] on the
+    device) down to its `keep` heaviest, the positions below `sink` and the last
+    `recent` before any other (hc_paged_evict in include/hc.h).  The outputs
+    receive new lengths, weights, positions and dropped counts (default: in
+    place); keys and values move in place."""
+    _paged_evict(pages.row_len, pages, keep, sink, recent, len_out, weights_out, pos_out, dropped_out, stream=stream)
+
+
+@_on_device
+def _paged_evict(row_len, pages, keep, sink, recent, len_out, weights_out, pos_out, dropped_out):
+    dev, rows = pages.dev, pages.rows
+    if pages.weights is None:
+        raise ValueError("the cache has no weights, positions and dropped counts")
+    at, every = None, 0
+    if torch.is_tensor(keep):
+        _meta(dev, "keep", keep, torch.int32, rows)
+        at = keep.data_ptr()
+    else:
+        every = int(keep)
+    if len_out is not None:
+        _meta(dev, "len_out", len_out, torch.int32, rows)
+    if dropped_out is not None:
+        _meta(dev, "dropped_out", dropped_out, torch.int32, rows)
+    if weights_out is not None:
+        pages._ledger("weights_out", weights_out, torch.float32, pages.batch * pages.kv_heads, like=pages.weights)
+    if pos_out is not None:
+        pages._ledger("pos_out", pos_out, torch.int32, rows, like=pages.pos)
+    ws, nbytes = pages._workspace("hc_paged_evict_scratch_size")
+    _lib.check(_lib.load().hc_paged_evict(pages.ref, at, every, sink, recent, _ptr(len_out), _ptr(weights_out), _ptr(pos_out),
+                                          _ptr(dropped_out), ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(dev)))

@@ -674,6 +674,94 @@ int hc_block_step(int dtype, const void* q, const int64_t* q_strides, const void
 size_t hc_block_step_workspace_size(int batch, int q_heads, int kv_heads, int queries, int block, int max_blocks,
                                     int keep);
 
+/*
+ * A paged cache: pools K and V of pages [pages][page_tokens][heads][128], any
+ * strides of whole 16 bytes (k_strides, v_strides: page, token, head, in
+ * elements; channels contiguous), holding the tokens of table rows.  Token t of
+ * table row r lies in page table[r * table_stride + t / page_tokens], at place
+ * t % page_tokens.  heads = 1: a table row is one (sequence, KV head) row b *
+ * kv_heads + h, as in the reference's pools ([blocks, 256, 1, 128] with block
+ * tables and lengths a row, heterocache/cache_utils.py:693-766); heads =
+ * kv_heads: a table row is a sequence, whose pages hold every head.  Lengths,
+ * tables and counts are read on the device, so captured calls replay while the
+ * rows grow.  A row may share pages with others as long as nothing is written
+ * to them.  An entry outside of the pools is never followed: attention over
+ * it is NaN, an append or move through it is left out, and status (an int32
+ * word or NULL) gets bit 1.  A row without room for its new tokens keeps its
+ * old ones and its length, attends NaN, and sets bit 0.
+ * weights, pos and dropped (all or none): what the attention of past queries
+ * gave each token ([batch * kv_heads][weight_stride], float32), its position
+ * ([table rows][pos_stride]), and how many tokens a table row has given up.
+ */
+typedef struct hc_paged_cache {
+  int32_t dtype, batch, kv_heads, heads;
+  int32_t pages, page_tokens, table_pages, reserved;
+  void *k, *v;
+  int64_t k_strides[3], v_strides[3];
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t* row_len;
+  float* weights;
+  int64_t weight_stride;
+  int32_t* pos;
+  int64_t pos_stride;
+  int32_t* dropped;
+  int32_t* status;
+} hc_paged_cache;
+
+/*
+ * New keys and values [batch][kv_heads][tokens][128] (element strides: batch,
+ * head, token) at the ends of their rows, counts[b] of them (clamped to
+ * [0, tokens]; NULL: all).  With weights: the new tokens' start at zero, their
+ * positions at row_len + dropped + i.  len_out: the new lengths (NULL: row_len
+ * itself).
+ */
+int hc_paged_append(const hc_paged_cache* c, const void* k, const int64_t* k_strides, const void* v,
+                    const int64_t* v_strides, const int32_t* counts, int tokens, int32_t* len_out, void* stream);
+
+/*
+ * Attention of the last n = counts[b] tokens of each sequence over its rows:
+ * query i < n sees tokens t < len - n + 1 + i, out[b, h, i] = softmax(scale *
+ * q . k_t) v_t; the others are padding and give zeros.  With k_new and v_new
+ * the call appends them first (len then counts them; see hc_paged_append),
+ * otherwise they are stored already.  Zeros where nothing is visible; NaN where
+ * a visible score is NaN or all are -inf.
+ * weigh: weights_out[r][t] = weights[r][t] + the sum over the row's queries and
+ * query heads of their probabilities of token t, for every token of the row; a
+ * token appended by this call starts at zero.  weights_out NULL: in place.
+ * q, out: element strides batch, head, token, all of whole 16 bytes; out shares
+ * no memory with q.  Stands where the reference calls flash attention over its
+ * pools (heterocache/llama_model.py:382-389), for one new token or many.
+ * workspace: hc_paged_workspace_size bytes, 16-byte aligned, no initialisation;
+ * calls that overlap in time need their own.  Up to 16 (query, head) pairs a row
+ * with weigh it holds their scores, 4 bytes a pair and token of a table row's capacity.
+ */
+int hc_paged_attn(const hc_paged_cache* c, const void* q, const int64_t* q_strides, int q_heads, int queries,
+                  const void* k_new, const int64_t* k_strides, const void* v_new, const int64_t* v_strides,
+                  const int32_t* counts, float scale, int weigh, float* weights_out, int32_t* len_out, void* out,
+                  const int64_t* out_strides, void* workspace, size_t workspace_bytes, void* stream);
+size_t hc_paged_workspace_size(const hc_paged_cache* c, int q_heads, int queries, int fresh, int weigh);
+
+/*
+ * Eviction by accumulated weight: of a table row's n tokens the first `keep`
+ * (keep[r], or keep_all where keep is NULL) stay, in this order: the protected
+ * ones, then by weight, the greatest first, and of equals the lower slot first.
+ * Protected, and alike: positions below `sink`, and the last `recent` (at or
+ * above n + dropped - recent).  NaN ranks below every number.  Where a table row serves all KV heads a token's weight is the
+ * sum of theirs, formed in 64 bits and rounded to float32, and all heads give it
+ * up.  A kept token in a slot below `keep` stays there; the others fill the
+ * freed slots, both in ascending order, with their keys, values, weights and
+ * positions.  The row's length becomes min(n, keep), its dropped count grows by
+ * the rest.  A row whose pages others share must not be evicted from.
+ * len_out, weights_out, pos_out, dropped_out: NULL for in place; else the new
+ * values, the old staying as they are (keys and values move in place).  scratch:
+ * hc_paged_evict_scratch_size bytes, 16-byte aligned, no initialisation.
+ */
+int hc_paged_evict(const hc_paged_cache* c, const int32_t* keep, int keep_all, int sink, int recent, int32_t* len_out,
+                   float* weights_out, int32_t* pos_out, int32_t* dropped_out, void* scratch, size_t scratch_bytes,
+                   void* stream);
+size_t hc_paged_evict_scratch_size(const hc_paged_cache* c);
+
 #ifdef __cplusplus
 }
 #endif
