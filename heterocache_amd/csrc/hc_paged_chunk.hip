@@ -35,48 +35,121 @@ constexpr int chunk_lds() {
   return 3 * kTiles * Tile<T>::kBytes;
 }
 
-// Copies of 64 tokens of keys or values by a workgroup: load r of a thread is
-// chunk tid % kChunks of token r * kPer + tid / kChunks.
+// LDS holds 64 tokens of keys or values in blocks of 1 KB, 16 tokens x 64 bytes
+// of channels each, block (group of 16, segment) at (group * kSegs + segment).
+// A copy of a wave fills one; which 16 bytes a lane fetches sets their order in
+// the block, chosen so that every operand is read at lane * (8 or 16) bytes
+// plus a constant, without conflicts:
+//   keys            [16-byte piece][token]
+//   values, 16 bit  [pair of pieces][token][piece of the pair]: the transposed
+//                   read of 16 channels takes 512 bytes in a row
+//   values, fp32    [token % 4][token / 4][piece]
+// (In fp32 key operands take channels 32 x + 16 half + 4 g + [0, 4), so that
+// their pieces also lie together.)
+constexpr int kBlock = 1024;
+template <typename T>
+constexpr int kSegs = Tile<T>::kRow / 64;
+
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::vec8 chunk_keys(const char* set, int lane, int group, int x) {
+  const char* p = set + 16 * lane;
+  if constexpr (sizeof(T) == 4) {
+    typename Elem<T>::vec8 r;
+    r.lo = *reinterpret_cast<const f32x4*>(p + (group * kSegs<T> + 2 * x) * kBlock);
+    r.hi = *reinterpret_cast<const f32x4*>(p + (group * kSegs<T> + 2 * x + 1) * kBlock);
+    return r;
+  } else {
+    return *reinterpret_cast<const typename Elem<T>::vec8*>(p + (group * kSegs<T> + x) * kBlock);
+  }
+}
+// Tokens 32 c + 16 (e / 4) + 4 g + e % 4 of channel 16 mt + n.
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::vec8 chunk_values(const char* set, int lane, int c, int mt) {
+  if constexpr (sizeof(T) == 4) {
+    typename Elem<T>::vec8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      set8<T>(r, e, *reinterpret_cast<const float*>(set + 4 * lane + ((2 * c + (e >> 2)) * kSegs<T> + mt) * kBlock + 256 * (e & 3)));
+    return r;
+  } else {
+    const char* p = set + 8 * lane + 2 * c * kSegs<T> * kBlock + 512 * mt;
+    const short4_t lo = lds_read_transposed(p), hi = lds_read_transposed(p + kSegs<T> * kBlock);
+    const short8_t both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(typename Elem<T>::vec8, both);
+  }
+}
+
+// Copies of 64 tokens by a workgroup: wave w takes segments w (and w + 4) of
+// every group.
 template <typename T, bool UNIFORM>
 struct Stage {
-  static constexpr int kPer = kThreads / Tile<T>::kChunks;  // tokens of one load of all threads: 16 or 8
-  static constexpr int kLoads = kKeys / kPer;
-  const Pool& p;
-  const int32_t* tab;
-  int total, tok, wave;
-  uint32_t chunk;
-  __device__ __forceinline__ Stage(const Pool& pool, int row, int total_tok) : p(pool), total(total_tok) {
-    tab = p.table + table_row(p, row) * p.table_stride;
-    tok = threadIdx.x / Tile<T>::kChunks;
-    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    chunk = 16 * ((threadIdx.x % Tile<T>::kChunks) ^ Tile<T>::swizzle(tok));
+  static constexpr int kGroups = kKeys / 16, kMine = kSegs<T> / kWaves;
+  typedef const __attribute__((address_space(4))) int32_t* Table;  // unchanged while the kernel runs: scalar loads
+  Table tab;
+  int total, wave, k_tok, v_tok;  // this lane's token of a group
+  uint32_t k_off, v_off;          // UNIFORM: its bytes behind the group's first token; else behind its own token
+  __device__ __forceinline__ Stage(const Pool& p, int row, int total_tok, int lane, int wv) : total(total_tok), wave(wv) {
+    tab = (Table)(uintptr_t)(p.table + table_row(p, row) * p.table_stride);
+    k_tok = lane & 15;
+    v_tok = sizeof(T) == 4 ? 4 * (lane >> 2 & 3) + (lane >> 4) : lane >> 1 & 15;
+    const int k_piece = lane >> 4, v_piece = sizeof(T) == 4 ? lane & 3 : 2 * (lane >> 5) + (lane & 1);
+    k_off = 64 * wave + 16 * k_piece + (UNIFORM ? (uint32_t)(k_tok * (int)p.k_tok) : 0u);
+    v_off = 64 * wave + 16 * v_piece + (UNIFORM ? (uint32_t)(v_tok * (int)p.v_tok) : 0u);
   }
-  // Pages of the tokens t0 + [0, 64): of each 16 of them, or of this thread's.
-  static constexpr int kEntries = UNIFORM ? kKeys / 16 : kLoads;
-  __device__ __forceinline__ int token(int t0, int r) const {
-    return UNIFORM ? min(t0 + 16 * r, (total - 1) & ~15) : min(t0 + r * kPer + tok, total - 1);
-  }
-  __device__ __forceinline__ void entries(int t0, int (&e)[kEntries]) const {
+  // UNIFORM: page and place of the 16-token groups of tokens t0 + [0, 64).
+  struct Places {
+    uint32_t page[kGroups], at[kGroups];
+  };
+  __device__ __forceinline__ void places(const Pool& p, int t0, Places& e, bool& bad) const {
+    if constexpr (UNIFORM) {
 #pragma unroll
-    for (int r = 0; r < kEntries; ++r) e[r] = tab[page_of(p, token(t0, r))];
-  }
-  __device__ __forceinline__ void copy(int t0, const int (&e)[kEntries], const char* pool, int64_t s_page, int64_t s_tok,
-                                       char* lds, bool& bad) const {
-#pragma unroll
-    for (int r = 0; r < kLoads; ++r) {
-      constexpr int kSame = UNIFORM ? 16 / kPer : 1;  // loads of one entry
-      int pg = e[r / kSame];
-      if ((uint32_t)pg >= (uint32_t)p.pages) bad = true, pg = 0;
-      const int t = token(t0, r / kSame);
-      const int at = t - page_of(p, t) * p.page_tokens;
-      const char* src = pool + pg * s_page + at * s_tok;
-      // (The swizzle is linear in the token's bits.)
-      src += chunk ^ (uint32_t)(16 * Tile<T>::swizzle(r * kPer & 15));
-      if constexpr (UNIFORM) src += (uint32_t)((r % kSame * kPer + tok) * (int)s_tok);
-      lds_dma16(src, lds + r * kThreads * 16 + wave * 1024);
+      for (int r = 0; r < kGroups; ++r) {
+        const uint32_t t = (uint32_t)min(t0 + 16 * r, (total - 1) & ~15);
+        const uint32_t pi = __umulhi(t, p.div_mul) >> (p.div_shift - 32);
+        uint32_t pg = (uint32_t)__builtin_amdgcn_readfirstlane(tab[pi]);
+        if (pg >= (uint32_t)p.pages) bad = true, pg = 0;
+        e.page[r] = pg, e.at[r] = t - pi * (uint32_t)p.page_tokens;
+      }
     }
   }
+  __device__ __forceinline__ void copy(const Pool& p, int t0, const Places& e, const char* pool, int64_t s_page,
+                                       int64_t s_tok, int tok, uint32_t off, char* lds, bool& bad) const {
+#pragma unroll
+    for (int r = 0; r < kGroups; ++r) {
+      const char* src;
+      if constexpr (UNIFORM) {  // (strides and a page's extent lie below 2^31)
+        src = pool + ((uint64_t)e.page[r] * (uint32_t)s_page + e.at[r] * (uint32_t)s_tok);
+      } else {
+        const int t = min(t0 + 16 * r + tok, total - 1);
+        const int pi = page_of(p, t);
+        int pg = tab[pi];
+        if ((uint32_t)pg >= (uint32_t)p.pages) bad = true, pg = 0;
+        src = pool + pg * s_page + (t - pi * p.page_tokens) * s_tok;
+      }
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) lds_dma16(src + (off + 256 * j), lds + (r * kSegs<T> + wave + kWaves * j) * kBlock);
+    }
+  }
+  __device__ __forceinline__ void keys(const Pool& p, int t0, const Places& e, int hd, char* lds, bool& bad) const {
+    copy(p, t0, e, p.k + hd * p.k_head, p.k_page, p.k_tok, k_tok, k_off, lds, bad);
+  }
+  __device__ __forceinline__ void values(const Pool& p, int t0, const Places& e, int hd, char* lds, bool& bad) const {
+    copy(p, t0, e, p.v + hd * p.v_head, p.v_page, p.v_tok, v_tok, v_off, lds, bad);
+  }
 };
+
+// A query operand, channels as chunk_keys takes them.
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::vec8 chunk_query(const T* q, int g, int x) {
+  if constexpr (sizeof(T) == 4) {
+    typename Elem<T>::vec8 r;
+    r.lo = *reinterpret_cast<const f32x4*>(q + 32 * x + 4 * g);
+    r.hi = *reinterpret_cast<const f32x4*>(q + 32 * x + 16 + 4 * g);
+    return r;
+  } else {
+    return load8<T>(q + 32 * x + 8 * g);
+  }
+}
 
 // The product of 16 channels of values with a tile's probabilities where some
 // column does not see some token: what lies behind `end`, which no column sees,
@@ -159,9 +232,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
     const bool ok = c < ncols;
     const int i = ok ? c / a.G : 0, gi = ok ? c % a.G : 0;
     lim[j] = ok ? min(max(base + i + 1, 0), total) : w_hi;  // (padding beside tokens sees what the last does)
-    const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_s[0] + (int64_t)(h * a.G + gi) * a.q_s[1] + i * a.q_s[2] + 8 * g4;
+    const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_s[0] + (int64_t)(h * a.G + gi) * a.q_s[1] + i * a.q_s[2];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) qop[j][s] = ok ? load8<T>(qp + 32 * s) : zero8<T>();
+    for (int s = 0; s < 4; ++s) qop[j][s] = ok ? chunk_query<T>(qp, g4, s) : zero8<T>();
   }
 
   f32x4 o[8][2];
@@ -173,27 +246,27 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
   bool bad = false;
 
   typedef Stage<T, UNIFORM> St;
-  const St st(p, row, max(total, 1));
-  const char* const kp = p.k + hd * p.k_head;
-  const char* const vp = p.v + hd * p.v_head;
+  const St st(p, row, max(total, 1), lane, wave);
   constexpr int kSet = kTiles * Tl::kBytes;
   char* const sv = lds + 2 * kSet;
-  int e0[St::kEntries], e1[St::kEntries];  // pages of this iteration's tokens, and of the next one's
+  typename St::Places pg;  // of the next iteration's tokens
   if (it0 < it1) {
-    st.entries(it0 * kKeys, e0);
-    st.copy(it0 * kKeys, e0, kp, p.k_page, p.k_tok, lds, bad);
-    st.copy(it0 * kKeys, e0, vp, p.v_page, p.v_tok, sv, bad);
-    if (it0 + 1 < it1) st.entries((it0 + 1) * kKeys, e1);
+    st.places(p, it0 * kKeys, pg, bad);
+    st.keys(p, it0 * kKeys, pg, hd, lds, bad);
+    st.values(p, it0 * kKeys, pg, hd, sv, bad);
+    if (it0 + 1 < it1) st.places(p, (it0 + 1) * kKeys, pg, bad);
   }
   wait_lds_dma();
   __syncthreads();
 
-  for (int it = it0; it < it1; ++it) {
+  // EDGE: some column may not see all of the tokens.
+  auto step = [&](auto edge_tag, int it) {
+    constexpr bool EDGE = decltype(edge_tag)::value;
     const int t0 = it * kKeys;
     const bool more = it + 1 < it1;
-    if (more) st.copy(t0 + kKeys, e1, kp, p.k_page, p.k_tok, lds + ((it - it0 + 1) & 1) * kSet, bad);
-    const bool work = active && t0 < w_hi;
-    const bool edge = t0 + kKeys > w_lo;  // some column does not see all of these tokens
+    if (more) st.keys(p, t0 + kKeys, pg, hd, lds + ((it - it0 + 1) & 1) * kSet, bad);
+    const bool work = active && (!EDGE || t0 < w_hi);
+    const bool edge = EDGE && t0 + kKeys > w_lo;
     vec8 pb[2][2];
     if (work) {
       __builtin_amdgcn_s_setprio(0);
@@ -209,19 +282,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
         if constexpr (sizeof(T) == 4) {
           // Sums of 32 channels apart: a rounding is half a step of the partial
           // sum that it falls on.
-          f32x4 sum[4][2];
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            const vec8 ka = key_operand<T>(sk + (tb >> 1) * Tl::kBytes, g4, n16, tb & 1, s);
+            const vec8 ka = chunk_keys<T>(sk, lane, tb, s);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) sum[s][j] = mma_16x16x32(ka, qop[j][s], f32x4{0.f, 0.f, 0.f, 0.f});
+            for (int j = 0; j < 2; ++j) sacc[tb][j] += mma_16x16x32(ka, qop[j][s], f32x4{0.f, 0.f, 0.f, 0.f});
           }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) sacc[tb][j] = (sum[0][j] + sum[1][j]) + (sum[2][j] + sum[3][j]);
         } else {
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            const vec8 ka = key_operand<T>(sk + (tb >> 1) * Tl::kBytes, g4, n16, tb & 1, s);
+            const vec8 ka = chunk_keys<T>(sk, lane, tb, s);
 #pragma unroll
             for (int j = 0; j < 2; ++j) sacc[tb][j] = mma_16x16x32(ka, qop[j][s], sacc[tb][j]);
           }
@@ -271,7 +341,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
 #pragma unroll
           for (int db = 0; db < 8; ++db) o[db][j] *= alpha;
           probs(mnew == -INFINITY ? 0.f : -mnew);
-          if (mnew == -INFINITY && t0 < lim[j]) ps += 1.f;
+          if (mnew == -INFINITY && (!EDGE || t0 < lim[j])) ps += 1.f;
         }
         l[j] += ps;
       }
@@ -280,31 +350,31 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
     wait_lds_dma();  // the values, and the next keys, which were requested before the scores
     __syncthreads();
     if (work) {
-      if (edge) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int db = 0; db < 8; ++db) {
-            vec8 va = value_operand<T>(sv + c * Tl::kBytes, g4, n16, db);
+        for (int db = 0; db < 8; ++db) {
+          const vec8 va = chunk_values<T>(sv, lane, c, db);
+          if (EDGE && edge) {
             edge_values<T>(va, pb[c], t0 + c * HC_TILE, w_hi, g4, o[db]);
-          }
-      } else {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int db = 0; db < 8; ++db) {
-            const vec8 va = value_operand<T>(sv + c * Tl::kBytes, g4, n16, db);
+          } else {
 #pragma unroll
             for (int j = 0; j < 2; ++j) o[db][j] = mma_16x16x32(va, pb[c][j], o[db][j]);
           }
-      }
+        }
     }
     __syncthreads();  // the values are no longer read
     if (more) {
-      st.copy(t0 + kKeys, e1, vp, p.v_page, p.v_tok, sv, bad);
-      if (it + 2 < it1) st.entries(t0 + 2 * kKeys, e1);
+      st.values(p, t0 + kKeys, pg, hd, sv, bad);
+      if (it + 2 < it1) st.places(p, t0 + 2 * kKeys, pg, bad);
     }
-  }
+  };
+  // Every column of the workgroup sees these iterations' tokens whole.
+  const int it_whole = min(max(min(max(base + c_first / a.G + 1, 0), total) / kKeys, it0), it1);
+  int it = it0;
+  for (; it < it_whole; ++it) step(std::false_type{}, it);
+#pragma unroll 1
+  for (; it < it1; ++it) step(std::true_type{}, it);
 
   // A page outside of the pool: NaN for all columns, and the status word.
   const bool any_bad = __syncthreads_or(bad);
@@ -537,7 +607,10 @@ int launch_weigh(const PagedAttn& a, hipStream_t s) {
 
 template <typename T>
 int launch(const PagedAttn& a, hipStream_t s) {
-  const bool uniform = a.pool.page_tokens % 16 == 0;
+  const Pool& p = a.pool;
+  const int64_t far = (int64_t)1 << 31;
+  const bool uniform = p.page_tokens % 16 == 0 && p.k_page < far && p.v_page < far && p.page_tokens * p.k_tok < far &&
+                       p.page_tokens * p.v_tok < far;
   int rc;
   if (a.parts > 1) {
     rc = uniform ? launch_attn<T, true, true>(a, s) : launch_attn<T, false, true>(a, s);
