@@ -114,6 +114,11 @@ struct PagedNew {  // the new keys and values [batch][Hkv][Q][128]: byte strides
   int64_t k_s[3], v_s[3];
 };
 
+// Rows of at most this many (query, head) columns are paged_rows_kernel's, the
+// others paged_chunk_kernel's; a padded batch may hold both.
+constexpr int kFewCols = 16;
+constexpr int kChunkCols = 128;  // columns of a workgroup of the latter
+
 struct PagedAttn {
   Pool pool;
   PagedNew fresh;
@@ -121,16 +126,19 @@ struct PagedAttn {
   int64_t q_s[3];  // element strides: batch, head, token
   void* out;
   int64_t o_s[3];
-  int G, cols;  // query heads of a KV head; columns of a row, (query, head) pairs i * G + g
+  int G, cols, few;  // query heads of a KV head; columns of a row, (query, head) pairs i * G + g; and of one of few
+  uint32_t g_mul;    // c / G = (c * g_mul) >> g_shift
+  int g_shift;
+  bool stored;  // an append ahead of the launch has stored the new tokens
   float scale_log2;
-  // Per row: its first tile among all rows' (paged_rows_kernel), its tokens
-  // with the new ones (-1 - len: no room for them).
-  int2* info;
-  int32_t* share;          // tiles of a workgroup
+  int2* info;      // few columns, per row: its first tile among all rows', its tokens with the new ones (-1 - len: no room for them)
+  int32_t* share;  // tiles of a workgroup
   float *part_o, *part_ml;  // partials: 128 channels; (m, l)
-  float *ml;                // a column's folded (m, l): [row][cols]
+  int4* plan;               // many columns, per row: first partial, parts, tokens as above
+  float *chunk_o, *chunk_ml;
+  float* ml;  // a column's folded (m, l): [row][cols]
   int32_t* len_out;
-  // Accumulated weights of every token and the columns' scores.
+  // Accumulated weights of every token and the scores of few columns.
   const float* weights;
   float* weights_out;
   int64_t weight_stride;
@@ -140,13 +148,17 @@ struct PagedAttn {
   int64_t pos_stride;
   const int32_t* dropped;
   float* zeroed;  // weights of new tokens are set to zero here (calls that do not accumulate)
-  int parts, blocks, grid;
+  int grid, chunk_grid, chunk_slots;
 };
+
+__device__ __forceinline__ int over_group(const PagedAttn& a, int c) {
+  return (int)(((uint64_t)(uint32_t)c * a.g_mul) >> a.g_shift);
+}
 
 int launch_paged_rows(int dtype, const PagedAttn& a, hipStream_t s);
 int launch_paged_chunk(int dtype, const PagedAttn& a, hipStream_t s);
 int launch_paged_append(int dtype, const PagedAttn& a, hipStream_t s);
 int paged_rows_slots(int dtype);
-int paged_chunk_parts(int dtype, int rows, int blocks, int capacity);
+int paged_chunk_slots(int dtype);
 
 }  // namespace hc

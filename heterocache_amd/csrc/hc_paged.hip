@@ -8,6 +8,14 @@ namespace hc {
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// t / d = (t * mul) >> shift for t < 2^31: mul = ceil(2^(31 + s) / d), shift = 31 + s, d <= 2^s.
+static void divider(int d, uint32_t& mul, int& shift) {
+  int s = 0;
+  while (((int64_t)1 << s) < d) ++s;
+  mul = (uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d);
+  shift = 31 + s;
+}
+
 // The cache's geometry, checked, as the kernels take it.
 int fill_pool(const char* name, const hc_paged_cache* c, Pool& p, int Q, const int32_t* counts) {
   if (!c) return set_error(HC_ERR_INVALID, "%s: null cache", name);
@@ -42,11 +50,7 @@ int fill_pool(const char* name, const hc_paged_cache* c, Pool& p, int Q, const i
   p.k_page = c->k_strides[0] * esz, p.k_tok = c->k_strides[1] * esz, p.k_head = c->k_strides[2] * esz;
   p.v_page = c->v_strides[0] * esz, p.v_tok = c->v_strides[1] * esz, p.v_head = c->v_strides[2] * esz;
   p.table = c->table, p.table_stride = c->table_stride, p.row_len = c->row_len, p.counts = counts, p.status = c->status;
-  // t / d = t * ceil(2^(31 + s) / d) >> (31 + s) for t < 2^31 and d <= 2^s.
-  int s = 0;
-  while ((1 << s) < c->page_tokens) ++s;
-  p.div_mul = (uint32_t)((((uint64_t)1 << (31 + s)) + c->page_tokens - 1) / c->page_tokens);
-  p.div_shift = 31 + s;
+  divider(c->page_tokens, p.div_mul, p.div_shift);
   p.page_tokens = c->page_tokens, p.pages = c->pages, p.capacity = (int)cap;
   p.heads = c->heads, p.Hkv = c->kv_heads, p.rows = c->batch * c->kv_heads, p.Q = Q;
   p.fresh = 0;
@@ -57,48 +61,49 @@ namespace {
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// The parts of a call's workspace, and its grid.
+// The parts of a call's workspace, and its grids.
 struct Layout {
-  bool rows;  // few columns: paged_rows_kernel
-  int cols, blocks, parts, grid;
-  size_t info, share, part_o, part_ml, ml, scores, bytes;
+  bool chunk;  // rows of many columns
+  int cols, few, grid, chunk_grid, chunk_slots;
+  size_t info, share, part_o, part_ml, plan, chunk_o, chunk_ml, ml, scores, bytes;
   int64_t score_stride;
 };
 
-Layout layout(const hc_paged_cache* c, int q_heads, int queries, bool fresh, bool weigh) {
-  Layout l;
+Layout layout(const hc_paged_cache* c, int q_heads, int queries, bool counts, bool weigh) {
+  Layout l = {};
   const int G = q_heads / c->kv_heads, rows = c->batch * c->kv_heads;
   const int64_t cap = (int64_t)c->table_pages * c->page_tokens;
   l.cols = G * queries;
-  l.rows = l.cols <= 16;
-  l.blocks = l.parts = l.grid = 0, l.score_stride = 0;
-  size_t at = 0;
+  l.chunk = l.cols > kFewCols;
+  // A padded batch's short rows are attended as such.
+  l.few = !l.chunk ? l.cols : counts && G <= kFewCols ? kFewCols : 0;
   auto take = [&](size_t bytes) {
-    const size_t here = at;
-    at += up256(bytes);
+    const size_t here = l.bytes;
+    l.bytes += up256(bytes);
     return here;
   };
-  l.info = take((size_t)rows * 8);
-  l.share = take(4);
-  l.ml = l.scores = 0;
-  if (l.rows) {
+  if (l.few) {
     l.grid = paged_rows_slots(c->dtype);
     const size_t slots = (size_t)l.grid + rows;
-    l.part_o = take(slots * l.cols * HC_HEAD_DIM * 4);
-    l.part_ml = take(slots * l.cols * 8);
+    l.info = take((size_t)rows * 8);
+    l.share = take(4);
+    l.part_o = take(slots * l.few * HC_HEAD_DIM * 4);
+    l.part_ml = take(slots * l.few * 8);
     if (weigh) {
       l.score_stride = (cap + HC_TILE - 1) / HC_TILE * HC_TILE;
-      l.scores = take((size_t)rows * l.cols * l.score_stride * 4);
+      l.scores = take((size_t)rows * l.few * l.score_stride * 4);
     }
-  } else {
-    l.blocks = (l.cols + 127) / 128;
-    l.parts = paged_chunk_parts(c->dtype, rows, l.blocks, (int)cap);
-    const size_t slots = l.parts > 1 ? (size_t)rows * l.cols * l.parts : 0;
-    l.part_o = take(slots * HC_HEAD_DIM * 4);
-    l.part_ml = take(slots * 8);
+  }
+  if (l.chunk) {
+    // One round of workgroups may be cut blocks' (see find_unit).
+    l.chunk_slots = paged_chunk_slots(c->dtype);
+    const int64_t blocks = (int64_t)rows * ((l.cols + kChunkCols - 1) / kChunkCols);
+    l.chunk_grid = (int)std::min<int64_t>((l.chunk_slots + blocks + 7) / 8 * 8, 0x7ffffff8);
+    l.plan = take((size_t)rows * sizeof(int4));
+    l.chunk_o = take((size_t)l.chunk_slots * kChunkCols * HC_HEAD_DIM * 4);
+    l.chunk_ml = take((size_t)l.chunk_slots * kChunkCols * 8);
     if (weigh) l.ml = take((size_t)rows * l.cols * 8);
   }
-  l.bytes = at;
   return l;
 }
 
@@ -131,22 +136,14 @@ void take_ledger(const hc_paged_cache* c, PagedAttn& a) {
 
 int paged_rows_slots(int dtype) { return device_cus() * (dtype == HC_DTYPE_F32 ? 1 : 2); }
 
-// Parts of the keys: one round of workgroups where the blocks of columns leave
-// most of the device idle, of eight iterations of 64 tokens at least.
-int paged_chunk_parts(int dtype, int rows, int blocks, int capacity) {
-  const int slots = device_cus() * (dtype == HC_DTYPE_F32 ? 1 : 3);
-  const int64_t natural = (int64_t)rows * blocks;
-  if (2 * natural > slots) return 1;
-  const int64_t by_keys = capacity / (64 * 8);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(by_keys, slots / natural), 64));
-}
+int paged_chunk_slots(int dtype) { return device_cus() * (dtype == HC_DTYPE_F32 ? 2 : 3); }
 
 }  // namespace hc
 
 using namespace hc;
 
-extern "C" size_t hc_paged_workspace_size(const hc_paged_cache* c, int q_heads, int queries, int fresh, int weigh) {
-  return sized(c, q_heads, queries) ? layout(c, q_heads, queries, fresh, weigh).bytes : 0;
+extern "C" size_t hc_paged_workspace_size(const hc_paged_cache* c, int q_heads, int queries, int counts, int weigh) {
+  return sized(c, q_heads, queries) ? layout(c, q_heads, queries, counts, weigh).bytes : 0;
 }
 
 extern "C" int hc_paged_append(const hc_paged_cache* c, const void* k, const int64_t* k_strides, const void* v,
@@ -191,22 +188,24 @@ extern "C" int hc_paged_attn(const hc_paged_cache* c, const void* q, const int64
   if (!aligned16(q) || !aligned16(out)) return set_error(HC_ERR_INVALID, "hc_paged_attn: tensors must be 16-byte aligned");
   if (fresh)
     if (int rc = check_fresh("hc_paged_attn", c, k_new, k_strides, v_new, v_strides, a.fresh)) return rc;
-  const Layout l = layout(c, q_heads, queries, fresh, weigh);
+  const Layout l = layout(c, q_heads, queries, counts != nullptr, weigh);
   if (workspace_bytes < l.bytes || !workspace || !aligned16(workspace))
     return set_error(HC_ERR_INVALID, "hc_paged_attn: workspace too small or unaligned (%zu < %zu bytes)", workspace_bytes, l.bytes);
-  const int64_t grid = l.rows ? 0 : (int64_t)a.pool.rows * l.blocks * l.parts;
-  if (grid > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_paged_attn: grid too large");
   char* const ws = reinterpret_cast<char*>(workspace);
   a.pool.fresh = fresh;
   a.q = q, a.out = out;
   for (int i = 0; i < 3; ++i) a.q_s[i] = q_strides[i], a.o_s[i] = out_strides[i];
-  a.G = q_heads / c->kv_heads, a.cols = l.cols;
+  a.G = q_heads / c->kv_heads, a.cols = l.cols, a.few = l.few;
+  divider(a.G, a.g_mul, a.g_shift);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.info = reinterpret_cast<int2*>(ws + l.info);
   a.share = reinterpret_cast<int32_t*>(ws + l.share);
   a.part_o = reinterpret_cast<float*>(ws + l.part_o);
   a.part_ml = reinterpret_cast<float*>(ws + l.part_ml);
-  a.parts = l.parts, a.blocks = l.blocks, a.grid = l.grid;
+  a.plan = reinterpret_cast<int4*>(ws + l.plan);
+  a.chunk_o = reinterpret_cast<float*>(ws + l.chunk_o);
+  a.chunk_ml = reinterpret_cast<float*>(ws + l.chunk_ml);
+  a.grid = l.grid, a.chunk_grid = l.chunk_grid, a.chunk_slots = l.chunk_slots;
   take_ledger(c, a);
   if (!fresh) a.pos = nullptr, a.zeroed = nullptr;
   if (weigh) {
@@ -218,15 +217,16 @@ extern "C" int hc_paged_attn(const hc_paged_cache* c, const void* q, const int64
   }
   hipStream_t s = (hipStream_t)stream;
   int32_t* const lens = fresh ? (len_out ? len_out : c->row_len) : nullptr;
-  if (l.rows) {
+  if (!l.chunk) {
     a.len_out = lens;
     return launch_paged_rows(c->dtype, a, s);
   }
-  if (fresh) {
+  // The lengths advance in the last launch that knows the old ones.
+  if (fresh)
     if (int rc = launch_paged_append(c->dtype, a, s)) return rc;
-  } else {
-    a.info = nullptr;
-  }
+  a.stored = true;
+  if (l.few)
+    if (int rc = launch_paged_rows(c->dtype, a, s)) return rc;
   a.len_out = lens;
   return launch_paged_chunk(c->dtype, a, s);
 }

@@ -27,15 +27,16 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kWaveCols = 32;
 constexpr int kCols = kWaves * kWaveCols;
-constexpr int kKeys = 64;  // tokens an iteration
-constexpr int kTiles = kKeys / HC_TILE;
-
+static_assert(kCols == kChunkCols, "columns of a workgroup");
+// Tokens of an iteration: 16 KB of keys and as much of values in any type.
+template <typename T>
+constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;
 template <typename T>
 constexpr int chunk_lds() {
-  return 3 * kTiles * Tile<T>::kBytes;
+  return 3 * kKeys<T> * Tile<T>::kRow;
 }
 
-// LDS holds 64 tokens of keys or values in blocks of 1 KB, 16 tokens x 64 bytes
+// LDS holds an iteration's tokens of keys or values in blocks of 1 KB, 16 tokens x 64 bytes
 // of channels each, block (group of 16, segment) at (group * kSegs + segment).
 // A copy of a wave fills one; which 16 bytes a lane fetches sets their order in
 // the block, chosen so that every operand is read at lane * (8 or 16) bytes
@@ -79,11 +80,11 @@ __device__ __forceinline__ typename Elem<T>::vec8 chunk_values(const char* set, 
   }
 }
 
-// Copies of 64 tokens by a workgroup: wave w takes segments w (and w + 4) of
+// Copies of an iteration's tokens by a workgroup: wave w takes segments w (and w + 4) of
 // every group.
 template <typename T, bool UNIFORM>
 struct Stage {
-  static constexpr int kGroups = kKeys / 16, kMine = kSegs<T> / kWaves;
+  static constexpr int kGroups = kKeys<T> / 16, kMine = kSegs<T> / kWaves;
   typedef const __attribute__((address_space(4))) int32_t* Table;  // unchanged while the kernel runs: scalar loads
   Table tab;
   int total, wave, k_tok, v_tok;  // this lane's token of a group
@@ -96,7 +97,7 @@ struct Stage {
     k_off = 64 * wave + 16 * k_piece + (UNIFORM ? (uint32_t)(k_tok * (int)p.k_tok) : 0u);
     v_off = 64 * wave + 16 * v_piece + (UNIFORM ? (uint32_t)(v_tok * (int)p.v_tok) : 0u);
   }
-  // UNIFORM: page and place of the 16-token groups of tokens t0 + [0, 64).
+  // UNIFORM: page and place of the iteration's 16-token groups.
   struct Places {
     uint32_t page[kGroups], at[kGroups];
   };
@@ -190,36 +191,110 @@ __device__ __forceinline__ void edge_values(typename Elem<T>::vec8 va, const typ
   for (int j = 0; j < 2; ++j) o[j] = mma_16x16x32(va, pb[j], o[j]);
 }
 
-template <typename T, bool UNIFORM, bool SPLIT>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_kernel(const PagedAttn a) {
+// What a workgroup does: a block of 128 columns of a row, and of its keys one
+// part of several.  The blocks' iterations, counted over all rows from the
+// lengths on the device, are cut where the blocks alone would leave half of the
+// device idle, or one row's far longer than the mean; parts of one block lie
+// beside each other, and neighbours on one XCD (workgroups are dealt to the 8
+// XCDs in turn), so that its L2 serves the keys that the blocks of a row share.
+struct Unit {
+  int row, block, part, parts, slot;
+};
+constexpr int kLeastIts = 8;  // iterations of a part at least
+
+__device__ __forceinline__ float wave_sum(float v) {
+  asm("" : "+v"(v));
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+__device__ __forceinline__ bool find_unit(const PagedAttn& a, int keys, int lane, Unit& u) {
+  const Pool& p = a.pool;
+  const int x = blockIdx.x;
+  int enc = 0, blocks = 0, its = 0;
+  auto load_rows = [&](int r0) {
+    const int r = min(r0 + lane, p.rows - 1);
+    const RowSpan s = row_span(p, r);
+    const int cols = s.n * a.G;
+    enc = s.room ? s.total : -1 - s.len;
+    blocks = r0 + lane < p.rows && s.room && (cols > kFewCols || a.few == 0) ? (cols + kCols - 1) / kCols : 0;
+    its = (s.total + keys - 1) / keys;
+    asm("" : "+v"(enc), "+v"(blocks), "+v"(its));  // opaque: the wave's sums take every lane
+  };
+  int units = 0;
+  float work = 0.f;
+  load_rows(0);
+  for (int r0 = 0;;) {
+    units += __builtin_amdgcn_readlane(wave_scan_add(blocks), 63);
+    work += wave_sum((float)blocks * (float)its);
+    r0 += 64;
+    if (r0 >= p.rows) break;
+    load_rows(r0);
+  }
+  // At most chunk_slots workgroups belong to blocks that are cut.
+  const int slots = a.chunk_slots;
+  const float cut = 2 * units <= slots ? work / (float)(slots - units) : 2.f * work / (float)slots;
+  const int share = __builtin_amdgcn_readfirstlane(max(kLeastIts, (int)cut + 1));
+  int count = 0, split = 0;
+  auto parts_of = [&]() { return blocks > 0 ? max((its + share - 1) / share, 1) : 0; };
+  for (int r0 = 0; r0 < p.rows; r0 += 64) {
+    if (p.rows > 64) load_rows(r0);
+    const int parts = parts_of();
+    const int incl = wave_scan_add(parts > 1 ? parts * blocks : 0);
+    if (x == 0 && r0 + lane < p.rows) a.plan[r0 + lane] = make_int4(split + incl - (parts > 1 ? parts * blocks : 0), parts, enc, 0);
+    split += __builtin_amdgcn_readlane(incl, 63);
+    count += __builtin_amdgcn_readlane(wave_scan_add(parts * blocks), 63);
+  }
+  const int per = (count + 7) / 8, y = x % 8 * per + x / 8;
+  if (x / 8 >= per || y >= count) return false;
+  int before = 0, cut_before = 0;
+  for (int r0 = 0; r0 < p.rows; r0 += 64) {
+    if (p.rows > 64) load_rows(r0);
+    const int parts = parts_of(), mine = parts * blocks;
+    const int incl = wave_scan_add(mine) + before, cuts = wave_scan_add(parts > 1 ? mine : 0) + cut_before;
+    const uint64_t hit = __ballot(y < incl);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      u.row = r0 + src;
+      u.parts = __builtin_amdgcn_readlane(parts, src);
+      const int nb = __builtin_amdgcn_readlane(blocks, src);
+      const int at = y - (__builtin_amdgcn_readlane(incl, src) - u.parts * nb);
+      u.block = nb - 1 - at / u.parts;  // the blocks with the most keys first
+      u.part = at % u.parts;
+      u.slot = u.parts > 1 ? __builtin_amdgcn_readlane(cuts, src) - u.parts * nb + at : 0;
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(incl, 63);
+    cut_before = __builtin_amdgcn_readlane(cuts, 63);
+  }
+  return false;
+}
+
+template <typename T, bool UNIFORM>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) void paged_chunk_kernel(const PagedAttn a) {
   typedef typename Elem<T>::vec8 vec8;
   typedef Tile<T> Tl;
+  constexpr int kStep = kKeys<T>, kBlocks16 = kStep / 16, kTiles = kStep / HC_TILE;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const Pool& p = a.pool;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g4 = lane >> 4, n16 = lane & 15;
-  // Workgroup -> (row, part, block of columns), the blocks with the most keys first.
-  const int row = blockIdx.x % p.rows, rest = blockIdx.x / p.rows;
-  const int part = SPLIT ? rest % a.parts : 0;
-  const int cb = a.blocks - 1 - (SPLIT ? rest / a.parts : rest);
+  Unit u;
+  if (!find_unit(a, kStep, lane, u)) return;
+  const int row = u.row;
   const int b = row / p.Hkv, h = row % p.Hkv;
   const int hd = p.heads == 1 ? 0 : h;
   const RowSpan span = row_span(p, row);
-  // An append ahead of this launch has left the rows' tokens behind.
-  const int info = a.info ? a.info[table_row(p, row)].y : span.total;
-  const bool room = info >= 0;
-  const int total = room ? info : -1 - info, nq = span.n, ncols = nq * a.G;
+  const int total = __builtin_amdgcn_readfirstlane(span.total), nq = __builtin_amdgcn_readfirstlane(span.n), ncols = nq * a.G;
   const int base = total - nq;
-  if (a.len_out && rest == 0 && tid == 0 && (p.heads == 1 || h == 0)) a.len_out[table_row(p, row)] = total;
-  const int c_first = cb * kCols, c_wave = c_first + wave * kWaveCols;
-  if (SPLIT && c_first >= ncols) return;  // (padding: the fold writes it)
-  // The last query of the workgroup, and of the wave, that is a token.
-  const int i_last = min(c_first + kCols, ncols) - 1;
-  const int seen = !room || c_first >= ncols ? 0 : min(max(base + i_last / a.G + 1, 0), total);
-  const int its_all = (seen + kKeys - 1) / kKeys;
-  const int share = SPLIT ? (its_all + a.parts - 1) / a.parts : its_all;
-  const int it0 = SPLIT ? min(part * share, its_all) : 0, it1 = SPLIT ? min(it0 + share, its_all) : its_all;
-  const bool active = c_wave < ncols && room;
+  const int c_first = u.block * kCols, c_wave = c_first + wave * kWaveCols;
+  // The last query of the workgroup, and of the wave.
+  const int i_last = (min(c_first + kCols, ncols) - 1) / a.G;
+  const int its_all = (min(max(base + i_last + 1, 0), total) + kStep - 1) / kStep;
+  const int share = (its_all + u.parts - 1) / u.parts;
+  const int it0 = min(u.part * share, its_all), it1 = min(it0 + share, its_all);
+  const bool active = c_wave < ncols;
   const int w_lo = min(max(base + c_wave / a.G + 1, 0), total);  // tokens that all columns of the wave see
   const int w_hi = active ? min(max(base + (min(c_wave + kWaveCols, ncols) - 1) / a.G + 1, 0), total) : 0;
 
@@ -247,14 +322,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
 
   typedef Stage<T, UNIFORM> St;
   const St st(p, row, max(total, 1), lane, wave);
-  constexpr int kSet = kTiles * Tl::kBytes;
+  constexpr int kSet = kStep * Tl::kRow;
   char* const sv = lds + 2 * kSet;
   typename St::Places pg;  // of the next iteration's tokens
   if (it0 < it1) {
-    st.places(p, it0 * kKeys, pg, bad);
-    st.keys(p, it0 * kKeys, pg, hd, lds, bad);
-    st.values(p, it0 * kKeys, pg, hd, sv, bad);
-    if (it0 + 1 < it1) st.places(p, (it0 + 1) * kKeys, pg, bad);
+    st.places(p, it0 * kStep, pg, bad);
+    st.keys(p, it0 * kStep, pg, hd, lds, bad);
+    st.values(p, it0 * kStep, pg, hd, sv, bad);
+    if (it0 + 1 < it1) st.places(p, (it0 + 1) * kStep, pg, bad);
   }
   wait_lds_dma();
   __syncthreads();
@@ -262,23 +337,23 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
   // EDGE: some column may not see all of the tokens.
   auto step = [&](auto edge_tag, int it) {
     constexpr bool EDGE = decltype(edge_tag)::value;
-    const int t0 = it * kKeys;
+    const int t0 = it * kStep;
     const bool more = it + 1 < it1;
-    if (more) st.keys(p, t0 + kKeys, pg, hd, lds + ((it - it0 + 1) & 1) * kSet, bad);
+    if (more) st.keys(p, t0 + kStep, pg, hd, lds + ((it - it0 + 1) & 1) * kSet, bad);
     const bool work = active && (!EDGE || t0 < w_hi);
-    const bool edge = EDGE && t0 + kKeys > w_lo;
-    vec8 pb[2][2];
+    const bool edge = EDGE && t0 + kStep > w_lo;
+    vec8 pb[kTiles][2];
     if (work) {
       __builtin_amdgcn_s_setprio(0);
       const char* sk = lds + ((it - it0) & 1) * kSet;
       // S^T blocks: rows = tokens 16 tb + 4 g4 + r, column = c_wave + 16 j + n16.
-      f32x4 sacc[4][2];
+      f32x4 sacc[kBlocks16][2];
 #pragma unroll
-      for (int tb = 0; tb < 4; ++tb)
+      for (int tb = 0; tb < kBlocks16; ++tb)
 #pragma unroll
         for (int j = 0; j < 2; ++j) sacc[tb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int tb = 0; tb < 4; ++tb) {
+      for (int tb = 0; tb < kBlocks16; ++tb) {
         if constexpr (sizeof(T) == 4) {
           // Sums of 32 channels apart: a rounding is half a step of the partial
           // sum that it falls on.
@@ -304,7 +379,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int tb = 0; tb < 4; ++tb)
+          for (int tb = 0; tb < kBlocks16; ++tb)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               if (t0 + 16 * tb + 4 * g4 + r >= lim[j]) sacc[tb][j][r] = -INFINITY;
@@ -315,7 +390,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
         auto probs = [&](float nm) {
           ps = 0.f;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < kTiles; ++c) {
             float pv[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -331,7 +406,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
         if (__any(!(ps <= Weights<T>::kLazy))) {
           float mx = -INFINITY;
 #pragma unroll
-          for (int tb = 0; tb < 4; ++tb)
+          for (int tb = 0; tb < kBlocks16; ++tb)
 #pragma unroll
             for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sacc[tb][j][r]);
           const float mnew = next_reference<T>(m[j], rows4_max(mx) * a.scale_log2);
@@ -351,7 +426,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
     __syncthreads();
     if (work) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < kTiles; ++c)
 #pragma unroll
         for (int db = 0; db < 8; ++db) {
           const vec8 va = chunk_values<T>(sv, lane, c, db);
@@ -365,12 +440,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
     }
     __syncthreads();  // the values are no longer read
     if (more) {
-      st.values(p, t0 + kKeys, pg, hd, sv, bad);
-      if (it + 2 < it1) st.places(p, t0 + 2 * kKeys, pg, bad);
+      st.values(p, t0 + kStep, pg, hd, sv, bad);
+      if (it + 2 < it1) st.places(p, t0 + 2 * kStep, pg, bad);
     }
   };
   // Every column of the workgroup sees these iterations' tokens whole.
-  const int it_whole = min(max(min(max(base + c_first / a.G + 1, 0), total) / kKeys, it0), it1);
+  const int it_whole = min(max(min(max(base + c_first / a.G + 1, 0), total) / kStep, it0), it1);
   int it = it0;
   for (; it < it_whole; ++it) step(std::false_type{}, it);
 #pragma unroll 1
@@ -383,17 +458,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
   for (int j = 0; j < 2; ++j) {
     float lt = rows4_sum(l[j]);
     const int c = c_wave + 16 * j + n16;
-    if (c >= a.cols) continue;
-    if (c < ncols && (any_bad || !room)) m[j] = -INFINITY, lt = NAN;
-    if (c >= ncols) m[j] = -INFINITY, lt = 0.f;
-    const int64_t col = (int64_t)row * a.cols + c;
-    if constexpr (SPLIT) {
-      float* pp = a.part_o + (col * a.parts + part) * HC_HEAD_DIM + 4 * g4;
+    if (c >= ncols) continue;  // (padding: the fold writes it)
+    if (any_bad) m[j] = -INFINITY, lt = NAN;
+    if (u.parts > 1) {
+      const int64_t at = (int64_t)u.slot * kCols + (c - c_first);
+      float* pp = a.chunk_o + at * HC_HEAD_DIM + 4 * g4;
 #pragma unroll
       for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4*>(pp + 16 * db) = o[db][j];
-      if (g4 == 0) *reinterpret_cast<float2*>(a.part_ml + (col * a.parts + part) * 2) = make_float2(m[j], lt);
+      if (g4 == 0) *reinterpret_cast<float2*>(a.chunk_ml + at * 2) = make_float2(m[j], lt);
     } else {
-      if (a.ml && g4 == 0) *reinterpret_cast<float2*>(a.ml + col * 2) = make_float2(m[j], lt);
+      if (a.ml && g4 == 0) *reinterpret_cast<float2*>(a.ml + ((int64_t)row * a.cols + c) * 2) = make_float2(m[j], lt);
       typedef T quad __attribute__((ext_vector_type(4)));
       T* op = reinterpret_cast<T*>(a.out) + b * a.o_s[0] + (int64_t)(h * a.G + c % a.G) * a.o_s[1] + (c / a.G) * a.o_s[2] + 4 * g4;
 #pragma unroll
@@ -407,46 +481,61 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 3) void paged_chunk_
   }
 }
 
-// A column's partials folded: 32 threads a column, 4 channels each.
+// The cut blocks' partials folded, 32 threads a column of 4 channels each; the
+// outputs of padding, of rows without room, and the new lengths.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_chunk_fold_kernel(const PagedAttn a) {
   const Pool& p = a.pool;
-  const int64_t col = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (col >= (int64_t)p.rows * a.cols) return;
   const int d0 = 4 * (threadIdx.x & 31);
-  const int row = (int)(col / a.cols), c = (int)(col % a.cols);
-  const int b = row / p.Hkv, h = row % p.Hkv;
-  float M = -INFINITY, L = 0.f;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  if (c < query_tokens(p.counts, b, p.Q) * a.G) {
-    const float* po = a.part_o + col * a.parts * HC_HEAD_DIM + d0;
-    const float* ml = a.part_ml + col * a.parts * 2;
-    for (int s0 = 0; s0 < a.parts; s0 += 4) {
-      f32x4 o4[4];
-      float2 m4[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int s = min(s0 + u, a.parts - 1);
-        o4[u] = *reinterpret_cast<const f32x4*>(po + s * HC_HEAD_DIM);
-        m4[u] = *reinterpret_cast<const float2*>(ml + 2 * s);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (s0 + u >= a.parts) continue;
-        const float mn = fmaxf(M, m4[u].x), f = state_weight(M, mn), e = state_weight(m4[u].x, mn);
-        L = L * f + m4[u].y * e;
-        acc = acc * f + o4[u] * e;
-        M = mn;
-      }
+  if (a.len_out) {
+    const int r = blockIdx.x * 256 + threadIdx.x, rows = p.heads == 1 ? p.rows : p.rows / p.Hkv;
+    if (r < rows) {
+      const int e = a.plan[p.heads == 1 ? r : r * p.Hkv].z;
+      a.len_out[r] = e >= 0 ? e : -1 - e;
     }
   }
-  if (a.ml && d0 == 0) *reinterpret_cast<float2*>(a.ml + col * 2) = make_float2(M, L);
-  typedef T quad __attribute__((ext_vector_type(4)));
-  T* op = reinterpret_cast<T*>(a.out) + b * a.o_s[0] + (int64_t)(h * a.G + c % a.G) * a.o_s[1] + (c / a.G) * a.o_s[2] + d0;
-  quad r;
+  const int64_t columns = (int64_t)p.rows * a.cols;
+  for (int64_t col = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); col < columns; col += (int64_t)gridDim.x * 8) {
+    const int row = (int)(col / a.cols), c = (int)(col % a.cols);
+    const int4 plan = a.plan[row];
+    const int b = row / p.Hkv, h = row % p.Hkv;
+    const int ncols = query_tokens(p.counts, b, p.Q) * a.G;
+    const bool few = a.few > 0 && ncols <= kFewCols, room = plan.z >= 0;
+    if (few ? c < a.few : c < ncols && room && plan.y == 1) continue;
+    float M = -INFINITY, L = c < ncols && !room ? NAN : 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (c < ncols && room) {
+      const int nb = (ncols + kCols - 1) / kCols;
+      const int64_t at = ((int64_t)plan.x + (nb - 1 - c / kCols) * plan.y) * kCols + c % kCols;
+      const float* po = a.chunk_o + at * HC_HEAD_DIM + d0;
+      const float* ml = a.chunk_ml + at * 2;
+      for (int s0 = 0; s0 < plan.y; s0 += 4) {
+        f32x4 o4[4];
+        float2 m4[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) r[e] = Elem<T>::from_f32(state_output(acc[e], M, L));
-  *reinterpret_cast<quad*>(op) = r;
+        for (int u = 0; u < 4; ++u) {
+          const int64_t s = min(s0 + u, plan.y - 1);
+          o4[u] = *reinterpret_cast<const f32x4*>(po + s * kCols * HC_HEAD_DIM);
+          m4[u] = *reinterpret_cast<const float2*>(ml + s * kCols * 2);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (s0 + u >= plan.y) continue;
+          const float mn = fmaxf(M, m4[u].x), f = state_weight(M, mn), e = state_weight(m4[u].x, mn);
+          L = L * f + m4[u].y * e;
+          acc = acc * f + o4[u] * e;
+          M = mn;
+        }
+      }
+      if (a.ml && d0 == 0) *reinterpret_cast<float2*>(a.ml + col * 2) = make_float2(M, L);
+    }
+    typedef T quad __attribute__((ext_vector_type(4)));
+    T* op = reinterpret_cast<T*>(a.out) + b * a.o_s[0] + (int64_t)(h * a.G + c % a.G) * a.o_s[1] + (c / a.G) * a.o_s[2] + d0;
+    quad r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = Elem<T>::from_f32(state_output(acc[e], M, L));
+    *reinterpret_cast<quad*>(op) = r;
+  }
 }
 
 // Every token's share of the chunk's attention,
@@ -462,7 +551,7 @@ constexpr int weigh_lds() {
 }
 
 template <typename T, int NC>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : NC == 4 ? 3 : 4) void paged_weigh_kernel(const PagedAttn a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) void paged_weigh_kernel(const PagedAttn a) {
   typedef typename Elem<T>::vec8 vec8;
   typedef Tile<T> Tl;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -472,11 +561,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : NC == 4 ? 3 : 4) voi
   const int row = blockIdx.x % p.rows, tb = blockIdx.x / p.rows;
   const int b = row / p.Hkv, h = row % p.Hkv;
   const int hd = p.heads == 1 ? 0 : h;
-  const RowSpan span = row_span(p, row);
-  const int info = a.info ? a.info[table_row(p, row)].y : span.total;
+  const int info = a.plan[row].z, nq = query_tokens(p.counts, b, p.Q);
   const bool room = info >= 0;
-  const int total = room ? info : -1 - info, ncols = room ? span.n * a.G : 0, base = total - span.n;
+  const int total = room ? info : -1 - info, ncols = room ? nq * a.G : 0, base = total - nq;
   const int old = p.fresh && room ? base : total;
+  if (a.few > 0 && nq * a.G <= kFewCols) return;  // (paged_fold_kernel's)
   const int t_block = tb * kWaves * 16 * NC;
   if (t_block >= total) return;
   const int t_wave = t_block + wave * 16 * NC;
@@ -507,7 +596,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : NC == 4 ? 3 : 4) voi
 #pragma unroll
     for (int r = 0; r < kLoads; ++r) {
       const int u = r * kPer + tid / Tl::kChunks, c = min(col + u, ncols - 1);
-      const int i = c / a.G, gi = c % a.G;
+      const int i = over_group(a, c), gi = c - i * a.G;
       const char* src = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.q) + b * a.q_s[0] +
                                                       (int64_t)(h * a.G + gi) * a.q_s[1] + i * a.q_s[2]);
       lds_dma16(src + 16 * ((tid % Tl::kChunks) ^ Tl::swizzle(u)), s + r * kThreads * 16 + wave * 1024);
@@ -517,8 +606,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : NC == 4 ? 3 : 4) voi
       const float2 ml = *reinterpret_cast<const float2*>(a.ml + ((int64_t)row * a.cols + c) * 2);
       // No number among the scores: NaN for each token; no token: nothing.
       const float inv = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : NAN) : 1.f / ml.y;
-      *reinterpret_cast<float2*>(s + 64 * Tl::kRow + 8 * tid) =
-          make_float2(ml.x == -INFINITY ? 0.f : ml.x, col + tid < ncols ? inv : 0.f);
+      float* const st = reinterpret_cast<float*>(s + 64 * Tl::kRow);
+      st[tid] = ml.x == -INFINITY ? 0.f : ml.x, st[64 + tid] = col + tid < ncols ? inv : 0.f;
     }
   };
   float sum[NC];
@@ -530,9 +619,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : NC == 4 ? 3 : 4) voi
     __syncthreads();
     if (col + 64 < ncols) stage((it + 1) & 1, col + 64);
     const char* s = lds + (it & 1) * kSet;
-    const float2* const ml = reinterpret_cast<const float2*>(s + 64 * Tl::kRow);
+    const float* const ml = reinterpret_cast<const float*>(s + 64 * Tl::kRow);
     // Some of these columns may not see some of the wave's tokens.
-    const bool edge = t_wave + 16 * NC > base + col / a.G + 1 || col + 64 > ncols;
+    const bool edge = t_wave + 16 * NC > base + over_group(a, col) + 1 || col + 64 > ncols;
     float part[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) part[c] = 0.f;
@@ -547,19 +636,19 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : NC == 4 ? 3 : 4) voi
 #pragma unroll
         for (int c = 0; c < NC; ++c) acc[c] = mma_16x16x32(qa, kop[c][x], acc[c]);
       }
+      const f32x4 top = *reinterpret_cast<const f32x4*>(ml + 16 * qb + 4 * g4);
+      const f32x4 inv = *reinterpret_cast<const f32x4*>(ml + 64 + 16 * qb + 4 * g4);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int u = 16 * qb + 4 * g4 + r;
-        const float2 y = ml[u];
         if (edge) {
-          const bool live = col + u < ncols;
-          const int lim = live ? base + (col + u) / a.G + 1 : 0;
+          const int u = col + 16 * qb + 4 * g4 + r;
+          const int lim = u < ncols ? base + over_group(a, u) + 1 : 0;
 #pragma unroll
           for (int c = 0; c < NC; ++c)
-            if (t_wave + 16 * c + n16 < lim) part[c] = fmaf(fast_exp2(fmaf(acc[c][r], a.scale_log2, -y.x)), y.y, part[c]);
+            if (t_wave + 16 * c + n16 < lim) part[c] = fmaf(fast_exp2(fmaf(acc[c][r], a.scale_log2, -top[r])), inv[r], part[c]);
         } else {
 #pragma unroll
-          for (int c = 0; c < NC; ++c) part[c] = fmaf(fast_exp2(fmaf(acc[c][r], a.scale_log2, -y.x)), y.y, part[c]);
+          for (int c = 0; c < NC; ++c) part[c] = fmaf(fast_exp2(fmaf(acc[c][r], a.scale_log2, -top[r])), inv[r], part[c]);
         }
       }
     }
@@ -576,17 +665,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : NC == 4 ? 3 : 4) voi
   }
 }
 
-template <typename T, bool UNIFORM, bool SPLIT>
+template <typename T, bool UNIFORM>
 int launch_attn(const PagedAttn& a, hipStream_t s) {
   static std::once_flag once;
   static hipError_t attr = hipSuccess;
   std::call_once(once, [] {
-    attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_chunk_kernel<T, UNIFORM, SPLIT>),
+    attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_chunk_kernel<T, UNIFORM>),
                                hipFuncAttributeMaxDynamicSharedMemorySize, chunk_lds<T>());
   });
   if (attr != hipSuccess) return set_error(HC_ERR_HIP, "hc_paged_attn: %s", hipGetErrorString(attr));
-  hipLaunchKernelGGL((paged_chunk_kernel<T, UNIFORM, SPLIT>), dim3((unsigned)((int64_t)a.pool.rows * a.blocks * a.parts)),
-                     dim3(kThreads), chunk_lds<T>(), s, a);
+  hipLaunchKernelGGL((paged_chunk_kernel<T, UNIFORM>), dim3(a.chunk_grid), dim3(kThreads), chunk_lds<T>(), s, a);
   return check_launch("hc_paged_attn(chunk)");
 }
 
@@ -611,20 +699,17 @@ int launch(const PagedAttn& a, hipStream_t s) {
   const int64_t far = (int64_t)1 << 31;
   const bool uniform = p.page_tokens % 16 == 0 && p.k_page < far && p.v_page < far && p.page_tokens * p.k_tok < far &&
                        p.page_tokens * p.v_tok < far;
-  int rc;
-  if (a.parts > 1) {
-    rc = uniform ? launch_attn<T, true, true>(a, s) : launch_attn<T, false, true>(a, s);
-    if (rc) return rc;
-    const int64_t cols = (int64_t)a.pool.rows * a.cols;
-    hipLaunchKernelGGL((paged_chunk_fold_kernel<T>), dim3((unsigned)((cols + 7) / 8)), dim3(256), 0, s, a);
-    rc = check_launch("hc_paged_attn(fold)");
-  } else {
-    rc = uniform ? launch_attn<T, true, false>(a, s) : launch_attn<T, false, false>(a, s);
-  }
+  int rc = uniform ? launch_attn<T, true>(a, s) : launch_attn<T, false>(a, s);
+  if (rc) return rc;
+  const int64_t cols = (int64_t)p.rows * a.cols;
+  const unsigned fold = (unsigned)std::max<int64_t>(std::min<int64_t>((cols + 7) / 8, 2048), (p.rows + 255) / 256);
+  hipLaunchKernelGGL((paged_chunk_fold_kernel<T>), dim3(fold), dim3(256), 0, s, a);
+  rc = check_launch("hc_paged_attn(fold)");
   if (rc || !a.weights_out) return rc;
-  // 64 tokens a wave halve the reads of the queries against 16, once there are workgroups enough.
-  const int64_t wide = (int64_t)a.pool.rows * ((a.pool.capacity + 255) / 256);
-  if (sizeof(T) == 2 && wide >= 512) return launch_weigh<T, 4>(a, s);
+  // More tokens a wave take fewer reads of the queries, once there are workgroups enough.
+  const int64_t wide = (int64_t)p.rows * ((p.capacity + 255) / 256);
+  if (sizeof(T) == 2 && wide >= 2048) return launch_weigh<T, 4>(a, s);
+  if (sizeof(T) == 2 && wide >= 256) return launch_weigh<T, 2>(a, s);
   return launch_weigh<T, 1>(a, s);
 }
 
@@ -638,7 +723,6 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAttn a, in
   const RowSpan s = row_span(p, row);
   const bool first = p.heads == 1 || h == 0;
   if (blk == 0 && threadIdx.x == 0 && first) {
-    if (a.info) a.info[trow] = make_int2(0, s.room ? s.total : -1 - s.len);
     if (a.len_out) a.len_out[trow] = s.total;
     if (!s.room && p.status) atomicOr(p.status, kStatusCapacity);
   }

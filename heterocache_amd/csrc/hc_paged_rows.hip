@@ -51,7 +51,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
     const int r = min(r0 + lane, p.rows - 1);
     const RowSpan s = row_span(p, r);
     row_e = s.room ? s.total : -1 - s.len;
-    nt = s.room && s.n > 0 ? tiles_of(s.total) : 0;
+    nt = s.room && s.n > 0 && s.n * a.G <= kFewCols ? tiles_of(s.total) : 0;
     nt = r0 + lane < p.rows ? nt : 0;
     asm("" : "+v"(row_e), "+v"(nt));  // opaque: the wave's sums take every lane
   };
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
         if (tile0 + kWaves < t1) next = entry(tile0 + kWaves);
       }
       // The run that begins the row stores its new tokens.
-      if (p.fresh && t0 == 0) {
+      if (p.fresh && !a.stored && t0 == 0) {
         for (int u = threadIdx.x; u < nq * Tl::kChunks; u += kThreads) {
           const int i = u / Tl::kChunks, off = 16 * (u % Tl::kChunks), t = old + i;
           const int pg = tab[page_of(p, t)], at = t - page_of(p, t) * p.page_tokens;
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
             if (tok0 + 16 * (e >> 2) + 4 * g + (e & 3) >= lim) s[e >> 2][e & 3] = -INFINITY;
         }
         if (WEIGH && col_ok) {
-          float* sp = a.scores + ((int64_t)row * a.cols + n) * a.score_stride + tok0 + 4 * g;
+          float* sp = a.scores + ((int64_t)row * a.few + n) * a.score_stride + tok0 + 4 * g;
           *reinterpret_cast<f32x4*>(sp) = s[0] * a.scale_log2;
           *reinterpret_cast<f32x4*>(sp + 16) = s[1] * a.scale_log2;
         }
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) *reinterpret_cast<f32x4*>(&s_o[wave][n][16 * mt + 4 * g]) = o[mt];
       __syncthreads();
-      const int64_t slot = ((int64_t)(x + row) * a.cols);
+      const int64_t slot = (int64_t)(x + row) * a.few;
       for (int c = threadIdx.x >> 5; c < nq * a.G; c += kThreads / 32) {
         const int d0 = 4 * (threadIdx.x & 31);
         float M = s_ml[0][c][0], L = 0.f;
@@ -248,22 +248,23 @@ __global__ __launch_bounds__(256) void paged_fold_kernel(const PagedAttn a, int 
   const Pool& p = a.pool;
   const int share = *a.share;
   int x = blockIdx.x;
-  const int columns = p.rows * a.cols;
+  const int columns = p.rows * a.few;
   const bool weigh = WEIGH && x >= columns;
-  const int row = weigh ? (x - columns) % p.rows : x / a.cols;
+  const int row = weigh ? (x - columns) % p.rows : x / a.few;
   const int2 info = a.info[row];
   const bool room = info.y >= 0;
   const int b = row / p.Hkv, h = row % p.Hkv, total = room ? info.y : -1 - info.y;
   const int nq = query_tokens(p.counts, b, p.Q), ncols = room ? nq * a.G : 0;
+  if (nq * a.G > kFewCols) return;
   const int nt = room && nq > 0 ? tiles_of(total) : 0;
   const int first = info.x / share, segs = nt > 0 ? (info.x + nt - 1) / share - first + 1 : 0;
-  const float* const ml = a.part_ml + (int64_t)(first + row) * a.cols * 2;  // [segment][column]
+  const float* const ml = a.part_ml + (int64_t)(first + row) * a.few * 2;  // [segment][column]
   if (!weigh) {
     __shared__ float s_m[8], s_l[8];
     __shared__ f32x4 s_o[8][32];
-    const int c = x % a.cols;
+    const int c = x % a.few;
     const int grp = threadIdx.x >> 5, d0 = 4 * (threadIdx.x & 31);
-    const float* const po = a.part_o + ((int64_t)(first + row) * a.cols + c) * HC_HEAD_DIM + d0;
+    const float* const po = a.part_o + ((int64_t)(first + row) * a.few + c) * HC_HEAD_DIM + d0;
     float m = -INFINITY, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     if (c < ncols) {
@@ -273,8 +274,8 @@ __global__ __launch_bounds__(256) void paged_fold_kernel(const PagedAttn a, int 
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int64_t s = min(s0 + 8 * u, segs - 1);
-          o4[u] = *reinterpret_cast<const f32x4*>(po + s * a.cols * HC_HEAD_DIM);
-          m4[u] = *reinterpret_cast<const float2*>(ml + (s * a.cols + c) * 2);
+          o4[u] = *reinterpret_cast<const f32x4*>(po + s * a.few * HC_HEAD_DIM);
+          m4[u] = *reinterpret_cast<const float2*>(ml + (s * a.few + c) * 2);
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -312,7 +313,7 @@ __global__ __launch_bounds__(256) void paged_fold_kernel(const PagedAttn a, int 
     float m = -INFINITY, l = 0.f;
     if (c < ncols) {
       for (int s = j; s < segs; s += 16) {
-        const float2 y = *reinterpret_cast<const float2*>(ml + ((int64_t)s * a.cols + c) * 2);
+        const float2 y = *reinterpret_cast<const float2*>(ml + ((int64_t)s * a.few + c) * 2);
         const float M = fmaxf(m, y.x);
         l = l * state_weight(m, M) + y.y * state_weight(y.x, M);
         m = M;
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(256) void paged_fold_kernel(const PagedAttn a, int 
       const int t = t0 + 4 * threadIdx.x;
       if (t >= total) break;
       f32x4 w = {0.f, 0.f, 0.f, 0.f};
-      const float* sp = a.scores + (int64_t)row * a.cols * a.score_stride + t;
+      const float* sp = a.scores + (int64_t)row * a.few * a.score_stride + t;
 #pragma unroll 4
       for (int u = 0; u < ncols; ++u) {
         const f32x4 s = *reinterpret_cast<const f32x4*>(sp + u * a.score_stride);
@@ -364,7 +365,7 @@ int launch(const PagedAttn& a, hipStream_t s) {
       if (attr == hipSuccess) attr = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, rows_lds<T>());
   });
   if (attr != hipSuccess) return set_error(HC_ERR_HIP, "hc_paged_attn: %s", hipGetErrorString(attr));
-  const int columns = a.pool.rows * a.cols;
+  const int columns = a.pool.rows * a.few;
   if (weigh) {
     hipLaunchKernelGGL((paged_rows_kernel<T, true>), dim3(a.grid), dim3(kThreads), rows_lds<T>(), s, a);
     if (int rc = check_launch("hc_paged_attn")) return rc;

@@ -1331,7 +1331,7 @@ def paged_attn(q, pages, scale, k_new=None, v_new=None, counts=None, weigh=False
             raise ValueError("weights_out without weigh, or for a cache without weights")
         pages._ledger("weights_out", weights_out, torch.float32, B * pages.kv_heads, like=pages.weights)
     out, o_st = _out_bthd(q, out, shape, dev)
-    ws, nbytes = pages._workspace("hc_paged_workspace_size", Hq, T, k_new is not None, bool(weigh))
+    ws, nbytes = pages._workspace("hc_paged_workspace_size", Hq, T, counts is not None, bool(weigh))
     _lib.check(_lib.load().hc_paged_attn(pages.ref, q.data_ptr(), _strides3((shape, q.stride())), Hq, T, kp, ks, vp, vs,
                                          _ptr(counts), scale, bool(weigh), _ptr(weights_out), _ptr(len_out), out.data_ptr(),
                                          o_st, ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(dev)))

@@ -732,15 +732,16 @@ int hc_paged_append(const hc_paged_cache* c, const void* k, const int64_t* k_str
  * q, out: element strides batch, head, token, all of whole 16 bytes; out shares
  * no memory with q.  Stands where the reference calls flash attention over its
  * pools (heterocache/llama_model.py:382-389), for one new token or many.
- * workspace: hc_paged_workspace_size bytes, 16-byte aligned, no initialisation;
- * calls that overlap in time need their own.  Up to 16 (query, head) pairs a row
- * with weigh it holds their scores, 4 bytes a pair and token of a table row's capacity.
+ * workspace: hc_paged_workspace_size bytes (counts: whether the call has them),
+ * 16-byte aligned, no initialisation; calls that overlap in time need their own.
+ * With weigh it holds the scores of rows of up to 16 (query, head) pairs, 4 bytes
+ * a pair and token of a table row's capacity.
  */
 int hc_paged_attn(const hc_paged_cache* c, const void* q, const int64_t* q_strides, int q_heads, int queries,
                   const void* k_new, const int64_t* k_strides, const void* v_new, const int64_t* v_strides,
                   const int32_t* counts, float scale, int weigh, float* weights_out, int32_t* len_out, void* out,
                   const int64_t* out_strides, void* workspace, size_t workspace_bytes, void* stream);
-size_t hc_paged_workspace_size(const hc_paged_cache* c, int q_heads, int queries, int fresh, int weigh);
+size_t hc_paged_workspace_size(const hc_paged_cache* c, int q_heads, int queries, int counts, int weigh);
 
 /*
  * Eviction by accumulated weight: of a table row's n tokens the first `keep`

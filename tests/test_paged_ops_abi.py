@@ -102,7 +102,7 @@ def test_attn(lib):
     c = _cache()
     for n in (1, 40):
         for weigh in (0, 1):
-            size = lib.hc_paged_workspace_size(ctypes.byref(c), 8, n, 1, weigh)
+            size = lib.hc_paged_workspace_size(ctypes.byref(c), 8, n, 0, weigh)
             assert size > 0
             _refused(lib, _attn(lib, c, n=n, weigh=weigh, wb=size - 1), b"workspace too small")
             _refused(lib, _attn(lib, c, n=n, weigh=weigh, wb=size, ws=FAKE + 8), b"workspace")
