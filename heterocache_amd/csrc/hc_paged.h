@@ -51,6 +51,13 @@ __device__ __forceinline__ RowSpan row_span(const Pool& p, int row) {
   return s;
 }
 
+// Whether 16 tokens from a multiple of 16 lie in one page, at offsets below 2^31.
+inline bool uniform_pages(const Pool& p) {
+  const int64_t far = (int64_t)1 << 31;
+  return p.page_tokens % 16 == 0 && p.k_page < far && p.v_page < far && p.page_tokens * p.k_tok < far &&
+         p.page_tokens * p.v_tok < far;
+}
+
 constexpr int kStatusCapacity = 1, kStatusPage = 2;
 
 template <typename T>
@@ -136,7 +143,8 @@ struct PagedAttn {
   float *part_o, *part_ml;  // partials: 128 channels; (m, l)
   int4* plan;               // many columns, per row: first partial, parts, tokens as above
   float *chunk_o, *chunk_ml;
-  float* ml;  // a column's folded (m, l): [row][cols]
+  float* ml;  // a column's folded state, as weigh_state: [row][ml_stride]
+  int64_t ml_stride;
   int32_t* len_out;
   // Accumulated weights of every token and the scores of few columns.
   const float* weights;

@@ -66,7 +66,7 @@ struct Layout {
   bool chunk;  // rows of many columns
   int cols, few, grid, chunk_grid, chunk_slots;
   size_t info, share, part_o, part_ml, plan, chunk_o, chunk_ml, ml, scores, bytes;
-  int64_t score_stride;
+  int64_t score_stride, ml_stride;
 };
 
 Layout layout(const hc_paged_cache* c, int q_heads, int queries, bool counts, bool weigh) {
@@ -102,7 +102,9 @@ Layout layout(const hc_paged_cache* c, int q_heads, int queries, bool counts, bo
     l.plan = take((size_t)rows * sizeof(int4));
     l.chunk_o = take((size_t)l.chunk_slots * kChunkCols * HC_HEAD_DIM * 4);
     l.chunk_ml = take((size_t)l.chunk_slots * kChunkCols * 8);
-    if (weigh) l.ml = take((size_t)rows * l.cols * 8);
+    // (Read 128 states at a time from multiples of 64.)
+    l.ml_stride = (l.cols + 63) / 64 * 64 + 64;
+    if (weigh) l.ml = take((size_t)rows * l.ml_stride * 8);
   }
   return l;
 }
@@ -211,7 +213,7 @@ extern "C" int hc_paged_attn(const hc_paged_cache* c, const void* q, const int64
   if (weigh) {
     a.weights_out = weights_out ? weights_out : c->weights;
     a.zeroed = nullptr;
-    a.ml = reinterpret_cast<float*>(ws + l.ml);
+    a.ml = reinterpret_cast<float*>(ws + l.ml), a.ml_stride = l.ml_stride;
     a.scores = reinterpret_cast<float*>(ws + l.scores);
     a.score_stride = l.score_stride;
   }

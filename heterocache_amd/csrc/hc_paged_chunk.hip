@@ -271,6 +271,14 @@ __device__ __forceinline__ bool find_unit(const PagedAttn& a, int keys, int lane
   return false;
 }
 
+// What paged_weigh_kernel takes of a column: the reference of its scores and the
+// inverse of their sum.  No token: nothing to add; no number among the scores:
+// NaN for each.
+__device__ __forceinline__ float2 weigh_state(float M, float L) {
+  if (M == -INFINITY) return make_float2(0.f, L == 0.f ? 0.f : NAN);
+  return make_float2(M, 1.f / L);
+}
+
 template <typename T, bool UNIFORM>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) void paged_chunk_kernel(const PagedAttn a) {
   typedef typename Elem<T>::vec8 vec8;
@@ -467,7 +475,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) void paged_chunk_
       for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4*>(pp + 16 * db) = o[db][j];
       if (g4 == 0) *reinterpret_cast<float2*>(a.chunk_ml + at * 2) = make_float2(m[j], lt);
     } else {
-      if (a.ml && g4 == 0) *reinterpret_cast<float2*>(a.ml + ((int64_t)row * a.cols + c) * 2) = make_float2(m[j], lt);
+      if (a.ml && g4 == 0) *reinterpret_cast<float2*>(a.ml + ((int64_t)row * a.ml_stride + c) * 2) = weigh_state(m[j], lt);
       typedef T quad __attribute__((ext_vector_type(4)));
       T* op = reinterpret_cast<T*>(a.out) + b * a.o_s[0] + (int64_t)(h * a.G + c % a.G) * a.o_s[1] + (c / a.G) * a.o_s[2] + 4 * g4;
 #pragma unroll
@@ -527,7 +535,7 @@ __global__ __launch_bounds__(256) void paged_chunk_fold_kernel(const PagedAttn a
           M = mn;
         }
       }
-      if (a.ml && d0 == 0) *reinterpret_cast<float2*>(a.ml + col * 2) = make_float2(M, L);
+      if (a.ml && d0 == 0) *reinterpret_cast<float2*>(a.ml + ((int64_t)row * a.ml_stride + c) * 2) = weigh_state(M, L);
     }
     typedef T quad __attribute__((ext_vector_type(4)));
     T* op = reinterpret_cast<T*>(a.out) + b * a.o_s[0] + (int64_t)(h * a.G + c % a.G) * a.o_s[1] + (c / a.G) * a.o_s[2] + d0;
@@ -547,7 +555,7 @@ __global__ __launch_bounds__(256) void paged_chunk_fold_kernel(const PagedAttn a
 // streamed through LDS 64 at a time, so a token's sum stays in its lane.
 template <typename T>
 constexpr int weigh_lds() {
-  return 2 * (64 * Tile<T>::kRow + 64 * 8);
+  return 2 * (64 * Tile<T>::kRow + 1024);
 }
 
 template <typename T, int NC>
@@ -587,8 +595,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) void paged_weigh_
 
   // Columns of the chunk, 64 an iteration, from the first that sees a token of
   // the workgroup on: unit u = r * 256 + tid is chunk u % kChunks of column u /
-  // kChunks.  Columns behind the last repeat it, with 1 / L = 0.
-  constexpr int kSet = 64 * Tl::kRow + 64 * 8;
+  // kChunks.  Columns behind the last repeat it, and no token is taken as seen by them.
+  constexpr int kSet = 64 * Tl::kRow + 1024;
   constexpr int kPer = kThreads / Tl::kChunks, kLoads = 64 / kPer;
   const int c0 = max(t_block - base, 0) * a.G / 64 * 64;
   auto stage = [&](int set, int col) {
@@ -601,14 +609,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) void paged_weigh_
                                                       (int64_t)(h * a.G + gi) * a.q_s[1] + i * a.q_s[2]);
       lds_dma16(src + 16 * ((tid % Tl::kChunks) ^ Tl::swizzle(u)), s + r * kThreads * 16 + wave * 1024);
     }
-    if (tid < 64) {
-      const int c = min(col + tid, ncols - 1);
-      const float2 ml = *reinterpret_cast<const float2*>(a.ml + ((int64_t)row * a.cols + c) * 2);
-      // No number among the scores: NaN for each token; no token: nothing.
-      const float inv = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : NAN) : 1.f / ml.y;
-      float* const st = reinterpret_cast<float*>(s + 64 * Tl::kRow);
-      st[tid] = ml.x == -INFINITY ? 0.f : ml.x, st[64 + tid] = col + tid < ncols ? inv : 0.f;
-    }
+    // Their states, and those of as many behind, which nothing reads.
+    if (wave == 0)
+      lds_dma16(reinterpret_cast<const char*>(a.ml + ((int64_t)row * a.ml_stride + col) * 2) + 16 * lane, s + 64 * Tl::kRow);
   };
   float sum[NC];
 #pragma unroll
@@ -636,8 +639,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) void paged_weigh_
 #pragma unroll
         for (int c = 0; c < NC; ++c) acc[c] = mma_16x16x32(qa, kop[c][x], acc[c]);
       }
-      const f32x4 top = *reinterpret_cast<const f32x4*>(ml + 16 * qb + 4 * g4);
-      const f32x4 inv = *reinterpret_cast<const f32x4*>(ml + 64 + 16 * qb + 4 * g4);
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(ml + 2 * (16 * qb + 4 * g4));
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(ml + 2 * (16 * qb + 4 * g4) + 4);
+      const float top[4] = {lo[0], lo[2], hi[0], hi[2]}, inv[4] = {lo[1], lo[3], hi[1], hi[3]};
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if (edge) {
@@ -696,13 +700,10 @@ int launch_weigh(const PagedAttn& a, hipStream_t s) {
 template <typename T>
 int launch(const PagedAttn& a, hipStream_t s) {
   const Pool& p = a.pool;
-  const int64_t far = (int64_t)1 << 31;
-  const bool uniform = p.page_tokens % 16 == 0 && p.k_page < far && p.v_page < far && p.page_tokens * p.k_tok < far &&
-                       p.page_tokens * p.v_tok < far;
-  int rc = uniform ? launch_attn<T, true>(a, s) : launch_attn<T, false>(a, s);
+  int rc = uniform_pages(p) ? launch_attn<T, true>(a, s) : launch_attn<T, false>(a, s);
   if (rc) return rc;
   const int64_t cols = (int64_t)p.rows * a.cols;
-  const unsigned fold = (unsigned)std::max<int64_t>(std::min<int64_t>((cols + 7) / 8, 2048), (p.rows + 255) / 256);
+  const unsigned fold = (unsigned)std::max<int64_t>(std::min<int64_t>((cols + 7) / 8, 8192), (p.rows + 255) / 256);
   hipLaunchKernelGGL((paged_chunk_fold_kernel<T>), dim3(fold), dim3(256), 0, s, a);
   rc = check_launch("hc_paged_attn(fold)");
   if (rc || !a.weights_out) return rc;

@@ -11,7 +11,10 @@
 // each token's address through the table (or, for the tokens that the call
 // appends, from their tensors: they are stored to the pages beside, so that
 // nothing waits for a launch of its own), takes the tile's operands into
-// registers and requests the next tile before it attends.
+// registers and requests the next tile before it attends.  Where page sizes are
+// multiples of 16, a copy's tokens lie in one page and its address is scalar;
+// other sizes, and the tiles that reach behind the stored tokens, take an
+// address a token.
 #include <algorithm>
 #include <mutex>
 
@@ -33,7 +36,7 @@ constexpr int rows_lds() {
 
 __device__ __forceinline__ int tiles_of(int tokens) { return (tokens + HC_TILE - 1) / HC_TILE; }
 
-template <typename T, bool WEIGH>
+template <typename T, bool WEIGH, bool UNIFORM>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_kernel(const PagedAttn a) {
   typedef typename Elem<T>::vec8 vec8;
   typedef Tile<T> Tl;
@@ -103,30 +106,87 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
       const int64_t s_fresh = is_v ? a.fresh.v_s[2] : a.fresh.k_s[2];
       bool bad = false;
 
-      // Lane l holds the address of token l % 32 of a tile: keys for the lower
-      // 32 lanes, values for the upper.  Tokens behind the last are the last.
-      auto entry = [&](int tile) { return tab[page_of(p, min(tile * HC_TILE + (lane & 31), total_tok - 1))]; };
-      auto copy = [&](int tile, int page) {
+      // A tile's page entries: UNIFORM, of its two groups of 16 tokens, the tile
+      // being whole in the pages; else of token l % 32 in lane l.  Tokens behind
+      // the last are the last.
+      typedef const __attribute__((address_space(4))) int32_t* Table;  // unchanged while the kernel runs: scalar loads
+      const Table stab = (Table)(uintptr_t)tab;
+      struct Entries {
+        int e[2];
+      };
+      auto whole = [&](int tile) { return UNIFORM && tile * HC_TILE + HC_TILE <= old; };
+      auto entries = [&](int tile) {
+        Entries r = {};
+        if (whole(tile)) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) r.e[u] = __builtin_amdgcn_readfirstlane(stab[page_of(p, tile * HC_TILE + 16 * u)]);
+        } else {
+          r.e[0] = tab[page_of(p, min(tile * HC_TILE + (lane & 31), total_tok - 1))];
+        }
+        return r;
+      };
+      // (Bytes of a lane's 16 within a token, for the first tokens of a group.)
+      const int tok0_lane = lane / Tl::kChunks;
+      const uint32_t off_lane = 16 * ((lane % Tl::kChunks) ^ Tl::swizzle(tok0_lane));
+      auto copy = [&](int tile, Entries en) {
+        if (whole(tile)) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t pg = (uint32_t)en.e[u];
+            if (pg >= (uint32_t)p.pages) bad = true, pg = 0;
+            const int t = tile * HC_TILE + 16 * u;
+            const uint32_t at = (uint32_t)(t - page_of(p, t) * p.page_tokens);
+            const char* const kp = p.k + hd * p.k_head + ((uint64_t)pg * (uint32_t)p.k_page + at * (uint32_t)p.k_tok);
+            const char* const vp = p.v + hd * p.v_head + ((uint64_t)pg * (uint32_t)p.v_page + at * (uint32_t)p.v_tok);
+#pragma unroll
+            for (int j = 0; j < Tl::kLoads / 2; ++j) {
+              // (The swizzle is linear in the token's bits.)
+              const uint32_t off = off_lane ^ (uint32_t)(16 * Tl::swizzle(j * Tl::kTokens & 15));
+              const uint32_t tok = j * Tl::kTokens + tok0_lane;
+              lds_dma16_run<1, true>(kp + (off + tok * (uint32_t)p.k_tok), sk + 1024 * (u * Tl::kLoads / 2 + j));
+              lds_dma16_run<1, true>(vp + (off + tok * (uint32_t)p.v_tok), sv + 1024 * (u * Tl::kLoads / 2 + j));
+            }
+          }
+          return;
+        }
+        // Lane l holds the address of token l % 32: keys for the lower 32 lanes,
+        // values for the upper.
         const int t = min(tile * HC_TILE + (lane & 31), total_tok - 1);
         const bool is_new = t >= old;
+        int page = en.e[0];
         if (!is_new && (uint32_t)page >= (uint32_t)p.pages) bad = true, page = 0;
         const int at = t - page_of(p, t) * p.page_tokens;
         const char* src = is_new ? fresh + (t - old) * s_fresh : pool + page * s_page + at * s_tok;
         __builtin_amdgcn_wave_barrier();
         addr[lane] = reinterpret_cast<int64_t>(src);
         __builtin_amdgcn_wave_barrier();
+        constexpr int kBatch = 8;  // addresses read together: each copy may write LDS, which orders the next read
 #pragma unroll
-        for (int j = 0; j < Tl::kLoads; ++j) {
-          const int tok = j * Tl::kTokens + lane / Tl::kChunks;
-          const int off = 16 * ((lane % Tl::kChunks) ^ Tl::swizzle(tok));
-          lds_dma16(reinterpret_cast<const char*>(addr[tok]) + off, sk + 1024 * j);
-          lds_dma16(reinterpret_cast<const char*>(addr[32 + tok]) + off, sv + 1024 * j);
-        }
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+          for (int j0 = 0; j0 < Tl::kLoads; j0 += kBatch) {
+            int64_t from[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+              const int tok = (j0 + j) * Tl::kTokens + lane / Tl::kChunks;
+              from[j] = addr[32 * v + tok] + 16 * ((lane % Tl::kChunks) ^ Tl::swizzle(tok));
+            }
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+              lds_dma16_run<1, true>(reinterpret_cast<const char*>(from[j]), (v ? sv : sk) + 1024 * (j0 + j));
+          }
       };
 
       const int tile0 = t0 + wave;
-      int page = 0, next = 0;
-      if (tile0 < t1) page = entry(tile0);
+      // The wave's tiles, every kWaves-th, from one that differs between the
+      // workgroups on and round: runs of equal length begin at equal places of
+      // their pages, and together they would draw on few memory channels.
+      const int mine = max((t1 - tile0 + kWaves - 1) / kWaves, 0);
+      const int end = tile0 + mine * kWaves;
+      auto after = [&](int tile) { return tile + kWaves < end ? tile + kWaves : tile0; };
+      int tile = tile0 + (mine > 0 ? (int)((uint32_t)x * 5u % (uint32_t)mine) * kWaves : 0);
+      Entries first_e = {}, next = {};
+      if (mine > 0) first_e = entries(tile);
       // Column n: query n / G, head n % G of the row's group.
       const bool col_ok = n < nq * a.G;
       const int qi = col_ok ? n / a.G : 0, gi = col_ok ? n % a.G : 0;
@@ -136,9 +196,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
 #pragma unroll
         for (int s = 0; s < 4; ++s) qreg[s] = col_ok ? load8<T>(qp + 32 * s) : zero8<T>();
       }
-      if (tile0 < t1) {
-        copy(tile0, page);
-        if (tile0 + kWaves < t1) next = entry(tile0 + kWaves);
+      if (mine > 0) {
+        copy(tile, first_e);
+        if (mine > 1) next = entries(after(tile));
       }
       // The run that begins the row stores its new tokens.
       if (p.fresh && !a.stored && t0 == 0) {
@@ -167,7 +227,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
       f32x4 o[8];
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) o[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int tile = tile0; tile < t1; tile += kWaves) {
+      for (int left = mine; left > 0; --left) {
         const int tok0 = tile * HC_TILE;
         wait_lds_dma();
         __builtin_amdgcn_wave_barrier();
@@ -176,13 +236,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
         for (int y = 0; y < 8; ++y) kr[y] = key_operand<T>(sk, g, n, y >> 2, y & 3);
 #pragma unroll
         for (int y = 0; y < 8; ++y) vr[y] = value_operand<T>(sv, g, n, y);
-        // The operands are here: the buffer takes the next tile.
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-        __builtin_amdgcn_sched_barrier(0);
-        if (tile + kWaves < t1) {
-          copy(tile + kWaves, next);
-          if (tile + 2 * kWaves < t1) next = entry(tile + 2 * kWaves);
-        }
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the operands are here
         __builtin_amdgcn_sched_barrier(0);
         f32x4 s[2];
         tile_scores<T>(kr, qreg, s);
@@ -191,16 +245,26 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
           for (int e = 0; e < 8; ++e)
             if (tok0 + 16 * (e >> 2) + 4 * g + (e & 3) >= lim) s[e >> 2][e & 3] = -INFINITY;
         }
+        // (Ahead of the copies, whose wait then finds the stores done.)
         if (WEIGH && col_ok) {
           float* sp = a.scores + ((int64_t)row * a.few + n) * a.score_stride + tok0 + 4 * g;
           *reinterpret_cast<f32x4*>(sp) = s[0] * a.scale_log2;
           *reinterpret_cast<f32x4*>(sp + 16) = s[1] * a.scale_log2;
         }
+        __builtin_amdgcn_sched_barrier(0);
+        // The buffer takes the next tile.
+        const int then = after(tile);
+        if (left > 1) {
+          copy(then, next);
+          if (left > 2) next = entries(after(then));
+        }
+        __builtin_amdgcn_sched_barrier(0);
         const vec8 pb = tile_probs<T>(s, tok0 < lim, a.scale_log2, m, l, o);
         if (tok0 + HC_TILE > lim_lo)
           tile_values<T, true>(vr, pb, tok0, total_tok, g, o);
         else
           tile_values<T, false>(vr, pb, tok0, total_tok, g, o);
+        tile = then;
       }
       l = rows4_sum(l);
       if (__any(bad)) {
@@ -354,29 +418,31 @@ __global__ __launch_bounds__(256) void paged_fold_kernel(const PagedAttn a, int 
   }
 }
 
-template <typename T>
-int launch(const PagedAttn& a, hipStream_t s) {
-  const bool weigh = a.weights_out != nullptr;
+template <typename T, bool WEIGH, bool UNIFORM>
+int launch_attn(const PagedAttn& a, hipStream_t s) {
   static std::once_flag once;
   static hipError_t attr = hipSuccess;
   std::call_once(once, [] {
-    for (const void* fn : {reinterpret_cast<const void*>(&paged_rows_kernel<T, false>),
-                           reinterpret_cast<const void*>(&paged_rows_kernel<T, true>)})
-      if (attr == hipSuccess) attr = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, rows_lds<T>());
+    attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_rows_kernel<T, WEIGH, UNIFORM>),
+                               hipFuncAttributeMaxDynamicSharedMemorySize, rows_lds<T>());
   });
   if (attr != hipSuccess) return set_error(HC_ERR_HIP, "hc_paged_attn: %s", hipGetErrorString(attr));
+  hipLaunchKernelGGL((paged_rows_kernel<T, WEIGH, UNIFORM>), dim3(a.grid), dim3(kThreads), rows_lds<T>(), s, a);
+  return check_launch("hc_paged_attn(rows)");
+}
+
+template <typename T, bool WEIGH>
+int launch(const PagedAttn& a, hipStream_t s) {
+  if (int rc = uniform_pages(a.pool) ? launch_attn<T, WEIGH, true>(a, s) : launch_attn<T, WEIGH, false>(a, s)) return rc;
   const int columns = a.pool.rows * a.few;
-  if (weigh) {
-    hipLaunchKernelGGL((paged_rows_kernel<T, true>), dim3(a.grid), dim3(kThreads), rows_lds<T>(), s, a);
-    if (int rc = check_launch("hc_paged_attn")) return rc;
-    const int runs = std::max(1, std::min((a.pool.capacity + kWeighTokens - 1) / kWeighTokens, 2048 / a.pool.rows));
-    hipLaunchKernelGGL((paged_fold_kernel<T, true>), dim3(columns + runs * a.pool.rows), dim3(256), 0, s, a, runs);
-  } else {
-    hipLaunchKernelGGL((paged_rows_kernel<T, false>), dim3(a.grid), dim3(kThreads), rows_lds<T>(), s, a);
-    if (int rc = check_launch("hc_paged_attn")) return rc;
-    hipLaunchKernelGGL((paged_fold_kernel<T, false>), dim3(columns), dim3(256), 0, s, a, 0);
-  }
+  const int runs = WEIGH ? std::max(1, std::min((a.pool.capacity + kWeighTokens - 1) / kWeighTokens, 2048 / a.pool.rows)) : 0;
+  hipLaunchKernelGGL((paged_fold_kernel<T, WEIGH>), dim3(columns + runs * a.pool.rows), dim3(256), 0, s, a, runs);
   return check_launch("hc_paged_attn(fold)");
+}
+
+template <typename T>
+int launch(const PagedAttn& a, hipStream_t s) {
+  return a.weights_out ? launch<T, true>(a, s) : launch<T, false>(a, s);
 }
 
 }  // namespace
