@@ -138,7 +138,7 @@ void take_ledger(const hc_paged_cache* c, PagedAttn& a) {
 
 int paged_rows_slots(int dtype) { return device_cus() * (dtype == HC_DTYPE_F32 ? 1 : 2); }
 
-int paged_chunk_slots(int dtype) { return device_cus() * (dtype == HC_DTYPE_F32 ? 2 : 3); }
+int paged_chunk_slots(int dtype) { return device_cus() * 2; }
 
 }  // namespace hc
 

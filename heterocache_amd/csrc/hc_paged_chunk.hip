@@ -559,17 +559,22 @@ constexpr int weigh_lds() {
 }
 
 template <typename T, int NC>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) void paged_weigh_kernel(const PagedAttn a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : NC == 4 ? 3 : 4) void paged_weigh_kernel(const PagedAttn a, int blocks) {
   typedef typename Elem<T>::vec8 vec8;
   typedef Tile<T> Tl;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const Pool& p = a.pool;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g4 = lane >> 4, n16 = lane & 15;
-  const int row = blockIdx.x % p.rows, tb = blockIdx.x / p.rows;
+  // Rows r, r + 8, .. on one XCD, the blocks of a row behind each other: workgroups
+  // are dealt in turn to the XCDs and within one to its four engines, where rows
+  // of a sequence each would all meet (4 ragged sequences: 160 us, now 82).
+  const int row = blockIdx.x % 8 + 8 * (blockIdx.x / 8 / blocks), tb = blockIdx.x / 8 % blocks;
+  if (row >= p.rows) return;
   const int b = row / p.Hkv, h = row % p.Hkv;
   const int hd = p.heads == 1 ? 0 : h;
-  const int info = a.plan[row].z, nq = query_tokens(p.counts, b, p.Q);
+  // (Scalar, as what follows from them.)
+  const int info = __builtin_amdgcn_readfirstlane(a.plan[row].z), nq = __builtin_amdgcn_readfirstlane(query_tokens(p.counts, b, p.Q));
   const bool room = info >= 0;
   const int total = room ? info : -1 - info, ncols = room ? nq * a.G : 0, base = total - nq;
   const int old = p.fresh && room ? base : total;
@@ -580,7 +585,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) void paged_weigh_
   const int32_t* const tab = p.table + table_row(p, row) * p.table_stride;
 
   // Key operands: token t_wave + 16 c + n16 (those behind the last repeat it and
-  // are not stored), channels 32 s + 8 g4 + [0, 8).
+  // are not stored), channels as the queries'.
   vec8 kop[NC][4];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -588,26 +593,27 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) void paged_weigh_
     const int pi = page_of(p, t);
     int pg = tab[pi];
     if ((uint32_t)pg >= (uint32_t)p.pages) pg = 0;  // (the columns' sums are NaN)
-    const T* kp = reinterpret_cast<const T*>(p.k + hd * p.k_head + pg * p.k_page + (t - pi * p.page_tokens) * p.k_tok) + 8 * g4;
+    const T* kp = reinterpret_cast<const T*>(p.k + hd * p.k_head + pg * p.k_page + (t - pi * p.page_tokens) * p.k_tok);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) kop[c][s] = load8<T>(kp + 32 * s);
+    for (int s = 0; s < 4; ++s) kop[c][s] = chunk_query<T>(kp, g4, s);
   }
 
   // Columns of the chunk, 64 an iteration, from the first that sees a token of
-  // the workgroup on: unit u = r * 256 + tid is chunk u % kChunks of column u /
-  // kChunks.  Columns behind the last repeat it, and no token is taken as seen by them.
-  constexpr int kSet = 64 * Tl::kRow + 1024;
-  constexpr int kPer = kThreads / Tl::kChunks, kLoads = 64 / kPer;
+  // the workgroup on, in LDS as chunk_keys reads them.  Columns behind the last
+  // repeat it, and no token is taken as seen by them.
+  constexpr int kSet = 64 * Tl::kRow + 1024, kMine = kSegs<T> / kWaves;
   const int c0 = max(t_block - base, 0) * a.G / 64 * 64;
+  const uint32_t q_off = 64 * wave + 16 * g4;
   auto stage = [&](int set, int col) {
     char* s = lds + set * kSet;
 #pragma unroll
-    for (int r = 0; r < kLoads; ++r) {
-      const int u = r * kPer + tid / Tl::kChunks, c = min(col + u, ncols - 1);
+    for (int r = 0; r < 4; ++r) {
+      const int c = min(col + 16 * r + n16, ncols - 1);
       const int i = over_group(a, c), gi = c - i * a.G;
       const char* src = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.q) + b * a.q_s[0] +
                                                       (int64_t)(h * a.G + gi) * a.q_s[1] + i * a.q_s[2]);
-      lds_dma16(src + 16 * ((tid % Tl::kChunks) ^ Tl::swizzle(u)), s + r * kThreads * 16 + wave * 1024);
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) lds_dma16(src + (q_off + 256 * j), s + (r * kSegs<T> + wave + kWaves * j) * kBlock);
     }
     // Their states, and those of as many behind, which nothing reads.
     if (wave == 0)
@@ -623,41 +629,44 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) void paged_weigh_
     if (col + 64 < ncols) stage((it + 1) & 1, col + 64);
     const char* s = lds + (it & 1) * kSet;
     const float* const ml = reinterpret_cast<const float*>(s + 64 * Tl::kRow);
-    // Some of these columns may not see some of the wave's tokens.
-    const bool edge = t_wave + 16 * NC > base + over_group(a, col) + 1 || col + 64 > ncols;
-    float part[NC];
+    auto add = [&](auto edge_tag) {
+      constexpr bool EDGE = decltype(edge_tag)::value;
+      float part[NC];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) part[c] = 0.f;
+      for (int c = 0; c < NC; ++c) part[c] = 0.f;
 #pragma unroll
-    for (int qb = 0; qb < 4; ++qb) {
-      f32x4 acc[NC];
+      for (int qb = 0; qb < 4; ++qb) {
+        f32x4 acc[NC];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const vec8 qa = key_operand<T>(s + (qb >> 1) * Tl::kBytes, g4, n16, qb & 1, x);
+        for (int x = 0; x < 4; ++x) {
+          const vec8 qa = chunk_keys<T>(s, lane, qb, x);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) acc[c] = mma_16x16x32(qa, kop[c][x], acc[c]);
-      }
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(ml + 2 * (16 * qb + 4 * g4));
-      const f32x4 hi = *reinterpret_cast<const f32x4*>(ml + 2 * (16 * qb + 4 * g4) + 4);
-      const float top[4] = {lo[0], lo[2], hi[0], hi[2]}, inv[4] = {lo[1], lo[3], hi[1], hi[3]};
+          for (int c = 0; c < NC; ++c) acc[c] = mma_16x16x32(qa, kop[c][x], acc[c]);
+        }
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(ml + 2 * (16 * qb + 4 * g4));
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(ml + 2 * (16 * qb + 4 * g4) + 4);
+        const float top[4] = {lo[0], lo[2], hi[0], hi[2]}, inv[4] = {lo[1], lo[3], hi[1], hi[3]};
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (edge) {
+        for (int r = 0; r < 4; ++r) {
           const int u = col + 16 * qb + 4 * g4 + r;
-          const int lim = u < ncols ? base + over_group(a, u) + 1 : 0;
+          const int lim = !EDGE ? 0 : u < ncols ? base + over_group(a, u) + 1 : 0;
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
-            if (t_wave + 16 * c + n16 < lim) part[c] = fmaf(fast_exp2(fmaf(acc[c][r], a.scale_log2, -top[r])), inv[r], part[c]);
-        } else {
-#pragma unroll
-          for (int c = 0; c < NC; ++c) part[c] = fmaf(fast_exp2(fmaf(acc[c][r], a.scale_log2, -top[r])), inv[r], part[c]);
+          for (int c = 0; c < NC; ++c) {
+            const float e = fast_exp2(fmaf(acc[c][r], a.scale_log2, -top[r])), more = fmaf(e, inv[r], part[c]);
+            part[c] = !EDGE || t_wave + 16 * c + n16 < lim ? more : part[c];
+          }
         }
       }
-    }
 #pragma unroll
-    for (int c = 0; c < NC; ++c) sum[c] += part[c];
+      for (int c = 0; c < NC; ++c) sum[c] += part[c];
+    };
+    // Some of these columns may not see some of the wave's tokens.
+    if (t_wave + 16 * NC > base + over_group(a, col) + 1 || col + 64 > ncols)
+      add(std::true_type{});
+    else
+      add(std::false_type{});
   }
   const float* const in = a.weights + row * a.weight_stride;
   float* const outw = a.weights_out + row * a.weight_stride;
@@ -692,8 +701,10 @@ int launch_weigh(const PagedAttn& a, hipStream_t s) {
   });
   if (attr != hipSuccess) return set_error(HC_ERR_HIP, "hc_paged_attn: %s", hipGetErrorString(attr));
   const int block = kWaves * 16 * NC;
-  const int64_t grid = (int64_t)a.pool.rows * ((a.pool.capacity + block - 1) / block);
-  hipLaunchKernelGGL((paged_weigh_kernel<T, NC>), dim3((unsigned)grid), dim3(kThreads), weigh_lds<T>(), s, a);
+  const int blocks = (a.pool.capacity + block - 1) / block;
+  const int64_t grid = (int64_t)(a.pool.rows + 7) / 8 * 8 * blocks;
+  if (grid > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_paged_attn: weights of %d rows of %d tokens", a.pool.rows, a.pool.capacity);
+  hipLaunchKernelGGL((paged_weigh_kernel<T, NC>), dim3((unsigned)grid), dim3(kThreads), weigh_lds<T>(), s, a, blocks);
   return check_launch("hc_paged_attn(weights)");
 }
 

@@ -93,7 +93,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
       const int t0 = max(lo - first, 0), t1 = min(hi - first, ntiles);
       const int b = row / p.Hkv, h = row % p.Hkv;
       const int trow = table_row(p, row), hd = p.heads == 1 ? 0 : h;
-      const int nq = query_tokens(p.counts, b, p.Q);
+      const int nq = __builtin_amdgcn_readfirstlane(query_tokens(p.counts, b, p.Q));
       const int base = total_tok - nq;  // query i sees tokens below base + i + 1
       const int old = p.fresh ? base : total_tok;
       const int32_t* const tab = p.table + trow * p.table_stride;
