@@ -42,6 +42,7 @@ extern "C" int hc_read_status(int32_t* status, int clear, int32_t* value, void* 
       return hc::set_error(HC_ERR_HIP, "hc_read_status: %s", hipGetErrorString(hipGetLastError()));
   }
   if (word & 1) return hc::set_error(HC_ERR_CAPACITY, "a row was at capacity when a token was appended (status 0x%x)", word);
+  if (word & 2) return hc::set_error(HC_ERR_INVALID, "a row of a paged cache reached an entry of its table that names no page (status 0x%x)", word);
   return HC_OK;
 }
 

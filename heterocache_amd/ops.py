@@ -890,12 +890,12 @@ def _query_counts(counts, batch, dev):
     return host_counts("query_counts", host, dev)
 
 
-def host_counts(name, host, device):
+def host_counts(name, host, device, dtype=torch.int32):
     """Host integers on the device, but not into a graph, whose replays would
     copy from staging memory that has long been reused."""
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{name} on the host cannot be captured: pass an int32 device tensor")
-    return to_device(host, device, torch.int32)
+    return to_device(host, device, dtype)
 
 
 @_on_device

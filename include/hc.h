@@ -43,7 +43,8 @@ const char* hc_last_error(void);
  * Read the device status word that hc_append and hc_decode_attn raise when a
  * row is at capacity: waits for `stream`, stores the word in *value (optional),
  * zeroes it when `clear` is set, and returns HC_ERR_CAPACITY when bit 0 is
- * set (HC_OK otherwise).  The one call that synchronises the host; it exists
+ * set, HC_ERR_INVALID when bit 1 alone is (a row of a paged cache reached a
+ * table entry that names no page), HC_OK otherwise.  The one call that synchronises the host; it exists
  * so that launches replayed from a HIP graph, which no host check precedes,
  * still surface the reference's pool exhaustion ("Layer i OOM.",
  * heterocache/cache_utils.py:988-990) as a typed error.

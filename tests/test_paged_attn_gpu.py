@@ -116,3 +116,204 @@ def test_append_alone(dev):
                 assert int(c.pages.row_len[r]) == n + counts[b]
                 assert not c.pages.weights[b * 2 + h, n:n + counts[b]].any()
                 assert c.pages.pos[r, n:n + counts[b]].tolist() == [n + i + int(c.pages.dropped[r]) for i in range(counts[b])]
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, FL])
+@pytest.mark.parametrize("T,n", [(4, 60), (40, 100)])
+def test_values_that_are_no_numbers_reach_those_who_see_them(dev, dtype, T, n):
+    """An infinite or NaN key or value of a later token does not reach the queries before it."""
+    rng = np.random.default_rng(T)
+    for what in ("v", "k"):
+        for value in (float("inf"), float("-inf"), float("nan")):
+            c = Cache(rng, 1, 1, [n], 16, dtype, dev, room=T)
+            q, kn, vn = (queries(rng, 1, h, T, dtype, dev) for h in (4, 1, 1))
+            at = T // 2
+            (vn if what == "v" else kn)[0, 0, at, 5] = value
+            got = ops.paged_attn(q, c.pages, SCALE, kn, vn)
+            k, v = torch.cat([c.kv[0][0], kn[0, 0]]), torch.cat([c.kv[0][1], vn[0, 0]])
+            out, tol, _, _ = attend_causal(q[0, :, :at].transpose(0, 1), k[:n + at], v[:n + at], n, SCALE, dtype)
+            close(got[0, :at], out, tol, f"{what} {value}")
+            late = got[0, at:].float()
+            if what == "v":
+                assert (torch.isnan(late[..., 5]).all() if value != value else (late[..., 5] == value).all())
+                keep = [d for d in range(D) if d != 5]
+                assert torch.isfinite(late[..., keep]).all()
+            elif value != value:
+                assert torch.isnan(late).all()
+            else:
+                # The score is +-inf by the query's sign there: no softmax, or a token of no weight.
+                bad = q[0, :, at:, 5].transpose(0, 1).float() * value == float("inf")
+                assert torch.isnan(late[bad]).all() and torch.isfinite(late[~bad]).all()
+
+
+@pytest.mark.parametrize("T", [1, 30])
+def test_no_visible_number(dev, T):
+    """All scores -inf: NaN, and NaN weights; no token: zeros."""
+    rng = np.random.default_rng(3)
+    c = Cache(rng, 2, 1, [5, 0], 16, BF, dev, room=T, ledger=True)
+    q, kn, vn = (queries(rng, 2, h, T, BF, dev) for h in (4, 1, 1))
+    q[0].fill_(1.0)
+    kn[0].fill_(float("-inf"))
+    for t in range(5):
+        pg, sl = c.slots(0, [t])
+        c.k[pg, sl, 0] = float("-inf")
+    got = ops.paged_attn(q, c.pages, SCALE, kn, vn, weigh=True, counts=[T, 0])
+    assert torch.isnan(got[0]).all() and not got[1].any()
+    assert torch.isnan(c.pages.weights[0, :5]).all() and torch.isfinite(c.pages.weights[1]).all()
+
+
+def test_small_weights_behind_a_dominant_token(dev):
+    """fp16: a long flat tail e^-17 below one token counts in the product with V as it does in the sum."""
+    n = 6000
+    for T in (1, 20):
+        rng = np.random.default_rng(T)
+        c = Cache(rng, 1, 1, [n], 64, FP, dev, room=T)
+        q, kn, vn = (queries(rng, 1, h, T, FP, dev) for h in (2, 1, 1))
+        q.zero_(), kn.zero_()
+        q[..., 0] = 16.0
+        pg, sl = c.slots(0, np.arange(n))
+        c.k[:] = 0.0
+        c.k[pg[:1], sl[:1], 0, 0] = 12.0
+        c.v[pg, sl] = 1.0
+        vn.fill_(1.0)
+        c.v[pg[:1], sl[:1]] = 0.0
+        c.kv[0] = (c.k[pg, sl, 0], c.v[pg, sl, 0])
+        got = ops.paged_attn(q, c.pages, SCALE, kn, vn)
+        k, v = torch.cat([c.kv[0][0], kn[0, 0]]), torch.cat([c.kv[0][1], vn[0, 0]])
+        out, tol, _, _ = attend_causal(q[0].transpose(0, 1), k, v, n, SCALE, FP)
+        close(got[0], out, tol, f"{T} queries")
+
+
+def test_rows_without_room(dev):
+    """They keep what they hold, attend NaN, and set the status word; the others go on."""
+    rng = np.random.default_rng(6)
+    for T in (2, 40):
+        c = Cache(rng, 3, 2, [60, 64 - T, 63], 16, BF, dev, width=4, room=0, ledger=True, spare=12)
+        for r in range(3):  # every entry of the tables names a page
+            free = sorted(set(range(c.k.shape[0])) - set(c.table.reshape(-1).tolist()))
+            hole = np.nonzero(c.table[r] < 0)[0]
+            c.table[r, hole] = free[:len(hole)]
+        c.pages.table.copy_(torch.as_tensor(c.table))
+        k0, w0 = c.k.clone(), c.pages.weights.clone()
+        q, kn, vn = (queries(rng, 3, h, T, BF, dev) for h in (4, 2, 2))
+        got = ops.paged_attn(q, c.pages, SCALE, kn, vn, weigh=True)
+        full = [64 - T < n for n in (60, 64 - T, 63)]
+        assert c.pages.row_len.tolist() == [n + (0 if f else T) for n, f in zip((60, 64 - T, 63), full)]
+        for b in range(3):
+            assert torch.isnan(got[b]).all() == full[b]
+            if full[b]:
+                assert torch.equal(c.pages.weights[2 * b:2 * b + 2], w0[2 * b:2 * b + 2])
+                pg = torch.as_tensor(c.table[b].astype(np.int64)).to(dev)
+                a, z = c.k[pg], k0[pg]
+                assert torch.equal(torch.isnan(a), torch.isnan(z)) and torch.equal(a.nan_to_num(), z.nan_to_num())
+        with pytest.raises(_lib.HCError, match="capacity"):
+            ops.read_status(c.status)
+
+
+def test_bad_pages(dev):
+    """Entries outside of the pool are not followed: NaN for the rows that need them, and the status word."""
+    rng = np.random.default_rng(7)
+    for T, page in ((1, 16), (1, 24), (40, 16), (40, 24)):
+        for value in (-1, 1 << 30, -(1 << 31)):
+            c = Cache(rng, 2, 2, [100, 90], page, BF, dev, room=T, ledger=True)
+            c.pages.table[1, 2] = value
+            q, kn, vn = (queries(rng, 2, h, T, BF, dev) for h in (4, 2, 2))
+            got = ops.paged_attn(q, c.pages, SCALE, kn, vn)
+            assert torch.isfinite(got[0].float()).all() and torch.isnan(got[1]).all()
+            with pytest.raises(_lib.HCError, match="names no page"):
+                ops.read_status(c.status)
+            ops.paged_evict(c.pages, 20)
+            with pytest.raises(_lib.HCError, match="names no page"):
+                ops.read_status(c.status)
+            assert c.pages.row_len.tolist() == [20, 20]
+
+
+def test_offsets_past_32_bits(dev):
+    """Pools of more than 2^31 elements, read and written at their end."""
+    rng = np.random.default_rng(8)
+    page, heads = 64, 2
+    total = (1 << 31) // (page * heads * D) + 300
+    k, v = (torch.empty((total, page, heads, D), dtype=BF, device=dev) for _ in range(2))
+    ids = (total - 1 - rng.permutation(200)).astype(np.int32)
+    for T in (1, 40):
+        n = 500
+        table = torch.as_tensor(ids[:10].reshape(1, 10)).to(dev)
+        p = ops.Pages(k, v, table, torch.tensor([n], dtype=torch.int32, device=dev), heads)
+        rows = torch.as_tensor(ids[:10].astype(np.int64)).to(dev)
+        k[rows], v[rows] = (torch.as_tensor(rng.standard_normal((10, page, heads, D)), dtype=torch.float32).to(BF).to(dev)
+                            for _ in range(2))
+        q, kn, vn = (queries(rng, 1, h, T, BF, dev) for h in (8, 2, 2))
+        got = ops.paged_attn(q, p, SCALE, kn, vn)
+        for h in range(2):
+            kk, vv = (torch.cat([x[rows].reshape(-1, heads, D)[:n, h], y[0, h]]) for x, y in ((k, kn), (v, vn)))
+            out, tol, _, _ = attend_causal(q[0, 4 * h:4 * h + 4].transpose(0, 1), kk, vv, n, SCALE, BF)
+            close(got[0, :, 4 * h:4 * h + 4], out, tol, f"{T} queries head {h}")
+            assert torch.equal(k[rows].reshape(-1, heads, D)[n:n + T, h], kn[0, h])
+
+
+def test_layouts_outputs_and_lengths_apart(dev):
+    """Contiguous [B, H, T, 128] inputs, an output slice of a larger tensor, a table and a ledger that are slices, lengths
+    and weights written elsewhere."""
+    rng = np.random.default_rng(9)
+    for T in (1, 40):
+        c = Cache(rng, 2, 2, [70, 33], 16, BF, dev, room=T, ledger=True)
+        p = c.pages
+        wide = torch.full((2, p.table.shape[1] + 3), -1, dtype=torch.int32, device=dev)
+        wide[:, :p.table.shape[1]] = p.table
+        ledger = torch.zeros((4, p.capacity + 37), device=dev)
+        ledger[:, :p.capacity] = p.weights
+        p2 = ops.Pages(c.k, c.v, wide[:, :p.table.shape[1]], p.row_len, 2, weights=ledger[:, :p.capacity], pos=p.pos,
+                       dropped=p.dropped)
+        q, kn, vn = (queries(rng, 2, h, T, BF, dev).contiguous() for h in (8, 2, 2))
+        big = torch.full((2, T + 2, 8, D + 8), 7.0, dtype=BF, device=dev)
+        lens, weights = torch.zeros_like(p.row_len), torch.full((4, p.capacity + 37), -1.0, device=dev)[:, :p.capacity]
+        got = ops.paged_attn(q, p2, SCALE, kn, vn, out=big[:, 1:T + 1, :, :D], weigh=True, len_out=lens, weights_out=weights)
+        want = ops.paged_attn(q, p, SCALE, kn, vn, weigh=True)
+        assert torch.equal(got, want)
+        assert (big[:, 0] == 7).all() and (big[:, T + 1] == 7).all() and (big[..., D:] == 7).all()
+        assert lens.tolist() == p.row_len.tolist() == [70 + T, 33 + T]
+        for r, n in ((0, 70 + T), (1, 70 + T), (2, 33 + T), (3, 33 + T)):
+            assert torch.equal(weights[r, :n], p.weights[r, :n]) and (weights[r, n:] == -1).all()
+
+
+def test_repeats_bit_for_bit(dev):
+    rng = np.random.default_rng(10)
+    for T in (1, 60):
+        c = Cache(rng, 3, 2, [700, 20, 333], 16, BF, dev, room=T, ledger=True)
+        q, kn, vn = (queries(rng, 3, h, T, BF, dev) for h in (8, 2, 2))
+        runs = []
+        for _ in range(3):
+            w, lens = torch.zeros_like(c.pages.weights), torch.zeros_like(c.pages.row_len)
+            runs.append((ops.paged_attn(q, c.pages, SCALE, kn, vn, weigh=True, weights_out=w, len_out=lens), w, lens))
+        for x in runs[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(x, runs[0]))
+
+
+def test_python_refusals(dev):
+    rng = np.random.default_rng(11)
+    c = Cache(rng, 2, 2, [20], 16, BF, dev, room=4, ledger=True)
+    p = c.pages
+    q, kn, vn = (queries(rng, 2, h, 1, BF, dev) for h in (4, 2, 2))
+    bad = [
+        (TypeError, lambda: ops.paged_attn(q.half(), p, SCALE, kn, vn)), (TypeError, lambda: ops.paged_attn(q, p, SCALE, kn.half(), vn)),
+        (ValueError, lambda: ops.paged_attn(q, p, SCALE, kn)), (ValueError, lambda: ops.paged_attn(q[:1], p, SCALE, kn, vn)),
+        (ValueError, lambda: ops.paged_attn(q[:, :3], p, SCALE, kn, vn)), (ValueError, lambda: ops.paged_attn(q, p, SCALE, kn[:, :1], vn[:, :1])),
+        (ValueError, lambda: ops.paged_attn(q, p, SCALE, kn.expand(2, 2, 3, D), vn.expand(2, 2, 3, D))),
+        (ValueError, lambda: ops.paged_attn(q.cpu(), p, SCALE)), (ValueError, lambda: ops.paged_attn(q, p, SCALE, weights_out=p.weights)),
+        (ValueError, lambda: ops.paged_attn(q, p, SCALE, weigh=True, weights_out=p.weights[:, :5])),
+        (ValueError, lambda: ops.paged_attn(q, p, SCALE, kn, vn, counts=[1])), (ValueError, lambda: ops.paged_attn(q, p, SCALE, out=q)),
+        (ValueError, lambda: ops.paged_attn(q, p, SCALE, kn, vn, len_out=p.row_len.long())),
+        (_lib.HCError, lambda: ops.paged_attn(q, p, 0.0, kn, vn)), (_lib.HCError, lambda: ops.paged_attn(q, p, SCALE, len_out=p.row_len)),
+        (ValueError, lambda: ops.paged_append(kn, vn[..., :64], p)), (ValueError, lambda: ops.paged_evict(p, torch.ones(3, dtype=torch.int32, device=dev))),
+        (_lib.HCError, lambda: ops.paged_evict(p, 3, sink=2, recent=2)), (ValueError, lambda: ops.paged_evict(p, 8, pos_out=p.pos[:, :4])),
+        (ValueError, lambda: ops.Pages(c.k, c.v, p.table, p.row_len, 3)), (ValueError, lambda: ops.Pages(c.k, c.v, p.table.long(), p.row_len, 2)),
+        (ValueError, lambda: ops.Pages(c.k, c.v[:, :8], p.table, p.row_len, 2)), (ValueError, lambda: ops.Pages(c.k, c.v, p.table, p.row_len[:1], 2)),
+        (ValueError, lambda: ops.Pages(c.k, c.v, p.table, p.row_len, 2, weights=p.weights)),
+        (ValueError, lambda: ops.Pages(c.k, c.v, p.table, p.row_len, 2, weights=p.weights[:, :9], pos=p.pos, dropped=p.dropped)),
+        (ValueError, lambda: ops.Pages(c.k[:1].expand(9, -1, -1, -1), c.v[:1].expand(9, -1, -1, -1), p.table, p.row_len, 2)),
+        (TypeError, lambda: ops.Pages(c.k.double(), c.v.double(), p.table, p.row_len, 2)),
+    ]
+    for i, (kind, call) in enumerate(bad):
+        with pytest.raises(kind):
+            call()
+            pytest.fail(f"call {i} was not refused")
