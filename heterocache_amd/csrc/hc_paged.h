@@ -138,8 +138,7 @@ struct PagedAttn {
   int g_shift;
   bool stored;  // an append ahead of the launch has stored the new tokens
   float scale_log2;
-  int2* info;      // few columns, per row: its first tile among all rows', its tokens with the new ones (-1 - len: no room for them)
-  int32_t* share;  // tiles of a workgroup
+  int4* info;  // few columns, per row: first partial, how many, its tokens with the new ones (-1 - len: no room for them)
   float *part_o, *part_ml;  // partials: 128 channels; (m, l)
   int4* plan;               // many columns, per row: first partial, parts, tokens as above
   float *chunk_o, *chunk_ml;

@@ -65,7 +65,7 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 struct Layout {
   bool chunk;  // rows of many columns
   int cols, few, grid, chunk_grid, chunk_slots;
-  size_t info, share, part_o, part_ml, plan, chunk_o, chunk_ml, ml, scores, bytes;
+  size_t info, part_o, part_ml, plan, chunk_o, chunk_ml, ml, scores, bytes;
   int64_t score_stride, ml_stride;
 };
 
@@ -85,8 +85,7 @@ Layout layout(const hc_paged_cache* c, int q_heads, int queries, bool counts, bo
   if (l.few) {
     l.grid = paged_rows_slots(c->dtype);
     const size_t slots = (size_t)l.grid + rows;
-    l.info = take((size_t)rows * 8);
-    l.share = take(4);
+    l.info = take((size_t)rows * sizeof(int4));
     l.part_o = take(slots * l.few * HC_HEAD_DIM * 4);
     l.part_ml = take(slots * l.few * 8);
     if (weigh) {
@@ -200,8 +199,7 @@ extern "C" int hc_paged_attn(const hc_paged_cache* c, const void* q, const int64
   a.G = q_heads / c->kv_heads, a.cols = l.cols, a.few = l.few;
   divider(a.G, a.g_mul, a.g_shift);
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.info = reinterpret_cast<int2*>(ws + l.info);
-  a.share = reinterpret_cast<int32_t*>(ws + l.share);
+  a.info = reinterpret_cast<int4*>(ws + l.info);
   a.part_o = reinterpret_cast<float*>(ws + l.part_o);
   a.part_ml = reinterpret_cast<float*>(ws + l.part_ml);
   a.plan = reinterpret_cast<int4*>(ws + l.plan);

@@ -66,31 +66,44 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
     if (r0 >= p.rows) break;
     load_rows(r0);
   }
-  // A whole number of tiles a wave.
-  const int share = max((total + a.grid - 1) / a.grid + kWaves - 1, kWaves) / kWaves * kWaves;
+  // Equal runs of all tiles, which may cross rows, or every row cut for itself:
+  // the latter leaves workgroups idle where lengths differ, but a run that
+  // crosses pays for a row's start and end again, about kCross rounds of a tile
+  // a wave.  Whichever has fewer rounds (64 rows of 66 tiles with weights: 30.0
+  // us in crossing runs, now 23.5).
+  constexpr int kCross = 3;
+  const int crossing = (total + a.grid - 1) / a.grid;
+  const int apart = 2 * p.rows <= a.grid ? (total + a.grid - p.rows - 1) / (a.grid - p.rows) : 1 << 30;
+  const bool cut = (apart + kWaves - 1) / kWaves <= (crossing + kWaves - 1) / kWaves + kCross;
+  // (A whole number of tiles a wave.)
+  const int share = cut ? max(apart, kWaves) : max(crossing + kWaves - 1, kWaves) / kWaves * kWaves;
   const int x = blockIdx.x;
   const int64_t lo64 = (int64_t)x * share;
   const int lo = (int)min(lo64, (int64_t)total), hi = (int)min(lo64 + share, (int64_t)total);
-  if (x == 0 && threadIdx.x == 0) *a.share = share;
-  if (lo >= hi && x != 0) return;
+  if (!cut && lo >= hi && x != 0) return;
 
-  int before = 0;  // tiles of the rows ahead of r0
+  int before = 0;  // of the rows ahead of r0: tiles, or parts
   for (int r0 = 0; r0 < p.rows; r0 += 64) {
     if (p.rows > 64) load_rows(r0);
-    const int incl = wave_scan_add(nt) + before, excl = incl - nt;
+    const int parts = cut ? (nt + share - 1) / share : nt;
+    const int incl = wave_scan_add(parts) + before, excl = incl - parts;
     before = __builtin_amdgcn_readlane(incl, 63);
     if (x == 0 && wave == 0 && r0 + lane < p.rows) {
-      a.info[r0 + lane] = make_int2(excl, row_e);
+      // The row's first partial, how many, its tokens.
+      const int w0 = excl / share, segs = parts == 0 ? 0 : cut ? parts : (incl - 1) / share - w0 + 1;
+      a.info[r0 + lane] = make_int4(cut ? excl : w0 + r0 + lane, segs, row_e, 0);
       if (row_e < 0 && p.status) atomicOr(p.status, kStatusCapacity);
     }
-    uint64_t mine = __ballot(nt > 0 && excl < hi && incl > lo);
+    uint64_t mine = __ballot(parts > 0 && (cut ? excl <= x && incl > x : excl < hi && incl > lo));
     while (mine) {
       const int src = __builtin_ctzll(mine);
       mine &= mine - 1;
       const int row = r0 + src;
       const int first = __builtin_amdgcn_readlane(excl, src), ntiles = __builtin_amdgcn_readlane(nt, src);
       const int total_tok = __builtin_amdgcn_readlane(row_e, src);
-      const int t0 = max(lo - first, 0), t1 = min(hi - first, ntiles);
+      const int np = __builtin_amdgcn_readlane(parts, src);
+      const int t0 = cut ? (int)((int64_t)ntiles * (x - first) / np) : max(lo - first, 0);
+      const int t1 = cut ? (int)((int64_t)ntiles * (x - first + 1) / np) : min(hi - first, ntiles);
       const int b = row / p.Hkv, h = row % p.Hkv;
       const int trow = table_row(p, row), hd = p.heads == 1 ? 0 : h;
       const int nq = __builtin_amdgcn_readfirstlane(query_tokens(p.counts, b, p.Q));
@@ -280,7 +293,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) *reinterpret_cast<f32x4*>(&s_o[wave][n][16 * mt + 4 * g]) = o[mt];
       __syncthreads();
-      const int64_t slot = (int64_t)(x + row) * a.few;
+      const int64_t slot = (int64_t)(cut ? x : x + row) * a.few;
       for (int c = threadIdx.x >> 5; c < nq * a.G; c += kThreads / 32) {
         const int d0 = 4 * (threadIdx.x & 31);
         float M = s_ml[0][c][0], L = 0.f;
@@ -298,7 +311,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
       }
       __syncthreads();  // the next row's copies take the buffer
     }
-    if (before >= hi && x != 0) break;
+    if ((cut ? before > x : before >= hi) && x != 0) break;
   }
 }
 
@@ -310,25 +323,23 @@ constexpr int kWeighTokens = 1024;
 template <typename T, bool WEIGH>
 __global__ __launch_bounds__(256) void paged_fold_kernel(const PagedAttn a, int runs) {
   const Pool& p = a.pool;
-  const int share = *a.share;
   int x = blockIdx.x;
   const int columns = p.rows * a.few;
   const bool weigh = WEIGH && x >= columns;
   const int row = weigh ? (x - columns) % p.rows : x / a.few;
-  const int2 info = a.info[row];
-  const bool room = info.y >= 0;
-  const int b = row / p.Hkv, h = row % p.Hkv, total = room ? info.y : -1 - info.y;
+  const int4 info = a.info[row];
+  const bool room = info.z >= 0;
+  const int b = row / p.Hkv, h = row % p.Hkv, total = room ? info.z : -1 - info.z;
   const int nq = query_tokens(p.counts, b, p.Q), ncols = room ? nq * a.G : 0;
   if (nq * a.G > kFewCols) return;
-  const int nt = room && nq > 0 ? tiles_of(total) : 0;
-  const int first = info.x / share, segs = nt > 0 ? (info.x + nt - 1) / share - first + 1 : 0;
-  const float* const ml = a.part_ml + (int64_t)(first + row) * a.few * 2;  // [segment][column]
+  const int segs = info.y;
+  const float* const ml = a.part_ml + (int64_t)info.x * a.few * 2;  // [segment][column]
   if (!weigh) {
     __shared__ float s_m[8], s_l[8];
     __shared__ f32x4 s_o[8][32];
     const int c = x % a.few;
     const int grp = threadIdx.x >> 5, d0 = 4 * (threadIdx.x & 31);
-    const float* const po = a.part_o + ((int64_t)(first + row) * a.few + c) * HC_HEAD_DIM + d0;
+    const float* const po = a.part_o + ((int64_t)info.x * a.few + c) * HC_HEAD_DIM + d0;
     float m = -INFINITY, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     if (c < ncols) {
