@@ -89,8 +89,8 @@ Layout layout(const hc_paged_cache* c, int q_heads, int queries, bool counts, bo
     l.part_o = take(slots * l.few * HC_HEAD_DIM * 4);
     l.part_ml = take(slots * l.few * 8);
     if (weigh) {
-      l.score_stride = (cap + HC_TILE - 1) / HC_TILE * HC_TILE;
-      l.scores = take((size_t)rows * l.few * l.score_stride * 4);
+      l.score_stride = (cap + HC_TILE - 1) / HC_TILE * HC_TILE * l.few;
+      l.scores = take((size_t)rows * l.score_stride * 4);
     }
   }
   if (l.chunk) {

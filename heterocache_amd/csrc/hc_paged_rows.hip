@@ -260,7 +260,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void paged_rows_k
         }
         // (Ahead of the copies, whose wait then finds the stores done.)
         if (WEIGH && col_ok) {
-          float* sp = a.scores + ((int64_t)row * a.few + n) * a.score_stride + tok0 + 4 * g;
+          // [row][tile][column][32]
+          float* sp = a.scores + row * a.score_stride + ((int64_t)tile * a.few + n) * HC_TILE + 4 * g;
           *reinterpret_cast<f32x4*>(sp) = s[0] * a.scale_log2;
           *reinterpret_cast<f32x4*>(sp + 16) = s[1] * a.scale_log2;
         }
@@ -412,10 +413,10 @@ __global__ __launch_bounds__(256) void paged_fold_kernel(const PagedAttn a, int 
       const int t = t0 + 4 * threadIdx.x;
       if (t >= total) break;
       f32x4 w = {0.f, 0.f, 0.f, 0.f};
-      const float* sp = a.scores + (int64_t)row * a.few * a.score_stride + t;
+      const float* sp = a.scores + row * a.score_stride + (int64_t)(t / HC_TILE) * a.few * HC_TILE + t % HC_TILE;
 #pragma unroll 4
       for (int u = 0; u < ncols; ++u) {
-        const f32x4 s = *reinterpret_cast<const f32x4*>(sp + u * a.score_stride);
+        const f32x4 s = *reinterpret_cast<const f32x4*>(sp + u * HC_TILE);
         const float top = s_top[u], inv = s_inv[u];
         const int lim = base + 1 + u / a.G;
 #pragma unroll
