@@ -51,6 +51,12 @@ __device__ __forceinline__ RowSpan row_span(const Pool& p, int row) {
   return s;
 }
 
+// Workgroups a row that add up the weights of few columns, and a launch's that folds many.
+inline int paged_weigh_runs(const Pool& p) {
+  const int most = 2048 / p.rows, runs = (p.capacity + 1023) / 1024;
+  return runs < most ? runs : most > 1 ? most : 1;
+}
+
 // Whether 16 tokens from a multiple of 16 lie in one page, at offsets below 2^31.
 inline bool uniform_pages(const Pool& p) {
   const int64_t far = (int64_t)1 << 31;
@@ -121,6 +127,8 @@ struct PagedNew {  // the new keys and values [batch][Hkv][Q][128]: byte strides
   int64_t k_s[3], v_s[3];
 };
 
+constexpr int kPagedWaves = 4, kPagedThreads = 64 * kPagedWaves;
+
 // Rows of at most this many (query, head) columns are paged_rows_kernel's, the
 // others paged_chunk_kernel's; a padded batch may hold both.
 constexpr int kFewCols = 16;
@@ -136,7 +144,6 @@ struct PagedAttn {
   int G, cols, few;  // query heads of a KV head; columns of a row, (query, head) pairs i * G + g; and of one of few
   uint32_t g_mul;    // c / G = (c * g_mul) >> g_shift
   int g_shift;
-  bool stored;  // an append ahead of the launch has stored the new tokens
   float scale_log2;
   int4* info;  // few columns, per row: first partial, how many, its tokens with the new ones (-1 - len: no room for them)
   float *part_o, *part_ml;  // partials: 128 channels; (m, l)
@@ -162,9 +169,17 @@ __device__ __forceinline__ int over_group(const PagedAttn& a, int c) {
   return (int)(((uint64_t)(uint32_t)c * a.g_mul) >> a.g_shift);
 }
 
-int launch_paged_rows(int dtype, const PagedAttn& a, hipStream_t s);
-int launch_paged_chunk(int dtype, const PagedAttn& a, hipStream_t s);
+inline unsigned paged_chunk_fold_grid(const PagedAttn& a) {
+  const int64_t work = ((int64_t)a.pool.rows * a.cols + 7) / 8, least = (a.pool.rows + 255) / 256;
+  return (unsigned)(work < least ? least : work < 8192 ? work : 8192);
+}
+
+// fold: the launch that folds the partials too.
+int launch_paged_rows(int dtype, const PagedAttn& a, bool fold, hipStream_t s);
+int launch_paged_chunk(int dtype, const PagedAttn& a, bool fold, hipStream_t s);
 int launch_paged_append(int dtype, const PagedAttn& a, hipStream_t s);
+int launch_paged_mixed(int dtype, const PagedAttn& a, hipStream_t s);
+int launch_paged_weights(int dtype, const PagedAttn& a, hipStream_t s);
 int paged_rows_slots(int dtype);
 int paged_chunk_slots(int dtype);
 

@@ -219,14 +219,17 @@ extern "C" int hc_paged_attn(const hc_paged_cache* c, const void* q, const int64
   int32_t* const lens = fresh ? (len_out ? len_out : c->row_len) : nullptr;
   if (!l.chunk) {
     a.len_out = lens;
-    return launch_paged_rows(c->dtype, a, s);
+    return launch_paged_rows(c->dtype, a, true, s);
   }
   // The lengths advance in the last launch that knows the old ones.
-  if (fresh)
-    if (int rc = launch_paged_append(c->dtype, a, s)) return rc;
-  a.stored = true;
-  if (l.few)
-    if (int rc = launch_paged_rows(c->dtype, a, s)) return rc;
-  a.len_out = lens;
-  return launch_paged_chunk(c->dtype, a, s);
+  int rc;
+  if (l.few) {
+    a.len_out = lens;
+    rc = launch_paged_mixed(c->dtype, a, s);
+  } else {
+    if (fresh && (rc = launch_paged_append(c->dtype, a, s))) return rc;
+    a.len_out = lens;
+    rc = launch_paged_chunk(c->dtype, a, true, s);
+  }
+  return rc || !weigh ? rc : launch_paged_weights(c->dtype, a, s);
 }
