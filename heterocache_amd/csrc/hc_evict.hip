@@ -435,14 +435,22 @@ __global__ __launch_bounds__(kRunThreads) void evict_list_kernel(const EvictArgs
     eqs[i] = __ballot(t < n && keep > 0 && k[i] == st.least);
     if (lane == 0) s_part[0][i * kW + wave] = __popcll(eqs[i]);
   }
+  // (Counts of 64 slots, in slot order, to what lies before them.)
+  static_assert(kRunPer * kW <= 64, "one scan");
+  auto prefix = [&](int* c) {
+    const int v = lane < kRunPer * kW ? c[lane] : 0;
+    const int incl = wave_scan_add(v);
+    if (lane < kRunPer * kW) c[lane] = incl - v;
+  };
+  __syncthreads();
+  if (wave == 0) prefix(s_part[0]);
   __syncthreads();
   const uint64_t below = (1ull << lane) - 1;
   uint64_t freed[kRunPer], moved[kRunPer];
 #pragma unroll
   for (int i = 0; i < kRunPer; ++i) {
     const int t = run * kRun + i * kRunThreads + tid;
-    int rank = eq_before + __popcll(eqs[i] & below);
-    for (int u = 0; u < i * kW + wave; ++u) rank += s_part[0][u];
+    const int rank = eq_before + s_part[0][i * kW + wave] + __popcll(eqs[i] & below);
     const bool kept = t < n && keep > 0 && (k[i] > st.least || (k[i] == st.least && rank < st.equal));
     freed[i] = __ballot(t < keep && t < n && !kept);
     moved[i] = __ballot(t >= keep && kept);
@@ -452,13 +460,13 @@ __global__ __launch_bounds__(kRunThreads) void evict_list_kernel(const EvictArgs
     }
   }
   __syncthreads();
+  if (wave < 2) prefix(s_part[1 + wave]);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < kRunPer; ++i) {
     const int t = run * kRun + i * kRunThreads + tid;
-    int f = free_before, m = free_all + move_before;
-    for (int u = 0; u < i * kW + wave; ++u) f += s_part[1][u], m += s_part[2][u];
-    if (freed[i] >> lane & 1) list[f + __popcll(freed[i] & below)] = t;
-    if (moved[i] >> lane & 1) list[m + __popcll(moved[i] & below)] = t;
+    if (freed[i] >> lane & 1) list[free_before + s_part[1][i * kW + wave] + __popcll(freed[i] & below)] = t;
+    if (moved[i] >> lane & 1) list[free_all + move_before + s_part[2][i * kW + wave] + __popcll(moved[i] & below)] = t;
   }
 }
 
