@@ -154,6 +154,10 @@ extern "C" int hc_paged_append(const hc_paged_cache* c, const void* k, const int
   if (int rc = fill_pool("hc_paged_append", c, a.pool, tokens, counts)) return rc;
   if (tokens < 0) return set_error(HC_ERR_INVALID, "hc_paged_append: tokens=%d", tokens);
   if (c->batch == 0 || (tokens == 0 && !len_out)) return HC_OK;
+  const intptr_t gap = 4 * (intptr_t)(a.pool.rows / c->heads);
+  const intptr_t apart = reinterpret_cast<intptr_t>(len_out) - reinterpret_cast<intptr_t>(c->row_len);
+  if (len_out && apart != 0 && apart > -gap && apart < gap)
+    return set_error(HC_ERR_INVALID, "hc_paged_append: len_out overlaps row_len without being it");
   if (tokens > 0)
     if (int rc = check_fresh("hc_paged_append", c, k, k_strides, v, v_strides, a.fresh)) return rc;
   if ((int64_t)a.pool.rows * ((tokens + 15) / 16) > 0x7fffffffLL)

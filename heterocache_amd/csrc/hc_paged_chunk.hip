@@ -29,7 +29,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAttn a, in
 //
 // from the columns' folded (M, L): the scores are formed again, tokens as the
 // columns of the matrix product (their operands stay in registers), queries
-// streamed through LDS 64 at a time, so a token's sum stays in its lane.
+// streamed through LDS 64 at a time, so a token's sum stays in its lane and no
+// atomics are needed.  Per score one matrix element, a fused multiply-add, an
+// exponential and an addition: bound by the vector units (4 sequences of up to 509
+// tokens over 8003, 216 M scores of 4 heads: 85 us, 44 of them vector work).
 template <typename T>
 constexpr int weigh_lds() {
   return 2 * (64 * Tile<T>::kRow + 1024);
@@ -45,7 +48,7 @@ __global__ __launch_bounds__(kPagedThreads, sizeof(T) == 4 ? 2 : NC == 4 ? 3 : 4
   const int g4 = lane >> 4, n16 = lane & 15;
   // Rows r, r + 8, .. on one XCD, the blocks of a row behind each other: workgroups
   // are dealt in turn to the XCDs and within one to its four engines, where rows
-  // of a sequence each would all meet (4 ragged sequences: 160 us, now 82).
+  // of a sequence each would all meet (4 ragged sequences: 162 us, now 85).
   const int row = blockIdx.x % 8 + 8 * (blockIdx.x / 8 / blocks), tb = blockIdx.x / 8 % blocks;
   if (row >= p.rows) return;
   const int b = row / p.Hkv, h = row % p.Hkv;

@@ -7,7 +7,7 @@
 // turn would meet on some of the XCDs and engines, to which workgroups are dealt
 // in turn as well).  Otherwise a launch each: the one kernel's registers and LDS
 // leave the chunks fewer waves (4 ragged sequences of up to 509 tokens: 201
-// against 165 us; 5 sequences of up to 18 tokens behind 889: 34 against 50).
+// against 165 us; 5 sequences of up to 18 tokens behind 889: 36 against 50).
 // Then one launch that folds both.
 #include <algorithm>
 #include <mutex>

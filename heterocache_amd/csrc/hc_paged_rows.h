@@ -14,7 +14,9 @@
 // registers and requests the next tile before it attends.  Where page sizes are
 // multiples of 16, a copy's tokens lie in one page and its address is scalar;
 // other sizes, and the tiles that reach behind the stored tokens, take an
-// address a token.
+// address a token.  Measured: 745 MB of a ragged fp16 batch in 122 us, 6.1 TB/s;
+// 17 MB in 10.6 us, of which some 9 are the chain of cold reads (lengths, table,
+// tiles), the launch and the end.
 #pragma once
 #include "hc_paged.h"
 
@@ -65,7 +67,7 @@ __device__ __forceinline__ void paged_rows_job(const PagedAttn& a, const int x, 
   // the latter leaves workgroups idle where lengths differ, but a run that
   // crosses pays for a row's start and end again, about kCross rounds of a tile
   // a wave.  Whichever has fewer rounds (64 rows of 66 tiles with weights: 30.0
-  // us in crossing runs, now 23.5).
+  // us in crossing runs, now 26.2).
   constexpr int kCross = 3;
   const int crossing = (total + a.grid - 1) / a.grid;
   const int apart = 2 * p.rows <= a.grid ? (total + a.grid - p.rows - 1) / (a.grid - p.rows) : 1 << 30;

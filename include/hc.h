@@ -729,7 +729,8 @@ int hc_paged_append(const hc_paged_cache* c, const void* k, const int64_t* k_str
  * a visible score is NaN or all are -inf.
  * weigh: weights_out[r][t] = weights[r][t] + the sum over the row's queries and
  * query heads of their probabilities of token t, for every token of the row; a
- * token appended by this call starts at zero.  weights_out NULL: in place.
+ * token appended by this call starts at zero.  weights_out NULL: in place; else
+ * memory that shares nothing with the old.
  * q, out: element strides batch, head, token, all of whole 16 bytes; out shares
  * no memory with q.  Stands where the reference calls flash attention over its
  * pools (heterocache/llama_model.py:382-389), for one new token or many.
@@ -756,7 +757,8 @@ size_t hc_paged_workspace_size(const hc_paged_cache* c, int q_heads, int queries
  * positions.  The row's length becomes min(n, keep), its dropped count grows by
  * the rest.  A row whose pages others share must not be evicted from.
  * len_out, weights_out, pos_out, dropped_out: NULL for in place; else the new
- * values, the old staying as they are (keys and values move in place).  scratch:
+ * values in memory of their own, the old staying as they are (keys and values
+ * move in place).  scratch:
  * hc_paged_evict_scratch_size bytes, 16-byte aligned, no initialisation.
  */
 int hc_paged_evict(const hc_paged_cache* c, const int32_t* keep, int keep_all, int sink, int recent, int32_t* len_out,

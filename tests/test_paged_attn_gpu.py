@@ -317,3 +317,85 @@ def test_python_refusals(dev):
         with pytest.raises(kind):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, FL])
+@pytest.mark.parametrize("page,apart,order", [(16, False, "token"), (5, True, "head"), (24, False, "head")])
+@pytest.mark.parametrize("fresh", [True, False])
+def test_padded_batches_of_other_pages_and_types(dev, dtype, page, apart, order, fresh):
+    rng = np.random.default_rng(page)
+    c = Cache(rng, 4, 2, [70, 3, 0, 210], page, dtype, dev, apart=apart, order=order, room=40, ledger=True)
+    _step(rng, c, 4, 40, dtype, dev, counts=[1, 40, 17, 4], fresh=fresh, weigh=True)
+
+
+@pytest.mark.parametrize("weigh", [False, True])
+@pytest.mark.parametrize("page,fresh", [(64, True), (64, False), (20, True)])
+def test_padded_batches_over_long_rows(dev, page, fresh, weigh):
+    """Chunks with much to do, which are launched apart from the single tokens."""
+    rng = np.random.default_rng(page)
+    c = Cache(rng, 4, 2, [20000, 30, 0, 7001], page, BF, dev, room=70, ledger=weigh)
+    _step(rng, c, 4, 70, BF, dev, counts=[70, 1, 9, 1], fresh=fresh, weigh=weigh)
+
+
+@pytest.mark.parametrize("counts", [None, "some"])
+@pytest.mark.parametrize("T,G", [(2, 8), (9, 3), (40, 4), (3, 24)])
+def test_more_rows_than_a_wave_scans_at_once(dev, T, G, counts):
+    rng = np.random.default_rng(T)
+    B = 45
+    c = Cache(rng, B, 2, [0, 40, 3, 17, 90], 16, BF, dev, room=T, ledger=True)
+    some = None if counts is None else [int(x) for x in rng.integers(0, T + 1, B)]
+    _step(rng, c, G, T, BF, dev, counts=some, weigh=True)
+
+
+def test_a_long_row_beside_short_ones(dev):
+    """One row's keys are cut although there are blocks enough."""
+    rng = np.random.default_rng(12)
+    c = Cache(rng, 40, 1, [30] * 39 + [30000], 64, BF, dev, room=150)
+    _step(rng, c, 8, 150, BF, dev, counts=[150] * 40)
+
+
+def test_thousands_of_rows(dev):
+    rng = np.random.default_rng(13)
+    c = Cache(rng, 700, 4, [5, 33, 0], 16, BF, dev, room=2, apart=True, ledger=True)
+    _step(rng, c, 2, 1, BF, dev, weigh=True)
+    _step(rng, c, 2, 1, BF, dev, counts=[b % 2 for b in range(700)])
+
+
+@pytest.mark.parametrize("T", [1, 30])
+def test_rows_that_share_pages(dev, T):
+    """A prefix whose whole pages stand in every sequence's table, each with pages of its own behind it."""
+    rng = np.random.default_rng(T)
+    c = Cache(rng, 3, 2, [64], 16, BF, dev, room=T, spare=9)
+    for b in (1, 2):
+        c.pages.table[b, :4] = c.pages.table[0, :4]
+        c.table[b, :4] = c.table[0, :4]
+        for h in range(2):
+            c.kv[b * 2 + h] = c.kv[h]
+    _step(rng, c, 4, T, BF, dev)
+
+
+@pytest.mark.parametrize("n,T", [(100, 9), (20000, 40)])
+def test_padded_batches_captured(dev, n, T):
+    """A padded chunk with weights, captured once: three replays beside eager calls on a twin, with other counts each."""
+    caches = [Cache(np.random.default_rng(1), 3, 2, [n, 5, 60], 16, BF, dev, room=3 * T, ledger=True) for _ in range(2)]
+    rng = np.random.default_rng(2)
+    new = lambda: [queries(rng, 3, h, T, BF, dev) for h in (8, 2, 2)]
+    static, counts = new(), torch.zeros(3, dtype=torch.int32, device=dev)
+    ops.paged_attn(static[0], caches[0].pages, SCALE, *static[1:], counts=counts, weigh=True)  # nothing is appended
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = ops.paged_attn(static[0], caches[0].pages, SCALE, *static[1:], counts=counts, weigh=True)
+    for some in ([T, 1, 0], [2, T, T], [T, 0, 3]):
+        args = new()
+        counts.copy_(torch.tensor(some, dtype=torch.int32))
+        for x, y in zip(static, args):
+            x.copy_(y)
+        graph.replay()
+        want = ops.paged_attn(args[0], caches[1].pages, SCALE, *args[1:], counts=some, weigh=True)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and caches[0].pages.row_len.tolist() == caches[1].pages.row_len.tolist()
+        for r, m in enumerate(caches[1].pages.row_len.tolist()):
+            assert torch.equal(caches[0].pages.weights[2 * r:2 * r + 2, :m], caches[1].pages.weights[2 * r:2 * r + 2, :m])
+            assert torch.equal(caches[0].pages.pos[r, :m], caches[1].pages.pos[r, :m])

@@ -91,3 +91,28 @@ def test_ties_infinities_and_nan(dev):
     c = Cache(rng, 1, 4, [500], 16, BF, dev, apart=False, ledger=True)
     c.pages.weights.copy_(torch.as_tensor(rng.choice([0.25, 0.5, 2.0 ** -30], c.pages.weights.shape), dtype=torch.float32))
     _evict(c, 333, 0, 16)
+
+
+@pytest.mark.parametrize("apart", [True, False])
+def test_long_tables(dev, apart):
+    """Tables of more than 16384 tokens: short rows among long ones, sums over heads, every weight equal, nothing kept."""
+    rng = np.random.default_rng(3)
+    heads = 2
+    lens = [20000, 500, 17001, 0] if apart else [18000, 40]
+    c = Cache(rng, 2, heads, lens, 64, BF, dev, apart=apart, ledger=True)
+    keep = [15000, 1000, 0, 7] if apart else [900, 39]
+    _evict(c, keep, 0, 0, apart_outputs=True)
+    _evict(c, keep, 0, 0)
+    for value in (0.0, 3.5):
+        c = Cache(rng, 1, heads, [18000], 256, FP, dev, apart=apart, ledger=True)
+        c.pages.weights.fill_(value)
+        _evict(c, 7000, 4, 300)
+        _evict(c, 6999, 4, 300)
+    c = Cache(rng, 1, heads, [50], 64, FP, dev, apart=apart, ledger=True, width=400)  # little in a large table
+    _evict(c, 33, 2, 9)
+
+
+def test_many_rows(dev):
+    rng = np.random.default_rng(4)
+    c = Cache(rng, 700, 4, [20, 33, 7], 16, BF, dev, apart=True, ledger=True)
+    _evict(c, 16, 1, 4)

@@ -94,6 +94,8 @@ def test_append(lib):
     _refused(lib, _append(lib, c, vs=None), b"null")
     _refused(lib, _append(lib, c, ks=_s(256, 128, 260)), b"strides")
     _refused(lib, _append(lib, c, v=FAKE + 2), b"aligned")
+    _refused(lib, _append(lib, c, lo=FAKE + 4), b"overlaps")
+    _refused(lib, _append(lib, c, lo=FAKE - 12), b"overlaps")
     _refused(lib, _append(lib, _cache(batch=1 << 20, table_pages=1, table_stride=1), t=1 << 20), b"rows x")
     assert _append(lib, _cache(batch=0)) == 0 and _append(lib, c, t=0, lo=None) == 0
 
