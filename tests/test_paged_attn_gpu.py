@@ -399,3 +399,21 @@ def test_padded_batches_captured(dev, n, T):
         for r, m in enumerate(caches[1].pages.row_len.tolist()):
             assert torch.equal(caches[0].pages.weights[2 * r:2 * r + 2, :m], caches[1].pages.weights[2 * r:2 * r + 2, :m])
             assert torch.equal(caches[0].pages.pos[r, :m], caches[1].pages.pos[r, :m])
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, FL])
+@pytest.mark.parametrize("T", [1, 20])
+def test_infinite_values_that_all_queries_see(dev, dtype, T):
+    """An infinite value of an earlier token is the output's channel; the others are as without it."""
+    rng = np.random.default_rng(T)
+    c = Cache(rng, 1, 1, [300], 16, dtype, dev, room=T)
+    pg, sl = c.slots(0, [100, 170])
+    c.v[pg[0], sl[0], 0, 3], c.v[pg[1], sl[1], 0, 9] = float("inf"), float("-inf")
+    q, kn, vn = (queries(rng, 1, h, T, dtype, dev) for h in (4, 1, 1))
+    got = ops.paged_attn(q, c.pages, SCALE, kn, vn)[0]
+    k, v = torch.cat([c.kv[0][0], kn[0, 0]]), torch.cat([c.kv[0][1], vn[0, 0]]).clone()
+    v[100, 3] = v[170, 9] = 0.0
+    out, tol, _, _ = attend_causal(q[0].transpose(0, 1), k, v, 300, SCALE, dtype)
+    assert (got[..., 3] == float("inf")).all() and (got[..., 9] == float("-inf")).all()
+    rest = [d for d in range(D) if d not in (3, 9)]
+    close(got[..., rest], out[..., rest], tol[..., rest], "the other channels")
