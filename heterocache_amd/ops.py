@@ -1247,7 +1247,7 @@ class Pages:
             table_stride=table.stride(0) if rows > 1 else entries, row_len=row_len.data_ptr(), weights=_ptr(weights),
             weight_stride=wide(weights), pos=_ptr(pos), pos_stride=wide(pos), dropped=_ptr(dropped), status=_ptr(status))
         self.ref = ctypes.addressof(self.struct)
-        self._sizes = {}
+        self._layouts, self._sizes = {}, {}
 
     def _ledger(self, name, t, dtype, rows, like=None):
         if (t.dim() != 2 or t.dtype is not dtype or t.get_device() != self.dev or t.shape[0] != rows
@@ -1305,37 +1305,61 @@ def paged_attn(q, pages, scale, k_new=None, v_new=None, counts=None, weigh=False
     integers.  weigh: every token's share of the attention is added to the
     cache's weights.  out: not q's memory; len_out, weights_out: receive the new
     lengths and weights (default: in place)."""
-    dt, dev = q.dtype, q.get_device()
-    shape = _queries(q)
-    B, Hq, T, _ = shape
-    if dt is not pages.dtype:
-        raise TypeError(f"q is {dt}, the pools {pages.dtype}: they must share a dtype")
-    if dev != pages.dev:
-        raise ValueError(f"q on {q.device} for pools on {pages.device}")
-    if B != pages.batch or Hq == 0 or Hq % pages.kv_heads:
-        raise ValueError(f"queries {tuple(shape)} for {pages.batch} sequences of {pages.kv_heads} KV heads")
-    if (k_new is None) != (v_new is None):
+    dev, fresh = pages.dev, k_new is not None
+    if fresh != (v_new is not None):
         raise ValueError("new keys and values come together")
-    kp = ks = vp = vs = None
-    if k_new is not None:
-        _new_tokens(pages, k_new, v_new, "new keys and values")
-        if k_new.shape[2] != T:
-            raise ValueError(f"{k_new.shape[2]} new tokens for {T} queries")
-        kp, ks, vp, vs = (k_new.data_ptr(), _strides3((k_new.shape, k_new.stride())), v_new.data_ptr(),
-                          _strides3((v_new.shape, v_new.stride())))
-    counts = _query_counts(counts, B, dev)
+    if q.dtype is not pages.dtype or fresh and (k_new.dtype is not pages.dtype or v_new.dtype is not pages.dtype):
+        raise TypeError(f"the pools are {pages.dtype}, q {q.dtype}{f', new keys {k_new.dtype}, values {v_new.dtype}' if fresh else ''}: "
+                        "they must share a dtype")
+    if q.get_device() != dev or fresh and (k_new.get_device() != dev or v_new.get_device() != dev):
+        raise ValueError(f"the pools are on {pages.device}, q on {q.device}: all tensors must be on one device")
+    # What the shapes and strides alone decide is checked once a layout.
+    key = (q.shape, q.stride(), k_new.shape if fresh else None, k_new.stride() if fresh else None, v_new.shape if fresh else None,
+           v_new.stride() if fresh else None, counts is None, bool(weigh))
+    lay = pages._layouts.get(key)
+    if lay is None:
+        lay = _paged_layout(pages, q, k_new, v_new, counts is not None, bool(weigh))
+        if len(pages._layouts) >= 256:
+            pages._layouts.clear()
+        pages._layouts[key] = lay
+    B, Hq, T, strides, at, out_shape, nbytes = lay
+    if counts is not None:
+        counts = _query_counts(counts, B, dev)
     if len_out is not None:
         _meta(dev, "len_out", len_out, torch.int32, pages.rows)
     if weights_out is not None:
         if not weigh or pages.weights is None:
             raise ValueError("weights_out without weigh, or for a cache without weights")
         pages._ledger("weights_out", weights_out, torch.float32, B * pages.kv_heads, like=pages.weights)
-    out, o_st = _out_bthd(q, out, shape, dev)
-    ws, nbytes = pages._workspace("hc_paged_workspace_size", Hq, T, counts is not None, bool(weigh))
-    _lib.check(_lib.load().hc_paged_attn(pages.ref, q.data_ptr(), _strides3((shape, q.stride())), Hq, T, kp, ks, vp, vs,
-                                         _ptr(counts), scale, bool(weigh), _ptr(weights_out), _ptr(len_out), out.data_ptr(),
-                                         o_st, ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(dev)))
+    device, o_st = pages.device, at + 72
+    if out is None:
+        out = torch.empty(out_shape, dtype=pages.dtype, device=device)
+    else:
+        out, o_st = _out_bthd(q, out, q.shape, dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _lib.check(_lib.load().hc_paged_attn(
+        pages.ref, q.data_ptr(), at, Hq, T, k_new.data_ptr() if fresh else None, at + 24, v_new.data_ptr() if fresh else None, at + 48,
+        _ptr(counts), scale, bool(weigh), _ptr(weights_out), _ptr(len_out), out.data_ptr(), o_st, ws.data_ptr(), nbytes,
+        torch._C._cuda_getCurrentRawStream(dev)))
     return out
+
+
+def _paged_layout(pages, q, k_new, v_new, counts, weigh):
+    """Sizes, strides (of q, new keys, new values and a contiguous output) and
+    their address, output shape and workspace bytes of a paged_attn call."""
+    shape = _queries(q)
+    B, Hq, T, D = shape
+    if B != pages.batch or Hq == 0 or Hq % pages.kv_heads:
+        raise ValueError(f"queries {tuple(shape)} for {pages.batch} sequences of {pages.kv_heads} KV heads")
+    if k_new is not None:
+        _new_tokens(pages, k_new, v_new, "new keys and values")
+        if k_new.shape[2] != T:
+            raise ValueError(f"{k_new.shape[2]} new tokens for {T} queries")
+    kl, vl = ((t.shape, t.stride()) if t is not None else ((1, 1, 1), (0, 0, 0)) for t in (k_new, v_new))
+    strides = (ctypes.c_int64 * 12)(*_strides3((shape, q.stride()), kl, vl, ((B, Hq, T), (T * Hq * D, D, Hq * D))))
+    with torch.cuda.device(pages.dev):
+        nbytes = _lib.load().hc_paged_workspace_size(pages.ref, Hq, T, counts, weigh)
+    return B, Hq, T, strides, ctypes.addressof(strides), (B, T, Hq, D), nbytes
 
 
 def paged_evict(pages, keep, sink=0, recent=0, len_out=None, weights_out=None, pos_out=None, dropped_out=None, stream=None):
