@@ -145,7 +145,7 @@ struct Stage {
       const int pi = page_of(p, t);
       const bool is_new = MIXED && t >= old;
       int pg = tab[pi];
-      if (!is_new && (uint32_t)pg >= (uint32_t)p.pages) bad = true, pg = 0;
+      if ((uint32_t)pg >= (uint32_t)p.pages) bad = true, pg = 0;  // (of a new token too: the append leaves it out)
       const char* src = pool + pg * s_page + (t - pi * p.page_tokens) * s_tok;
       if (is_new) src = fresh + (t - old) * s_new;
 #pragma unroll

@@ -1,0 +1,53 @@
+"""The paged cache at the edges of what its calls allow."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from heterocache_amd import _lib, ops
+from tests.paged_util import Cache, queries
+from tests.serving_util import D
+
+pytestmark = pytest.mark.gpu
+BF, FP, FL = torch.bfloat16, torch.float16, torch.float32
+SCALE = 1 / math.sqrt(D)
+
+
+@pytest.mark.parametrize("weigh", [False, True])
+@pytest.mark.parametrize("page,dtype,apart", [(16, BF, False), (24, BF, True), (16, FL, True)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_new_tokens_without_a_page(dev, wide, page, dtype, apart, weigh):
+    """A padded batch of which one row's table names no page for some of its new tokens: the queries that see them get
+    NaN, and so does every weight that they add to; the other sequences and all stored pages are as in a call without the
+    fault.  Tables as wide as their rows, and far wider, take the batch in one launch and in several."""
+    T, lens, counts = 40, [60, 48, 47], [40, 1, 17]
+    width = -(-(24000 if wide else 112) // page)
+    for b, value in ((0, -1), (0, 1 << 30), (1, -1), (2, -(1 << 31))):
+        good, c = (Cache(np.random.default_rng(10 * page + b), 3, 2, [n for n in lens for _ in range(2 if apart else 1)], page, dtype,
+                         dev, apart=apart, room=T, stale=0.0, ledger=True, width=width) for _ in range(2))
+        n = lens[b] + counts[b]
+        entry = (n - 1) // page
+        assert entry * page >= lens[b]  # its tokens are new
+        rows = [2 * b, 2 * b + 1] if apart else [b]
+        c.pages.table[rows, entry] = value
+        rng = np.random.default_rng(b)
+        q, kn, vn = (queries(rng, 3, h, T, dtype, dev) for h in (8, 2, 2))
+        dc = torch.tensor(counts, dtype=torch.int32, device=dev)
+        want = ops.paged_attn(q, good.pages, SCALE, kn, vn, counts=dc, weigh=weigh)
+        got = ops.paged_attn(q, c.pages, SCALE, kn, vn, counts=dc, weigh=weigh)
+        others = [x for x in range(3) if x != b]
+        assert torch.isfinite(want.float()).all() and torch.equal(got[others], want[others])
+        assert torch.isnan(got[b, entry * page - lens[b]:counts[b]].float()).all(), (b, value)
+        assert not got[b, counts[b]:].any()
+        with pytest.raises(_lib.HCError, match="names no page"):
+            ops.read_status(c.status)
+        assert torch.equal(c.pages.row_len, good.pages.row_len)
+        if weigh:
+            mine = torch.arange(6, device=dev) // 2 == b
+            assert torch.isnan(c.pages.weights[mine, :n]).all(), (b, value)
+            assert torch.equal(c.pages.weights[~mine], good.pages.weights[~mine])
+        # The entry's tokens are left out, and nothing else.
+        left = torch.ones(len(good.k), dtype=torch.bool, device=dev)
+        left[torch.as_tensor(good.table[rows, entry].astype(np.int64)).to(dev)] = False
+        assert torch.equal(c.k[left], good.k[left]) and torch.equal(c.v[left], good.v[left])
