@@ -178,6 +178,7 @@ inline unsigned paged_chunk_fold_grid(const PagedAttn& a) {
 int launch_paged_rows(int dtype, const PagedAttn& a, bool fold, hipStream_t s);
 int launch_paged_chunk(int dtype, const PagedAttn& a, bool fold, hipStream_t s);
 int launch_paged_append(int dtype, const PagedAttn& a, hipStream_t s);
+int launch_paged_carry(const PagedAttn& a, hipStream_t s);
 int launch_paged_mixed(int dtype, const PagedAttn& a, hipStream_t s);
 int launch_paged_weights(int dtype, const PagedAttn& a, hipStream_t s);
 int paged_rows_slots(int dtype);

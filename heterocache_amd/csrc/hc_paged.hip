@@ -182,7 +182,16 @@ extern "C" int hc_paged_attn(const hc_paged_cache* c, const void* q, const int64
     return set_error(HC_ERR_INVALID, "hc_paged_attn: scale must be finite and positive");
   if (weigh && !c->weights) return set_error(HC_ERR_INVALID, "hc_paged_attn: the cache has no weights to add to");
   if (weights_out && !weigh) return set_error(HC_ERR_INVALID, "hc_paged_attn: weights_out without weigh");
-  if (c->batch == 0 || queries == 0) return HC_OK;
+  if (c->batch == 0) return HC_OK;
+  if (queries == 0) {
+    // No outputs; the lengths and weights behind the call are those before it.
+    if (weights_out && weights_out != c->weights) {
+      take_ledger(c, a);
+      a.weights_out = weights_out;
+      if (int rc = launch_paged_carry(a, (hipStream_t)stream)) return rc;
+    }
+    return hc_paged_append(c, nullptr, nullptr, nullptr, nullptr, counts, 0, len_out, stream);
+  }
   const bool fresh = k_new || v_new;
   if (len_out && !fresh) return set_error(HC_ERR_INVALID, "hc_paged_attn: len_out without new tokens");
   if (!q || !q_strides || !out || !out_strides) return set_error(HC_ERR_INVALID, "hc_paged_attn: null pointer argument");

@@ -213,6 +213,14 @@ __global__ __launch_bounds__(256) void paged_advance_kernel(const PagedAttn a, i
   a.len_out[r] = s.total;
 }
 
+// The weights of a call without queries, in memory of their own.
+__global__ __launch_bounds__(256) void paged_carry_kernel(const PagedAttn a, int runs) {
+  const int row = blockIdx.x % a.pool.rows, total = row_span(a.pool, row).total;
+  const float* const in = a.weights + row * a.weight_stride;
+  float* const out = a.weights_out + row * a.weight_stride;
+  for (int t = (int)(blockIdx.x / a.pool.rows) * 256 + threadIdx.x; t < total; t += runs * 256) out[t] = in[t];
+}
+
 }  // namespace
 
 int launch_paged_chunk(int dtype, const PagedAttn& a, bool fold, hipStream_t s) {
@@ -229,6 +237,12 @@ int launch_paged_weights(int dtype, const PagedAttn& a, hipStream_t s) {
     case HC_DTYPE_F16: return launch_weights<_Float16>(a, s);
     default: return launch_weights<float>(a, s);
   }
+}
+
+int launch_paged_carry(const PagedAttn& a, hipStream_t s) {
+  const int runs = paged_weigh_runs(a.pool);
+  hipLaunchKernelGGL(paged_carry_kernel, dim3((unsigned)(a.pool.rows * runs)), dim3(256), 0, s, a, runs);
+  return check_launch("hc_paged_attn(weights)");
 }
 
 int launch_paged_append(int dtype, const PagedAttn& a, hipStream_t s) {

@@ -731,6 +731,8 @@ int hc_paged_append(const hc_paged_cache* c, const void* k, const int64_t* k_str
  * query heads of their probabilities of token t, for every token of the row; a
  * token appended by this call starts at zero.  weights_out NULL: in place; else
  * memory that shares nothing with the old.
+ * queries = 0: nothing is attended or appended (the tensors may be NULL), and
+ * len_out and weights_out, where given, receive the old lengths and weights.
  * q, out: element strides batch, head, token, all of whole 16 bytes; out shares
  * no memory with q.  Stands where the reference calls flash attention over its
  * pools (heterocache/llama_model.py:382-389), for one new token or many.

@@ -51,3 +51,30 @@ def test_new_tokens_without_a_page(dev, wide, page, dtype, apart, weigh):
         left = torch.ones(len(good.k), dtype=torch.bool, device=dev)
         left[torch.as_tensor(good.table[rows, entry].astype(np.int64)).to(dev)] = False
         assert torch.equal(c.k[left], good.k[left]) and torch.equal(c.v[left], good.v[left])
+
+
+@pytest.mark.parametrize("apart", [True, False])
+@pytest.mark.parametrize("counts", [False, True])
+def test_no_tokens(dev, apart, counts):
+    """A call of no tokens has no outputs, but lengths and weights: the old ones, also in memory of their own."""
+    c = Cache(np.random.default_rng(1), 2, 3, [70, 0, 33], 16, BF, dev, apart=apart, ledger=True)
+    p = c.pages
+    lens, w0 = p.row_len.clone(), p.weights.clone()
+    q, kn, vn = (torch.zeros((2, h, 0, D), dtype=BF, device=dev) for h in (6, 3, 3))
+    dc = torch.zeros(2, dtype=torch.int32, device=dev) if counts else None
+    len_out, w_out = torch.full_like(lens, -9), torch.full_like(w0, -9.0)
+    for weigh in (True, False):
+        len_out.fill_(-9), w_out.fill_(-9.0)
+        got = ops.paged_attn(q, p, SCALE, kn, vn, counts=dc, weigh=weigh, len_out=len_out, weights_out=w_out if weigh else None)
+        assert got.shape == (2, 0, 6, D) and torch.equal(len_out, lens)
+        for x in range(6):
+            n = int(lens[c.row(x // 3, x % 3)[0]])
+            if weigh:
+                assert torch.equal(w_out[x, :n], w0[x, :n]) and (w_out[x, n:] == -9.0).all()
+    w_out.fill_(-9.0)
+    ops.paged_attn(q, p, SCALE, counts=dc, weigh=True, weights_out=w_out)  # of tokens that are stored
+    assert all(torch.equal(w_out[x, :n], w0[x, :n]) for x in range(6) for n in [int(lens[c.row(x // 3, x % 3)[0]])])
+    ops.paged_attn(q, p, SCALE, kn, vn, counts=dc, weigh=True)             # in place
+    len_out.fill_(-9)
+    ops.paged_append(kn, vn, p, counts=dc, len_out=len_out)
+    assert torch.equal(len_out, lens) and torch.equal(p.row_len, lens) and torch.equal(p.weights, w0) and c.status.item() == 0
