@@ -26,9 +26,9 @@ class PagedStore:
     attention weight, its position, and the tokens that a row has given up.
 
     `host_len` bounds the rows' lengths on the host (exact unless counts were
-    given on the device): pages are reserved by it, the kernels read the lengths
-    on the device.  Pages are handed out in host order: calls that use one store
-    go to one stream, or are ordered by the caller.
+    given on the device or calls captured): pages are reserved by it, the
+    kernels read the lengths on the device.  Pages are handed out in host order:
+    calls that use one store go to one stream, or are ordered by the caller.
     """
 
     def __init__(self, batch, kv_heads, pages, dtype, device, max_tokens, page_tokens=64, per_head=False, track=False,
@@ -156,7 +156,8 @@ class PagedStore:
     def evict(self, keep, sink=0, recent=0, stream=None):
         """Holds every row to its `keep` heaviest tokens (an integer, or one a
         row), the positions below `sink` and the last `recent` first
-        (ops.paged_evict); pages that no token is left in become free."""
+        (ops.paged_evict); pages that no token is left in become free (not by a
+        captured call: the next eager one after sync_host_lengths frees them)."""
         host = np.broadcast_to(np.asarray(keep, dtype=np.int64), (self.rows,))
         if (host < sink + recent).any():
             raise ValueError(f"keep={keep} holds less than sink={sink} and recent={recent}")
@@ -164,8 +165,9 @@ class PagedStore:
         with torch.cuda.stream(stream):
             arg = int(keep) if np.ndim(keep) == 0 else ops.host_counts("keep", host.copy(), self.device)
             ops.paged_evict(self.pages, arg, sink=sink, recent=recent)
-            if not torch.cuda.is_current_stream_capturing():
-                self._give_back(lens, range(self.rows))
+            if torch.cuda.is_current_stream_capturing():
+                return  # nothing has run: the old bound holds, and the pages are the rows' own
+            self._give_back(lens, range(self.rows))
         self.host_len = lens
 
     def release(self, sequences, stream=None):

@@ -261,3 +261,34 @@ def test_two_streams(dev):
             p.extend(o, *x, [T, T], BF, w)
     for p in plains:
         p.check()
+
+
+def test_an_eviction_that_is_captured_and_not_replayed(dev):
+    """Capturing runs nothing: the rows keep their tokens, and what the host knows of them still bounds their lengths."""
+    rng = np.random.default_rng(10)
+    s = PagedStore(2, 2, 60, BF, dev, max_tokens=128, page_tokens=16, per_head=True, track=True)
+    plain = Plain(s)
+    _extend(rng, s, plain, 4, 32, BF)                        # full pages
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            s.evict(20, sink=2, recent=6)
+    torch.cuda.current_stream().wait_stream(side)
+    assert (s.host_len >= s.row_len.cpu().numpy()).all()
+    _extend(rng, s, plain, 4, 1, BF)                         # into a page that is not reserved yet
+    plain.check()
+    s.check_status()
+    weights = s.pages.weights.cpu().numpy()
+    graph.replay()
+    plain.evict([20] * s.rows, 2, 6, weights)
+    torch.cuda.synchronize()
+    s.sync_host_lengths(s.row_len.cpu().numpy())
+    plain.check()
+    _extend(rng, s, plain, 4, 5, BF)
+    weights = s.pages.weights.cpu().numpy()
+    s.evict(9, sink=2, recent=6)                             # the pages behind come back now
+    plain.evict([9] * s.rows, 2, 6, weights)
+    plain.check()
+    assert (s.held == 1).all()
