@@ -248,6 +248,9 @@ __global__ __launch_bounds__(256) void evict_clear_kernel(const EvictArgs a) {
   }
 }
 
+// (Beyond 2^19 rows the offsets of their counters pass 2^31.)
+__device__ __forceinline__ int32_t* row_hist(const EvictArgs& a, int row) { return a.hist + (int64_t)row * kTop; }
+
 // Second: the keys, counted by their top bits.
 __global__ __launch_bounds__(kRunThreads) void evict_count_kernel(const EvictArgs a) {
   __shared__ int s_hist[kTop];
@@ -274,7 +277,7 @@ __global__ __launch_bounds__(kRunThreads) void evict_count_kernel(const EvictArg
   }
   __syncthreads();
   for (int i = tid; i < kTop; i += kRunThreads)
-    if (s_hist[i]) atomicAdd(a.hist + row * kTop + i, s_hist[i]);
+    if (s_hist[i]) atomicAdd(row_hist(a, row) + i, s_hist[i]);
 }
 
 // Bin, from the top, that holds the want-th of the counts (kRunThreads * PER of
@@ -310,7 +313,7 @@ __global__ __launch_bounds__(kRunThreads) void evict_collect_kernel(const EvictA
   const int row = blockIdx.x % a.rows, run = blockIdx.x / a.rows, tid = threadIdx.x;
   const int n = a.state[row].n, keep = a.state[row].keep;
   if (n <= keep || keep == 0 || run * kRun >= n) return;
-  const uint32_t top = (uint32_t)pick_bin<kTop / kRunThreads>(a.hist + row * kTop, keep, s_wave, s_pick, tid).x;
+  const uint32_t top = (uint32_t)pick_bin<kTop / kRunThreads>(row_hist(a, row), keep, s_wave, s_pick, tid).x;
   const uint32_t* const keys = a.keys + (int64_t)row * a.pool.capacity;
   uint32_t* const out = a.candidates + (int64_t)row * a.pool.capacity;
   uint32_t k[kRunPer];
@@ -345,7 +348,7 @@ __global__ __launch_bounds__(kRunThreads) void evict_rank_kernel(const EvictArgs
   uint32_t least = 0xffffffffu;
   int equal = 0;
   if (keep > 0) {
-    const int2 top = pick_bin<kTop / kRunThreads>(a.hist + row * kTop, keep, s_wave, s_pick, tid);
+    const int2 top = pick_bin<kTop / kRunThreads>(row_hist(a, row), keep, s_wave, s_pick, tid);
     const int found = a.found[row];
     const uint32_t* const cand = a.candidates + (int64_t)row * a.pool.capacity;
     // The 20 bits left, 11 and 9 at a time.

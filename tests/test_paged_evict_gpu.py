@@ -116,3 +116,34 @@ def test_many_rows(dev):
     rng = np.random.default_rng(4)
     c = Cache(rng, 700, 4, [20, 33, 7], 16, BF, dev, apart=True, ledger=True)
     _evict(c, 16, 1, 4)
+
+
+def test_counters_past_32_bits(dev):
+    """Long table rows with more than 2^31 counters: the rows at both ends are evicted from, the others are
+    empty."""
+    rows, cap, n, keep = (1 << 19) + 5, 16385, 16384, 9000
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info(dev)[0] < 210 * 10 ** 9:
+        pytest.skip("needs 182 GB of free device memory")
+    rng = np.random.default_rng(5)
+    k, v = (torch.as_tensor(rng.standard_normal((2, cap, 1, 128)), dtype=torch.float32).to(BF).to(dev) for _ in range(2))
+    table = torch.full((rows, 1), -1, dtype=torch.int32, device=dev)
+    row_len, dropped, status = (torch.zeros(x, dtype=torch.int32, device=dev) for x in (rows, rows, 1))
+    weights, pos = (torch.empty((rows, cap), dtype=t, device=dev) for t in (FL, torch.int32))
+    want = {}
+    for r, page in ((0, 0), (rows - 1, 1)):
+        table[r, 0], row_len[r] = page, n
+        w = rng.exponential(size=(1, cap)).astype(np.float32)
+        weights[r], pos[r] = torch.as_tensor(w[0]).to(dev), torch.arange(cap, dtype=torch.int32, device=dev)
+        src = evict_order(w, np.arange(cap), n, keep, 4, 100, 0)
+        want[r] = [src, k[page, :n, 0].cpu()[src], v[page, :n, 0].cpu()[src], w[0, src]]
+    p = ops.Pages(k, v, table, row_len, 1, weights=weights, pos=pos, dropped=dropped, status=status)
+    ops.paged_evict(p, keep, sink=4, recent=100)
+    for r, page in ((0, 0), (rows - 1, 1)):
+        src, wk, wv, ww = want[r]
+        assert int(row_len[r]) == keep and int(dropped[r]) == n - keep
+        assert pos[r, :keep].tolist() == src.tolist() and np.array_equal(weights[r, :keep].cpu().numpy(), ww)
+        assert torch.equal(k[page, :keep, 0].cpu(), wk) and torch.equal(v[page, :keep, 0].cpu(), wv)
+    assert int(row_len.sum()) == 2 * keep and status.item() == 0
+    del weights, pos, p
+    torch.cuda.empty_cache()
