@@ -123,7 +123,8 @@ __device__ __forceinline__ RowState row_state(const EvictArgs& a, int row) {
 
 // Keys of rows whose weights are sums over heads, by more workgroups than rows.
 __global__ __launch_bounds__(kRunThreads) void evict_keys_kernel(const EvictArgs a) {
-  const int row = blockIdx.x % a.rows, t = blockIdx.x / a.rows * kRunThreads + threadIdx.x;
+  const uint32_t x = group_id();
+  const int row = x % a.rows, t = x / a.rows * kRunThreads + threadIdx.x;
   const RowState s = row_state(a, row);
   if (s.n > s.keep && t < s.n) a.keys[(int64_t)row * a.pool.capacity + t] = token_key(a, row, t, s.n + s.dropped - a.recent);
 }
@@ -136,7 +137,8 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(const EvictArgs 
   __shared__ int s_count[PER * kWaves];
   __shared__ uint32_t s_range[2];
   __shared__ int s_pick[2];
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row = (int)group_id(), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (row >= a.rows) return;
   RowState st = row_state(a, row);
   const int n = st.n, keep = st.keep;
   int32_t* const list = a.moves + (int64_t)row * a.pool.capacity;
@@ -254,7 +256,8 @@ __device__ __forceinline__ int32_t* row_hist(const EvictArgs& a, int row) { retu
 // Second: the keys, counted by their top bits.
 __global__ __launch_bounds__(kRunThreads) void evict_count_kernel(const EvictArgs a) {
   __shared__ int s_hist[kTop];
-  const int row = blockIdx.x % a.rows, run = blockIdx.x / a.rows, tid = threadIdx.x;
+  const uint32_t x = group_id();
+  const int row = x % a.rows, run = x / a.rows, tid = threadIdx.x;
   const int n = a.state[row].n, keep = a.state[row].keep;
   if (n <= keep || run * kRun >= n) return;
   const int first_recent = n + a.state[row].dropped - a.recent;
@@ -310,7 +313,8 @@ __device__ __forceinline__ int2 pick_bin(const int* hist, int want, int* s_wave,
 __global__ __launch_bounds__(kRunThreads) void evict_collect_kernel(const EvictArgs a) {
   __shared__ int s_wave[kRunThreads / 64 + 1], s_pick[2];
   __shared__ int s_base[kRunThreads / 64];
-  const int row = blockIdx.x % a.rows, run = blockIdx.x / a.rows, tid = threadIdx.x;
+  const uint32_t x = group_id();
+  const int row = x % a.rows, run = x / a.rows, tid = threadIdx.x;
   const int n = a.state[row].n, keep = a.state[row].keep;
   if (n <= keep || keep == 0 || run * kRun >= n) return;
   const uint32_t top = (uint32_t)pick_bin<kTop / kRunThreads>(row_hist(a, row), keep, s_wave, s_pick, tid).x;
@@ -342,7 +346,8 @@ __global__ __launch_bounds__(kRunThreads) void evict_rank_kernel(const EvictArgs
   __shared__ int s_hist[kRunThreads * 8];
   __shared__ int s_wave[kRunThreads / 64 + 1], s_pick[2];
   __shared__ RunCount s_count;
-  const int row = blockIdx.x % a.rows, run = blockIdx.x / a.rows, tid = threadIdx.x;
+  const uint32_t x = group_id();
+  const int row = x % a.rows, run = x / a.rows, tid = threadIdx.x;
   const int n = a.state[row].n, keep = a.state[row].keep;
   if (n <= keep || run * kRun >= n) return;
   uint32_t least = 0xffffffffu;
@@ -403,7 +408,8 @@ __global__ __launch_bounds__(kRunThreads) void evict_rank_kernel(const EvictArgs
 // Fifth: the lists.  What the runs ahead free and move follows from their counts.
 __global__ __launch_bounds__(kRunThreads) void evict_list_kernel(const EvictArgs a) {
   __shared__ int s_part[3][kRunPer * kRunThreads / 64];
-  const int row = blockIdx.x % a.rows, run = blockIdx.x / a.rows, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t x = group_id();
+  const int row = x % a.rows, run = x / a.rows, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const RowState st = a.state[row];
   const int n = st.n, keep = st.keep;
   if (n <= keep && run == 0 && tid == 0) a.state[row].moved = 0;
@@ -481,7 +487,9 @@ __global__ __launch_bounds__(kRunThreads) void evict_list_kernel(const EvictArgs
 // token's keys and values stay where they are and the status word says so.
 __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a) {
   const Pool& p = a.pool;
-  const int row = blockIdx.x / a.move_blocks, blk = blockIdx.x % a.move_blocks;
+  const uint32_t x = group_id();
+  const int row = x / a.move_blocks, blk = x % a.move_blocks;
+  if (row >= a.rows) return;
   const RowState st = a.state[row];
   const int count = st.moved, kept = min(st.n, st.keep);
   const int32_t* const list = a.moves + (int64_t)row * p.capacity;
@@ -627,25 +635,23 @@ extern "C" int hc_paged_evict(const hc_paged_cache* c, const int32_t* keep, int 
   a.move_blocks = (int)std::max<int64_t>(1, std::min<int64_t>((most + 511) / 512, 4096 / (a.rows * (2 * a.pool.heads + 1))));
   hipStream_t s = (hipStream_t)stream;
   const int64_t grid = (int64_t)a.rows * l.runs;
-  if (grid > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_paged_evict: %d rows of %d tokens", a.rows, a.pool.capacity);
   if (a.pool.heads > 32767) return set_error(HC_ERR_INVALID, "hc_paged_evict: %d heads", a.pool.heads);
-  const dim3 move((unsigned)((int64_t)a.rows * a.move_blocks), 2 * a.pool.heads + 1);
+  const dim3 move = groups((int64_t)a.rows * a.move_blocks, 256, 2 * a.pool.heads + 1);
   if (l.is_long) {
     hipLaunchKernelGGL(evict_clear_kernel, dim3((unsigned)std::min<int64_t>(((int64_t)a.rows * kTop + 255) / 256, 1024)), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(evict_count_kernel, dim3((unsigned)grid), dim3(kRunThreads), 0, s, a);
-    hipLaunchKernelGGL(evict_collect_kernel, dim3((unsigned)grid), dim3(kRunThreads), 0, s, a);
-    hipLaunchKernelGGL(evict_rank_kernel, dim3((unsigned)grid), dim3(kRunThreads), 0, s, a);
-    hipLaunchKernelGGL(evict_list_kernel, dim3((unsigned)grid), dim3(kRunThreads), 0, s, a);
+    hipLaunchKernelGGL(evict_count_kernel, groups(grid), dim3(kRunThreads), 0, s, a);
+    hipLaunchKernelGGL(evict_collect_kernel, groups(grid), dim3(kRunThreads), 0, s, a);
+    hipLaunchKernelGGL(evict_rank_kernel, groups(grid), dim3(kRunThreads), 0, s, a);
+    hipLaunchKernelGGL(evict_list_kernel, groups(grid), dim3(kRunThreads), 0, s, a);
     if (int rc = check_launch("hc_paged_evict")) return rc;
     hipLaunchKernelGGL(evict_move_kernel, move, dim3(256), 0, s, a);
     return check_launch("hc_paged_evict(move)");
   }
-  const dim3 rows(a.rows), threads(kThreads);
+  const dim3 rows = groups(a.rows, kThreads), threads(kThreads);
   const bool few = a.pool.capacity <= 4 * kThreads;
   if (a.pool.heads > 1) {
     const int64_t blocks = (int64_t)a.rows * ((a.pool.capacity + kRunThreads - 1) / kRunThreads);
-    if (blocks > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_paged_evict: %d rows of %d tokens", a.rows, a.pool.capacity);
-    hipLaunchKernelGGL(evict_keys_kernel, dim3((unsigned)blocks), dim3(kRunThreads), 0, s, a);
+    hipLaunchKernelGGL(evict_keys_kernel, groups(blocks), dim3(kRunThreads), 0, s, a);
     if (few)
       hipLaunchKernelGGL((evict_select_kernel<4, true>), rows, threads, 0, s, a);
     else

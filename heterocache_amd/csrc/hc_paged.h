@@ -14,6 +14,17 @@
 
 namespace hc {
 
+// A launch of n workgroups.  HIP takes fewer than 2^32 threads along x, so more
+// lie along z, in layers of whole XCD turns; a kernel takes group_id() for its
+// workgroup, and those behind the last leave at once.
+constexpr int64_t kLayerThreads = (int64_t)1 << 31;
+constexpr int64_t kMostGroups = 0x7fffffffLL - kLayerThreads / 256;  // a layer's rest included an int
+inline dim3 groups(int64_t n, int threads = 256, unsigned y = 1) {
+  const int64_t layer = kLayerThreads / threads;
+  return n <= layer ? dim3((unsigned)n, y) : dim3((unsigned)layer, y, (unsigned)((n + layer - 1) / layer));
+}
+__device__ __forceinline__ uint32_t group_id() { return blockIdx.x + blockIdx.z * gridDim.x; }
+
 struct Pool {
   const char *k, *v;
   int64_t k_page, k_tok, k_head, v_page, v_tok, v_head;  // byte strides

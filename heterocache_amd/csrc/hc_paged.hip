@@ -160,7 +160,7 @@ extern "C" int hc_paged_append(const hc_paged_cache* c, const void* k, const int
     return set_error(HC_ERR_INVALID, "hc_paged_append: len_out overlaps row_len without being it");
   if (tokens > 0)
     if (int rc = check_fresh("hc_paged_append", c, k, k_strides, v, v_strides, a.fresh)) return rc;
-  if ((int64_t)a.pool.rows * ((tokens + 15) / 16) > 0x7fffffffLL)
+  if ((int64_t)a.pool.rows * ((tokens + 15) / 16) > kMostGroups)
     return set_error(HC_ERR_INVALID, "hc_paged_append: %d rows x %d tokens", a.pool.rows, tokens);
   a.pool.fresh = 1;
   a.len_out = len_out ? len_out : c->row_len;

@@ -11,7 +11,7 @@ namespace {
 template <typename T, bool UNIFORM>
 __global__ __launch_bounds__(kPagedThreads, sizeof(T) == 4 ? 2 : 3) void paged_chunk_kernel(const PagedAttn a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  paged_chunk_job<T, UNIFORM, false>(a, blockIdx.x, lds);
+  paged_chunk_job<T, UNIFORM, false>(a, (int)group_id(), lds);
 }
 
 template <typename T>
@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256) void paged_chunk_fold_kernel(const PagedAttn a
 }
 
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAttn a, int chunks, int blocks) {
-  paged_append_job<false>(a, blockIdx.x, chunks, blocks);
+  paged_append_job<false>(a, (int)group_id(), chunks, blocks);
 }
 
 // Every token's share of the chunk's attention,
@@ -49,7 +49,8 @@ __global__ __launch_bounds__(kPagedThreads, sizeof(T) == 4 ? 2 : NC == 4 ? 3 : 4
   // Rows r, r + 8, .. on one XCD, the blocks of a row behind each other: workgroups
   // are dealt in turn to the XCDs and within one to its four engines, where rows
   // of a sequence each would all meet (4 ragged sequences: 162 us, now 85).
-  const int row = blockIdx.x % 8 + 8 * (blockIdx.x / 8 / blocks), tb = blockIdx.x / 8 % blocks;
+  const uint32_t x = group_id();
+  const int row = x % 8 + 8 * (x / 8 / blocks), tb = x / 8 % blocks;
   if (row >= p.rows) return;
   const int b = row / p.Hkv, h = row % p.Hkv;
   const int hd = p.heads == 1 ? 0 : h;
@@ -167,7 +168,7 @@ int launch_attn(const PagedAttn& a, hipStream_t s) {
                                hipFuncAttributeMaxDynamicSharedMemorySize, chunk_lds<T>());
   });
   if (attr != hipSuccess) return set_error(HC_ERR_HIP, "hc_paged_attn: %s", hipGetErrorString(attr));
-  hipLaunchKernelGGL((paged_chunk_kernel<T, UNIFORM>), dim3(a.chunk_grid), dim3(kPagedThreads), chunk_lds<T>(), s, a);
+  hipLaunchKernelGGL((paged_chunk_kernel<T, UNIFORM>), groups(a.chunk_grid), dim3(kPagedThreads), chunk_lds<T>(), s, a);
   return check_launch("hc_paged_attn(chunk)");
 }
 
@@ -183,8 +184,7 @@ int launch_weigh(const PagedAttn& a, hipStream_t s) {
   const int block = kPagedWaves * 16 * NC;
   const int blocks = (a.pool.capacity + block - 1) / block;
   const int64_t grid = (int64_t)(a.pool.rows + 7) / 8 * 8 * blocks;
-  if (grid > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_paged_attn: weights of %d rows of %d tokens", a.pool.rows, a.pool.capacity);
-  hipLaunchKernelGGL((paged_weigh_kernel<T, NC>), dim3((unsigned)grid), dim3(kPagedThreads), weigh_lds<T>(), s, a, blocks);
+  hipLaunchKernelGGL((paged_weigh_kernel<T, NC>), groups(grid), dim3(kPagedThreads), weigh_lds<T>(), s, a, blocks);
   return check_launch("hc_paged_attn(weights)");
 }
 
@@ -215,10 +215,11 @@ __global__ __launch_bounds__(256) void paged_advance_kernel(const PagedAttn a, i
 
 // The weights of a call without queries, in memory of their own.
 __global__ __launch_bounds__(256) void paged_carry_kernel(const PagedAttn a, int runs) {
-  const int row = blockIdx.x % a.pool.rows, total = row_span(a.pool, row).total;
+  const int x = (int)group_id(), row = x % a.pool.rows, total = row_span(a.pool, row).total;
   const float* const in = a.weights + row * a.weight_stride;
   float* const out = a.weights_out + row * a.weight_stride;
-  for (int t = (int)(blockIdx.x / a.pool.rows) * 256 + threadIdx.x; t < total; t += runs * 256) out[t] = in[t];
+  if (x >= a.pool.rows * runs) return;
+  for (int t = x / a.pool.rows * 256 + (int)threadIdx.x; t < total; t += runs * 256) out[t] = in[t];
 }
 
 }  // namespace
@@ -241,7 +242,7 @@ int launch_paged_weights(int dtype, const PagedAttn& a, hipStream_t s) {
 
 int launch_paged_carry(const PagedAttn& a, hipStream_t s) {
   const int runs = paged_weigh_runs(a.pool);
-  hipLaunchKernelGGL(paged_carry_kernel, dim3((unsigned)(a.pool.rows * runs)), dim3(256), 0, s, a, runs);
+  hipLaunchKernelGGL(paged_carry_kernel, groups(a.pool.rows * runs), dim3(256), 0, s, a, runs);
   return check_launch("hc_paged_attn(weights)");
 }
 
@@ -250,7 +251,7 @@ int launch_paged_append(int dtype, const PagedAttn& a, hipStream_t s) {
   PagedAttn first = a;
   const bool in_place = a.len_out && a.len_out == a.pool.row_len;
   if (in_place) first.len_out = nullptr;
-  hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)((int64_t)a.pool.rows * blocks)), dim3(256), 0, s, first, chunks, blocks);
+  hipLaunchKernelGGL(paged_append_kernel, groups((int64_t)a.pool.rows * blocks), dim3(256), 0, s, first, chunks, blocks);
   int rc = check_launch("hc_paged_append");
   if (rc || !in_place) return rc;
   const int table_rows = a.pool.heads == 1 ? a.pool.rows : a.pool.rows / a.pool.Hkv;

@@ -36,11 +36,12 @@ __global__ __launch_bounds__(kPagedThreads, sizeof(T) == 4 ? 1 : 2) void paged_m
 }
 
 template <typename T, bool WEIGH>
-__global__ __launch_bounds__(256) void paged_mixed_fold_kernel(const PagedAttn a, int runs, int few) {
-  if ((int)blockIdx.x < few)
-    paged_fold_job<T, WEIGH>(a, blockIdx.x, runs);
-  else
-    paged_chunk_fold_job<T>(a, blockIdx.x - few, gridDim.x - few);
+__global__ __launch_bounds__(256) void paged_mixed_fold_kernel(const PagedAttn a, int runs, int few, int many) {
+  const int x = (int)group_id();
+  if (x < few)
+    paged_fold_job<T, WEIGH>(a, x, runs);
+  else if (x < few + many)
+    paged_chunk_fold_job<T>(a, x - few, many);
 }
 
 template <typename T, bool WEIGH, bool UNIFORM>
@@ -53,9 +54,8 @@ int launch_attn(const PagedAttn& a, hipStream_t s) {
   });
   if (attr != hipSuccess) return set_error(HC_ERR_HIP, "hc_paged_attn: %s", hipGetErrorString(attr));
   const int blocks = (a.pool.Q + 15) / 16;
-  const int64_t grid = (int64_t)a.grid + a.chunk_grid + (a.pool.fresh ? (int64_t)a.pool.rows * blocks : 0);
-  if (grid > 0x7fffffffLL) return set_error(HC_ERR_INVALID, "hc_paged_attn: %d rows x %d tokens", a.pool.rows, a.pool.Q);
-  hipLaunchKernelGGL((paged_mixed_kernel<T, WEIGH, UNIFORM>), dim3((unsigned)grid), dim3(kPagedThreads), mixed_lds<T>(), s, a, device_cus(), blocks);
+  const int grid = a.grid + a.chunk_grid + (a.pool.fresh ? a.pool.rows * blocks : 0);  // (few: the work is bounded)
+  hipLaunchKernelGGL((paged_mixed_kernel<T, WEIGH, UNIFORM>), dim3(grid), dim3(kPagedThreads), mixed_lds<T>(), s, a, device_cus(), blocks);
   return check_launch("hc_paged_attn(mixed)");
 }
 
@@ -77,7 +77,8 @@ int launch(int dtype, const PagedAttn& a, hipStream_t s) {
   }
   if (rc) return rc;
   const int runs = WEIGH ? paged_weigh_runs(a.pool) : 0, few = a.pool.rows * (a.few + runs);
-  hipLaunchKernelGGL((paged_mixed_fold_kernel<T, WEIGH>), dim3(few + paged_chunk_fold_grid(a)), dim3(256), 0, s, a, runs, few);
+  const int many = (int)paged_chunk_fold_grid(a);
+  hipLaunchKernelGGL((paged_mixed_fold_kernel<T, WEIGH>), groups((int64_t)few + many), dim3(256), 0, s, a, runs, few, many);
   return check_launch("hc_paged_attn(fold)");
 }
 

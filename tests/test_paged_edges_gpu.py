@@ -78,3 +78,81 @@ def test_no_tokens(dev, apart, counts):
     len_out.fill_(-9)
     ops.paged_append(kn, vn, p, counts=dc, len_out=len_out)
     assert torch.equal(len_out, lens) and torch.equal(p.row_len, lens) and torch.equal(p.weights, w0) and c.status.item() == 0
+
+
+def _table(rows, entries, row_pages, dev):
+    """A table of -1 but for the rows given."""
+    table = torch.full((rows, entries), -1, dtype=torch.int32, device=dev)
+    for r, page in row_pages.items():
+        table[r] = page
+    return table
+
+
+def _pool(rng, pages, page, dtype, dev):
+    return (torch.as_tensor(rng.standard_normal((pages, page, 1, D)), dtype=torch.float32).to(dtype).to(dev) for _ in range(2))
+
+
+def _i32(a, dev):
+    return torch.as_tensor(a, dtype=torch.int32).to(dev)
+
+
+def test_as_many_columns_as_a_launch_holds_threads(dev):
+    """2^20 rows of 16 columns are folded by 2^24 workgroups, 2^32 threads: every 64 rows as in a call of 64."""
+    rng = np.random.default_rng(20)
+    k, v = _pool(rng, 1, 16, BF, dev)
+    q = queries(rng, 64, 16, 1, BF, dev)
+    lens = _i32(np.arange(64) % 17, dev)
+    want = ops.paged_attn(q, ops.Pages(k, v, torch.zeros((64, 1), dtype=torch.int32, device=dev), lens, 1), SCALE)
+    n = 1 << 14
+    p = ops.Pages(k, v, torch.zeros((64 * n, 1), dtype=torch.int32, device=dev), lens.repeat(n), 1)
+    got = ops.paged_attn(q.repeat(n, 1, 1, 1), p, SCALE)
+    assert torch.isfinite(want.float()).all()
+    assert all(torch.equal(x.view(-1, 64, 1, 16, D), want.expand(x.shape[0] // 64, -1, -1, -1, -1)) for x in got.split(1 << 16))
+
+
+def test_as_many_weights_as_a_launch_holds_threads(dev):
+    """2^16 rows of wide tables take 2^24 workgroups to weigh in fp32."""
+    rng = np.random.default_rng(21)
+    T, page, n = 5, 1 << 14, 1 << 10
+    k, v = _pool(rng, 1, page, FL, dev)
+    q = queries(rng, 64, 4, T, FL, dev)
+    lens = _i32(1 + 7 * np.arange(64) % 73, dev)
+
+    def call(times):
+        rows = 64 * times
+        led = {"weights": torch.zeros((rows, page), device=dev), "pos": torch.zeros((rows, page), dtype=torch.int32, device=dev),
+               "dropped": torch.zeros(rows, dtype=torch.int32, device=dev)}
+        p = ops.Pages(k, v, torch.zeros((rows, 1), dtype=torch.int32, device=dev), lens.repeat(times), 1, **led)
+        return ops.paged_attn(q.repeat(times, 1, 1, 1), p, SCALE, weigh=True), p.weights
+
+    (out, w), (outs, ws) = call(1), call(n)
+    assert torch.isfinite(out).all() and (w.sum(1) > 0).all()
+    assert torch.equal(outs.view(n, *out.shape), out.expand(n, *out.shape))
+    assert torch.equal(ws.view(n, 64, page)[:, :, :128], w[:, :128].expand(n, -1, -1)) and not ws[:, 128:].any()
+
+
+def test_as_many_rows_as_a_cache_holds(dev):
+    """2^24 table rows: an append and an eviction reach the last ones."""
+    rng = np.random.default_rng(22)
+    rows, page = 1 << 24, 4
+    some = {0: 0, 1 << 23: 1, rows - 1: 2}
+    k, v = _pool(rng, 4, page, BF, dev)
+    table = _table(rows, 1, some, dev)
+    row_len, status = torch.zeros(rows, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    led = {"weights": torch.full((rows, page), -1.0, device=dev), "pos": torch.full((rows, page), -1, dtype=torch.int32, device=dev),
+           "dropped": torch.zeros(rows, dtype=torch.int32, device=dev)}
+    p = ops.Pages(k, v, table, row_len, 1, status=status, **led)
+    kn, vn = (queries(rng, 1, 1, page, BF, dev) for _ in range(2))
+    counts = torch.zeros(rows, dtype=torch.int32, device=dev)
+    counts[list(some)] = page
+    ops.paged_append(kn.expand(rows, -1, -1, -1), vn.expand(rows, -1, -1, -1), p, counts=counts)
+    assert torch.equal(row_len, counts) and status.item() == 0
+    for r, pg in some.items():
+        assert torch.equal(k[pg, :, 0], kn[0, 0]) and torch.equal(v[pg, :, 0], vn[0, 0])
+        assert p.pos[r].tolist() == [0, 1, 2, 3] and p.weights[r].tolist() == [0.0] * page
+        p.weights[r] = torch.tensor([2.0, 1.0, 4.0, 3.0], device=dev)
+    ops.paged_evict(p, 2)
+    assert torch.equal(row_len, counts // 2) and torch.equal(p.dropped, counts // 2) and status.item() == 0
+    for r, pg in some.items():
+        assert p.pos[r, :2].tolist() == [2, 3] and p.weights[r, :2].tolist() == [4.0, 3.0]
+        assert torch.equal(k[pg, :2, 0], kn[0, 0, 2:]) and torch.equal(v[pg, :2, 0], vn[0, 0, 2:])
