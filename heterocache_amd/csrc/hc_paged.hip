@@ -108,9 +108,14 @@ Layout layout(const hc_paged_cache* c, int q_heads, int queries, bool counts, bo
   return l;
 }
 
+// More than 2^26 query rows (whose product may pass 64 bits).
+bool too_many(const hc_paged_cache* c, int q_heads, int queries) {
+  return (int64_t)c->batch * q_heads > 1 << 26 || (int64_t)c->batch * q_heads * queries > 1 << 26;
+}
+
 bool sized(const hc_paged_cache* c, int q_heads, int queries) {
   return c && c->batch > 0 && c->kv_heads > 0 && q_heads > 0 && q_heads % c->kv_heads == 0 && queries > 0 && c->table_pages > 0 &&
-         c->page_tokens > 0;
+         c->page_tokens > 0 && !too_many(c, q_heads, queries);
 }
 
 int check_fresh(const char* name, const hc_paged_cache* c, const void* k, const int64_t* ks, const void* v, const int64_t* vs,
@@ -175,7 +180,7 @@ extern "C" int hc_paged_attn(const hc_paged_cache* c, const void* q, const int64
   clear_error();
   PagedAttn a = {};
   if (int rc = fill_pool("hc_paged_attn", c, a.pool, queries, counts)) return rc;
-  if (q_heads < 1 || q_heads % c->kv_heads || queries < 0 || (int64_t)c->batch * q_heads * queries > 1 << 26)
+  if (q_heads < 1 || q_heads % c->kv_heads || queries < 0 || too_many(c, q_heads, queries))
     return set_error(HC_ERR_INVALID, "hc_paged_attn: q_heads=%d kv_heads=%d queries=%d (at most 2^26 query rows)", q_heads,
                      c->kv_heads, queries);
   if (!std::isfinite(scale) || !(scale > 0.f))

@@ -140,3 +140,12 @@ def test_evict(lib):
     _refused(lib, _evict(lib, c, recent=7), b"exceed keep=8")
     _refused(lib, _evict(lib, _cache(weights=None)), b"no weights")
     assert _evict(lib, _cache(batch=0)) == 0
+
+
+def test_query_rows_past_64_bits(lib):
+    c = _cache(batch=16)
+    _refused(lib, _attn(lib, c, hq=1 << 30, n=1 << 30), b"2^26")
+    _refused(lib, _attn(lib, c, hq=1 << 24, n=1 << 30), b"2^26")
+    assert lib.hc_paged_workspace_size(ctypes.byref(c), 1 << 30, 1 << 30, 0, 0) == 0
+    assert lib.hc_paged_workspace_size(ctypes.byref(c), 8, 1 << 20, 0, 0) == 0
+    assert lib.hc_paged_workspace_size(ctypes.byref(c), 8, 1 << 19, 0, 0) > 0
