@@ -122,8 +122,8 @@ __device__ __forceinline__ RowState row_state(const EvictArgs& a, int row) {
 }
 
 // Keys of rows whose weights are sums over heads, by more workgroups than rows.
-__global__ __launch_bounds__(kRunThreads) void evict_keys_kernel(const EvictArgs a) {
-  const uint32_t x = group_id();
+__global__ __launch_bounds__(kRunThreads) void evict_keys_kernel(const EvictArgs a, uint32_t group0) {
+  const uint32_t x = group0 + blockIdx.x;
   const int row = x % a.rows, t = x / a.rows * kRunThreads + threadIdx.x;
   const RowState s = row_state(a, row);
   if (s.n > s.keep && t < s.n) a.keys[(int64_t)row * a.pool.capacity + t] = token_key(a, row, t, s.n + s.dropped - a.recent);
@@ -131,14 +131,13 @@ __global__ __launch_bounds__(kRunThreads) void evict_keys_kernel(const EvictArgs
 
 // Short rows: one workgroup a row, PER keys a thread.  READY: evict_keys_kernel has formed them.
 template <int PER, bool READY>
-__global__ __launch_bounds__(kThreads) void evict_select_kernel(const EvictArgs a) {
+__global__ __launch_bounds__(kThreads) void evict_select_kernel(const EvictArgs a, uint32_t group0) {
   __shared__ int s_hist[kBins];
   __shared__ int s_wave[kWaves + 1];
   __shared__ int s_count[PER * kWaves];
   __shared__ uint32_t s_range[2];
   __shared__ int s_pick[2];
-  const int row = (int)group_id(), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (row >= a.rows) return;
+  const int row = group0 + blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   RowState st = row_state(a, row);
   const int n = st.n, keep = st.keep;
   int32_t* const list = a.moves + (int64_t)row * a.pool.capacity;
@@ -254,9 +253,9 @@ __global__ __launch_bounds__(256) void evict_clear_kernel(const EvictArgs a) {
 __device__ __forceinline__ int32_t* row_hist(const EvictArgs& a, int row) { return a.hist + (int64_t)row * kTop; }
 
 // Second: the keys, counted by their top bits.
-__global__ __launch_bounds__(kRunThreads) void evict_count_kernel(const EvictArgs a) {
+__global__ __launch_bounds__(kRunThreads) void evict_count_kernel(const EvictArgs a, uint32_t group0) {
   __shared__ int s_hist[kTop];
-  const uint32_t x = group_id();
+  const uint32_t x = group0 + blockIdx.x;
   const int row = x % a.rows, run = x / a.rows, tid = threadIdx.x;
   const int n = a.state[row].n, keep = a.state[row].keep;
   if (n <= keep || run * kRun >= n) return;
@@ -310,10 +309,10 @@ __device__ __forceinline__ int2 pick_bin(const int* hist, int want, int* s_wave,
 }
 
 // Third: the keys that share the threshold's top bits (in any order).
-__global__ __launch_bounds__(kRunThreads) void evict_collect_kernel(const EvictArgs a) {
+__global__ __launch_bounds__(kRunThreads) void evict_collect_kernel(const EvictArgs a, uint32_t group0) {
   __shared__ int s_wave[kRunThreads / 64 + 1], s_pick[2];
   __shared__ int s_base[kRunThreads / 64];
-  const uint32_t x = group_id();
+  const uint32_t x = group0 + blockIdx.x;
   const int row = x % a.rows, run = x / a.rows, tid = threadIdx.x;
   const int n = a.state[row].n, keep = a.state[row].keep;
   if (n <= keep || keep == 0 || run * kRun >= n) return;
@@ -342,11 +341,11 @@ __global__ __launch_bounds__(kRunThreads) void evict_collect_kernel(const EvictA
 }
 
 // Fourth: the threshold, and the run's keys above it and at it.
-__global__ __launch_bounds__(kRunThreads) void evict_rank_kernel(const EvictArgs a) {
+__global__ __launch_bounds__(kRunThreads) void evict_rank_kernel(const EvictArgs a, uint32_t group0) {
   __shared__ int s_hist[kRunThreads * 8];
   __shared__ int s_wave[kRunThreads / 64 + 1], s_pick[2];
   __shared__ RunCount s_count;
-  const uint32_t x = group_id();
+  const uint32_t x = group0 + blockIdx.x;
   const int row = x % a.rows, run = x / a.rows, tid = threadIdx.x;
   const int n = a.state[row].n, keep = a.state[row].keep;
   if (n <= keep || run * kRun >= n) return;
@@ -406,9 +405,9 @@ __global__ __launch_bounds__(kRunThreads) void evict_rank_kernel(const EvictArgs
 }
 
 // Fifth: the lists.  What the runs ahead free and move follows from their counts.
-__global__ __launch_bounds__(kRunThreads) void evict_list_kernel(const EvictArgs a) {
+__global__ __launch_bounds__(kRunThreads) void evict_list_kernel(const EvictArgs a, uint32_t group0) {
   __shared__ int s_part[3][kRunPer * kRunThreads / 64];
-  const uint32_t x = group_id();
+  const uint32_t x = group0 + blockIdx.x;
   const int row = x % a.rows, run = x / a.rows, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const RowState st = a.state[row];
   const int n = st.n, keep = st.keep;
@@ -485,11 +484,10 @@ __global__ __launch_bounds__(kRunThreads) void evict_list_kernel(const EvictArgs
 // values (16 bytes a thread, neighbouring threads a token), then a head's
 // weights, then the positions.  Both pages of a move lie in the pool, or the
 // token's keys and values stay where they are and the status word says so.
-__global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a) {
+__global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, uint32_t group0) {
   const Pool& p = a.pool;
-  const uint32_t x = group_id();
+  const uint32_t x = group0 + blockIdx.x;
   const int row = x / a.move_blocks, blk = x % a.move_blocks;
-  if (row >= a.rows) return;
   const RowState st = a.state[row];
   const int count = st.moved, kept = min(st.n, st.keep);
   const int32_t* const list = a.moves + (int64_t)row * p.capacity;
@@ -634,34 +632,31 @@ extern "C" int hc_paged_evict(const hc_paged_cache* c, const int32_t* keep, int 
   const int64_t most = (int64_t)(a.pool.capacity / 2) * (HC_HEAD_DIM * a.esz / 16);
   a.move_blocks = (int)std::max<int64_t>(1, std::min<int64_t>((most + 511) / 512, 4096 / (a.rows * (2 * a.pool.heads + 1))));
   hipStream_t s = (hipStream_t)stream;
-  const int64_t grid = (int64_t)a.rows * l.runs;
   if (a.pool.heads > 32767) return set_error(HC_ERR_INVALID, "hc_paged_evict: %d heads", a.pool.heads);
-  const dim3 move = groups((int64_t)a.rows * a.move_blocks, 256, 2 * a.pool.heads + 1);
+  auto launch = [&](auto kernel, int64_t n, int threads, unsigned y = 1) {
+    return in_launches(n, threads, [&](dim3 grid, uint32_t group0) {
+      grid.y = y;
+      hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, a, group0);
+      return check_launch("hc_paged_evict");
+    });
+  };
+  int rc;
   if (l.is_long) {
+    const int64_t runs = (int64_t)a.rows * l.runs;
     hipLaunchKernelGGL(evict_clear_kernel, dim3((unsigned)std::min<int64_t>(((int64_t)a.rows * kTop + 255) / 256, 1024)), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(evict_count_kernel, groups(grid), dim3(kRunThreads), 0, s, a);
-    hipLaunchKernelGGL(evict_collect_kernel, groups(grid), dim3(kRunThreads), 0, s, a);
-    hipLaunchKernelGGL(evict_rank_kernel, groups(grid), dim3(kRunThreads), 0, s, a);
-    hipLaunchKernelGGL(evict_list_kernel, groups(grid), dim3(kRunThreads), 0, s, a);
-    if (int rc = check_launch("hc_paged_evict")) return rc;
-    hipLaunchKernelGGL(evict_move_kernel, move, dim3(256), 0, s, a);
-    return check_launch("hc_paged_evict(move)");
-  }
-  const dim3 rows = groups(a.rows, kThreads), threads(kThreads);
-  const bool few = a.pool.capacity <= 4 * kThreads;
-  if (a.pool.heads > 1) {
-    const int64_t blocks = (int64_t)a.rows * ((a.pool.capacity + kRunThreads - 1) / kRunThreads);
-    hipLaunchKernelGGL(evict_keys_kernel, groups(blocks), dim3(kRunThreads), 0, s, a);
-    if (few)
-      hipLaunchKernelGGL((evict_select_kernel<4, true>), rows, threads, 0, s, a);
-    else
-      hipLaunchKernelGGL((evict_select_kernel<16, true>), rows, threads, 0, s, a);
-  } else if (few) {
-    hipLaunchKernelGGL((evict_select_kernel<4, false>), rows, threads, 0, s, a);
+    rc = check_launch("hc_paged_evict");
+    if (!rc) rc = launch(evict_count_kernel, runs, kRunThreads);
+    if (!rc) rc = launch(evict_collect_kernel, runs, kRunThreads);
+    if (!rc) rc = launch(evict_rank_kernel, runs, kRunThreads);
+    if (!rc) rc = launch(evict_list_kernel, runs, kRunThreads);
   } else {
-    hipLaunchKernelGGL((evict_select_kernel<16, false>), rows, threads, 0, s, a);
+    const bool few = a.pool.capacity <= 4 * kThreads;
+    if (a.pool.heads > 1) {
+      rc = launch(evict_keys_kernel, (int64_t)a.rows * ((a.pool.capacity + kRunThreads - 1) / kRunThreads), kRunThreads);
+      if (!rc) rc = few ? launch(evict_select_kernel<4, true>, a.rows, kThreads) : launch(evict_select_kernel<16, true>, a.rows, kThreads);
+    } else {
+      rc = few ? launch(evict_select_kernel<4, false>, a.rows, kThreads) : launch(evict_select_kernel<16, false>, a.rows, kThreads);
+    }
   }
-  if (int rc = check_launch("hc_paged_evict")) return rc;
-  hipLaunchKernelGGL(evict_move_kernel, move, dim3(256), 0, s, a);
-  return check_launch("hc_paged_evict(move)");
+  return rc ? rc : launch(evict_move_kernel, (int64_t)a.rows * a.move_blocks, 256, 2 * a.pool.heads + 1);
 }

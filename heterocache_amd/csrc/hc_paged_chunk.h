@@ -575,7 +575,6 @@ template <bool MIXED>
 __device__ __forceinline__ void paged_append_job(const PagedAttn& a, const int x, int chunks, int blocks) {
   const Pool& p = a.pool;
   const int row = x / blocks, blk = x % blocks;
-  if (row >= p.rows) return;
   const int b = row / p.Hkv, h = row % p.Hkv;
   const int trow = table_row(p, row), hd = p.heads == 1 ? 0 : h;
   const RowSpan s = row_span(p, row);

@@ -9,9 +9,9 @@ namespace hc {
 namespace {
 
 template <typename T, bool UNIFORM>
-__global__ __launch_bounds__(kPagedThreads, sizeof(T) == 4 ? 2 : 3) void paged_chunk_kernel(const PagedAttn a) {
+__global__ __launch_bounds__(kPagedThreads, sizeof(T) == 4 ? 2 : 3) void paged_chunk_kernel(const PagedAttn a, uint32_t group0) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  paged_chunk_job<T, UNIFORM, false>(a, (int)group_id(), lds);
+  paged_chunk_job<T, UNIFORM, false>(a, group0 + blockIdx.x, lds);
 }
 
 template <typename T>
@@ -19,8 +19,8 @@ __global__ __launch_bounds__(256) void paged_chunk_fold_kernel(const PagedAttn a
   paged_chunk_fold_job<T>(a, blockIdx.x, gridDim.x);
 }
 
-__global__ __launch_bounds__(256) void paged_append_kernel(const PagedAttn a, int chunks, int blocks) {
-  paged_append_job<false>(a, (int)group_id(), chunks, blocks);
+__global__ __launch_bounds__(256) void paged_append_kernel(const PagedAttn a, int chunks, int blocks, uint32_t group0) {
+  paged_append_job<false>(a, group0 + blockIdx.x, chunks, blocks);
 }
 
 // Every token's share of the chunk's attention,
@@ -39,7 +39,7 @@ constexpr int weigh_lds() {
 }
 
 template <typename T, int NC>
-__global__ __launch_bounds__(kPagedThreads, sizeof(T) == 4 ? 2 : NC == 4 ? 3 : 4) void paged_weigh_kernel(const PagedAttn a, int blocks) {
+__global__ __launch_bounds__(kPagedThreads, sizeof(T) == 4 ? 2 : NC == 4 ? 3 : 4) void paged_weigh_kernel(const PagedAttn a, int blocks, uint32_t group0) {
   typedef typename Elem<T>::vec8 vec8;
   typedef Tile<T> Tl;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(kPagedThreads, sizeof(T) == 4 ? 2 : NC == 4 ? 3 : 4
   // Rows r, r + 8, .. on one XCD, the blocks of a row behind each other: workgroups
   // are dealt in turn to the XCDs and within one to its four engines, where rows
   // of a sequence each would all meet (4 ragged sequences: 162 us, now 85).
-  const uint32_t x = group_id();
+  const uint32_t x = group0 + blockIdx.x;
   const int row = x % 8 + 8 * (x / 8 / blocks), tb = x / 8 % blocks;
   if (row >= p.rows) return;
   const int b = row / p.Hkv, h = row % p.Hkv;
@@ -168,8 +168,10 @@ int launch_attn(const PagedAttn& a, hipStream_t s) {
                                hipFuncAttributeMaxDynamicSharedMemorySize, chunk_lds<T>());
   });
   if (attr != hipSuccess) return set_error(HC_ERR_HIP, "hc_paged_attn: %s", hipGetErrorString(attr));
-  hipLaunchKernelGGL((paged_chunk_kernel<T, UNIFORM>), groups(a.chunk_grid), dim3(kPagedThreads), chunk_lds<T>(), s, a);
-  return check_launch("hc_paged_attn(chunk)");
+  return in_launches(a.chunk_grid, kPagedThreads, [&](dim3 grid, uint32_t group0) {
+    hipLaunchKernelGGL((paged_chunk_kernel<T, UNIFORM>), grid, dim3(kPagedThreads), chunk_lds<T>(), s, a, group0);
+    return check_launch("hc_paged_attn(chunk)");
+  });
 }
 
 template <typename T, int NC>
@@ -183,9 +185,10 @@ int launch_weigh(const PagedAttn& a, hipStream_t s) {
   if (attr != hipSuccess) return set_error(HC_ERR_HIP, "hc_paged_attn: %s", hipGetErrorString(attr));
   const int block = kPagedWaves * 16 * NC;
   const int blocks = (a.pool.capacity + block - 1) / block;
-  const int64_t grid = (int64_t)(a.pool.rows + 7) / 8 * 8 * blocks;
-  hipLaunchKernelGGL((paged_weigh_kernel<T, NC>), groups(grid), dim3(kPagedThreads), weigh_lds<T>(), s, a, blocks);
-  return check_launch("hc_paged_attn(weights)");
+  return in_launches((int64_t)(a.pool.rows + 7) / 8 * 8 * blocks, kPagedThreads, [&](dim3 grid, uint32_t group0) {
+    hipLaunchKernelGGL((paged_weigh_kernel<T, NC>), grid, dim3(kPagedThreads), weigh_lds<T>(), s, a, blocks, group0);
+    return check_launch("hc_paged_attn(weights)");
+  });
 }
 
 template <typename T>
@@ -214,11 +217,10 @@ __global__ __launch_bounds__(256) void paged_advance_kernel(const PagedAttn a, i
 }
 
 // The weights of a call without queries, in memory of their own.
-__global__ __launch_bounds__(256) void paged_carry_kernel(const PagedAttn a, int runs) {
-  const int x = (int)group_id(), row = x % a.pool.rows, total = row_span(a.pool, row).total;
+__global__ __launch_bounds__(256) void paged_carry_kernel(const PagedAttn a, int runs, uint32_t group0) {
+  const int x = group0 + blockIdx.x, row = x % a.pool.rows, total = row_span(a.pool, row).total;
   const float* const in = a.weights + row * a.weight_stride;
   float* const out = a.weights_out + row * a.weight_stride;
-  if (x >= a.pool.rows * runs) return;
   for (int t = x / a.pool.rows * 256 + (int)threadIdx.x; t < total; t += runs * 256) out[t] = in[t];
 }
 
@@ -242,17 +244,21 @@ int launch_paged_weights(int dtype, const PagedAttn& a, hipStream_t s) {
 
 int launch_paged_carry(const PagedAttn& a, hipStream_t s) {
   const int runs = paged_weigh_runs(a.pool);
-  hipLaunchKernelGGL(paged_carry_kernel, groups(a.pool.rows * runs), dim3(256), 0, s, a, runs);
-  return check_launch("hc_paged_attn(weights)");
+  return in_launches(a.pool.rows * runs, 256, [&](dim3 grid, uint32_t group0) {
+    hipLaunchKernelGGL(paged_carry_kernel, grid, dim3(256), 0, s, a, runs, group0);
+    return check_launch("hc_paged_attn(weights)");
+  });
 }
 
 int launch_paged_append(int dtype, const PagedAttn& a, hipStream_t s) {
   const int chunks = dtype == HC_DTYPE_F32 ? 32 : 16, blocks = std::max(1, (a.pool.Q + 15) / 16);
-  PagedAttn first = a;
+  PagedAttn store = a;
   const bool in_place = a.len_out && a.len_out == a.pool.row_len;
-  if (in_place) first.len_out = nullptr;
-  hipLaunchKernelGGL(paged_append_kernel, groups((int64_t)a.pool.rows * blocks), dim3(256), 0, s, first, chunks, blocks);
-  int rc = check_launch("hc_paged_append");
+  if (in_place) store.len_out = nullptr;
+  const int rc = in_launches((int64_t)a.pool.rows * blocks, 256, [&](dim3 grid, uint32_t group0) {
+    hipLaunchKernelGGL(paged_append_kernel, grid, dim3(256), 0, s, store, chunks, blocks, group0);
+    return check_launch("hc_paged_append");
+  });
   if (rc || !in_place) return rc;
   const int table_rows = a.pool.heads == 1 ? a.pool.rows : a.pool.rows / a.pool.Hkv;
   hipLaunchKernelGGL(paged_advance_kernel, dim3((table_rows + 255) / 256), dim3(256), 0, s, a, table_rows);

@@ -36,11 +36,11 @@ __global__ __launch_bounds__(kPagedThreads, sizeof(T) == 4 ? 1 : 2) void paged_m
 }
 
 template <typename T, bool WEIGH>
-__global__ __launch_bounds__(256) void paged_mixed_fold_kernel(const PagedAttn a, int runs, int few, int many) {
-  const int x = (int)group_id();
+__global__ __launch_bounds__(256) void paged_mixed_fold_kernel(const PagedAttn a, int runs, int few, int many, uint32_t group0) {
+  const int x = group0 + blockIdx.x;
   if (x < few)
     paged_fold_job<T, WEIGH>(a, x, runs);
-  else if (x < few + many)
+  else
     paged_chunk_fold_job<T>(a, x - few, many);
 }
 
@@ -78,8 +78,10 @@ int launch(int dtype, const PagedAttn& a, hipStream_t s) {
   if (rc) return rc;
   const int runs = WEIGH ? paged_weigh_runs(a.pool) : 0, few = a.pool.rows * (a.few + runs);
   const int many = (int)paged_chunk_fold_grid(a);
-  hipLaunchKernelGGL((paged_mixed_fold_kernel<T, WEIGH>), groups((int64_t)few + many), dim3(256), 0, s, a, runs, few, many);
-  return check_launch("hc_paged_attn(fold)");
+  return in_launches((int64_t)few + many, 256, [&](dim3 grid, uint32_t group0) {
+    hipLaunchKernelGGL((paged_mixed_fold_kernel<T, WEIGH>), grid, dim3(256), 0, s, a, runs, few, many, group0);
+    return check_launch("hc_paged_attn(fold)");
+  });
 }
 
 }  // namespace

@@ -14,9 +14,8 @@ __global__ __launch_bounds__(kPagedThreads, sizeof(T) == 4 ? 1 : 2) void paged_r
 }
 
 template <typename T, bool WEIGH>
-__global__ __launch_bounds__(256) void paged_fold_kernel(const PagedAttn a, int runs) {
-  const int x = (int)group_id();
-  if (x < a.pool.rows * (a.few + runs)) paged_fold_job<T, WEIGH>(a, x, runs);
+__global__ __launch_bounds__(256) void paged_fold_kernel(const PagedAttn a, int runs, uint32_t group0) {
+  paged_fold_job<T, WEIGH>(a, group0 + blockIdx.x, runs);
 }
 
 template <typename T, bool WEIGH, bool UNIFORM>
@@ -37,8 +36,10 @@ int launch(const PagedAttn& a, bool fold, hipStream_t s) {
   if (int rc = uniform_pages(a.pool) ? launch_attn<T, WEIGH, true>(a, s) : launch_attn<T, WEIGH, false>(a, s)) return rc;
   if (!fold) return HC_OK;
   const int runs = WEIGH ? paged_weigh_runs(a.pool) : 0;
-  hipLaunchKernelGGL((paged_fold_kernel<T, WEIGH>), groups(a.pool.rows * (a.few + runs)), dim3(256), 0, s, a, runs);
-  return check_launch("hc_paged_attn(fold)");
+  return in_launches(a.pool.rows * (a.few + runs), 256, [&](dim3 grid, uint32_t group0) {
+    hipLaunchKernelGGL((paged_fold_kernel<T, WEIGH>), grid, dim3(256), 0, s, a, runs, group0);
+    return check_launch("hc_paged_attn(fold)");
+  });
 }
 
 template <typename T>
