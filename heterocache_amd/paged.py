@@ -55,6 +55,7 @@ class PagedStore:
                       "pos": i32(self.rows, self.capacity), "dropped": i32(self.rows)}
         self.pages = ops.Pages(self.k, self.v, self.table, self.row_len, kv_heads, status=self.status, **ledger)
         self.host_len = np.zeros(self.rows, dtype=np.int64)
+        self._along = None                                   # the same along a graph that is being captured
         self.held = np.zeros(self.rows, dtype=np.int64)      # pages of each row
         self._ids = np.full((self.rows, width), -1, dtype=np.int32)
         self._free = list(range(pages - 1, -1, -1))          # the next page is the last
@@ -62,6 +63,20 @@ class PagedStore:
     @property
     def free_pages(self):
         return len(self._free)
+
+    # -- lengths ---------------------------------------------------------------
+    def _bound(self):
+        """Bound of the lengths ahead of a call on the current stream."""
+        if not torch.cuda.is_current_stream_capturing():
+            self._along = None
+        return self.host_len if self._along is None else self._along
+
+    def _advance(self, lens):
+        """The lengths behind a call.  One that is captured has not run: the host's bound falls with none, and holds
+        at every point of the first replay."""
+        if torch.cuda.is_current_stream_capturing():
+            self._along, lens = lens, np.maximum(self.host_len, lens)
+        self.host_len = lens
 
     # -- pages ---------------------------------------------------------------
     def _oom(self):
@@ -77,7 +92,7 @@ class PagedStore:
         more = np.asarray(tokens, dtype=np.int64)
         if (more < 0).any():
             raise ValueError(f"tokens={tokens}")
-        self._reserve(self.host_len + (np.repeat(more, self.per_sequence) if more.ndim else more))
+        self._reserve(self._bound() + (np.repeat(more, self.per_sequence) if more.ndim else more))
 
     def _reserve(self, lens):
         need = -(-lens // self.page_tokens)
@@ -130,23 +145,23 @@ class PagedStore:
         (ops.paged_append), for instance of a prompt that ops.prefill_attn
         attends.  counts: tokens of each sequence (host integers, or an int32
         device tensor; None: all T)."""
-        lens = self.host_len + self._added(counts, k.shape[2])
         with torch.cuda.stream(stream):  # (None: the current one)
+            lens = self._bound() + self._added(counts, k.shape[2])
             self._reserve(lens)
             ops.paged_append(k, v, self.pages, counts=counts)
-        self.host_len = lens
+            self._advance(lens)
 
     def extend(self, q, k, v, scale, counts=None, weigh=None, out=None, stream=None):
         """Appends new tokens and attends them over their rows: queries [B, Hq,
         T, 128], keys and values [B, Hkv, T, 128], turned by their positions;
         [B, T, Hq, 128] (ops.paged_attn).  weigh (default: whether the store
         tracks): every token's share of the attention is added to its weight."""
-        lens = self.host_len + self._added(counts, k.shape[2])
         weigh = self.pages.weights is not None if weigh is None else weigh
         with torch.cuda.stream(stream):
+            lens = self._bound() + self._added(counts, k.shape[2])
             self._reserve(lens)
             out = ops.paged_attn(q, self.pages, scale, k, v, counts=counts, weigh=weigh, out=out)
-        self.host_len = lens
+            self._advance(lens)
         return out
 
     def attend(self, q, scale, counts=None, weigh=False, out=None, stream=None):
@@ -161,14 +176,13 @@ class PagedStore:
         host = np.broadcast_to(np.asarray(keep, dtype=np.int64), (self.rows,))
         if (host < sink + recent).any():
             raise ValueError(f"keep={keep} holds less than sink={sink} and recent={recent}")
-        lens = np.minimum(self.host_len, host)
         with torch.cuda.stream(stream):
+            lens = np.minimum(self._bound(), host)
             arg = int(keep) if np.ndim(keep) == 0 else ops.host_counts("keep", host.copy(), self.device)
             ops.paged_evict(self.pages, arg, sink=sink, recent=recent)
-            if torch.cuda.is_current_stream_capturing():
-                return  # nothing has run: the old bound holds, and the pages are the rows' own
-            self._give_back(lens, range(self.rows))
-        self.host_len = lens
+            if not torch.cuda.is_current_stream_capturing():
+                self._give_back(lens, range(self.rows))
+            self._advance(lens)
 
     def release(self, sequences, stream=None):
         """Ends sequences: their rows are empty, their pages free."""
@@ -183,7 +197,7 @@ class PagedStore:
             if self.pages.dropped is not None:
                 self.pages.dropped.index_fill_(0, at, 0)
             self._give_back(np.zeros(len(rows), dtype=np.int64), rows)
-        self.host_len[rows] = 0
+        self.host_len[rows], self._along = 0, None
 
     def sync_host_lengths(self, lens):
         """The lengths that the device holds, where the host has only a bound
@@ -191,7 +205,7 @@ class PagedStore:
         lens = np.asarray(lens, dtype=np.int64)
         if lens.shape != (self.rows,) or (lens > self.held * self.page_tokens).any() or (lens < 0).any():
             raise RuntimeError("row lengths outside their pages")
-        self.host_len = lens.copy()
+        self.host_len, self._along = lens.copy(), None
 
     def check_status(self, stream=None):
         """Wait for the stream and raise "Layer i OOM." if a row had no room

@@ -292,3 +292,41 @@ def test_an_eviction_that_is_captured_and_not_replayed(dev):
     plain.evict([9] * s.rows, 2, 6, weights)
     plain.check()
     assert (s.held == 1).all()
+
+
+def test_steps_and_evictions_in_one_graph(dev):
+    """A graph of more steps than its evictions leave pages for: what the first replay needs is known along the graph,
+    while the host's bound holds for the rows as they are before it."""
+    rng = np.random.default_rng(11)
+    s = PagedStore(1, 2, 40, BF, dev, max_tokens=64, page_tokens=4, per_head=True, track=True)
+    plain = Plain(s)
+    _extend(rng, s, plain, 4, 32, BF)
+    s.reserve(1)                                             # room for 36 tokens a row, and the graph appends 6
+    args = [_new(rng, s, 4, 1, BF) for _ in range(6)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph, outs, before = torch.cuda.CUDAGraph(), [], []
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            for a in args:
+                before.append(s.pages.weights.clone())
+                outs.append((s.extend(*a, SCALE), s.pages.weights.clone()))
+                s.evict(32, sink=1, recent=4)
+    torch.cuda.current_stream().wait_stream(side)
+    assert (s.host_len >= 32).all() and (s.host_len <= 36).all()
+    for _ in range(3):                                       # the graph runs when it is replayed, not before
+        _extend(rng, s, plain, 4, 1, BF)
+    weights = s.pages.weights.cpu().numpy()
+    s.evict(32, sink=1, recent=4)
+    plain.evict([32] * s.rows, 1, 4, weights)
+    s.reserve(1)
+    graph.replay()
+    torch.cuda.synchronize()
+    kept = s.pages.weights
+    for a, b, (out, w) in zip(args, before, outs):
+        kept.copy_(w)                                        # (as it was behind the step, for its check)
+        plain.extend(out, *a, [1], BF, b)
+        plain.evict([32] * s.rows, 1, 4, w.cpu().numpy())
+    s.sync_host_lengths(s.row_len.cpu().numpy())
+    plain.check()
+    s.check_status()
