@@ -14,11 +14,16 @@
 // into equal steps between the least and the greatest left until a step holds
 // one value (the top bits alone put most weights into a few counters, whose
 // additions run one after another: 8190 tokens 48 us, so 34).  Long rows, of
-// which one CU would draw some 33 GB/s: workgroups of 2048 tokens in four
-// launches, keys counted by their top 12 bits, those that share the threshold's
-// collected, the threshold found among them by every workgroup for itself, and
-// the lists written from the workgroups' counts (8 rows of up to 131072 tokens:
-// 37 us, one workgroup a row 346).  Ties at the threshold go to the lower slots
+// which one CU would draw some 33 GB/s: workgroups of 2048 tokens in five
+// launches, counters cleared, keys counted by their top 12 bits, those that share
+// the threshold's collected, the threshold found among them by every workgroup
+// for itself, and the lists written from the workgroups' counts (8 rows of up to
+// 131072 tokens: 37 us, one workgroup a row 346).  The candidates grow with what
+// shares those bits, and every workgroup counts them all: with the inputs cached
+// the whole call takes 60 us on spread weights, 146 where all lie within an eighth
+// of a binade and 475 where all are equal, as a stored prompt's are.  Which way a
+// row goes is decided by its table's capacity, which the host knows, not by its
+// length.  Ties at the threshold go to the lower slots
 // by a prefix count in slot order; freed slots and movers are ranked the same way
 // and paired by rank.  Moves run at the copy rate: 134 MB in 34 us.
 #include <algorithm>

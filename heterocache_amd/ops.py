@@ -1303,8 +1303,8 @@ def paged_attn(q, pages, scale, k_new=None, v_new=None, counts=None, weigh=False
     k_new, v_new [B, Hkv, T, 128]: the tokens' keys and values, appended by this
     call (None: the pages hold them).  counts: int32 device tensor [B] or host
     integers.  weigh: every token's share of the attention is added to the
-    cache's weights.  out: not q's memory; len_out, weights_out: receive the new
-    lengths and weights (default: in place)."""
+    cache's weights.  out: memory that no input holds; len_out, weights_out: receive
+    the new lengths and weights (default: in place)."""
     dev, fresh = pages.dev, k_new is not None
     if fresh != (v_new is not None):
         raise ValueError("new keys and values come together")

@@ -734,8 +734,9 @@ int hc_paged_append(const hc_paged_cache* c, const void* k, const int64_t* k_str
  * queries = 0: nothing is attended or appended (the tensors may be NULL), and
  * len_out and weights_out, where given, receive the old lengths and weights.
  * q, out: element strides batch, head, token, all of whole 16 bytes; out shares
- * no memory with q.  Stands where the reference calls flash attention over its
- * pools (heterocache/llama_model.py:382-389), for one new token or many.
+ * no memory with q, k_new or v_new.  Stands where the reference calls flash
+ * attention over its pools (heterocache/llama_model.py:382-389), for one new
+ * token or many.
  * workspace: hc_paged_workspace_size bytes (counts: whether the call has them),
  * 16-byte aligned, no initialisation; calls that overlap in time need their own.
  * With weigh it holds the scores of rows of up to 16 (query, head) pairs, 4 bytes
